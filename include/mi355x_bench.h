@@ -252,6 +252,119 @@ const char* mb_gemm_launched_kernel(int format, const mb_gemm_config* config, ui
 const char* mb_gemm_exact_tile_kernel(int format, const mb_gemm_config* config, uint32_t m, uint32_t n, uint32_t k,
                                       const void* scale_a, const void* scale_b);
 
+/* ---- layer operators: MXFP4 linear layers and routing to experts ----------
+ *
+ * What a mixture-of-experts layer calls around the MXFP4 GEMM: tensors to its
+ * operands and back, the products of a linear layer (one weight, or one for
+ * each expert), the choice of experts, the sort of the choices by expert and
+ * the weighted sum of the experts' outputs. The reference has none of these.
+ *
+ * Element types are MB_DTYPE_*. A tensor's rows are contiguous; inputs x and
+ * logits take a row stride in elements (0 repeats a row) and lie at any
+ * element's address. A size of zero is a call without work. */
+
+/* Rows of x [rows][k] to an MXFP4 operand: codes [out_rows][ceil(k/32)*16]
+ * bytes (16-byte aligned; even k in the low nibble, zero past k) and scales
+ * [ceil(k/256)][out_rows][8] (8-byte aligned; 127 for groups past k). The
+ * scale of a group of 32 elements is 2^e, e = clamp(floor(log2 max|x|) - 2,
+ * -127, 127), -127 for zeros; its elements are the E2M1 values nearest to
+ * x / 2^e, ties to the even code, saturating at 6. A group holding an infinity
+ * or NaN gets the scale 255 (NaN) and codes 0.
+ * slots NULL: row r becomes operand row r, out_rows = rows. Otherwise row r
+ * becomes the operand rows slots[r][0 .. copies), entries outside
+ * 0 .. out_rows-1 left out; operand rows that no entry names stay as they are. */
+int mb_mx_quantize(int dtype, const void* x, uint64_t x_bytes, uint32_t rows, uint32_t k, uint64_t row_stride,
+                   const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t out_rows, void* codes,
+                   uint64_t codes_bytes, void* scales, uint64_t scales_bytes, void* stream);
+
+/* The columns of x [rows][columns] to an operand of `columns` rows and
+ * k = `rows`: x transposed, groups of 32 along x's rows. */
+int mb_mx_quantize_columns(int dtype, const void* x, uint64_t x_bytes, uint32_t rows, uint32_t columns,
+                           uint64_t row_stride, void* codes, uint64_t codes_bytes, void* scales,
+                           uint64_t scales_bytes, void* stream);
+
+/* An operand to the values it stands for, out [rows][k]: exact in fp32 and
+ * bf16, rounded once in fp16. */
+int mb_mx_dequantize(int dtype, const void* codes, uint64_t codes_bytes, const void* scales, uint64_t scales_bytes,
+                     void* out, uint64_t out_bytes, uint32_t rows, uint32_t k, void* stream);
+
+/* C [rows][n] = A . B^T for operands A of `rows` rows and B of `experts`
+ * matrices of n rows (codes [experts][n][..], scales [experts][..][n][8]), K =
+ * k, sums in fp32, rounded once to dtype. offsets [experts+1] (device memory):
+ * A's rows offsets[e] .. offsets[e+1]-1 meet B's matrix e; rows from
+ * offsets[experts] on are not written. NULL with experts = 1: all rows. */
+int mb_mx_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
+                  const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes, void* c,
+                  uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets,
+                  uint64_t offsets_bytes, uint32_t experts, void* stream);
+
+/* Bytes of workspace (16-byte aligned) mb_mx_linear needs for `rows` rows of output. */
+uint64_t mb_mx_linear_workspace(uint32_t rows, uint32_t n, uint32_t k);
+
+/* Y = Q(X) . W^T: mb_mx_quantize of X, then mb_mx_product with the weight.
+ * offsets NULL: Y [tokens][n], one weight. With offsets and slots NULL: X's rows
+ * are already in the order of the experts. With order and slots (mb_dispatch,
+ * [tokens][copies]): X holds tokens, and Y [tokens*copies][n] their routed rows
+ * in the order of the experts; Y's rows from offsets[experts] on are not
+ * written. */
+int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,
+                 uint64_t w_bytes, const void* scale_w, uint64_t scale_w_bytes, void* y, uint64_t y_bytes, uint32_t n,
+                 uint32_t k, const int32_t* offsets, uint64_t offsets_bytes, const int32_t* order,
+                 const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t experts, void* workspace,
+                 uint64_t workspace_bytes, void* stream);
+
+/* Scores of mb_route. */
+#define MB_SCORES_SOFTMAX 0u
+#define MB_SCORES_SIGMOID 1u
+
+/* The `top` experts of every token and their weights. With s = softmax or
+ * sigmoid of the logits and c = s + bias (NULL: 0), in fp32: a logit of -inf
+ * masks its expert; of `groups` equal groups of consecutive experts the
+ * top_groups with the largest sum of their two largest c stay (of equal ones the
+ * lower); among the rest the `top` largest c, in falling order, of equal ones the
+ * lower index. chosen [tokens][top] is -1, with weight 0, where nothing is left;
+ * weights are s, divided by their sum if renormalize, times scale. A NaN score
+ * ranks below all others and gives a NaN weight.
+ * experts <= 1024, top <= 64, groups <= 64. */
+int mb_route(int dtype, const void* logits, uint64_t logits_bytes, uint32_t tokens, uint32_t experts,
+             uint64_t row_stride, const float* bias, uint64_t bias_bytes, uint32_t top, uint32_t scores,
+             uint32_t groups, uint32_t top_groups, uint32_t renormalize, float scale, int32_t* chosen,
+             uint64_t chosen_bytes, float* weights, uint64_t weights_bytes, void* stream);
+
+/* d_logits [tokens][experts] (contiguous, dtype) from the gradient of mb_route's
+ * weights, for the experts it chose: through the weights alone, the choice has
+ * no gradient. */
+int mb_route_backward(int dtype, const void* logits, uint64_t logits_bytes, uint32_t tokens, uint32_t experts,
+                      uint64_t row_stride, const int32_t* chosen, uint64_t chosen_bytes, const float* d_weights,
+                      uint64_t d_weights_bytes, uint32_t top, uint32_t scores, uint32_t renormalize, float scale,
+                      void* d_logits, uint64_t d_logits_bytes, void* stream);
+
+/* Bytes of workspace (4-byte aligned) of mb_dispatch. */
+uint64_t mb_dispatch_workspace(uint64_t entries, uint32_t experts);
+
+/* Sorts `entries` choices by expert, stably: offsets [experts+1] (the last the
+ * number of entries with an expert), order[slot] = entry, slots[entry] = slot,
+ * -1 for an entry without an expert (outside 0 .. experts-1) and in order's
+ * places past offsets[experts]. */
+int mb_dispatch(const int32_t* chosen, uint64_t chosen_bytes, uint64_t entries, uint32_t experts, int32_t* offsets,
+                uint64_t offsets_bytes, int32_t* order, uint64_t order_bytes, int32_t* slots, uint64_t slots_bytes,
+                void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* out [tokens][n] = sum over j of weights[t][j] * y[slots[t][j]] in fp32, in the
+ * order of j, rounded once; entries outside 0 .. y_rows-1 left out. */
+int mb_combine(int dtype, const void* y, uint64_t y_bytes, uint32_t y_rows, const int32_t* slots,
+               uint64_t slots_bytes, const float* weights, uint64_t weights_bytes, void* out, uint64_t out_bytes,
+               uint32_t tokens, uint32_t top, uint32_t n, void* stream);
+
+/* Gradients of mb_combine: d_y[slots[t][j]] = weights[t][j] * d_out[t] and
+ * d_weights[t][j] = the sum over n of d_out[t] * y[slots[t][j]] in fp32, 0 for
+ * entries left out. No two entries name one row; rows of d_y that none names
+ * stay as they are. */
+int mb_combine_backward(int dtype, const void* d_out, uint64_t d_out_bytes, const void* y, uint64_t y_bytes,
+                        uint32_t y_rows, const int32_t* slots, uint64_t slots_bytes, const float* weights,
+                        uint64_t weights_bytes, void* d_y, uint64_t d_y_bytes, float* d_weights,
+                        uint64_t d_weights_bytes, uint32_t tokens, uint32_t top, uint32_t n, void* stream);
+
 /* ---- vector: register-resident arithmetic chains ------------------------ */
 
 /* Vector chain kinds. Storage of input/output/coefficients per kind:

@@ -83,6 +83,7 @@ class GemmConfig(ctypes.Structure):
 MATRIX_FORMATS = {"bf16": 0, "fp16": 1, "fp32": 2, "tf32": 3, "int8": 4, "fp64": 5, "fp8": 6, "fp4": 7}
 
 _u64, _u32, _i32, _ptr = ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_void_p
+_f32 = ctypes.c_float
 
 # name -> (restype, argtypes). Every symbol here is declared in
 # include/mi355x_bench.h; tests check the two lists agree.
@@ -110,6 +111,23 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mb_gemm_exact_tile": (_i32, [_i32, ctypes.POINTER(GemmConfig), _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64,
                                   _ptr, _u64, _u32, _u32, _u32, _u32, _ptr]),
     "mb_gemm_exact_tile_kernel": (ctypes.c_char_p, [_i32, ctypes.POINTER(GemmConfig), _u32, _u32, _u32, _ptr, _ptr]),
+    "mb_mx_quantize": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr, _u64, _ptr]),
+    "mb_mx_quantize_columns": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _ptr, _u64, _ptr]),
+    "mb_mx_dequantize": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _ptr]),
+    "mb_mx_product": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _ptr,
+                             _u64, _u32, _ptr]),
+    "mb_mx_linear_workspace": (_u64, [_u32, _u32, _u32]),
+    "mb_mx_linear": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _ptr, _u64,
+                            _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
+    "mb_route": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _u32, _u32, _u32, _u32, _u32, _f32, _ptr, _u64,
+                        _ptr, _u64, _ptr]),
+    "mb_route_backward": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _f32,
+                                 _ptr, _u64, _ptr]),
+    "mb_dispatch_workspace": (_u64, [_u64, _u32]),
+    "mb_dispatch": (_i32, [_ptr, _u64, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr]),
+    "mb_combine": (_i32, [_i32, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _ptr]),
+    "mb_combine_backward": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64,
+                                   _u32, _u32, _u32, _ptr]),
     "mb_vector_kernel_name": (ctypes.c_char_p, [_i32, _u32]),
     "mb_vector_chains": (_i32, [_i32, _ptr, _ptr, _ptr, _u64, _u32, _u32, _u32, _u64, _u64, _u64, _ptr]),
 }

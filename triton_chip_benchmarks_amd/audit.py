@@ -36,6 +36,11 @@ _COPY_RE = re.compile(r"copy_kernelILi(\d+)ELi([012])E")
 _COPY_EDGES_RE = re.compile(r"copy_edges_kernelILi(\d+)ELi([012])E")
 _READ_RE = re.compile(r"read_sum_kernelI(f|DF16_|t)E")
 _READ_PACKED_RE = re.compile(r"read_sum_packed_kernelI(f|DF16_|t)Li(\d+)E")
+_ELEMENT_TYPE = {"f": "f32", "DF16_": "f16", "DF16b": "bf16"}
+_ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)E")
+_LAYER_RE = re.compile(r"(mx_quantize|mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
+                       r"_kernelI(f|DF16_|DF16b)E")
+_DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
 _VECTOR_RE = re.compile(r"vector_(\w+?)_kernelILi(\d+)E")
 _READ_TYPE = {"f": "f32", "DF16_": "f16", "t": "bf16"}
 
@@ -83,6 +88,15 @@ def registered_name(symbol: str) -> str | None:
     match = _READ_RE.search(symbol)
     if match:
         return f"read_sum_{_READ_TYPE[match.group(1)]}_vec"
+    match = _ROUTE_RE.search(symbol)
+    if match:
+        return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}_v{match.group(3)}"
+    match = _LAYER_RE.search(symbol)
+    if match:
+        return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}"
+    match = _DISPATCH_RE.search(symbol)
+    if match:
+        return match.group(1)
     match = _VECTOR_RE.search(symbol)
     if match:
         kind, unroll = match.groups()

@@ -1,0 +1,294 @@
+// MX quantisation: tensors to MXFP4 operands of the GEMMs, and back.
+//
+// A group of 32 elements along K shares a power-of-two scale 2^e,
+//   e = clamp(floor(log2 max|x|) - 2, -127, 127)   (-127 for a group of zeros),
+// and holds every element as the E2M1 value nearest to x / 2^e (ties to the even
+// code, saturating at 6). floor(log2) - 2 puts the largest element into [4, 8),
+// E2M1's top binade. The scale byte is S = e + 127; with the fp32 exponent field
+// f of max|x| it is max(f - 2, 0). A group that holds an infinity or a NaN has no
+// such scale: S = 255, the format's NaN, codes 0.
+//
+// Codes are [rows][ceil(k / 32) * 16] bytes, even k in the low nibble, zero past
+// k; scales [ceil(k / 256)][rows][8], 127 for groups past k: mb_gemm's operands.
+#include "mb_elem.h"
+#include "mb_mx.h"
+
+namespace mb {
+namespace {
+
+constexpr uint32_t kGroup = 32;   // elements sharing a scale
+constexpr uint32_t kBlock = 256;  // elements along K whose 8 scales a row holds together
+
+__device__ __forceinline__ float bits_float(uint32_t v) { return __builtin_bit_cast(float, v); }
+
+// Scale byte of a group whose largest magnitude has these fp32 bits.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
+  const int field = static_cast<int>(largest >> 23);
+  return field == 255 ? 255u : static_cast<uint32_t>(field > 2 ? field - 2 : 0);
+}
+
+// Two E2M1 codes in byte SEL of `word`.
+template <int SEL>
+__device__ __forceinline__ uint32_t encode_pair(uint32_t word, float a, float b, uint32_t scale) {
+  const int up = 127 - static_cast<int>(scale);
+  const float x = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(a, up), -6.0f, 6.0f);
+  const float y = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(b, up), -6.0f, 6.0f);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x, y, 1.0f, SEL);
+}
+
+__device__ __forceinline__ uint32_t encode8(const float (&v)[8], uint32_t scale) {
+  uint32_t word = 0;
+  word = encode_pair<0>(word, v[0], v[1], scale);
+  word = encode_pair<1>(word, v[2], v[3], scale);
+  word = encode_pair<2>(word, v[4], v[5], scale);
+  word = encode_pair<3>(word, v[6], v[7], scale);
+  return scale == 255 ? 0 : word;
+}
+
+__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+constexpr int kRowsPerWorkgroup = 32;
+
+// Rows of x to codes and scales. A lane takes eight elements, four lanes a
+// group, half a wave one row's 256 elements, a workgroup 32 rows of them. With
+// `slots` [rows][copies], row r goes to the operand's rows slots[r][0 .. copies),
+// those outside 0 .. out_rows - 1 left out; without, to row r.
+template <class T>
+__global__ void __launch_bounds__(256)
+    mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t row_stride,
+                       const int32_t* __restrict__ slots, uint32_t copies, uint32_t out_rows,
+                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  constexpr int U = 4;  // rows a lane loads at once
+  const uint32_t blocks = (k + kBlock - 1) / kBlock;
+  const uint32_t block = blockIdx.x % blocks;
+  const uint32_t row0 = blockIdx.x / blocks * kRowsPerWorkgroup + threadIdx.x / 32;
+  const uint32_t k0 = block * kBlock + threadIdx.x % 32 * 8;
+  const int count = static_cast<int>(k > k0 ? k - k0 : 0);
+  const uint32_t code_bytes = (k + kGroup - 1) / kGroup * 16;
+  Raw8<T> raw[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + 8 * u;
+    if (row < rows)
+      raw[u].load(x + row * row_stride + k0, count);
+    else
+      raw[u].zero();
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + 8 * u;
+    float v[8];
+    uint32_t largest = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = raw[u][i];
+      largest = max(largest, magnitude(v[i]));
+    }
+    largest = max(largest, quad_swap<kQuadXor1>(largest));
+    largest = max(largest, quad_swap<kQuadXor2>(largest));
+    const uint32_t scale = scale_byte(largest);
+    const uint32_t word = encode8(v, scale);
+    if (row >= rows) continue;
+    for (uint32_t c = 0; c < copies; ++c) {
+      const uint32_t out = slots ? static_cast<uint32_t>(slots[static_cast<uint64_t>(row) * copies + c]) : row;
+      if (out >= out_rows) continue;
+      if (k0 / 2 < code_bytes)
+        *reinterpret_cast<uint32_t*>(codes + static_cast<uint64_t>(out) * code_bytes + k0 / 2) = word;
+      if (threadIdx.x % 4 == 0)
+        scales[(static_cast<uint64_t>(block) * out_rows + out) * 8 + threadIdx.x % 32 / 4] =
+            static_cast<uint8_t>(k0 < k ? scale : 127);
+    }
+  }
+}
+
+// Columns of x to the rows of the transposed operand: groups of 32 run along
+// x's rows. A lane holds 32 rows of one column, so a group's largest magnitude
+// needs no other lane; a wave takes 64 columns of 32 rows.
+template <class T>
+__global__ void __launch_bounds__(256)
+    mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const uint32_t groups = (rows + kGroup - 1) / kGroup;
+  const uint32_t strips = (columns + 63) / 64;
+  const uint32_t strip = blockIdx.x % strips;
+  const uint32_t group = blockIdx.x / strips * 4 + threadIdx.x / 64;
+  const uint32_t column = strip * 64 + threadIdx.x % 64;
+  if (column >= columns || group >= (groups + 7) / 8 * 8) return;
+  uint8_t* scale_at = scales + (static_cast<uint64_t>(group / 8) * columns + column) * 8 + group % 8;
+  if (group >= groups) {
+    *scale_at = 127;
+    return;
+  }
+  float v[32];
+  uint32_t largest = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < 32; ++i) {
+    const uint32_t row = group * kGroup + i;
+    v[i] = row < rows ? widen(x[row * row_stride + column]) : 0.0f;
+    largest = max(largest, magnitude(v[i]));
+  }
+  const uint32_t scale = scale_byte(largest);
+  elem_u32x4 word;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    float part[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[i] = v[8 * q + i];
+    word[q] = encode8(part, scale);
+  }
+  *reinterpret_cast<elem_u32x4*>(codes + (static_cast<uint64_t>(column) * groups + group) * 16) = word;
+  *scale_at = static_cast<uint8_t>(scale);
+}
+
+// Codes and scales to values, rounded once to T (exact in fp32 and bf16).
+template <class T>
+__global__ void __launch_bounds__(256)
+    mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
+                         uint32_t rows, uint32_t k) {
+  const uint32_t per_row = (k + 7) / 8;
+  const uint64_t index = blockIdx.x * uint64_t{256} + threadIdx.x;
+  const uint64_t row = index / per_row;
+  if (row >= rows) return;
+  const uint32_t k0 = static_cast<uint32_t>(index % per_row) * 8;
+  const uint32_t code_bytes = (k + kGroup - 1) / kGroup * 16;
+  const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + row * code_bytes + k0 / 2);
+  const uint32_t scale = scales[(k0 / kBlock * uint64_t{rows} + row) * 8 + k0 % kBlock / kGroup];
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t code = word >> (4 * i) & 15u;
+    const float unit = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 0)[0];
+    v[i] = scale == 255 ? bits_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(unit, static_cast<int>(scale) - 127);
+  }
+  store8(out + row * k + k0, v, static_cast<int>(min(8u, k - k0)));
+}
+
+#define MB_MX_REGISTER(T, NAME)                                      \
+  MB_REGISTER_KERNEL("mx_quantize_" NAME, mx_quantize_kernel<T>);    \
+  MB_REGISTER_KERNEL("mx_quantize_columns_" NAME, mx_quantize_columns_kernel<T>); \
+  MB_REGISTER_KERNEL("mx_dequantize_" NAME, mx_dequantize_kernel<T>)
+MB_MX_REGISTER(float, "f32");
+MB_MX_REGISTER(_Float16, "f16");
+MB_MX_REGISTER(__bf16, "bf16");
+
+}  // namespace
+
+int check_operand(const char* entry, const char* what, uint64_t rows, uint64_t k, uint64_t copies, const void* codes,
+                  uint64_t codes_bytes, const void* scales, uint64_t scales_bytes) {
+  if (codes == nullptr || scales == nullptr) return fail(MB_ERR_INVALID, "%s: %s codes or scales are NULL", entry, what);
+  if (!aligned(codes, 16) || !aligned(scales, 8))
+    return fail(MB_ERR_ALIGNMENT, "%s: %s codes must lie on 16 bytes and scales on 8", entry, what);
+  if (codes_bytes < copies * mx_code_bytes(rows, k) || scales_bytes < copies * mx_scale_bytes(rows, k))
+    return fail(MB_ERR_INVALID, "%s: %s of %llu x %llu x %llu needs %llu code and %llu scale bytes; too small", entry,
+                what, (unsigned long long)copies, (unsigned long long)rows, (unsigned long long)k,
+                (unsigned long long)(copies * mx_code_bytes(rows, k)),
+                (unsigned long long)(copies * mx_scale_bytes(rows, k)));
+  return MB_OK;
+}
+
+int check_rows(const char* entry, int dtype, const void* x, uint64_t x_bytes, uint64_t rows, uint64_t k,
+               uint64_t row_stride) {
+  const uint32_t item = elem_bytes(dtype);
+  if (!item) return fail(MB_ERR_INVALID, "%s: unknown element type %d", entry, dtype);
+  if (x == nullptr) return fail(MB_ERR_INVALID, "%s: x is NULL", entry);
+  if (!aligned(x, item)) return fail(MB_ERR_ALIGNMENT, "%s: x must lie on its elements' %u bytes", entry, item);
+  if (rows > kMxMostRows || k > kMxMostK)
+    return fail(MB_ERR_UNSUPPORTED, "%s: %llu x %llu: at most %u rows of at most %u elements", entry,
+                (unsigned long long)rows, (unsigned long long)k, kMxMostRows, kMxMostK);
+  if (row_stride > UINT64_MAX / 8 / (rows ? rows : 1) || strided_bytes(rows, k, row_stride, item) > x_bytes)
+    return fail(MB_ERR_INVALID, "%s: x is too small for %llu rows of %llu elements at a stride of %llu", entry,
+                (unsigned long long)rows, (unsigned long long)k, (unsigned long long)row_stride);
+  return MB_OK;
+}
+
+int launch_quantize(int dtype, const void* x, uint32_t rows, uint32_t k, uint64_t row_stride, const int32_t* slots,
+                    uint32_t copies, uint32_t out_rows, void* codes, void* scales, hipStream_t stream) {
+  const uint64_t grid = (rows + uint64_t{kRowsPerWorkgroup} - 1) / kRowsPerWorkgroup * ((k + kBlock - 1) / kBlock);
+  if (grid > 0xffffffu)
+    return fail(MB_ERR_UNSUPPORTED, "mx_quantize: %u x %u exceeds one launch", rows, k);
+  MB_FOR_DTYPE(dtype, (mx_quantize_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream>>>(
+                          static_cast<const T*>(x), rows, k, row_stride, slots, copies, out_rows,
+                          static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales))));
+  return launch_status("mx_quantize");
+}
+
+int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                            void* codes, void* scales, hipStream_t stream) {
+  const uint64_t groups = (rows + kGroup - 1) / kGroup;
+  const uint64_t grid = (columns + uint64_t{63}) / 64 * ((groups + 7) / 8 * 2);
+  if (grid > 0xffffffu)
+    return fail(MB_ERR_UNSUPPORTED, "mx_quantize_columns: %u x %u exceeds one launch", rows, columns);
+  MB_FOR_DTYPE(dtype, (mx_quantize_columns_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream>>>(
+                          static_cast<const T*>(x), rows, columns, row_stride, static_cast<uint8_t*>(codes),
+                          static_cast<uint8_t*>(scales))));
+  return launch_status("mx_quantize_columns");
+}
+
+}  // namespace mb
+
+extern "C" {
+
+int mb_mx_quantize(int dtype, const void* x, uint64_t x_bytes, uint32_t rows, uint32_t k, uint64_t row_stride,
+                   const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t out_rows, void* codes,
+                   uint64_t codes_bytes, void* scales, uint64_t scales_bytes, void* stream) {
+  const char* entry = "mb_mx_quantize";
+  if (rows == 0 || k == 0) return mb::elem_bytes(dtype) ? MB_OK
+                                                        : mb::fail(MB_ERR_INVALID, "%s: unknown element type %d",
+                                                                   entry, dtype);
+  if (int rc = mb::check_rows(entry, dtype, x, x_bytes, rows, k, row_stride)) return rc;
+  if (slots == nullptr) {
+    copies = 1;
+    out_rows = rows;
+  } else if (copies == 0 || copies > 64 || slots_bytes < uint64_t{rows} * copies * 4) {
+    return mb::fail(MB_ERR_INVALID, "%s: slots must hold 1 to 64 entries for each of %u rows", entry, rows);
+  } else if (!mb::aligned(slots, 4)) {
+    return mb::fail(MB_ERR_ALIGNMENT, "%s: slots must lie on 4 bytes", entry);
+  }
+  if (out_rows > mb::kMxMostRows)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: at most %u operand rows", entry, mb::kMxMostRows);
+  if (int rc = mb::check_operand(entry, "the operand", out_rows, k, 1, codes, codes_bytes, scales, scales_bytes))
+    return rc;
+  return mb::launch_quantize(dtype, x, rows, k, row_stride, slots, copies, out_rows, codes, scales,
+                             static_cast<hipStream_t>(stream));
+}
+
+int mb_mx_quantize_columns(int dtype, const void* x, uint64_t x_bytes, uint32_t rows, uint32_t columns,
+                           uint64_t row_stride, void* codes, uint64_t codes_bytes, void* scales,
+                           uint64_t scales_bytes, void* stream) {
+  const char* entry = "mb_mx_quantize_columns";
+  if (rows == 0 || columns == 0) return mb::elem_bytes(dtype) ? MB_OK
+                                                              : mb::fail(MB_ERR_INVALID, "%s: unknown element type %d",
+                                                                         entry, dtype);
+  if (int rc = mb::check_rows(entry, dtype, x, x_bytes, rows, columns, row_stride)) return rc;
+  if (columns > mb::kMxMostRows || rows > mb::kMxMostK)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: %u x %u: at most %u rows", entry, rows, columns, mb::kMxMostK);
+  if (int rc = mb::check_operand(entry, "the operand", columns, rows, 1, codes, codes_bytes, scales, scales_bytes))
+    return rc;
+  return mb::launch_quantize_columns(dtype, x, rows, columns, row_stride, codes, scales,
+                                     static_cast<hipStream_t>(stream));
+}
+
+int mb_mx_dequantize(int dtype, const void* codes, uint64_t codes_bytes, const void* scales, uint64_t scales_bytes,
+                     void* out, uint64_t out_bytes, uint32_t rows, uint32_t k, void* stream) {
+  const char* entry = "mb_mx_dequantize";
+  const uint32_t item = mb::elem_bytes(dtype);
+  if (!item) return mb::fail(MB_ERR_INVALID, "%s: unknown element type %d", entry, dtype);
+  if (rows == 0 || k == 0) return MB_OK;
+  if (rows > mb::kMxMostRows || k > mb::kMxMostK)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: %u x %u: at most %u rows of at most %u elements", entry, rows, k,
+                    mb::kMxMostRows, mb::kMxMostK);
+  if (int rc = mb::check_operand(entry, "the operand", rows, k, 1, codes, codes_bytes, scales, scales_bytes))
+    return rc;
+  if (out == nullptr || out_bytes < uint64_t{rows} * k * item)
+    return mb::fail(MB_ERR_INVALID, "%s: out is NULL or too small for %u x %u", entry, rows, k);
+  if (!mb::aligned(out, item)) return mb::fail(MB_ERR_ALIGNMENT, "%s: out must lie on its elements' %u bytes", entry, item);
+  const uint64_t grid = (uint64_t{rows} * ((k + 7) / 8) + 255) / 256;
+  if (grid > 0xffffffu) return mb::fail(MB_ERR_UNSUPPORTED, "%s: %u x %u exceeds one launch", entry, rows, k);
+  MB_FOR_DTYPE(dtype, (mb::mx_dequantize_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0,
+                                                     static_cast<hipStream_t>(stream)>>>(
+                          static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
+                          static_cast<T*>(out), rows, k)));
+  return mb::launch_status("mx_dequantize");
+}
+
+}  // extern "C"

@@ -1,0 +1,622 @@
+// Routing of tokens to experts: choice and weights with their gradient, the
+// sort of the choices by expert, and the weighted sum of the experts' outputs
+// with its gradients.
+#include <type_traits>
+
+#include "mb_elem.h"
+
+namespace mb {
+namespace {
+
+constexpr uint32_t kMostExperts = 1024, kMostTop = 64;
+constexpr float kNegInf = -__builtin_inff();
+
+__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+// Orders a wave's LDS writes before its later LDS reads.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+}
+
+// Scores s of a token's logits, lane l holding experts l * V .. l * V + V - 1;
+// logits past the last expert and masked ones (-inf) are -inf and score 0.
+template <int V>
+__device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax, float (&score)[V]) {
+  if (!softmax) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) score[i] = sigmoid(logit[i]);
+    return;
+  }
+  float top = kNegInf;
+#pragma unroll
+  for (int i = 0; i < V; ++i) top = fmaxf(top, logit[i]);
+  top = wave_max(top);
+  if (top == kNegInf) top = 0.0f;  // nothing but masked experts
+  float total = 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    score[i] = expf(logit[i] - top);
+    total += score[i];
+  }
+  total = wave_add(total);
+#pragma unroll
+  for (int i = 0; i < V; ++i) score[i] = total == 0.0f ? 0.0f : score[i] / total;
+}
+
+template <class T, int V>
+__device__ __forceinline__ void load_logits(const T* __restrict__ row, uint32_t experts, int lane, float (&logit)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t e = lane * V + i;
+    logit[i] = e < experts ? widen(row[e]) : kNegInf;
+  }
+}
+
+// One wave a token. Selection values: score + bias; -inf where masked (a logit
+// of -inf) or outside the kept groups; a NaN counts as -1e38, below any score and
+// a finite sum with another, so that a token of NaNs still gets different
+// experts, with NaN weights.
+template <class T, int V>
+__global__ void __launch_bounds__(256)
+    route_kernel(const T* __restrict__ logits, uint32_t tokens, uint32_t experts, uint64_t row_stride,
+                 const float* __restrict__ bias, uint32_t top, bool softmax, uint32_t groups, uint32_t top_groups,
+                 bool renormalize, float scale, int32_t* __restrict__ chosen, float* __restrict__ weights) {
+  __shared__ float lds[4][64 * V];
+  __shared__ float group_lds[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t token = blockIdx.x * 4 + wave;
+  if (token >= tokens) return;
+  float logit[V], score[V], value[V];
+  load_logits(logits + token * row_stride, experts, lane, logit);
+  scores_of(logit, softmax, score);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t e = lane * V + i;
+    value[i] = score[i] + (bias && e < experts ? bias[e] : 0.0f);
+    if (value[i] != value[i]) value[i] = -1e38f;
+    if (logit[i] == kNegInf) value[i] = kNegInf;
+  }
+  if (groups > 1) {
+    const uint32_t size = experts / groups;
+#pragma unroll
+    for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = value[i];
+    wave_lds_fence();
+    float first = kNegInf, second = kNegInf;
+    if (static_cast<uint32_t>(lane) < groups) {
+      for (uint32_t i = 0; i < size; ++i) {
+        const float v = lds[wave][lane * size + i];
+        second = fmaxf(second, fminf(first, v));
+        first = fmaxf(first, v);
+      }
+      group_lds[wave][lane] = first + (second == kNegInf ? 0.0f : second);
+    }
+    wave_lds_fence();
+    // A group is kept if fewer than top_groups come before it: larger ones, or
+    // as large ones of a lower index.
+    bool kept = false;
+    if (static_cast<uint32_t>(lane) < groups) {
+      const float mine = group_lds[wave][lane];
+      uint32_t before = 0;
+      for (uint32_t g = 0; g < groups; ++g) {
+        const float other = group_lds[wave][g];
+        before += other > mine || (other == mine && g < static_cast<uint32_t>(lane));
+      }
+      kept = before < top_groups;
+    }
+    const uint64_t mask = __ballot(kept);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const uint32_t e = lane * V + i;
+      if (e < experts && !(mask >> (e / size) & 1)) value[i] = kNegInf;
+    }
+  }
+  int mine = -1;
+  float mine_score = 0.0f;
+  for (uint32_t j = 0; j < top; ++j) {
+    float best = value[0];
+    int at = 0;
+#pragma unroll
+    for (int i = 1; i < V; ++i) {
+      if (value[i] > best) {
+        best = value[i];
+        at = i;
+      }
+    }
+    const float largest = wave_max(best);
+    if (largest == kNegInf) break;
+    const int winner = __builtin_ctzll(__ballot(best == largest));
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (i == at) {
+        s = score[i];
+        if (lane == winner) value[i] = kNegInf;
+      }
+    }
+    const int expert = __shfl(lane * V + at, winner, 64);
+    s = __shfl(s, winner, 64);
+    if (lane == static_cast<int>(j)) {
+      mine = expert;
+      mine_score = s;
+    }
+  }
+  float weight = mine_score;
+  if (renormalize) {
+    const float total = wave_add(mine_score);
+    weight = total == 0.0f ? 0.0f : weight / total;
+  }
+  if (static_cast<uint32_t>(lane) < top) {
+    chosen[static_cast<uint64_t>(token) * top + lane] = mine;
+    weights[static_cast<uint64_t>(token) * top + lane] = weight * scale;
+  }
+}
+
+// Gradient of route's weights with respect to the logits, one wave a token.
+// With w_j = r s_j / Z over the chosen (Z = 1 unless renormalised) and g their
+// gradient, d s_j = r (g_j - sum_i g_i s_i / Z) / Z, then through the scores:
+// softmax d l = s (d s - sum d s s), sigmoid d l = d s s (1 - s). The choice
+// itself has no gradient.
+template <class T, int V>
+__global__ void __launch_bounds__(256)
+    route_backward_kernel(const T* __restrict__ logits, uint32_t tokens, uint32_t experts, uint64_t row_stride,
+                          const int32_t* __restrict__ chosen, const float* __restrict__ d_weights, uint32_t top,
+                          bool softmax, bool renormalize, float scale, T* __restrict__ d_logits) {
+  __shared__ float lds[4][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t token = blockIdx.x * 4 + wave;
+  if (token >= tokens) return;
+  float logit[V], score[V];
+  load_logits(logits + token * row_stride, experts, lane, logit);
+  scores_of(logit, softmax, score);
+  int expert = -1;
+  float d = 0.0f;
+  if (static_cast<uint32_t>(lane) < top) {
+    expert = chosen[static_cast<uint64_t>(token) * top + lane];
+    if (static_cast<uint32_t>(expert) >= experts) expert = -1;
+    if (expert >= 0) d = d_weights[static_cast<uint64_t>(token) * top + lane] * scale;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = score[i];
+  wave_lds_fence();
+  const float s = expert >= 0 ? lds[wave][expert] : 0.0f;
+  wave_lds_fence();
+  if (renormalize) {
+    const float total = wave_add(s);
+    const float mean = total == 0.0f ? 0.0f : wave_add(d * s) / total;
+    d = expert < 0 || total == 0.0f ? 0.0f : (d - mean) / total;
+  }
+  // Renormalised softmax weights do not change with the unchosen logits.
+  const float common = softmax && !renormalize ? wave_add(d * s) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = 0.0f;
+  wave_lds_fence();
+  if (expert >= 0) lds[wave][expert] = d;
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t e = lane * V + i;
+    const float ds = lds[wave][e];
+    if (e < experts)
+      d_logits[static_cast<uint64_t>(token) * experts + e] =
+          static_cast<T>(softmax ? score[i] * (ds - common) : ds * score[i] * (1.0f - score[i]));
+  }
+}
+
+// ---- dispatch ----------------------------------------------------------------
+
+constexpr int kDispatchWaves = 16, kDispatchRounds = 4;
+constexpr uint32_t kDispatchItems = kDispatchWaves * kDispatchRounds * 64;  // entries of a workgroup
+
+// Lanes whose expert equals this lane's; none for a lane without one.
+__device__ __forceinline__ uint64_t same_expert(int expert, uint32_t bits) {
+  uint64_t mask = __ballot(expert >= 0);
+  for (uint32_t b = 0; b < bits; ++b) {
+    const bool set = expert >> b & 1;
+    const uint64_t with = __ballot(set);
+    mask &= set ? with : ~with;
+  }
+  return expert < 0 ? 0 : mask;
+}
+
+__device__ __forceinline__ int load_expert(const int32_t* __restrict__ chosen, uint32_t i, uint32_t entries,
+                                           uint32_t experts) {
+  if (i >= entries) return -1;
+  const int e = chosen[i];
+  return static_cast<uint32_t>(e) < experts ? e : -1;
+}
+
+// Adds this wave's entries of each expert to its own row of the histogram.
+__device__ __forceinline__ void count_entries(const int32_t* __restrict__ chosen, uint32_t base, uint32_t entries,
+                                              uint32_t experts, uint32_t bits, uint32_t* hist, int lane) {
+  for (int r = 0; r < kDispatchRounds; ++r) {
+    const int e = load_expert(chosen, base + r * 64 + lane, entries, experts);
+    const uint64_t same = same_expert(e, bits);
+    if (same && __builtin_ctzll(same) == lane) hist[e] += __builtin_popcountll(same);
+    wave_lds_fence();
+  }
+}
+
+// Counts of each expert's entries, one row a workgroup.
+__global__ void __launch_bounds__(1024)
+    dispatch_count_kernel(const int32_t* __restrict__ chosen, uint32_t entries, uint32_t experts, uint32_t bits,
+                          uint32_t* __restrict__ counts) {
+  extern __shared__ uint32_t hist[];  // [waves][experts]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (uint32_t i = threadIdx.x; i < kDispatchWaves * experts; i += 1024) hist[i] = 0;
+  __syncthreads();
+  count_entries(chosen, blockIdx.x * kDispatchItems + wave * kDispatchRounds * 64, entries, experts, bits,
+                hist + wave * experts, lane);
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < experts; e += 1024) {
+    uint32_t total = 0;
+    for (int w = 0; w < kDispatchWaves; ++w) total += hist[w * experts + e];
+    counts[static_cast<uint64_t>(blockIdx.x) * experts + e] = total;
+  }
+}
+
+// Places every entry: an expert's entries follow those of the experts before
+// it, its own of earlier workgroups, waves, rounds and lanes. `counts` are the
+// rows of dispatch_count_kernel; NULL in a launch of one workgroup.
+__global__ void __launch_bounds__(1024)
+    dispatch_place_kernel(const int32_t* __restrict__ chosen, uint32_t entries, uint32_t experts, uint32_t bits,
+                          const uint32_t* __restrict__ counts, int32_t* __restrict__ offsets,
+                          int32_t* __restrict__ order, int32_t* __restrict__ slots) {
+  extern __shared__ uint32_t hist[];  // [waves][experts]
+  __shared__ uint32_t wave_total[kDispatchWaves];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const uint32_t base = blockIdx.x * kDispatchItems + wave * kDispatchRounds * 64;
+  for (uint32_t i = threadIdx.x; i < kDispatchWaves * experts; i += 1024) hist[i] = 0;
+  __syncthreads();
+  count_entries(chosen, base, entries, experts, bits, hist + wave * experts, lane);
+  __syncthreads();
+  // Thread e: the expert's entries in all workgroups, and in earlier ones.
+  const uint32_t e = threadIdx.x;
+  uint32_t total = 0, before = 0;
+  if (e < experts) {
+    if (counts) {
+      for (uint32_t b = 0; b < gridDim.x; ++b) {
+        const uint32_t c = counts[static_cast<uint64_t>(b) * experts + e];
+        before += b < blockIdx.x ? c : 0;
+        total += c;
+      }
+    } else {
+      for (int w = 0; w < kDispatchWaves; ++w) total += hist[w * experts + e];
+    }
+  }
+  uint32_t scan = total;
+#pragma unroll
+  for (int offset = 1; offset < 64; offset <<= 1) {
+    const uint32_t v = __shfl_up(scan, offset, 64);
+    if (lane >= offset) scan += v;
+  }
+  if (lane == 63) wave_total[wave] = scan;
+  __syncthreads();
+  uint32_t all = 0, start = scan - total;
+  for (int w = 0; w < kDispatchWaves; ++w) {
+    if (w < wave) start += wave_total[w];
+    all += wave_total[w];
+  }
+  if (e < experts) {
+    if (blockIdx.x == 0) offsets[e] = static_cast<int32_t>(start);
+    uint32_t at = start + before;
+    for (int w = 0; w < kDispatchWaves; ++w) {
+      const uint32_t c = hist[w * experts + e];
+      hist[w * experts + e] = at;
+      at += c;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) offsets[experts] = static_cast<int32_t>(all);
+  __syncthreads();
+  uint32_t* next = hist + wave * experts;
+  for (int r = 0; r < kDispatchRounds; ++r) {
+    const uint32_t i = base + r * 64 + lane;
+    const int expert = load_expert(chosen, i, entries, experts);
+    const uint64_t same = same_expert(expert, bits);
+    const uint32_t rank = __builtin_popcountll(same & ((uint64_t{1} << lane) - 1));
+    uint32_t slot = 0;
+    if (same) slot = next[expert] + rank;
+    wave_lds_fence();
+    if (same && rank == 0) next[expert] += __builtin_popcountll(same);
+    wave_lds_fence();
+    if (i < entries) {
+      slots[i] = same ? static_cast<int32_t>(slot) : -1;
+      if (same) order[slot] = static_cast<int32_t>(i);
+      if (i >= all) order[i] = -1;  // places of entries without an expert, at the end
+    }
+  }
+}
+
+// ---- combine -----------------------------------------------------------------
+
+// out[t] = sum over j of weights[t][j] * y[slots[t][j]], in the order of j. One
+// wave a token and 512 columns, eight a lane.
+template <class T>
+__global__ void __launch_bounds__(256)
+    combine_kernel(const T* __restrict__ y, uint32_t y_rows, const int32_t* __restrict__ slots,
+                   const float* __restrict__ weights, T* __restrict__ out, uint32_t tokens, uint32_t top, uint32_t n) {
+  const uint32_t strips = (n + 511) / 512;
+  const uint64_t task = blockIdx.x * uint64_t{4} + (threadIdx.x >> 6);
+  const uint64_t token = task / strips;
+  if (token >= tokens) return;
+  const uint32_t column = static_cast<uint32_t>(task % strips) * 512 + (threadIdx.x & 63) * 8;
+  if (column >= n) return;
+  const int count = static_cast<int>(min(8u, n - column));
+  float sum[8] = {};
+  for (uint32_t j = 0; j < top; ++j) {
+    const uint32_t slot = static_cast<uint32_t>(slots[token * top + j]);
+    if (slot >= y_rows) continue;
+    const float weight = weights[token * top + j];
+    Raw8<T> raw;
+    raw.load(y + uint64_t{slot} * n + column, count);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = fmaf(weight, raw[i], sum[i]);
+  }
+  store8(out + token * n + column, sum, count);
+}
+
+// d_y[slots[t][j]] = weights[t][j] * d_out[t] and d_weights[t][j] = the product
+// of d_out[t] and y[slots[t][j]]. One wave a token and j.
+template <class T>
+__global__ void __launch_bounds__(256)
+    combine_backward_kernel(const T* __restrict__ d_out, const T* __restrict__ y, uint32_t y_rows,
+                            const int32_t* __restrict__ slots, const float* __restrict__ weights, T* __restrict__ d_y,
+                            float* __restrict__ d_weights, uint32_t tokens, uint32_t top, uint32_t n) {
+  const uint64_t task = blockIdx.x * uint64_t{4} + (threadIdx.x >> 6);
+  if (task >= uint64_t{tokens} * top) return;
+  const int lane = threadIdx.x & 63;
+  const uint64_t token = task / top;
+  const uint32_t slot = static_cast<uint32_t>(slots[task]);
+  float dot = 0.0f;
+  if (slot < y_rows) {
+    const float weight = weights[task];
+    for (uint32_t column = lane * 8; column < n; column += 512) {
+      const int count = static_cast<int>(min(8u, n - column));
+      Raw8<T> g, v;
+      g.load(d_out + token * n + column, count);
+      v.load(y + uint64_t{slot} * n + column, count);
+      float d[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        dot = fmaf(g[i], v[i], dot);
+        d[i] = weight * g[i];
+      }
+      store8(d_y + uint64_t{slot} * n + column, d, count);
+    }
+  }
+  dot = wave_add(dot);
+  if (lane == 0) d_weights[task] = dot;
+}
+
+#define MB_ROUTE_REGISTER_V(T, NAME, V)                                            \
+  MB_REGISTER_KERNEL("route_" NAME "_v" #V, (route_kernel<T, V>));                 \
+  MB_REGISTER_KERNEL("route_backward_" NAME "_v" #V, (route_backward_kernel<T, V>))
+#define MB_ROUTE_REGISTER(T, NAME)                              \
+  MB_ROUTE_REGISTER_V(T, NAME, 1);                              \
+  MB_ROUTE_REGISTER_V(T, NAME, 2);                              \
+  MB_ROUTE_REGISTER_V(T, NAME, 4);                              \
+  MB_ROUTE_REGISTER_V(T, NAME, 8);                              \
+  MB_ROUTE_REGISTER_V(T, NAME, 16);                             \
+  MB_REGISTER_KERNEL("combine_" NAME, combine_kernel<T>);       \
+  MB_REGISTER_KERNEL("combine_backward_" NAME, combine_backward_kernel<T>)
+MB_ROUTE_REGISTER(float, "f32");
+MB_ROUTE_REGISTER(_Float16, "f16");
+MB_ROUTE_REGISTER(__bf16, "bf16");
+MB_REGISTER_KERNEL("dispatch_count", dispatch_count_kernel);
+MB_REGISTER_KERNEL("dispatch_place", dispatch_place_kernel);
+
+int check_logits(const char* entry, int dtype, const void* logits, uint64_t logits_bytes, uint32_t tokens,
+                 uint32_t experts, uint64_t row_stride, uint32_t top) {
+  const uint32_t item = elem_bytes(dtype);
+  if (!item) return fail(MB_ERR_INVALID, "%s: unknown element type %d", entry, dtype);
+  if (experts == 0 || experts > kMostExperts)
+    return fail(MB_ERR_INVALID, "%s: %u experts outside 1..%u", entry, experts, kMostExperts);
+  if (top == 0 || top > kMostTop || top > experts)
+    return fail(MB_ERR_INVALID, "%s: top %u outside 1..%u of %u experts", entry, top, kMostTop, experts);
+  if (tokens > (1u << 24)) return fail(MB_ERR_UNSUPPORTED, "%s: at most %u tokens", entry, 1u << 24);
+  if (tokens == 0) return MB_OK;
+  if (logits == nullptr || row_stride > UINT64_MAX / 8 / tokens ||
+      logits_bytes < strided_bytes(tokens, experts, row_stride, item))
+    return fail(MB_ERR_INVALID, "%s: logits are NULL or too small for %u tokens of %u experts", entry, tokens, experts);
+  if (!aligned(logits, item))
+    return fail(MB_ERR_ALIGNMENT, "%s: logits must lie on their elements' %u bytes", entry, item);
+  return MB_OK;
+}
+
+int check_chosen(const char* entry, const void* chosen, uint64_t chosen_bytes, const void* weights,
+                 uint64_t weights_bytes, uint64_t entries) {
+  if (chosen == nullptr || weights == nullptr || chosen_bytes < entries * 4 || weights_bytes < entries * 4)
+    return fail(MB_ERR_INVALID, "%s: experts or weights are NULL or too small for %llu entries", entry,
+                (unsigned long long)entries);
+  if (!aligned(chosen, 4) || !aligned(weights, 4))
+    return fail(MB_ERR_ALIGNMENT, "%s: experts and weights must lie on 4 bytes", entry);
+  return MB_OK;
+}
+
+template <class F>
+void for_experts(uint32_t experts, F&& f) {
+  if (experts <= 64)
+    f(std::integral_constant<int, 1>{});
+  else if (experts <= 128)
+    f(std::integral_constant<int, 2>{});
+  else if (experts <= 256)
+    f(std::integral_constant<int, 4>{});
+  else if (experts <= 512)
+    f(std::integral_constant<int, 8>{});
+  else
+    f(std::integral_constant<int, 16>{});
+}
+
+uint64_t dispatch_blocks(uint64_t entries) { return (entries + kDispatchItems - 1) / kDispatchItems; }
+
+}  // namespace
+}  // namespace mb
+
+extern "C" {
+
+int mb_route(int dtype, const void* logits, uint64_t logits_bytes, uint32_t tokens, uint32_t experts,
+             uint64_t row_stride, const float* bias, uint64_t bias_bytes, uint32_t top, uint32_t scores,
+             uint32_t groups, uint32_t top_groups, uint32_t renormalize, float scale, int32_t* chosen,
+             uint64_t chosen_bytes, float* weights, uint64_t weights_bytes, void* stream) {
+  const char* entry = "mb_route";
+  if (int rc = mb::check_logits(entry, dtype, logits, logits_bytes, tokens, experts, row_stride, top)) return rc;
+  if (scores > MB_SCORES_SIGMOID) return mb::fail(MB_ERR_INVALID, "%s: unknown scores %u", entry, scores);
+  if (groups == 0 || groups > 64 || experts % groups || top_groups == 0 || top_groups > groups)
+    return mb::fail(MB_ERR_INVALID, "%s: %u of %u groups: 1 to 64 groups that divide the %u experts", entry,
+                    top_groups, groups, experts);
+  if (top > experts / groups * top_groups)
+    return mb::fail(MB_ERR_INVALID, "%s: top %u exceeds the %u experts of %u groups", entry, top,
+                    experts / groups * top_groups, top_groups);
+  if (bias && (bias_bytes < uint64_t{experts} * 4 || !mb::aligned(bias, 4)))
+    return mb::fail(MB_ERR_INVALID, "%s: the bias must hold %u floats, on 4 bytes", entry, experts);
+  if (tokens == 0) return MB_OK;
+  if (int rc = mb::check_chosen(entry, chosen, chosen_bytes, weights, weights_bytes, uint64_t{tokens} * top))
+    return rc;
+  const dim3 grid((tokens + 3) / 4);
+  MB_FOR_DTYPE(dtype, mb::for_experts(experts, [&](auto v) {
+    mb::route_kernel<T, decltype(v)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const T*>(logits), tokens, experts, row_stride, bias, top, scores == MB_SCORES_SOFTMAX,
+        top_groups == groups ? 1 : groups, top_groups, renormalize != 0, scale, chosen, weights);
+  }));
+  return mb::launch_status("route");
+}
+
+int mb_route_backward(int dtype, const void* logits, uint64_t logits_bytes, uint32_t tokens, uint32_t experts,
+                      uint64_t row_stride, const int32_t* chosen, uint64_t chosen_bytes, const float* d_weights,
+                      uint64_t d_weights_bytes, uint32_t top, uint32_t scores, uint32_t renormalize, float scale,
+                      void* d_logits, uint64_t d_logits_bytes, void* stream) {
+  const char* entry = "mb_route_backward";
+  if (int rc = mb::check_logits(entry, dtype, logits, logits_bytes, tokens, experts, row_stride, top)) return rc;
+  if (scores > MB_SCORES_SIGMOID) return mb::fail(MB_ERR_INVALID, "%s: unknown scores %u", entry, scores);
+  if (tokens == 0) return MB_OK;
+  if (int rc = mb::check_chosen(entry, chosen, chosen_bytes, d_weights, d_weights_bytes, uint64_t{tokens} * top))
+    return rc;
+  const uint32_t item = mb::elem_bytes(dtype);
+  if (d_logits == nullptr || d_logits_bytes < uint64_t{tokens} * experts * item)
+    return mb::fail(MB_ERR_INVALID, "%s: d_logits are NULL or too small for %u tokens of %u experts", entry, tokens,
+                    experts);
+  if (!mb::aligned(d_logits, item))
+    return mb::fail(MB_ERR_ALIGNMENT, "%s: d_logits must lie on their elements' %u bytes", entry, item);
+  const dim3 grid((tokens + 3) / 4);
+  MB_FOR_DTYPE(dtype, mb::for_experts(experts, [&](auto v) {
+    mb::route_backward_kernel<T, decltype(v)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const T*>(logits), tokens, experts, row_stride, chosen, d_weights, top,
+        scores == MB_SCORES_SOFTMAX, renormalize != 0, scale, static_cast<T*>(d_logits));
+  }));
+  return mb::launch_status("route_backward");
+}
+
+uint64_t mb_dispatch_workspace(uint64_t entries, uint32_t experts) {
+  const uint64_t blocks = mb::dispatch_blocks(entries);
+  return blocks > 1 ? blocks * experts * 4 : 0;
+}
+
+int mb_dispatch(const int32_t* chosen, uint64_t chosen_bytes, uint64_t entries, uint32_t experts, int32_t* offsets,
+                uint64_t offsets_bytes, int32_t* order, uint64_t order_bytes, int32_t* slots, uint64_t slots_bytes,
+                void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* entry = "mb_dispatch";
+  if (experts == 0 || experts > mb::kMostExperts)
+    return mb::fail(MB_ERR_INVALID, "%s: %u experts outside 1..%u", entry, experts, mb::kMostExperts);
+  if (entries > (1u << 24)) return mb::fail(MB_ERR_UNSUPPORTED, "%s: at most %u entries", entry, 1u << 24);
+  if (offsets == nullptr || offsets_bytes < (uint64_t{experts} + 1) * 4)
+    return mb::fail(MB_ERR_INVALID, "%s: offsets are NULL or too small for %u experts", entry, experts);
+  if (entries && (chosen == nullptr || order == nullptr || slots == nullptr || chosen_bytes < entries * 4 ||
+                  order_bytes < entries * 4 || slots_bytes < entries * 4))
+    return mb::fail(MB_ERR_INVALID, "%s: experts, order or slots are NULL or too small for %llu entries", entry,
+                    (unsigned long long)entries);
+  if (!mb::aligned(chosen, 4) || !mb::aligned(offsets, 4) || !mb::aligned(order, 4) || !mb::aligned(slots, 4) ||
+      !mb::aligned(workspace, 4))
+    return mb::fail(MB_ERR_ALIGNMENT, "%s: every buffer must lie on 4 bytes", entry);
+  const uint64_t needed = mb_dispatch_workspace(entries, experts);
+  if (needed && (workspace == nullptr || workspace_bytes < needed))
+    return mb::fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
+                    (unsigned long long)needed);
+  const uint32_t blocks = static_cast<uint32_t>(entries ? mb::dispatch_blocks(entries) : 1);
+  uint32_t bits = 1;
+  while ((1u << bits) < experts) ++bits;
+  const uint32_t lds = mb::kDispatchWaves * experts * 4;
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  uint32_t* counts = blocks > 1 ? static_cast<uint32_t*>(workspace) : nullptr;
+  if (counts) {
+    mb::dispatch_count_kernel<<<dim3(blocks), dim3(1024), lds, on>>>(chosen, static_cast<uint32_t>(entries), experts,
+                                                                    bits, counts);
+    if (int rc = mb::launch_status("dispatch_count")) return rc;
+  }
+  mb::dispatch_place_kernel<<<dim3(blocks), dim3(1024), lds, on>>>(chosen, static_cast<uint32_t>(entries), experts,
+                                                                  bits, counts, offsets, order, slots);
+  return mb::launch_status("dispatch_place");
+}
+
+static int check_combine(const char* entry, int dtype, const void* y, uint64_t y_bytes, uint64_t y_rows,
+                         const int32_t* slots, uint64_t slots_bytes, const float* weights, uint64_t weights_bytes,
+                         uint64_t tokens, uint32_t top, uint64_t n) {
+  const uint32_t item = mb::elem_bytes(dtype);
+  if (!item) return mb::fail(MB_ERR_INVALID, "%s: unknown element type %d", entry, dtype);
+  if (top == 0 || top > mb::kMostTop)
+    return mb::fail(MB_ERR_INVALID, "%s: %u slots a token outside 1..%u", entry, top, mb::kMostTop);
+  if (tokens > (1u << 24) || y_rows > (1u << 24) || n > (1u << 20) || tokens * ((n + 511) / 512) > (1u << 25))
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: %llu tokens of %llu columns exceed one launch", entry,
+                    (unsigned long long)tokens, (unsigned long long)n);
+  if (tokens * n == 0) return MB_OK;
+  if (y_bytes < y_rows * n * item || (y == nullptr && y_rows))
+    return mb::fail(MB_ERR_INVALID, "%s: y is NULL or too small for %llu x %llu", entry, (unsigned long long)y_rows,
+                    (unsigned long long)n);
+  if (!mb::aligned(y, item)) return mb::fail(MB_ERR_ALIGNMENT, "%s: y must lie on its elements' %u bytes", entry, item);
+  if (slots == nullptr || weights == nullptr || slots_bytes < tokens * top * 4 || weights_bytes < tokens * top * 4)
+    return mb::fail(MB_ERR_INVALID, "%s: slots or weights are NULL or too small for %llu x %u", entry,
+                    (unsigned long long)tokens, top);
+  if (!mb::aligned(slots, 4) || !mb::aligned(weights, 4))
+    return mb::fail(MB_ERR_ALIGNMENT, "%s: slots and weights must lie on 4 bytes", entry);
+  return MB_OK;
+}
+
+static int check_rows_out(const char* entry, const char* what, const void* p, uint64_t bytes, uint64_t rows,
+                          uint64_t n, uint32_t item) {
+  if (rows * n && (p == nullptr || bytes < rows * n * item))
+    return mb::fail(MB_ERR_INVALID, "%s: %s is NULL or too small for %llu x %llu", entry, what,
+                    (unsigned long long)rows, (unsigned long long)n);
+  if (!mb::aligned(p, item))
+    return mb::fail(MB_ERR_ALIGNMENT, "%s: %s must lie on its elements' %u bytes", entry, what, item);
+  return MB_OK;
+}
+
+int mb_combine(int dtype, const void* y, uint64_t y_bytes, uint32_t y_rows, const int32_t* slots,
+               uint64_t slots_bytes, const float* weights, uint64_t weights_bytes, void* out, uint64_t out_bytes,
+               uint32_t tokens, uint32_t top, uint32_t n, void* stream) {
+  const char* entry = "mb_combine";
+  if (int rc = check_combine(entry, dtype, y, y_bytes, y_rows, slots, slots_bytes, weights, weights_bytes, tokens, top,
+                             n))
+    return rc;
+  if (tokens == 0 || n == 0) return MB_OK;
+  if (int rc = check_rows_out(entry, "out", out, out_bytes, tokens, n, mb::elem_bytes(dtype))) return rc;
+  const uint64_t tasks = uint64_t{tokens} * ((n + 511) / 512);
+  MB_FOR_DTYPE(dtype, (mb::combine_kernel<T><<<dim3(static_cast<uint32_t>((tasks + 3) / 4)), dim3(256), 0,
+                                               static_cast<hipStream_t>(stream)>>>(
+                          static_cast<const T*>(y), y_rows, slots, weights, static_cast<T*>(out), tokens, top, n)));
+  return mb::launch_status("combine");
+}
+
+int mb_combine_backward(int dtype, const void* d_out, uint64_t d_out_bytes, const void* y, uint64_t y_bytes,
+                        uint32_t y_rows, const int32_t* slots, uint64_t slots_bytes, const float* weights,
+                        uint64_t weights_bytes, void* d_y, uint64_t d_y_bytes, float* d_weights,
+                        uint64_t d_weights_bytes, uint32_t tokens, uint32_t top, uint32_t n, void* stream) {
+  const char* entry = "mb_combine_backward";
+  if (int rc = check_combine(entry, dtype, y, y_bytes, y_rows, slots, slots_bytes, weights, weights_bytes, tokens, top,
+                             n))
+    return rc;
+  const uint32_t item = mb::elem_bytes(dtype);
+  const uint64_t tasks = uint64_t{tokens} * top;
+  if (tasks > (1u << 24)) return mb::fail(MB_ERR_UNSUPPORTED, "%s: at most %u entries", entry, 1u << 24);
+  if (tokens == 0) return MB_OK;
+  if (int rc = check_rows_out(entry, "d_out", d_out, d_out_bytes, tokens, n, item)) return rc;
+  if (int rc = check_rows_out(entry, "d_y", d_y, d_y_bytes, y_rows, n, item)) return rc;
+  if (int rc = check_rows_out(entry, "d_weights", d_weights, d_weights_bytes, tokens, top, 4)) return rc;
+  MB_FOR_DTYPE(dtype, (mb::combine_backward_kernel<T><<<dim3(static_cast<uint32_t>((tasks + 3) / 4)), dim3(256), 0,
+                                                        static_cast<hipStream_t>(stream)>>>(
+                          static_cast<const T*>(d_out), static_cast<const T*>(y), y_rows, slots, weights,
+                          static_cast<T*>(d_y), d_weights, tokens, top, n)));
+  return mb::launch_status("combine_backward");
+}
+
+}  // extern "C"

@@ -1,0 +1,157 @@
+"""Routing of tokens to experts, and back.
+
+`route` chooses each token's experts and their weights from its logits,
+`dispatch` sorts the choices by expert (the `Plan` that mx.linear takes), and
+`combine` sums the experts' outputs into the tokens'. `route_backward` and
+`combine_backward` are the gradients. Every call launches on the current
+stream, allocates only the outputs that it is not given, and raises ValueError
+for tensors that do not fit it.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+from . import _native
+from .mx import bytes_of, check_device, check_output, dtype_code, strided_rows
+
+SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+class Plan(NamedTuple):
+    """Choices sorted by expert (int32): expert e's are order[offsets[e] .. offsets[e + 1] - 1], each the number of an
+    entry of the [tokens][top] choices; slots [tokens][top] is an entry's place in order. -1 where an entry has no
+    expert, and in order past the last entry that has one."""
+
+    offsets: object
+    order: object
+    slots: object
+    workspace: object = None
+
+
+def _torch():
+    import torch
+
+    return torch
+
+
+def _score_code(scores: str) -> int:
+    if scores not in SCORES:
+        raise ValueError(f"scores must be one of {', '.join(SCORES)}, not {scores!r}")
+    return SCORES[scores]
+
+
+def route(logits, top: int, bias=None, scores: str = "softmax", groups: int = 1, top_groups: int = 1,
+          renormalize: bool = True, scale: float = 1.0, experts=None, weights=None, stream=None):
+    """(experts, weights), int32 and float32 [tokens][top], of logits [tokens][experts].
+
+    s = softmax or sigmoid of the logits; c = s + bias decides: of `groups` equal groups the `top_groups` with the
+    largest sum of their two largest c stay, then the `top` largest c, in falling order and of equal ones the lower
+    index. A logit of -inf masks its expert; -1, with weight 0, stands where none is left. The weights are s, divided
+    by their sum if `renormalize`, times `scale`.
+    """
+    torch = _torch()
+    code = dtype_code(logits, "logits")
+    stride, span = strided_rows(logits, "logits")
+    tokens, count = logits.shape
+    experts = check_output(experts, "experts", (tokens, top), torch.int32, logits.device)
+    weights = check_output(weights, "weights", (tokens, top), torch.float32, logits.device)
+    if bias is not None:
+        bias = check_output(bias, "bias", (count,), torch.float32, logits.device)
+        check_device(bias)
+    check_device(logits, experts, weights)
+    _native.call("mb_route", code, logits.data_ptr(), span, tokens, count, stride,
+                 None if bias is None else bias.data_ptr(), 0 if bias is None else bytes_of(bias), top,
+                 _score_code(scores), groups, top_groups, int(renormalize), scale, experts.data_ptr(),
+                 bytes_of(experts), weights.data_ptr(), bytes_of(weights), _native.stream_handle(stream))
+    return experts, weights
+
+
+def route_backward(logits, experts, d_weights, scores: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+                   d_logits=None, stream=None):
+    """d_logits, in the logits' type, for the gradient d_weights of route's weights and the experts it chose."""
+    torch = _torch()
+    code = dtype_code(logits, "logits")
+    stride, span = strided_rows(logits, "logits")
+    tokens, count = logits.shape
+    if experts.dim() != 2 or experts.shape[0] != tokens:
+        raise ValueError(f"experts must be [{tokens}][top], not {tuple(experts.shape)}")
+    top = experts.shape[1]
+    check_output(experts, "experts", (tokens, top), torch.int32, logits.device)
+    check_output(d_weights, "d_weights", (tokens, top), torch.float32, logits.device)
+    d_logits = check_output(d_logits, "d_logits", (tokens, count), logits.dtype, logits.device)
+    check_device(logits, experts, d_weights, d_logits)
+    _native.call("mb_route_backward", code, logits.data_ptr(), span, tokens, count, stride, experts.data_ptr(),
+                 bytes_of(experts), d_weights.data_ptr(), bytes_of(d_weights), top, _score_code(scores),
+                 int(renormalize), scale, d_logits.data_ptr(), bytes_of(d_logits), _native.stream_handle(stream))
+    return d_logits
+
+
+def empty_plan(tokens: int, top: int, experts: int, device="cuda") -> Plan:
+    """A plan's buffers and workspace, for `dispatch` to fill."""
+    torch = _torch()
+    needed = _native.load().mb_dispatch_workspace(tokens * top, experts)
+    return Plan(torch.empty(experts + 1, dtype=torch.int32, device=device),
+                torch.empty(tokens * top, dtype=torch.int32, device=device),
+                torch.empty((tokens, top), dtype=torch.int32, device=device),
+                torch.empty(needed, dtype=torch.uint8, device=device))
+
+
+def dispatch(experts, count: int, plan: Plan | None = None, stream=None) -> Plan:
+    """The plan of the choices `experts` [tokens][top] (int32; outside 0 .. count - 1: none) of `count` experts."""
+    torch = _torch()
+    if experts.dim() != 2:
+        raise ValueError(f"experts must be [tokens][top], not {tuple(experts.shape)}")
+    tokens, top = experts.shape
+    check_output(experts, "experts", (tokens, top), torch.int32, experts.device)
+    if plan is None:
+        plan = empty_plan(tokens, top, count, experts.device)
+    check_output(plan.offsets, "plan.offsets", (count + 1,), torch.int32, experts.device)
+    check_output(plan.order, "plan.order", (tokens * top,), torch.int32, experts.device)
+    check_output(plan.slots, "plan.slots", (tokens, top), torch.int32, experts.device)
+    workspace = plan.workspace
+    check_device(experts, plan.offsets, plan.order, plan.slots, *(() if workspace is None else (workspace,)))
+    _native.call("mb_dispatch", experts.data_ptr(), bytes_of(experts), tokens * top, count, plan.offsets.data_ptr(),
+                 bytes_of(plan.offsets), plan.order.data_ptr(), bytes_of(plan.order), plan.slots.data_ptr(),
+                 bytes_of(plan.slots), None if workspace is None else workspace.data_ptr(),
+                 0 if workspace is None else bytes_of(workspace), _native.stream_handle(stream))
+    return plan
+
+
+def _combine_sizes(y, slots, weights):
+    torch = _torch()
+    if y.dim() != 2 or slots.dim() != 2:
+        raise ValueError(f"y must be [rows][n] and slots [tokens][top], not {tuple(y.shape)} and {tuple(slots.shape)}")
+    check_output(y, "y", y.shape, y.dtype, y.device)
+    check_output(slots, "slots", slots.shape, torch.int32, y.device)
+    check_output(weights, "weights", slots.shape, torch.float32, y.device)
+    check_device(y, slots, weights)
+    return dtype_code(y, "y"), *y.shape, *slots.shape
+
+
+def combine(y, slots, weights, out=None, stream=None):
+    """out[t] = the sum over j of weights[t][j] * y[slots[t][j]], in y's type; slots of -1 are left out."""
+    code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
+    out = check_output(out, "out", (tokens, n), y.dtype, y.device)
+    check_device(out)
+    _native.call("mb_combine", code, y.data_ptr(), bytes_of(y), rows, slots.data_ptr(), bytes_of(slots),
+                 weights.data_ptr(), bytes_of(weights), out.data_ptr(), bytes_of(out), tokens, top, n,
+                 _native.stream_handle(stream))
+    return out
+
+
+def combine_backward(d_out, y, slots, weights, d_y=None, d_weights=None, stream=None):
+    """(d_y, d_weights) of combine for the gradient d_out; rows of a given d_y that no slot names stay as they are."""
+    torch = _torch()
+    code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
+    check_output(d_out, "d_out", (tokens, n), y.dtype, y.device)
+    if d_y is None:
+        d_y = torch.zeros_like(y)
+    check_output(d_y, "d_y", (rows, n), y.dtype, y.device)
+    d_weights = check_output(d_weights, "d_weights", (tokens, top), torch.float32, y.device)
+    check_device(d_out, d_y, d_weights)
+    _native.call("mb_combine_backward", code, d_out.data_ptr(), bytes_of(d_out), y.data_ptr(), bytes_of(y), rows,
+                 slots.data_ptr(), bytes_of(slots), weights.data_ptr(), bytes_of(weights), d_y.data_ptr(),
+                 bytes_of(d_y), d_weights.data_ptr(), bytes_of(d_weights), tokens, top, n,
+                 _native.stream_handle(stream))
+    return d_y, d_weights
