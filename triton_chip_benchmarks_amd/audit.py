@@ -40,6 +40,7 @@ _ELEMENT_TYPE = {"f": "f32", "DF16_": "f16", "DF16b": "bf16"}
 _ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)E")
 _LAYER_RE = re.compile(r"(mx_quantize|mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
                        r"_kernelI(f|DF16_|DF16b)E")
+_PRODUCT_RING_RE = re.compile(r"mx_product_ring_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi(\d+)EE")
 _DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
 _VECTOR_RE = re.compile(r"vector_(\w+?)_kernelILi(\d+)E")
 _READ_TYPE = {"f": "f32", "DF16_": "f16", "t": "bf16"}
@@ -94,6 +95,11 @@ def registered_name(symbol: str) -> str | None:
     match = _LAYER_RE.search(symbol)
     if match:
         return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}"
+    match = _PRODUCT_RING_RE.search(symbol)
+    if match:
+        dtype, features, rows, stages = match.groups()
+        pair = "_pair" if (features, stages) == ("128", "2") else ""
+        return f"mx_product_{_ELEMENT_TYPE[dtype]}_{features}x{rows}{pair}"
     match = _DISPATCH_RE.search(symbol)
     if match:
         return match.group(1)

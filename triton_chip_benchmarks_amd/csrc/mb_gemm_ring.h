@@ -96,30 +96,23 @@ struct RingTile {
 // step and vmcnt counts them; stores past the edge are dropped the same way.
 // MXFP4 scale bytes past K are masked to 0 (2^-127) in registers: whatever the
 // caller's padding holds, NaN included, never meets the zeroed operands.
+//
+// The tile at row m0 of A (M rows) and n0 of B (N rows), M and N the rows that
+// the scales are laid out for; `rows_a` and `rows_b` rows of A and B from there
+// on are taken. On return no DMA is in flight.
 template <class Op, int BM, int BN, int STAGES>
-__global__ void __launch_bounds__(256)
-    gemm_ring_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, const uint8_t* __restrict__ SA,
-                     const uint8_t* __restrict__ SB, typename Op::Out* __restrict__ C, int M, int N, int K,
-                     int group_m) {
+__device__ __forceinline__ void ring_accumulate(
+    uint8_t* lds, const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, const uint8_t* __restrict__ SA,
+    const uint8_t* __restrict__ SB, int M, int N, int K, int m0, int n0, int rows_a, int rows_b, int lane,
+    int wave, typename Op::Acc (&acc)[RingTile<Op, BM, BN, STAGES>::FM][RingTile<Op, BM, BN, STAGES>::FN]) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using T = RingTile<Op, BM, BN, STAGES>;
   constexpr int ROWB = T::ROWB, FM = T::FM, FN = T::FN, CH = T::CHUNKS;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * T::STAGE];
-  if (K < 0) lds[threadIdx.x] = 0;  // keeps DMA-written reads live; never executed
-
-  int tile_m, tile_n;
-  band_tile_any((static_cast<uint32_t>(M) + BM - 1) / BM, (static_cast<uint32_t>(N) + BN - 1) / BN, group_m, tile_m,
-                tile_n);
-  const int m0 = tile_m * BM, n0 = tile_n * BN;
   const int row_bytes = K * Op::ELEM_BITS / 8;
   const int k_steps = (row_bytes + ROWB - 1) / ROWB;
 
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const __amdgpu_buffer_rsrc_t ra =
-      buffer_rsrc(A + static_cast<int64_t>(m0) * row_bytes, min(BM, M - m0) * row_bytes);
-  const __amdgpu_buffer_rsrc_t rb =
-      buffer_rsrc(B + static_cast<int64_t>(n0) * row_bytes, min(BN, N - n0) * row_bytes);
+  const __amdgpu_buffer_rsrc_t ra = buffer_rsrc(A + static_cast<int64_t>(m0) * row_bytes, rows_a * row_bytes);
+  const __amdgpu_buffer_rsrc_t rb = buffer_rsrc(B + static_cast<int64_t>(n0) * row_bytes, rows_b * row_bytes);
   // Lane l of a DMA fills row l/8, physical chunk l%8, from the logical chunk
   // stored there; rows 8 apart alternate between two swizzles. A chunk lies
   // inside its row in step kt while kt * 128 < its limit.
@@ -200,7 +193,6 @@ __global__ void __launch_bounds__(256)
     for (int f = 0; f < FN; ++f) set.sb[f] = scale(T::SCALES_A / 8 + wn * T::WN + f * Op::M + lrow);
   };
 
-  typename Op::Acc acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -275,6 +267,30 @@ __global__ void __launch_bounds__(256)
   if (kt < k_steps) step(kt, set0, set1);
   if constexpr (Op::LANE_BYTES == 8) fence();
   __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // no DMA of a step past the last may land in a later workgroup's LDS
+#endif
+}
+
+template <class Op, int BM, int BN, int STAGES>
+__global__ void __launch_bounds__(256)
+    gemm_ring_kernel(const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, const uint8_t* __restrict__ SA,
+                     const uint8_t* __restrict__ SB, typename Op::Out* __restrict__ C, int M, int N, int K,
+                     int group_m) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using T = RingTile<Op, BM, BN, STAGES>;
+  constexpr int FM = T::FM, FN = T::FN;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * T::STAGE];
+  if (K < 0) lds[threadIdx.x] = 0;  // keeps DMA-written reads live; never executed
+
+  int tile_m, tile_n;
+  band_tile_any((static_cast<uint32_t>(M) + BM - 1) / BM, (static_cast<uint32_t>(N) + BN - 1) / BN, group_m, tile_m,
+                tile_n);
+  const int m0 = tile_m * BM, n0 = tile_n * BN;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typename Op::Acc acc[FM][FN];
+  ring_accumulate<Op, BM, BN, STAGES>(lds, A, B, SA, SB, M, N, K, m0, n0, min(BM, M - m0), min(BN, N - n0), lane, wave,
+                                      acc);
+  const int wm = wave & 1, wn = wave >> 1;
 
   // Rows past M lie past num_records; columns past N get an out-of-range offset.
   constexpr int ES = sizeof(typename Op::Out);

@@ -1,7 +1,10 @@
 // Products of MXFP4 operands for linear layers: Y = X . W^T, each row of X with
 // the weight of its expert where there are several.
+#include <type_traits>
+
 #include "mb_elem.h"
-#include "mb_mfma.h"
+#include "mb_gemm_host.h"
+#include "mb_gemm_ring.h"
 #include "mb_mx.h"
 
 namespace mb {
@@ -63,7 +66,173 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-#define MB_PRODUCT_REGISTER(T, NAME) MB_REGISTER_KERNEL("mx_product_" NAME, mx_product_kernel<T>)
+// ---- tiles through the ring GEMM -----------------------------------------------
+
+// Expert and first row of row tile `tile` (BN rows each, an expert's rows
+// starting a tile of their own), for the whole wave.
+struct ExpertTile {
+  int expert, first, last;
+};
+
+template <int BN>
+__device__ __forceinline__ int expert_tile_count(const int32_t* __restrict__ offsets, int e, int experts, int rows) {
+  if (e >= experts) return 0;
+  int first, last;
+  expert_rows(offsets, e, rows, first, last);
+  return (last - first + BN - 1) / BN;
+}
+
+template <int BN>
+__device__ __forceinline__ int count_row_tiles(const int32_t* __restrict__ offsets, int experts, int rows, int lane) {
+  if (offsets == nullptr) return (rows + BN - 1) / BN;
+  int total = 0;
+  for (int e = lane; e < experts; e += 64) total += expert_tile_count<BN>(offsets, e, experts, rows);
+#pragma unroll
+  for (int offset = 32; offset > 0; offset >>= 1) total += __shfl_xor(total, offset, 64);
+  return __builtin_amdgcn_readfirstlane(total);
+}
+
+template <int BN>
+__device__ __forceinline__ ExpertTile find_row_tile(const int32_t* __restrict__ offsets, int experts, int rows,
+                                                    int tile, int lane) {
+  if (offsets == nullptr) return {0, tile * BN, rows};
+  int before = 0;  // tiles of the experts below `base`
+  for (int base = 0; base < experts; base += 64) {
+    const int mine = expert_tile_count<BN>(offsets, base + lane, experts, rows);
+    int scan = mine;
+#pragma unroll
+    for (int offset = 1; offset < 64; offset <<= 1) {
+      const int v = __shfl_up(scan, offset, 64);
+      if (lane >= offset) scan += v;
+    }
+    const uint64_t past = __ballot(before + scan > tile);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      const int start = before + __builtin_amdgcn_readlane(scan - mine, at);
+      const int e = base + at;
+      int first, last;
+      expert_rows(offsets, e, rows, first, last);
+      return {e, first + (tile - start) * BN, last};
+    }
+    before += __builtin_amdgcn_readlane(scan, 63);
+  }
+  return {0, rows, rows};  // no such tile
+}
+
+// BM columns (features) of BN rows of one expert by gemm_ring_kernel's loop, W as
+// its A and X as its B: a lane then holds four neighbouring features of a row.
+// The tile leaves through LDS, so that rows are stored in whole 16-byte pieces.
+template <class T, int BM, int BN, int STAGES>
+__global__ void __launch_bounds__(256)
+    mx_product_ring_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ sx,
+                           const uint8_t* __restrict__ w, const uint8_t* __restrict__ sw, T* __restrict__ y, int rows,
+                           int n, int k, const int32_t* __restrict__ offsets, int experts, int band) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using Op = MfmaMxfp4;
+  using Tile = RingTile<Op, BM, BN, STAGES>;
+  constexpr int FM = Tile::FM, FN = Tile::FN;
+  constexpr int LDS_ROW = BM * sizeof(T) + 16;  // padded: neighbouring rows start in other banks
+  static_assert(BN * LDS_ROW <= STAGES * Tile::STAGE, "the output tile fits the ring's LDS");
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * Tile::STAGE];
+  if (k < 0) lds[threadIdx.x] = 0;  // keeps DMA-written reads live; never executed
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // The grid bounds the number of tiles, which the experts' row counts decide.
+  // XCD x (ids x, x + 8, ..) takes a contiguous share of the real ones.
+  const int row_tiles = count_row_tiles<BN>(offsets, experts, rows, lane);
+  const int columns = (n + BM - 1) / BM;
+  if (static_cast<int64_t>(row_tiles) * columns > gridDim.x) return;  // offsets that do not rise: nothing to rely on
+  const int count = row_tiles * columns, xcd = blockIdx.x % kXcds, index = blockIdx.x / kXcds;
+  if (index >= count / kXcds + (xcd < count % kXcds)) return;
+  const int pid = xcd * (count / kXcds) + min(xcd, count % kXcds) + index;
+  const int per_band = band * columns, first_tile = pid / per_band * band;
+  const int in_band = min(row_tiles - first_tile, band);
+  const int row_tile = first_tile + pid % per_band % in_band;
+  const int m0 = pid % per_band / in_band * BM;
+  const ExpertTile at = find_row_tile<BN>(offsets, experts, rows, row_tile, lane);
+  const int n0 = at.first, live = min(BN, at.last - at.first);
+  const int64_t e = at.expert;
+  const int steps = (k + 255) / 256;
+
+  typename Op::Acc acc[FM][FN];
+  ring_accumulate<Op, BM, BN, STAGES>(lds, w + e * n * (k / 2), x, sw + e * steps * n * 8, sx, n, rows, k, m0, n0,
+                                      min(BM, n - m0), live, lane, wave, acc);
+  lds_barrier();  // every wave's reads of the ring have ended
+  const int wm = wave & 1, wn = wave >> 1;
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        T out[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) out[r] = static_cast<T>(acc[i][j][4 * q + r]);
+        const int row = wn * Tile::WN + j * 32 + (lane & 31);
+        const int column = wm * Tile::WM + i * 32 + Op::out_row(lane, 4 * q);
+        __builtin_memcpy(__builtin_assume_aligned(lds + row * LDS_ROW + column * sizeof(T), 4 * sizeof(T)), out,
+                         sizeof(out));
+      }
+  lds_barrier();
+  constexpr int PIECE = 16 / sizeof(T), PIECES = BM / PIECE;  // a row's 16-byte pieces
+  T* tile_y = y + static_cast<int64_t>(n0) * n + m0;
+#pragma unroll 4
+  for (int piece = threadIdx.x; piece < BN * PIECES; piece += 256) {
+    const int row = piece / PIECES, column = piece % PIECES * PIECE;
+    if (row >= live || m0 + column >= n) continue;
+    const elem_u32x4 value = *reinterpret_cast<const elem_u32x4*>(lds + row * LDS_ROW + column * sizeof(T));
+    T* to = tile_y + static_cast<int64_t>(row) * n + column;
+    if (m0 + column + PIECE <= n) {
+      *reinterpret_cast<elem_u32x4_any*>(to) = value;
+    } else {
+      T part[PIECE];
+      __builtin_memcpy(part, &value, 16);
+#pragma unroll
+      for (int i = 0; i < PIECE; ++i)
+        if (m0 + column + i < n) to[i] = part[i];
+    }
+  }
+#endif
+}
+
+using ProductLauncher = void (*)(const uint8_t*, const uint8_t*, const uint8_t*, const uint8_t*, void*, int, int, int,
+                                 const int32_t*, int, uint32_t, int, hipStream_t);
+
+template <class T, int BM, int BN, int STAGES>
+void launch_ring(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const uint8_t* sw, void* y, int rows, int n,
+                 int k, const int32_t* offsets, int experts, uint32_t grid, int band, hipStream_t stream) {
+  mx_product_ring_kernel<T, BM, BN, STAGES><<<dim3(grid), dim3(256), 0, stream>>>(
+      x, sx, w, sw, static_cast<T*>(y), rows, n, k, offsets, experts, band);
+}
+
+// A ring tile: BM features of BN rows.
+struct ProductKernel {
+  int features, rows;
+  int band;      // row tiles that share their weight's panels in an XCD's L2
+  int resident;  // workgroups a CU holds
+  GemmCost cost;
+  ProductLauncher launch[3];  // by MB_DTYPE_*
+};
+#define MB_PRODUCT(BM, BN, STAGES, BAND, COST)                                                               \
+  ProductKernel {                                                                                            \
+    BM, BN, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, COST, {                                     \
+      launch_ring<float, BM, BN, STAGES>, launch_ring<_Float16, BM, BN, STAGES>, launch_ring<__bf16, BM, BN, STAGES> \
+    }                                                                                                        \
+  }
+const ProductKernel kProductKernels[] = {
+    MB_PRODUCT(256, 128, 3, 4, kCostMx256x128),
+    MB_PRODUCT(128, 128, 4, 6, kCostMx128),
+    MB_PRODUCT(128, 128, 2, 8, kCostMx128Pair),
+    MB_PRODUCT(64, 64, 3, 8, kCostMx64),
+};
+
+#define MB_PRODUCT_REGISTER(T, NAME)                                                                        \
+  MB_REGISTER_KERNEL("mx_product_" NAME, mx_product_kernel<T>);                                             \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_256x128", (mx_product_ring_kernel<T, 256, 128, 3>));              \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_128x128", (mx_product_ring_kernel<T, 128, 128, 4>));              \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_128x128_pair", (mx_product_ring_kernel<T, 128, 128, 2>));         \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_64x64", (mx_product_ring_kernel<T, 64, 64, 3>))
 MB_PRODUCT_REGISTER(float, "f32");
 MB_PRODUCT_REGISTER(_Float16, "f16");
 MB_PRODUCT_REGISTER(__bf16, "bf16");
@@ -99,14 +268,59 @@ int check_offsets(const char* entry, const int32_t* offsets, uint64_t offsets_by
   return MB_OK;
 }
 
-int launch_product(int dtype, const void* x, const void* sx, const void* w, const void* sw, void* y, uint32_t rows,
-                   uint32_t n, uint32_t k, const int32_t* offsets, uint32_t experts, hipStream_t stream) {
+// Row tiles of `tile` rows: at most, and as many as experts of even numbers of
+// rows have (a last one half empty on average).
+uint64_t most_row_tiles(uint32_t rows, uint32_t experts, int tile) {
+  return experts > 1 ? rows / tile + (rows < experts ? rows : experts) : (rows + uint64_t{1} * tile - 1) / tile;
+}
+
+double mean_row_tiles(uint32_t rows, uint32_t experts, int tile) {
+  if (experts == 1) return static_cast<double>(most_row_tiles(rows, 1, tile));
+  const double each = static_cast<double>(rows) / experts;
+  return experts * (each >= tile ? each / tile + 0.5 : each >= 1 ? 1.0 : each);
+}
+
+// Estimated microseconds of a launch (see GemmCost).
+double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint32_t steps, uint32_t experts) {
+  const double tiles = mean_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
+  const double round = 256.0 * kernel.resident, whole = static_cast<double>(static_cast<uint64_t>(tiles / round));
+  const double rest = tiles / round - whole;
+  auto one = [&](double filled) {
+    return kernel.cost.tile + steps * (kernel.cost.step_empty + (kernel.cost.step_full - kernel.cost.step_empty) * filled);
+  };
+  return whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
+}
+
+int launch_product(int dtype, const void* x_codes, const void* sx, const void* w_codes, const void* sw, void* y,
+                   uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, uint32_t experts,
+                   hipStream_t stream) {
+  const uint8_t *x = static_cast<const uint8_t*>(x_codes), *w = static_cast<const uint8_t*>(w_codes);
+  const uint8_t *sxb = static_cast<const uint8_t*>(sx), *swb = static_cast<const uint8_t*>(sw);
+  const uint32_t padded = (k + 31) / 32 * 32, steps = (k + 255) / 256;
+  // The ring addresses a matrix's scales, and a tile's rows, with 32-bit offsets.
+  const uint64_t scale_rows = rows > n ? rows : n;
+  if (steps * scale_rows * 8 <= 0x7fffffffu) {
+    const ProductKernel* best = nullptr;
+    double best_cost = 0;
+    for (const ProductKernel& kernel : kProductKernels) {
+      const uint64_t grid = most_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
+      if (grid > 0xffffff) continue;
+      const double cost = product_cost(kernel, rows, n, steps, experts);
+      if (best == nullptr || cost < best_cost) best = &kernel, best_cost = cost;
+    }
+    if (best) {
+      const uint64_t grid = most_row_tiles(rows, experts, best->rows) * ((n + best->features - 1) / best->features);
+      best->launch[dtype](x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
+                          offsets, static_cast<int>(experts), static_cast<uint32_t>((grid + 7) / 8 * 8), best->band,
+                          stream);
+      return launch_status("mx_product_ring");
+    }
+  }
   const uint32_t tiles = (rows / experts + 15) / 16;
   const dim3 grid((n + 63) / 64, experts, tiles < 1 ? 1 : tiles < 256 ? tiles : 256);
   MB_FOR_DTYPE(dtype, (mx_product_kernel<T><<<grid, dim3(256), 0, stream>>>(
-                          static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(sx),
-                          static_cast<const uint8_t*>(w), static_cast<const uint8_t*>(sw), static_cast<T*>(y),
-                          static_cast<int>(rows), static_cast<int>(n), static_cast<int>(k), offsets)));
+                          x, sxb, w, swb, static_cast<T*>(y), static_cast<int>(rows), static_cast<int>(n),
+                          static_cast<int>(k), offsets)));
   return launch_status("mx_product");
 }
 
