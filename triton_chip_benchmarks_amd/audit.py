@@ -41,6 +41,7 @@ _ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)E")
 _LAYER_RE = re.compile(r"(mx_quantize|mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
                        r"_kernelI(f|DF16_|DF16b)E")
 _PRODUCT_RING_RE = re.compile(r"mx_product_ring_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi(\d+)EE")
+_FEW_RE = re.compile(r"mx_few_kernelI(h|f|DF16_|DF16b)(S\d*_|T_|f|DF16_|DF16b)?Li(\d+)ELi(\d+)EE")
 _DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
 _VECTOR_RE = re.compile(r"vector_(\w+?)_kernelILi(\d+)E")
 _READ_TYPE = {"f": "f32", "DF16_": "f16", "t": "bf16"}
@@ -100,6 +101,11 @@ def registered_name(symbol: str) -> str | None:
         dtype, features, rows, stages = match.groups()
         pair = "_pair" if (features, stages) == ("128", "2") else ""
         return f"mx_product_{_ELEMENT_TYPE[dtype]}_{features}x{rows}{pair}"
+    match = _FEW_RE.search(symbol)
+    if match:
+        x, y, blocks, split = match.groups()
+        family = "product" if x == "h" else "linear"
+        return f"mx_{family}_few_{_ELEMENT_TYPE[y if x == 'h' else x]}_{16 * int(blocks)}x{split}"
     match = _DISPATCH_RE.search(symbol)
     if match:
         return match.group(1)

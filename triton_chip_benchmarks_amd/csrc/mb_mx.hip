@@ -10,8 +10,8 @@
 //
 // Codes are [rows][ceil(k / 32) * 16] bytes, even k in the low nibble, zero past
 // k; scales [ceil(k / 256)][rows][8], 127 for groups past k: mb_gemm's operands.
-#include "mb_elem.h"
 #include "mb_mx.h"
+#include "mb_mx_device.h"
 
 namespace mb {
 namespace {
@@ -20,32 +20,6 @@ constexpr uint32_t kGroup = 32;   // elements sharing a scale
 constexpr uint32_t kBlock = 256;  // elements along K whose 8 scales a row holds together
 
 __device__ __forceinline__ float bits_float(uint32_t v) { return __builtin_bit_cast(float, v); }
-
-// Scale byte of a group whose largest magnitude has these fp32 bits.
-__device__ __forceinline__ uint32_t scale_byte(uint32_t largest) {
-  const int field = static_cast<int>(largest >> 23);
-  return field == 255 ? 255u : static_cast<uint32_t>(field > 2 ? field - 2 : 0);
-}
-
-// Two E2M1 codes in byte SEL of `word`.
-template <int SEL>
-__device__ __forceinline__ uint32_t encode_pair(uint32_t word, float a, float b, uint32_t scale) {
-  const int up = 127 - static_cast<int>(scale);
-  const float x = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(a, up), -6.0f, 6.0f);
-  const float y = __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(b, up), -6.0f, 6.0f);
-  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x, y, 1.0f, SEL);
-}
-
-__device__ __forceinline__ uint32_t encode8(const float (&v)[8], uint32_t scale) {
-  uint32_t word = 0;
-  word = encode_pair<0>(word, v[0], v[1], scale);
-  word = encode_pair<1>(word, v[2], v[3], scale);
-  word = encode_pair<2>(word, v[4], v[5], scale);
-  word = encode_pair<3>(word, v[6], v[7], scale);
-  return scale == 255 ? 0 : word;
-}
-
-__device__ __forceinline__ uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
 constexpr int kRowsPerWorkgroup = 32;
 
@@ -77,17 +51,11 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t row = row0 + 8 * u;
-    float v[8];
-    uint32_t largest = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = raw[u][i];
-      largest = max(largest, magnitude(v[i]));
-    }
-    largest = max(largest, quad_swap<kQuadXor1>(largest));
-    largest = max(largest, quad_swap<kQuadXor2>(largest));
-    const uint32_t scale = scale_byte(largest);
-    const uint32_t word = encode8(v, scale);
+    uint32_t largest = raw_magnitude(raw[u]);
+    largest = join_magnitudes(T(), largest, quad_swap<kQuadXor1>(largest));
+    largest = join_magnitudes(T(), largest, quad_swap<kQuadXor2>(largest));
+    const uint32_t scale = scale_byte(magnitude_bits<T>(largest));
+    const uint32_t word = encode8(raw[u], scale);
     if (row >= rows) continue;
     for (uint32_t c = 0; c < copies; ++c) {
       const uint32_t out = slots ? static_cast<uint32_t>(slots[static_cast<uint64_t>(row) * copies + c]) : row;
@@ -119,23 +87,24 @@ __global__ void __launch_bounds__(256)
     *scale_at = 127;
     return;
   }
-  float v[32];
-  uint32_t largest = 0;
-#pragma unroll
-  for (uint32_t i = 0; i < 32; ++i) {
-    const uint32_t row = group * kGroup + i;
-    v[i] = row < rows ? widen(x[row * row_stride + column]) : 0.0f;
-    largest = max(largest, magnitude(v[i]));
-  }
-  const uint32_t scale = scale_byte(largest);
-  elem_u32x4 word;
+  Raw8<T> raw[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    float part[8];
+    T v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) part[i] = v[8 * q + i];
-    word[q] = encode8(part, scale);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t row = group * kGroup + 8 * q + i;
+      v[i] = row < rows ? x[row * row_stride + column] : T(0);
+    }
+    __builtin_memcpy(raw[q].part, v, sizeof(v));
   }
+  uint32_t largest = raw_magnitude(raw[0]);
+#pragma unroll
+  for (int q = 1; q < 4; ++q) largest = join_magnitudes(T(), largest, raw_magnitude(raw[q]));
+  const uint32_t scale = scale_byte(magnitude_bits<T>(largest));
+  elem_u32x4 word;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) word[q] = encode8(raw[q], scale);
   *reinterpret_cast<elem_u32x4*>(codes + (static_cast<uint64_t>(column) * groups + group) * 16) = word;
   *scale_at = static_cast<uint8_t>(scale);
 }

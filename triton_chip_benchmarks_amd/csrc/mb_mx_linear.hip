@@ -6,6 +6,7 @@
 #include "mb_gemm_host.h"
 #include "mb_gemm_ring.h"
 #include "mb_mx.h"
+#include "mb_mx_device.h"
 
 namespace mb {
 namespace {
@@ -62,6 +63,173 @@ __global__ void __launch_bounds__(256)
         const int col = n0 + 4 * part + r;
         if (col < n) y[int64_t{m} * n + col] = static_cast<T>(acc[r]);
       }
+    }
+  }
+}
+
+// ---- few rows ------------------------------------------------------------------
+
+// Rows of X with one expert's weight, for few rows: quantisation and product in
+// one launch. A workgroup quantises up to 16 rows into LDS (or copies codes that
+// are quantised already), then multiplies them by its features' weight, which
+// goes from memory into the registers of v_mfma_scale_f32_16x16x128_f8f6f4 and is
+// read once for the 16 rows. SPLIT waves share the K of FB * 16 features, in
+// turns of 256 elements, and add their parts in LDS in a fixed order; the
+// workgroup's other waves take other features.
+//
+// Bound by the weight's bytes from memory, and at one row by the latency of a
+// launch and one pass over K. A wave keeps one turn's loads in flight (2.2 KiB of
+// 32 features): many waves cover the latency better than deep ones, whose
+// registers cost them (two turns deep 5 to 20% slower with many experts, four
+// 60%), and non-temporal loads lose 5 to 10%. Quantising in the kernel costs it
+// 0.4 us of 8.6 at 1x8192x8192, 4 of 42 for two rows of each of 128 experts of
+// 2048x4096, and spares a launch of 3.
+constexpr int kFewWaves = 8, kFewRows = 16;
+
+// Expert and rows of a workgroup's blockIdx.y; false where it has none. With
+// fewer rows than experts there is one grid row a row of X, and the first row of
+// an expert stands for all of them; its expert is the number of those that end
+// at or before it.
+__device__ __forceinline__ bool few_expert(const int32_t* __restrict__ offsets, int experts, int rows, int lane, int& e,
+                                           int& first, int& last) {
+  e = 0;
+  if (offsets) {
+    e = blockIdx.y;
+    if (rows < experts) {
+      int ended = 0;
+      for (int base = 0; base < experts; base += 64)
+        ended += __builtin_popcountll(__ballot(base + lane < experts && offsets[min(base + lane, experts - 1) + 1] <=
+                                                                            static_cast<int>(blockIdx.y)));
+      e = ended;
+      if (e >= experts || offsets[e] != static_cast<int>(blockIdx.y)) return false;
+    }
+  }
+  expert_rows(offsets, e, rows, first, last);
+  return first < last;
+}
+
+// LDS of the quantised rows: a row's codes, then a row's scales, each row a bank
+// group past the one before.
+constexpr uint32_t few_code_stride(uint32_t blocks) { return blocks * 128 + 16; }
+constexpr uint32_t few_scale_stride(uint32_t blocks) { return blocks * 8 + 8; }
+constexpr uint64_t few_lds_bytes(uint32_t blocks, uint32_t rows) {
+  return uint64_t{rows} * (few_code_stride(blocks) + few_scale_stride(blocks));
+}
+
+// X: fp32, fp16 or bf16 rows at `row_stride`, or uint8_t, codes with `sx`.
+template <class X, class T, int FB, int SPLIT>
+__global__ void __launch_bounds__(64 * kFewWaves)
+    mx_few_kernel(const X* __restrict__ x, uint64_t row_stride, const uint8_t* __restrict__ sx,
+                  const uint8_t* __restrict__ w, const uint8_t* __restrict__ sw, T* __restrict__ y, int rows, int n,
+                  int k, const int32_t* __restrict__ offsets, const int32_t* __restrict__ order, int copies,
+                  int tokens, int experts, int lds_rows) {
+  using Op = MfmaMxfp4x16;
+  constexpr int TILES = kFewWaves / SPLIT, COLUMNS = FB * 16;
+  __shared__ float parts[kFewWaves][kFewRows][COLUMNS + 1];
+  extern __shared__ __attribute__((aligned(16))) uint8_t staged[];
+  const int lane = threadIdx.x & 63, part = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int e, first, last;
+  if (!few_expert(offsets, experts, rows, lane, e, first, last)) return;
+  const int n0 = (blockIdx.x * TILES + wave / SPLIT) * COLUMNS, turn0 = wave % SPLIT;
+  const int groups = (k + 31) / 32, blocks = (k + 255) / 256;
+  const int row_bytes = groups * 16;
+  const int turns = (blocks - turn0 + SPLIT - 1) / SPLIT;
+  const int code_stride = few_code_stride(blocks), scale_stride = few_scale_stride(blocks);
+  uint8_t* const staged_scales = staged + lds_rows * code_stride;
+  const uint8_t* wr[FB];
+  const uint8_t* swr[FB];
+#pragma unroll
+  for (int f = 0; f < FB; ++f) {
+    const int feature = min(n0 + f * 16 + (lane & 15), n - 1);
+    wr[f] = w + (int64_t{e} * n + feature) * row_bytes;
+    swr[f] = sw + (int64_t{e} * blocks * n + feature) * 8;
+  }
+  struct Unit {
+    i32x4 w[FB][2];
+    elem_u32x2 s[FB];
+  };
+  auto load = [&](Unit& unit, int turn) __attribute__((always_inline)) {
+    const int b = turn0 + turn * SPLIT;
+#pragma unroll
+    for (int f = 0; f < FB; ++f) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        unit.w[f][h] =
+            *reinterpret_cast<const i32x4*>(wr[f] + min(b * 128 + h * 64 + part * 16, row_bytes - 16));
+      unit.s[f] = *reinterpret_cast<const elem_u32x2*>(swr[f] + int64_t{b} * n * 8);
+    }
+  };
+  for (int m0 = first; m0 < last; m0 += kFewRows) {
+    Unit unit;
+    if (turns > 0) load(unit, 0);  // in flight while the rows are quantised
+    const int live = min(kFewRows, last - m0);
+    for (int task = threadIdx.x; task < live * blocks * 8; task += 64 * kFewWaves) {
+      const int row = task / (blocks * 8), group = task % (blocks * 8);
+      i32x4 codes = {0, 0, 0, 0};
+      uint32_t scale = 0;  // groups past K: zeros of the scale 2^-127
+      if constexpr (sizeof(X) == 1) {
+        if (group < groups) {
+          codes = *reinterpret_cast<const i32x4*>(x + int64_t{m0 + row} * row_bytes + group * 16);
+          scale = sx[(int64_t{group >> 3} * rows + m0 + row) * 8 + (group & 7)];
+        }
+      } else if (group < groups) {
+        int token = m0 + row;
+        if (order) token = max(0, min(order[token] / copies, tokens - 1));
+        const X* from = x + static_cast<uint64_t>(token) * row_stride + group * 32;
+        Raw8<X> raw[4];
+        if (group * 32 + 32 <= k) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) raw[q].load(from + q * 8);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) raw[q].load(from + q * 8, k - group * 32 - q * 8);
+        }
+        uint32_t largest = raw_magnitude(raw[0]);
+#pragma unroll
+        for (int q = 1; q < 4; ++q) largest = join_magnitudes(X(), largest, raw_magnitude(raw[q]));
+        scale = scale_byte(magnitude_bits<X>(largest));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) codes[q] = static_cast<int>(encode8(raw[q], scale));
+      }
+      *reinterpret_cast<i32x4*>(staged + row * code_stride + group * 16) = codes;
+      staged_scales[row * scale_stride + group] = static_cast<uint8_t>(scale);
+    }
+    __syncthreads();
+    const int mine = min(lane & 15, live - 1);
+    const uint8_t* xc = staged + mine * code_stride + part * 16;
+    const uint8_t* xs = staged_scales + mine * scale_stride;
+    Op::Acc acc[FB] = {};
+    auto multiply = [&](const Unit& unit, int turn) __attribute__((always_inline)) {
+      const int b = turn0 + turn * SPLIT;
+      const elem_u32x2 sb = *reinterpret_cast<const elem_u32x2*>(xs + b * 8);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const i32x4 codes = *reinterpret_cast<const i32x4*>(xc + b * 128 + h * 64);
+        // Past K the codes are zeros; whatever the weight's scales hold there must not be NaN.
+        const bool past = b * 8 + h * 4 + part >= groups;
+#pragma unroll
+        for (int f = 0; f < FB; ++f)
+          acc[f] = Op::mma(unit.w[f][h], codes, acc[f], past ? 0 : static_cast<int>(unit.s[f][h] >> (8 * part)),
+                           static_cast<int>(sb[h] >> (8 * part)));
+      }
+    };
+    for (int turn = 0; turn < turns; ++turn) {
+      multiply(unit, turn);
+      if (turn + 1 < turns) load(unit, turn + 1);
+    }
+#pragma unroll
+    for (int f = 0; f < FB; ++f)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) parts[wave][lane & 15][f * 16 + 4 * part + r] = acc[f][r];
+    __syncthreads();
+    const int n_wg = blockIdx.x * TILES * COLUMNS;
+    for (int i = threadIdx.x; i < live * TILES * COLUMNS; i += 64 * kFewWaves) {
+      const int r = i / (TILES * COLUMNS), column = i % (TILES * COLUMNS), tile = column / COLUMNS;
+      float sum = 0.0f;
+#pragma unroll
+      for (int v = 0; v < SPLIT; ++v) sum += parts[tile * SPLIT + v][r][column % COLUMNS];
+      if (n_wg + column < n) y[static_cast<int64_t>(m0 + r) * n + n_wg + column] = static_cast<T>(sum);
     }
   }
 }
@@ -233,6 +401,16 @@ const ProductKernel kProductKernels[] = {
   MB_REGISTER_KERNEL("mx_product_" NAME "_128x128", (mx_product_ring_kernel<T, 128, 128, 4>));              \
   MB_REGISTER_KERNEL("mx_product_" NAME "_128x128_pair", (mx_product_ring_kernel<T, 128, 128, 2>));         \
   MB_REGISTER_KERNEL("mx_product_" NAME "_64x64", (mx_product_ring_kernel<T, 64, 64, 3>))
+#define MB_FEW_REGISTER_SPLIT(T, NAME, FB, SPLIT, SIZE)                                             \
+  MB_REGISTER_KERNEL("mx_linear_few_" NAME "_" SIZE, (mx_few_kernel<T, T, FB, SPLIT>));            \
+  MB_REGISTER_KERNEL("mx_product_few_" NAME "_" SIZE, (mx_few_kernel<uint8_t, T, FB, SPLIT>))
+#define MB_FEW_REGISTER(T, NAME)                   \
+  MB_FEW_REGISTER_SPLIT(T, NAME, 1, 8, "16x8");    \
+  MB_FEW_REGISTER_SPLIT(T, NAME, 2, 8, "32x8");    \
+  MB_FEW_REGISTER_SPLIT(T, NAME, 2, 4, "32x4")
+MB_FEW_REGISTER(float, "f32");
+MB_FEW_REGISTER(_Float16, "f16");
+MB_FEW_REGISTER(__bf16, "bf16");
 MB_PRODUCT_REGISTER(float, "f32");
 MB_PRODUCT_REGISTER(_Float16, "f16");
 MB_PRODUCT_REGISTER(__bf16, "bf16");
@@ -291,12 +469,52 @@ double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint
   return whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
 }
 
+// Whether mx_few_kernel takes a call: up to 16 rows of one weight, up to two an
+// expert on average (it reads a weight once for 16 rows, but its rows are
+// quantised, or copied, once a workgroup), whose codes fit the LDS. us, it and
+// the ring with its quantisation: 1x8192x8192 9.0 and 15, 16x8192x8192 14.3 and
+// 15.3; 128 experts of 2048x4096, two rows each 46 and 55, four 87 and 78.
+bool few_rows(uint64_t rows, uint32_t k, uint32_t experts) {
+  const uint64_t most = experts > 1 ? 2 * uint64_t{experts} : kFewRows;
+  return rows <= most && few_lds_bytes((k + 255) / 256, rows < kFewRows ? rows : kFewRows) <= 128 * 1024;
+}
+
+template <class X, class T>
+void launch_few(const void* x, uint64_t row_stride, const void* sx, const void* w, const void* sw, void* y,
+                uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, const int32_t* order, uint32_t copies,
+                uint32_t tokens, uint32_t experts, hipStream_t stream) {
+  const uint32_t grid_rows = rows < experts ? rows : experts, lds_rows = rows < kFewRows ? rows : kFewRows;
+  const uint64_t wide = (n + uint64_t{31}) / 32 * grid_rows;
+  auto launch = [&](auto kernel, uint32_t columns) {
+    kernel<<<dim3((n + columns - 1) / columns, grid_rows), dim3(64 * kFewWaves),
+             static_cast<uint32_t>(few_lds_bytes((k + 255) / 256, lds_rows)), stream>>>(
+        static_cast<const X*>(x), row_stride, static_cast<const uint8_t*>(sx), static_cast<const uint8_t*>(w),
+        static_cast<const uint8_t*>(sw), static_cast<T*>(y), static_cast<int>(rows), static_cast<int>(n),
+        static_cast<int>(k), offsets, order, static_cast<int>(copies), static_cast<int>(tokens),
+        static_cast<int>(experts), static_cast<int>(lds_rows));
+  };
+  // 32 features a workgroup where that gives every CU one, else 16 (1x4096x14336
+  // 7.7 us, with 32 10.2); with many workgroups, half the waves on each K (two
+  // rows of 128 experts 46 us, with eight 58).
+  if (wide < 256)
+    launch(mx_few_kernel<X, T, 1, 8>, 16);
+  else if (wide < 2048)
+    launch(mx_few_kernel<X, T, 2, 8>, 32);
+  else
+    launch(mx_few_kernel<X, T, 2, 4>, 64);
+}
+
 int launch_product(int dtype, const void* x_codes, const void* sx, const void* w_codes, const void* sw, void* y,
                    uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, uint32_t experts,
                    hipStream_t stream) {
   const uint8_t *x = static_cast<const uint8_t*>(x_codes), *w = static_cast<const uint8_t*>(w_codes);
   const uint8_t *sxb = static_cast<const uint8_t*>(sx), *swb = static_cast<const uint8_t*>(sw);
   const uint32_t padded = (k + 31) / 32 * 32, steps = (k + 255) / 256;
+  if (few_rows(rows, k, experts)) {
+    MB_FOR_DTYPE(dtype, (launch_few<uint8_t, T>(x, 0, sx, w, sw, y, rows, n, k, offsets, nullptr, 1, rows, experts,
+                                                stream)));
+    return launch_status("mx_product_few");
+  }
   // The ring addresses a matrix's scales, and a tile's rows, with 32-bit offsets.
   const uint64_t scale_rows = rows > n ? rows : n;
   if (steps * scale_rows * 8 <= 0x7fffffffu) {
@@ -380,6 +598,11 @@ int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, ui
   if (!mb::aligned(codes, 16)) return mb::fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
   uint8_t* scales = codes + codes_bytes;
   const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (mb::few_rows(rows, k, experts)) {
+    MB_FOR_DTYPE(dtype, (mb::launch_few<T, T>(x, row_stride, nullptr, w, scale_w, y, static_cast<uint32_t>(rows), n, k,
+                                              offsets, gathered ? order : nullptr, copies, tokens, experts, on)));
+    return mb::launch_status("mx_linear_few");
+  }
   if (int rc = mb::launch_quantize(dtype, x, tokens, k, row_stride, slots, gathered ? copies : 1,
                                    static_cast<uint32_t>(rows), codes, scales, on))
     return rc;

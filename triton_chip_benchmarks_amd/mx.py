@@ -16,7 +16,7 @@ fit it.
 
 from __future__ import annotations
 
-from typing import NamedTuple
+import torch
 
 from . import _native, formats
 
@@ -24,39 +24,47 @@ GROUP = formats.MX_GROUP_SIZE
 STEP = 256  # K elements whose scales a row holds together
 
 
-class Packed(NamedTuple):
-    """An operand of rows x k: codes [rows][ceil(k/32)*16] and scales [ceil(k/256)][rows][8], uint8; with a leading
-    dimension each, one such matrix for each expert."""
-
-    codes: object
-    scales: object
-    k: int
-
-    @property
-    def rows(self) -> int:
-        return self.codes.shape[-2]
+DTYPE_CODES = {torch.float32: _native.MB_DTYPE_F32, torch.float16: _native.MB_DTYPE_F16,
+               torch.bfloat16: _native.MB_DTYPE_BF16}
 
 
-def _torch():
-    import torch
+class Packed:
+    """An operand of rows x k: codes [rows][ceil(k/32)*16] and scales [ceil(k/256)][rows][8], contiguous uint8
+    tensors; with a leading dimension each, one such matrix for each of `experts`."""
 
-    return torch
+    __slots__ = ("codes", "scales", "k", "rows", "experts")
+
+    def __init__(self, codes, scales, k: int):
+        lead = codes.shape[:-2]
+        rows = codes.shape[-2] if codes.dim() >= 2 else -1
+        if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or len(lead) > 1 or not codes.is_contiguous()
+                or not scales.is_contiguous() or codes.shape != (*lead, rows, -(-k // GROUP) * (GROUP // 2))
+                or scales.shape != (*lead, -(-k // STEP), rows, STEP // GROUP)):
+            raise ValueError(f"an operand of k = {k} has contiguous uint8 codes [rows][{-(-k // GROUP) * 16}] and "
+                             f"scales [{-(-k // STEP)}][rows][8], not {tuple(codes.shape)} and {tuple(scales.shape)}")
+        self.codes, self.scales, self.k, self.rows = codes, scales, k, rows
+        self.experts = lead[0] if lead else None
+
+
+# The checks below run at every call, beside which a kernel takes a few microseconds: get_device and comparisons of
+# shapes cost tens of nanoseconds, tensor.device and torch.cuda.current_device several hundred.
 
 
 def dtype_code(tensor, what: str) -> int:
-    torch = _torch()
-    code = {torch.float32: _native.MB_DTYPE_F32, torch.float16: _native.MB_DTYPE_F16,
-            torch.bfloat16: _native.MB_DTYPE_BF16}.get(tensor.dtype)
+    code = DTYPE_CODES.get(tensor.dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, not {tensor.dtype}")
     return code
 
 
 def check_device(*tensors) -> None:
-    device = _torch().cuda.current_device()
+    device = tensors[0].get_device()
+    if device != (torch._C._cuda_getDevice() if torch.cuda.is_initialized() else torch.cuda.current_device()):
+        raise ValueError(f"tensors must lie on the current HIP device (cuda:{torch.cuda.current_device()}), not "
+                         f"{tensors[0].device}")
     for tensor in tensors:
-        if not tensor.is_cuda or tensor.device.index != device:
-            raise ValueError(f"tensors must lie on the current HIP device (cuda:{device}), not {tensor.device}")
+        if tensor.get_device() != device:
+            raise ValueError(f"tensors must lie on one device, cuda:{device}, not {tensor.device}")
 
 
 def strided_rows(tensor, what: str) -> tuple[int, int]:
@@ -75,8 +83,8 @@ def strided_rows(tensor, what: str) -> tuple[int, int]:
 def check_output(tensor, what: str, shape, dtype, device):
     """`tensor`, checked, or a new one in its place."""
     if tensor is None:
-        return _torch().empty(shape, dtype=dtype, device=device)
-    if tuple(tensor.shape) != tuple(shape) or tensor.dtype != dtype or not tensor.is_contiguous():
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tensor.shape != shape or tensor.dtype != dtype or not tensor.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of {tuple(shape)}, not {tensor.dtype} of "
                          f"{tuple(tensor.shape)}")
     return tensor
@@ -88,22 +96,15 @@ def bytes_of(tensor) -> int:
 
 def empty(rows: int, k: int, device="cuda", experts: int | None = None) -> Packed:
     """An operand's buffers, for `quantize` to fill."""
-    torch = _torch()
     lead = () if experts is None else (experts,)
     return Packed(torch.empty((*lead, rows, -(-k // GROUP) * (GROUP // 2)), dtype=torch.uint8, device=device),
                   torch.empty((*lead, -(-k // STEP), rows, STEP // GROUP), dtype=torch.uint8, device=device), k)
 
 
-def check_packed(packed: Packed, what: str, experts: int | None = None) -> None:
-    torch = _torch()
-    codes, scales, k = packed
-    lead = () if experts is None else (experts,)
-    rows = codes.shape[-2] if codes.dim() >= 2 else -1
-    if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or not codes.is_contiguous()
-            or not scales.is_contiguous() or tuple(codes.shape) != (*lead, rows, -(-k // GROUP) * (GROUP // 2))
-            or tuple(scales.shape) != (*lead, -(-k // STEP), rows, STEP // GROUP)):
-        raise ValueError(f"{what} must hold contiguous uint8 codes and scales of {'one matrix' if experts is None else f'{experts} matrices'}"
-                         f" with k = {k}, not {tuple(codes.shape)} and {tuple(scales.shape)}")
+def _check_experts(packed: Packed, what: str, experts: int | None) -> None:
+    if packed.experts != experts:
+        raise ValueError(f"{what} must hold {'one matrix' if experts is None else f'a matrix for each of {experts} experts'},"
+                         f" not codes of {tuple(packed.codes.shape)}")
 
 
 def quantize(x, packed: Packed | None = None, columns: bool = False, stream=None) -> Packed:
@@ -113,7 +114,7 @@ def quantize(x, packed: Packed | None = None, columns: bool = False, stream=None
     rows, k = x.shape[::-1] if columns else x.shape
     if packed is None:
         packed = empty(rows, k, x.device)
-    check_packed(packed, "packed")
+    _check_experts(packed, "packed", None)
     if (packed.rows, packed.k) != (rows, k):
         raise ValueError(f"packed must be an operand of {rows} x {k}, not {packed.rows} x {packed.k}")
     check_device(x, packed.codes, packed.scales)
@@ -128,8 +129,8 @@ def quantize(x, packed: Packed | None = None, columns: bool = False, stream=None
 
 def dequantize(packed: Packed, out=None, stream=None):
     """The values of an operand [rows][k]: bfloat16 (exact) unless `out` is of another type."""
-    check_packed(packed, "packed")
-    dtype = _torch().bfloat16 if out is None else out.dtype
+    _check_experts(packed, "packed", None)
+    dtype = torch.bfloat16 if out is None else out.dtype
     out = check_output(out, "out", (packed.rows, packed.k), dtype, packed.codes.device)
     code = dtype_code(out, "out")
     check_device(packed.codes, packed.scales, out)
@@ -145,10 +146,9 @@ def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=Non
     With `offsets` ([experts + 1] int32, on the device) b holds a matrix for each expert, and a's rows offsets[e] ..
     offsets[e + 1] - 1 meet matrix e; output rows from offsets[experts] on are not written.
     """
-    torch = _torch()
     experts = None if offsets is None else offsets.numel() - 1
-    check_packed(a, "a")
-    check_packed(b, "b", experts)
+    _check_experts(a, "a", None)
+    _check_experts(b, "b", experts)
     if a.k != b.k:
         raise ValueError(f"a and b must have the same k, not {a.k} and {b.k}")
     if dtype is None:
@@ -164,7 +164,7 @@ def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=Non
 
 
 def _check_indices(tensor, what: str) -> None:
-    if tensor is not None and (tensor.dtype != _torch().int32 or not tensor.is_contiguous()):
+    if tensor is not None and (tensor.dtype != torch.int32 or not tensor.is_contiguous()):
         raise ValueError(f"{what} must be a contiguous int32 tensor, not {tensor.dtype}")
 
 
@@ -173,7 +173,6 @@ def _pointer(tensor) -> tuple[int | None, int]:
 
 
 def _workspace(tensor, needed: int, device):
-    torch = _torch()
     if tensor is None:
         return torch.empty(needed, dtype=torch.uint8, device=device)
     if tensor.dtype != torch.uint8 or not tensor.is_contiguous() or tensor.numel() < needed:
@@ -183,7 +182,6 @@ def _workspace(tensor, needed: int, device):
 
 def linear_workspace(rows: int, n: int, k: int, dtype, experts: int = 1, device="cuda"):
     """A workspace for `linear` with `rows` output rows (routed ones, with a plan)."""
-    torch = _torch()
     return torch.empty(_native.load().mb_mx_linear_workspace(rows, n, k), dtype=torch.uint8, device=device)
 
 
@@ -213,7 +211,7 @@ def linear(x, weight: Packed, out=None, plan=None, sorted_rows: bool = False, wo
         check_device(offsets, *(() if sorted_rows else (order, slots)))
     elif sorted_rows:
         raise ValueError("sorted rows need the plan that they are sorted by")
-    check_packed(weight, "weight", experts)
+    _check_experts(weight, "weight", experts)
     if weight.k != k:
         raise ValueError(f"the weight must have k = {k}, not {weight.k}")
     n, routed = weight.rows, rows * copies
@@ -244,7 +242,6 @@ def _carve(workspace, at: int, rows: int, k: int) -> Packed:
 
 def linear_backward_workspace(rows: int, n: int, k: int, dtype, device="cuda"):
     """A workspace for `linear_backward`, and for `linear` of the same sizes."""
-    torch = _torch()
     needed = max(_backward_bytes(rows, n, k), _native.load().mb_mx_linear_workspace(rows, n, k))
     return torch.empty(needed, dtype=torch.uint8, device=device)
 

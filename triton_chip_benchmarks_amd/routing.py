@@ -12,6 +12,8 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
+import torch
+
 from . import _native
 from .mx import bytes_of, check_device, check_output, dtype_code, strided_rows
 
@@ -29,12 +31,6 @@ class Plan(NamedTuple):
     workspace: object = None
 
 
-def _torch():
-    import torch
-
-    return torch
-
-
 def _score_code(scores: str) -> int:
     if scores not in SCORES:
         raise ValueError(f"scores must be one of {', '.join(SCORES)}, not {scores!r}")
@@ -50,7 +46,6 @@ def route(logits, top: int, bias=None, scores: str = "softmax", groups: int = 1,
     index. A logit of -inf masks its expert; -1, with weight 0, stands where none is left. The weights are s, divided
     by their sum if `renormalize`, times `scale`.
     """
-    torch = _torch()
     code = dtype_code(logits, "logits")
     stride, span = strided_rows(logits, "logits")
     tokens, count = logits.shape
@@ -70,7 +65,6 @@ def route(logits, top: int, bias=None, scores: str = "softmax", groups: int = 1,
 def route_backward(logits, experts, d_weights, scores: str = "softmax", renormalize: bool = True, scale: float = 1.0,
                    d_logits=None, stream=None):
     """d_logits, in the logits' type, for the gradient d_weights of route's weights and the experts it chose."""
-    torch = _torch()
     code = dtype_code(logits, "logits")
     stride, span = strided_rows(logits, "logits")
     tokens, count = logits.shape
@@ -89,7 +83,6 @@ def route_backward(logits, experts, d_weights, scores: str = "softmax", renormal
 
 def empty_plan(tokens: int, top: int, experts: int, device="cuda") -> Plan:
     """A plan's buffers and workspace, for `dispatch` to fill."""
-    torch = _torch()
     needed = _native.load().mb_dispatch_workspace(tokens * top, experts)
     return Plan(torch.empty(experts + 1, dtype=torch.int32, device=device),
                 torch.empty(tokens * top, dtype=torch.int32, device=device),
@@ -99,7 +92,6 @@ def empty_plan(tokens: int, top: int, experts: int, device="cuda") -> Plan:
 
 def dispatch(experts, count: int, plan: Plan | None = None, stream=None) -> Plan:
     """The plan of the choices `experts` [tokens][top] (int32; outside 0 .. count - 1: none) of `count` experts."""
-    torch = _torch()
     if experts.dim() != 2:
         raise ValueError(f"experts must be [tokens][top], not {tuple(experts.shape)}")
     tokens, top = experts.shape
@@ -119,7 +111,6 @@ def dispatch(experts, count: int, plan: Plan | None = None, stream=None) -> Plan
 
 
 def _combine_sizes(y, slots, weights):
-    torch = _torch()
     if y.dim() != 2 or slots.dim() != 2:
         raise ValueError(f"y must be [rows][n] and slots [tokens][top], not {tuple(y.shape)} and {tuple(slots.shape)}")
     check_output(y, "y", y.shape, y.dtype, y.device)
@@ -142,7 +133,6 @@ def combine(y, slots, weights, out=None, stream=None):
 
 def combine_backward(d_out, y, slots, weights, d_y=None, d_weights=None, stream=None):
     """(d_y, d_weights) of combine for the gradient d_out; rows of a given d_y that no slot names stay as they are."""
-    torch = _torch()
     code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
     check_output(d_out, "d_out", (tokens, n), y.dtype, y.device)
     if d_y is None:
