@@ -183,7 +183,9 @@ def check(status: int) -> None:
 
 
 def call(name: str, *arguments) -> None:
-    check(getattr(load(), name)(*arguments))
+    status = getattr(_library or load(), name)(*arguments)
+    if status != MB_OK:
+        check(status)
 
 
 def device_query(device: int) -> dict:

@@ -39,7 +39,7 @@ _READ_PACKED_RE = re.compile(r"read_sum_packed_kernelI(f|DF16_|t)Li(\d+)E")
 _ELEMENT_TYPE = {"f": "f32", "DF16_": "f16", "DF16b": "bf16"}
 _ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)E")
 _LAYER_RE = re.compile(r"(mx_quantize|mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
-                       r"_kernelI(f|DF16_|DF16b)E")
+                       r"_kernelI(f|DF16_|DF16b)(?:Lb([01])E)?E")
 _PRODUCT_RING_RE = re.compile(r"mx_product_ring_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi(\d+)EE")
 _FEW_RE = re.compile(r"mx_few_kernelI(h|f|DF16_|DF16b)(S\d*_|T_|f|DF16_|DF16b)?Li(\d+)ELi(\d+)EE")
 _DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
@@ -95,7 +95,7 @@ def registered_name(symbol: str) -> str | None:
         return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}_v{match.group(3)}"
     match = _LAYER_RE.search(symbol)
     if match:
-        return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}"
+        return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}{'_stream' if match.group(3) == '1' else ''}"
     match = _PRODUCT_RING_RE.search(symbol)
     if match:
         dtype, features, rows, stages = match.groups()

@@ -58,7 +58,8 @@ struct Raw8 {
   }
 };
 
-template <class T>
+// STREAM: non-temporal, for outputs that the L2s cannot hold (see streams()).
+template <bool STREAM, class T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8], int count) {
   T out[8];
 #pragma unroll
@@ -67,8 +68,13 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8], int count) {
     elem_u32x4 part[sizeof(T) / 2];
     __builtin_memcpy(part, out, sizeof(part));
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
-      *reinterpret_cast<elem_u32x4_any*>(reinterpret_cast<uint8_t*>(p) + 16 * i) = part[i];
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
+      elem_u32x4_any* to = reinterpret_cast<elem_u32x4_any*>(reinterpret_cast<uint8_t*>(p) + 16 * i);
+      if constexpr (STREAM)
+        __builtin_nontemporal_store(part[i], to);
+      else
+        *to = part[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -83,22 +89,45 @@ __device__ __forceinline__ uint32_t quad_swap(uint32_t v) {
 }
 constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E;
 
+// One step of a reduction over the wave: v joined with another lane's, by data
+// parallel primitives, which take no LDS trip as a shuffle does (about 8 cycles
+// against 60). Lanes that CTRL leaves out get `none`.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_lane(float none, float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none),
+                                                               __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+
+// f over the wave's lanes, in every lane: rows of 16 by shifts of 1, 2, 4 and 8,
+// then row after row; lane 63 has all.
+template <class F>
+__device__ __forceinline__ float wave_reduce(float v, float none, F&& f) {
+  v = f(v, dpp_lane<0x111, 0xf>(none, v));
+  v = f(v, dpp_lane<0x112, 0xf>(none, v));
+  v = f(v, dpp_lane<0x114, 0xf>(none, v));
+  v = f(v, dpp_lane<0x118, 0xf>(none, v));
+  v = f(v, dpp_lane<0x142, 0xa>(none, v));  // lane 15 of rows 0 and 2 to rows 1 and 3
+  v = f(v, dpp_lane<0x143, 0xc>(none, v));  // lane 31 to rows 2 and 3
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 __device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, 64);
-  return v;
+  return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
 }
 
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int offset = 32; offset > 0; offset >>= 1) v = fmaxf(v, __shfl_xor(v, offset, 64));
-  return v;
+  return wave_reduce(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
 }
 
 // Host: bytes of one element of MB_DTYPE_*, 0 for another code.
 inline uint32_t elem_bytes(int dtype) {
   return dtype == MB_DTYPE_F32 ? 4 : dtype == MB_DTYPE_F16 || dtype == MB_DTYPE_BF16 ? 2 : 0;
 }
+
+// Host: whether an output of so many bytes is stored non-temporally: past the 32
+// MiB that the eight L2s hold together (combine of 8192x4 rows of 4096 bf16 58 us,
+// so 49; smaller outputs stay where the next kernel finds them).
+inline bool streams(uint64_t bytes) { return bytes > (32u << 20); }
 
 // Host: bytes that `rows` rows of `k` elements span at a row stride (elements).
 inline uint64_t strided_bytes(uint64_t rows, uint64_t k, uint64_t row_stride, uint32_t item) {

@@ -70,47 +70,122 @@ __global__ void __launch_bounds__(256)
 }
 
 // Columns of x to the rows of the transposed operand: groups of 32 run along
-// x's rows. A lane holds 32 rows of one column, so a group's largest magnitude
-// needs no other lane; a wave takes 64 columns of 32 rows.
+// x's rows. A workgroup takes 256 rows of 128 columns, a wave a group of 32
+// rows, a lane two neighbouring columns, so that a group's largest magnitude
+// needs no other lane; the codes cross LDS, so that an operand row's 128 bytes
+// leave together.
+constexpr int kTileColumns = 128, kTilePitch = 128 + 16;  // LDS bytes of a column, a bank group apart
+
+// 32 rows of two columns, a pair a row as it is stored.
 template <class T>
-__global__ void __launch_bounds__(256)
-    mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
-                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const uint32_t groups = (rows + kGroup - 1) / kGroup;
-  const uint32_t strips = (columns + 63) / 64;
-  const uint32_t strip = blockIdx.x % strips;
-  const uint32_t group = blockIdx.x / strips * 4 + threadIdx.x / 64;
-  const uint32_t column = strip * 64 + threadIdx.x % 64;
-  if (column >= columns || group >= (groups + 7) / 8 * 8) return;
-  uint8_t* scale_at = scales + (static_cast<uint64_t>(group / 8) * columns + column) * 8 + group % 8;
-  if (group >= groups) {
-    *scale_at = 127;
-    return;
-  }
-  Raw8<T> raw[4];
+struct ColumnPairs {
+  typedef uint32_t Pair __attribute__((ext_vector_type(sizeof(T) / 2), aligned(sizeof(T))));
+  typedef uint32_t Word __attribute__((ext_vector_type(sizeof(T) / 2)));
+  Word at[32];
+
+  // Largest magnitudes of the columns, in the form of magnitude_bits.
+  __device__ __forceinline__ void largest(uint32_t (&out)[2]) const {
+    if constexpr (sizeof(T) == 4) {
+      out[0] = out[1] = 0;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    T v[8];
+      for (int r = 0; r < 32; ++r) {
+        out[0] = max(out[0], at[r][0] & 0x7fffffffu);
+        out[1] = max(out[1], at[r][1] & 0x7fffffffu);
+      }
+    } else {
+      uint32_t both = 0;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) both = join_magnitudes(T(), both, word(r) & 0x7fff7fffu);
+      out[0] = both & 0xffffu;
+      out[1] = both >> 16;
+    }
+  }
+  // Rows 8q .. 8q + 7 of a column.
+  template <int COLUMN>
+  __device__ __forceinline__ Raw8<T> piece(int q) const {
+    Raw8<T> raw;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t row = group * kGroup + 8 * q + i;
-      v[i] = row < rows ? x[row * row_stride + column] : T(0);
+      const int r = 8 * q + i;
+      if constexpr (sizeof(T) == 4)
+        raw.part[i / 4][i % 4] = at[r][COLUMN];
+      else if (i % 2 == 0)  // one 16-bit half of each of two rows
+        raw.part[0][i / 2] =
+            __builtin_amdgcn_perm(word(r + 1), word(r), COLUMN ? 0x07060302u : 0x05040100u);
     }
-    __builtin_memcpy(raw[q].part, v, sizeof(v));
+    return raw;
   }
-  uint32_t largest = raw_magnitude(raw[0]);
-#pragma unroll
-  for (int q = 1; q < 4; ++q) largest = join_magnitudes(T(), largest, raw_magnitude(raw[q]));
+
+ private:
+  __device__ __forceinline__ uint32_t word(int r) const { return at[r][0]; }
+};
+
+template <class T, int COLUMN>
+__device__ __forceinline__ void quantize_column(const ColumnPairs<T>& values, uint32_t largest, uint8_t* codes,
+                                                uint8_t* scale_at) {
   const uint32_t scale = scale_byte(magnitude_bits<T>(largest));
   elem_u32x4 word;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) word[q] = encode8(raw[q], scale);
-  *reinterpret_cast<elem_u32x4*>(codes + (static_cast<uint64_t>(column) * groups + group) * 16) = word;
+  for (int q = 0; q < 4; ++q) word[q] = encode8(values.template piece<COLUMN>(q), scale);
+  *reinterpret_cast<elem_u32x4*>(codes) = word;
   *scale_at = static_cast<uint8_t>(scale);
 }
 
-// Codes and scales to values, rounded once to T (exact in fp32 and bf16).
 template <class T>
+__global__ void __launch_bounds__(512)
+    mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[kTileColumns * kTilePitch];
+  __shared__ __attribute__((aligned(8))) uint8_t tile_scales[kTileColumns * 8];
+  using Pair = typename ColumnPairs<T>::Pair;
+  const uint32_t groups = (rows + kGroup - 1) / kGroup;
+  const uint32_t strips = (columns + kTileColumns - 1) / kTileColumns;
+  const uint32_t strip = blockIdx.x % strips, block = blockIdx.x / strips;
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t local = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t group = block * 8 + local, column = lane * 2;
+  const uint32_t live = min(static_cast<uint32_t>(kTileColumns), columns - strip * kTileColumns);
+  if (group < groups) {
+    const uint32_t row0 = group * kGroup;
+    const T* from = x + row0 * row_stride + strip * kTileColumns;
+    ColumnPairs<T> values;
+    if (row0 + kGroup <= rows && live == kTileColumns) {
+#pragma unroll
+      for (int r = 0; r < 32; ++r, from += row_stride) values.at[r] = *reinterpret_cast<const Pair*>(from + column);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 32; ++r, from += row_stride) {
+        T pair[2] = {T(0), T(0)};
+        if (row0 + r < rows) {
+          if (column < live) pair[0] = from[column];
+          if (column + 1 < live) pair[1] = from[column + 1];
+        }
+        __builtin_memcpy(&values.at[r], pair, sizeof(pair));
+      }
+    }
+    uint32_t largest[2];
+    values.largest(largest);
+    quantize_column<T, 0>(values, largest[0], tile + column * kTilePitch + local * 16, tile_scales + column * 8 + local);
+    quantize_column<T, 1>(values, largest[1], tile + (column + 1) * kTilePitch + local * 16,
+                          tile_scales + (column + 1) * 8 + local);
+  } else {
+    tile_scales[column * 8 + local] = tile_scales[(column + 1) * 8 + local] = 127;
+  }
+  __syncthreads();
+  const uint64_t first = strip * uint64_t{kTileColumns};
+  for (uint32_t i = threadIdx.x; i < live * 8; i += 512) {
+    const uint32_t c = i / 8, chunk = i % 8;
+    if (block * 8 + chunk < groups)
+      *reinterpret_cast<elem_u32x4*>(codes + ((first + c) * groups + block * 8 + chunk) * 16) =
+          *reinterpret_cast<const elem_u32x4*>(tile + c * kTilePitch + chunk * 16);
+  }
+  if (threadIdx.x < live)
+    *reinterpret_cast<elem_u32x2*>(scales + (block * uint64_t{columns} + first + threadIdx.x) * 8) =
+        *reinterpret_cast<const elem_u32x2*>(tile_scales + threadIdx.x * 8);
+}
+
+// Codes and scales to values, rounded once to T (exact in fp32 and bf16).
+template <class T, bool STREAM>
 __global__ void __launch_bounds__(256)
     mx_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
                          uint32_t rows, uint32_t k) {
@@ -129,13 +204,14 @@ __global__ void __launch_bounds__(256)
     const float unit = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(code, 1.0f, 0)[0];
     v[i] = scale == 255 ? bits_float(0x7fc00000u) : __builtin_amdgcn_ldexpf(unit, static_cast<int>(scale) - 127);
   }
-  store8(out + row * k + k0, v, static_cast<int>(min(8u, k - k0)));
+  store8<STREAM>(out + row * k + k0, v, static_cast<int>(min(8u, k - k0)));
 }
 
 #define MB_MX_REGISTER(T, NAME)                                      \
   MB_REGISTER_KERNEL("mx_quantize_" NAME, mx_quantize_kernel<T>);    \
   MB_REGISTER_KERNEL("mx_quantize_columns_" NAME, mx_quantize_columns_kernel<T>); \
-  MB_REGISTER_KERNEL("mx_dequantize_" NAME, mx_dequantize_kernel<T>)
+  MB_REGISTER_KERNEL("mx_dequantize_" NAME, (mx_dequantize_kernel<T, false>)); \
+  MB_REGISTER_KERNEL("mx_dequantize_" NAME "_stream", (mx_dequantize_kernel<T, true>))
 MB_MX_REGISTER(float, "f32");
 MB_MX_REGISTER(_Float16, "f16");
 MB_MX_REGISTER(__bf16, "bf16");
@@ -183,11 +259,10 @@ int launch_quantize(int dtype, const void* x, uint32_t rows, uint32_t k, uint64_
 
 int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint32_t columns, uint64_t row_stride,
                             void* codes, void* scales, hipStream_t stream) {
-  const uint64_t groups = (rows + kGroup - 1) / kGroup;
-  const uint64_t grid = (columns + uint64_t{63}) / 64 * ((groups + 7) / 8 * 2);
-  if (grid > 0xffffffu)
+  const uint64_t grid = (columns + uint64_t{kTileColumns} - 1) / kTileColumns * ((rows + uint64_t{kBlock} - 1) / kBlock);
+  if (grid > 0x7fffffu)
     return fail(MB_ERR_UNSUPPORTED, "mx_quantize_columns: %u x %u exceeds one launch", rows, columns);
-  MB_FOR_DTYPE(dtype, (mx_quantize_columns_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream>>>(
+  MB_FOR_DTYPE(dtype, (mx_quantize_columns_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(512), 0, stream>>>(
                           static_cast<const T*>(x), rows, columns, row_stride, static_cast<uint8_t*>(codes),
                           static_cast<uint8_t*>(scales))));
   return launch_status("mx_quantize_columns");
@@ -253,10 +328,18 @@ int mb_mx_dequantize(int dtype, const void* codes, uint64_t codes_bytes, const v
   if (!mb::aligned(out, item)) return mb::fail(MB_ERR_ALIGNMENT, "%s: out must lie on its elements' %u bytes", entry, item);
   const uint64_t grid = (uint64_t{rows} * ((k + 7) / 8) + 255) / 256;
   if (grid > 0xffffffu) return mb::fail(MB_ERR_UNSUPPORTED, "%s: %u x %u exceeds one launch", entry, rows, k);
-  MB_FOR_DTYPE(dtype, (mb::mx_dequantize_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0,
-                                                     static_cast<hipStream_t>(stream)>>>(
-                          static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales),
-                          static_cast<T*>(out), rows, k)));
+  auto launch = [&](auto kernel, auto t) {
+    kernel<<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), static_cast<decltype(t)*>(out), rows,
+        k);
+  };
+  const bool streamed = mb::streams(uint64_t{rows} * k * item);
+  MB_FOR_DTYPE(dtype, {
+    if (streamed)
+      launch(mb::mx_dequantize_kernel<T, true>, T());
+    else
+      launch(mb::mx_dequantize_kernel<T, false>, T());
+  });
   return mb::launch_status("mx_dequantize");
 }
 

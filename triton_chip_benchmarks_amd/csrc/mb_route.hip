@@ -45,12 +45,22 @@ __device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax,
   for (int i = 0; i < V; ++i) score[i] = total == 0.0f ? 0.0f : score[i] / total;
 }
 
+// A lane's V consecutive elements of a row, at any element's address.
+template <class T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) LaneValues {
+  T at[V];
+};
+
 template <class T, int V>
 __device__ __forceinline__ void load_logits(const T* __restrict__ row, uint32_t experts, int lane, float (&logit)[V]) {
+  const uint32_t first = lane * V;
+  if (first + V <= experts) {
+    const LaneValues<T, V> values = *reinterpret_cast<const LaneValues<T, V>*>(row + first);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const uint32_t e = lane * V + i;
-    logit[i] = e < experts ? widen(row[e]) : kNegInf;
+    for (int i = 0; i < V; ++i) logit[i] = widen(values.at[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) logit[i] = first + i < experts ? widen(row[first + i]) : kNegInf;
   }
 }
 
@@ -64,7 +74,6 @@ __global__ void __launch_bounds__(256)
                  const float* __restrict__ bias, uint32_t top, bool softmax, uint32_t groups, uint32_t top_groups,
                  bool renormalize, float scale, int32_t* __restrict__ chosen, float* __restrict__ weights) {
   __shared__ float lds[4][64 * V];
-  __shared__ float group_lds[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const uint32_t token = blockIdx.x * 4 + wave;
   if (token >= tokens) return;
@@ -85,26 +94,23 @@ __global__ void __launch_bounds__(256)
     wave_lds_fence();
     float first = kNegInf, second = kNegInf;
     if (static_cast<uint32_t>(lane) < groups) {
+#pragma unroll 8
       for (uint32_t i = 0; i < size; ++i) {
         const float v = lds[wave][lane * size + i];
         second = fmaxf(second, fminf(first, v));
         first = fmaxf(first, v);
       }
-      group_lds[wave][lane] = first + (second == kNegInf ? 0.0f : second);
     }
-    wave_lds_fence();
+    const float mine = first + (second == kNegInf ? 0.0f : second);
     // A group is kept if fewer than top_groups come before it: larger ones, or
     // as large ones of a lower index.
-    bool kept = false;
-    if (static_cast<uint32_t>(lane) < groups) {
-      const float mine = group_lds[wave][lane];
-      uint32_t before = 0;
-      for (uint32_t g = 0; g < groups; ++g) {
-        const float other = group_lds[wave][g];
-        before += other > mine || (other == mine && g < static_cast<uint32_t>(lane));
-      }
-      kept = before < top_groups;
+    uint32_t before = 0;
+    for (uint32_t g = 0; g < groups; ++g) {
+      const float other = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), static_cast<int>(g)));
+      before += other > mine || (other == mine && g < static_cast<uint32_t>(lane));
     }
+    const bool kept = static_cast<uint32_t>(lane) < groups && before < top_groups;
     const uint64_t mask = __ballot(kept);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -135,11 +141,11 @@ __global__ void __launch_bounds__(256)
         if (lane == winner) value[i] = kNegInf;
       }
     }
-    const int expert = __shfl(lane * V + at, winner, 64);
-    s = __shfl(s, winner, 64);
+    const int expert = __builtin_amdgcn_readlane(lane * V + at, winner);
+    const int bits = __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), winner);
     if (lane == static_cast<int>(j)) {
       mine = expert;
-      mine_score = s;
+      mine_score = __builtin_bit_cast(float, bits);
     }
   }
   float weight = mine_score;
@@ -194,13 +200,19 @@ __global__ void __launch_bounds__(256)
   wave_lds_fence();
   if (expert >= 0) lds[wave][expert] = d;
   wave_lds_fence();
+  LaneValues<T, V> out;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const uint32_t e = lane * V + i;
-    const float ds = lds[wave][e];
-    if (e < experts)
-      d_logits[static_cast<uint64_t>(token) * experts + e] =
-          static_cast<T>(softmax ? score[i] * (ds - common) : ds * score[i] * (1.0f - score[i]));
+    const float ds = lds[wave][lane * V + i];
+    out.at[i] = static_cast<T>(softmax ? score[i] * (ds - common) : ds * score[i] * (1.0f - score[i]));
+  }
+  T* to = d_logits + static_cast<uint64_t>(token) * experts + lane * V;
+  if (static_cast<uint32_t>(lane) * V + V <= experts) {
+    *reinterpret_cast<LaneValues<T, V>*>(to) = out;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane * V + i < static_cast<int>(experts)) to[i] = out.at[i];
   }
 }
 
@@ -220,22 +232,40 @@ __device__ __forceinline__ uint64_t same_expert(int expert, uint32_t bits) {
   return expert < 0 ? 0 : mask;
 }
 
-__device__ __forceinline__ int load_expert(const int32_t* __restrict__ chosen, uint32_t i, uint32_t entries,
-                                           uint32_t experts) {
-  if (i >= entries) return -1;
-  const int e = chosen[i];
-  return static_cast<uint32_t>(e) < experts ? e : -1;
-}
+// A wave's entries: `rounds` of 64 consecutive ones from `base` on.
+struct DispatchEntries {
+  uint32_t base;
+  int rounds;
+  int expert[kDispatchRounds];     // -1 without one
+  uint64_t same[kDispatchRounds];  // lanes of the round with the same expert
+};
 
-// Adds this wave's entries of each expert to its own row of the histogram.
-__device__ __forceinline__ void count_entries(const int32_t* __restrict__ chosen, uint32_t base, uint32_t entries,
-                                              uint32_t experts, uint32_t bits, uint32_t* hist, int lane) {
+// Loads a wave's entries and adds them to its own row of the histogram.
+__device__ __forceinline__ void count_entries(const int32_t* __restrict__ chosen, uint32_t entries, uint32_t experts,
+                                              uint32_t bits, int wave, int lane, DispatchEntries& mine,
+                                              uint32_t* hist) {
+  // A launch of one workgroup shares few entries out over its waves.
+  const uint32_t here = min(kDispatchItems, entries - min(entries, blockIdx.x * kDispatchItems));
+  mine.rounds = static_cast<int>((here + kDispatchWaves * 64 - 1) / (kDispatchWaves * 64));
+  mine.base = blockIdx.x * kDispatchItems + wave * mine.rounds * 64;
+#pragma unroll
   for (int r = 0; r < kDispatchRounds; ++r) {
-    const int e = load_expert(chosen, base + r * 64 + lane, entries, experts);
-    const uint64_t same = same_expert(e, bits);
-    if (same && __builtin_ctzll(same) == lane) hist[e] += __builtin_popcountll(same);
+    const uint32_t i = mine.base + r * 64 + lane;
+    const int e = r < mine.rounds && i < entries ? chosen[i] : -1;
+    mine.expert[r] = static_cast<uint32_t>(e) < experts ? e : -1;
+  }
+  for (uint32_t i = threadIdx.x; i < kDispatchWaves * experts; i += 1024) hist[i] = 0;
+  __syncthreads();
+  uint32_t* row = hist + wave * experts;
+#pragma unroll
+  for (int r = 0; r < kDispatchRounds; ++r) {
+    mine.same[r] = 0;
+    if (r >= mine.rounds) continue;
+    const uint64_t same = mine.same[r] = same_expert(mine.expert[r], bits);
+    if (same && __builtin_ctzll(same) == lane) row[mine.expert[r]] += __builtin_popcountll(same);
     wave_lds_fence();
   }
+  __syncthreads();
 }
 
 // Counts of each expert's entries, one row a workgroup.
@@ -243,14 +273,11 @@ __global__ void __launch_bounds__(1024)
     dispatch_count_kernel(const int32_t* __restrict__ chosen, uint32_t entries, uint32_t experts, uint32_t bits,
                           uint32_t* __restrict__ counts) {
   extern __shared__ uint32_t hist[];  // [waves][experts]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (uint32_t i = threadIdx.x; i < kDispatchWaves * experts; i += 1024) hist[i] = 0;
-  __syncthreads();
-  count_entries(chosen, blockIdx.x * kDispatchItems + wave * kDispatchRounds * 64, entries, experts, bits,
-                hist + wave * experts, lane);
-  __syncthreads();
+  DispatchEntries mine;
+  count_entries(chosen, entries, experts, bits, threadIdx.x >> 6, threadIdx.x & 63, mine, hist);
   for (uint32_t e = threadIdx.x; e < experts; e += 1024) {
     uint32_t total = 0;
+#pragma unroll
     for (int w = 0; w < kDispatchWaves; ++w) total += hist[w * experts + e];
     counts[static_cast<uint64_t>(blockIdx.x) * experts + e] = total;
   }
@@ -266,24 +293,22 @@ __global__ void __launch_bounds__(1024)
   extern __shared__ uint32_t hist[];  // [waves][experts]
   __shared__ uint32_t wave_total[kDispatchWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t base = blockIdx.x * kDispatchItems + wave * kDispatchRounds * 64;
-  for (uint32_t i = threadIdx.x; i < kDispatchWaves * experts; i += 1024) hist[i] = 0;
-  __syncthreads();
-  count_entries(chosen, base, entries, experts, bits, hist + wave * experts, lane);
-  __syncthreads();
   // Thread e: the expert's entries in all workgroups, and in earlier ones.
   const uint32_t e = threadIdx.x;
   uint32_t total = 0, before = 0;
-  if (e < experts) {
-    if (counts) {
-      for (uint32_t b = 0; b < gridDim.x; ++b) {
-        const uint32_t c = counts[static_cast<uint64_t>(b) * experts + e];
-        before += b < blockIdx.x ? c : 0;
-        total += c;
-      }
-    } else {
-      for (int w = 0; w < kDispatchWaves; ++w) total += hist[w * experts + e];
+  if (e < experts && counts) {
+#pragma unroll 16  // loads in flight
+    for (uint32_t b = 0; b < gridDim.x; ++b) {
+      const uint32_t c = counts[static_cast<uint64_t>(b) * experts + e];
+      before += b < blockIdx.x ? c : 0;
+      total += c;
     }
+  }
+  DispatchEntries mine;
+  count_entries(chosen, entries, experts, bits, wave, lane, mine, hist);
+  if (e < experts && !counts) {
+#pragma unroll
+    for (int w = 0; w < kDispatchWaves; ++w) total += hist[w * experts + e];
   }
   uint32_t scan = total;
 #pragma unroll
@@ -294,6 +319,7 @@ __global__ void __launch_bounds__(1024)
   if (lane == 63) wave_total[wave] = scan;
   __syncthreads();
   uint32_t all = 0, start = scan - total;
+#pragma unroll
   for (int w = 0; w < kDispatchWaves; ++w) {
     if (w < wave) start += wave_total[w];
     all += wave_total[w];
@@ -301,6 +327,7 @@ __global__ void __launch_bounds__(1024)
   if (e < experts) {
     if (blockIdx.x == 0) offsets[e] = static_cast<int32_t>(start);
     uint32_t at = start + before;
+#pragma unroll
     for (int w = 0; w < kDispatchWaves; ++w) {
       const uint32_t c = hist[w * experts + e];
       hist[w * experts + e] = at;
@@ -310,15 +337,16 @@ __global__ void __launch_bounds__(1024)
   if (blockIdx.x == 0 && threadIdx.x == 0) offsets[experts] = static_cast<int32_t>(all);
   __syncthreads();
   uint32_t* next = hist + wave * experts;
+#pragma unroll
   for (int r = 0; r < kDispatchRounds; ++r) {
-    const uint32_t i = base + r * 64 + lane;
-    const int expert = load_expert(chosen, i, entries, experts);
-    const uint64_t same = same_expert(expert, bits);
+    if (r >= mine.rounds) continue;
+    const uint32_t i = mine.base + r * 64 + lane;
+    const uint64_t same = mine.same[r];
     const uint32_t rank = __builtin_popcountll(same & ((uint64_t{1} << lane) - 1));
     uint32_t slot = 0;
-    if (same) slot = next[expert] + rank;
+    if (same) slot = next[mine.expert[r]] + rank;
     wave_lds_fence();
-    if (same && rank == 0) next[expert] += __builtin_popcountll(same);
+    if (same && rank == 0) next[mine.expert[r]] += __builtin_popcountll(same);
     wave_lds_fence();
     if (i < entries) {
       slots[i] = same ? static_cast<int32_t>(slot) : -1;
@@ -330,63 +358,105 @@ __global__ void __launch_bounds__(1024)
 
 // ---- combine -----------------------------------------------------------------
 
+// Rows of one token's slots whose loads are in flight together.
+constexpr int kCombineRows = 8;
+
 // out[t] = sum over j of weights[t][j] * y[slots[t][j]], in the order of j. One
 // wave a token and 512 columns, eight a lane.
-template <class T>
+template <class T, bool STREAM>
 __global__ void __launch_bounds__(256)
     combine_kernel(const T* __restrict__ y, uint32_t y_rows, const int32_t* __restrict__ slots,
                    const float* __restrict__ weights, T* __restrict__ out, uint32_t tokens, uint32_t top, uint32_t n) {
   const uint32_t strips = (n + 511) / 512;
-  const uint64_t task = blockIdx.x * uint64_t{4} + (threadIdx.x >> 6);
-  const uint64_t token = task / strips;
+  const uint32_t task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const uint32_t token = task / strips;
   if (token >= tokens) return;
-  const uint32_t column = static_cast<uint32_t>(task % strips) * 512 + (threadIdx.x & 63) * 8;
+  const uint32_t column = task % strips * 512 + (threadIdx.x & 63) * 8;
+  // Lane j holds entry j: the loads of all slots and weights go out together.
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t my_slot = ~0u;
+  float my_weight = 0.0f;
+  if (lane < top) {
+    my_slot = static_cast<uint32_t>(slots[uint64_t{token} * top + lane]);
+    my_weight = weights[uint64_t{token} * top + lane];
+  }
   if (column >= n) return;
   const int count = static_cast<int>(min(8u, n - column));
   float sum[8] = {};
-  for (uint32_t j = 0; j < top; ++j) {
-    const uint32_t slot = static_cast<uint32_t>(slots[token * top + j]);
-    if (slot >= y_rows) continue;
-    const float weight = weights[token * top + j];
-    Raw8<T> raw;
-    raw.load(y + uint64_t{slot} * n + column, count);
+  for (uint32_t j0 = 0; j0 < top; j0 += kCombineRows) {
+    Raw8<T> raw[kCombineRows];
+    uint32_t slot[kCombineRows];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] = fmaf(weight, raw[i], sum[i]);
+    for (int j = 0; j < kCombineRows; ++j) {
+      slot[j] = j0 + j < top ? __builtin_amdgcn_readlane(my_slot, j0 + j) : ~0u;
+      if (slot[j] < y_rows) raw[j].load(y + uint64_t{slot[j]} * n + column, count);
+    }
+#pragma unroll
+    for (int j = 0; j < kCombineRows; ++j) {
+      if (slot[j] >= y_rows) continue;
+      const float weight = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, my_weight), j0 + j));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = fmaf(weight, raw[j][i], sum[i]);
+    }
   }
-  store8(out + token * n + column, sum, count);
+  store8<STREAM>(out + uint64_t{token} * n + column, sum, count);
 }
 
+constexpr int kGradientRows = 4;
+
 // d_y[slots[t][j]] = weights[t][j] * d_out[t] and d_weights[t][j] = the product
-// of d_out[t] and y[slots[t][j]]. One wave a token and j.
-template <class T>
+// of d_out[t] and y[slots[t][j]]. One workgroup a token, 2048 columns at a time;
+// a part of d_out serves kGradientRows slots.
+template <class T, bool STREAM>
 __global__ void __launch_bounds__(256)
     combine_backward_kernel(const T* __restrict__ d_out, const T* __restrict__ y, uint32_t y_rows,
                             const int32_t* __restrict__ slots, const float* __restrict__ weights, T* __restrict__ d_y,
-                            float* __restrict__ d_weights, uint32_t tokens, uint32_t top, uint32_t n) {
-  const uint64_t task = blockIdx.x * uint64_t{4} + (threadIdx.x >> 6);
-  if (task >= uint64_t{tokens} * top) return;
-  const int lane = threadIdx.x & 63;
-  const uint64_t token = task / top;
-  const uint32_t slot = static_cast<uint32_t>(slots[task]);
-  float dot = 0.0f;
-  if (slot < y_rows) {
-    const float weight = weights[task];
-    for (uint32_t column = lane * 8; column < n; column += 512) {
-      const int count = static_cast<int>(min(8u, n - column));
-      Raw8<T> g, v;
-      g.load(d_out + token * n + column, count);
-      v.load(y + uint64_t{slot} * n + column, count);
-      float d[8];
+                            float* __restrict__ d_weights, uint32_t top, uint32_t n) {
+  __shared__ float parts[4][kGradientRows];
+  const uint32_t token = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (uint32_t j0 = 0; j0 < top; j0 += kGradientRows) {
+    const uint64_t entry = uint64_t{token} * top + j0;
+    const uint32_t rows = min(static_cast<uint32_t>(kGradientRows), top - j0);
+    uint32_t slot[kGradientRows];
+    float weight[kGradientRows], dot[kGradientRows];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dot = fmaf(g[i], v[i], dot);
-        d[i] = weight * g[i];
-      }
-      store8(d_y + uint64_t{slot} * n + column, d, count);
+    for (int j = 0; j < kGradientRows; ++j) {
+      slot[j] = j < static_cast<int>(rows) ? static_cast<uint32_t>(slots[entry + j]) : ~0u;
+      weight[j] = slot[j] < y_rows ? weights[entry + j] : 0.0f;
+      dot[j] = 0.0f;
     }
+    for (uint32_t column = threadIdx.x * 8; column < n; column += 2048) {
+      const int count = static_cast<int>(min(8u, n - column));
+      Raw8<T> g, v[kGradientRows];
+      g.load(d_out + uint64_t{token} * n + column, count);
+#pragma unroll
+      for (int j = 0; j < kGradientRows; ++j)
+        if (slot[j] < y_rows) v[j].load(y + uint64_t{slot[j]} * n + column, count);
+#pragma unroll
+      for (int j = 0; j < kGradientRows; ++j) {
+        if (slot[j] >= y_rows) continue;
+        float d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          dot[j] = fmaf(g[i], v[j][i], dot[j]);
+          d[i] = weight[j] * g[i];
+        }
+        store8<STREAM>(d_y + uint64_t{slot[j]} * n + column, d, count);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kGradientRows; ++j) {
+      const float sum = wave_add(dot[j]);
+      if (lane == 0) parts[wave][j] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < rows)
+      d_weights[entry + threadIdx.x] = (parts[0][threadIdx.x] + parts[1][threadIdx.x]) +
+                                       (parts[2][threadIdx.x] + parts[3][threadIdx.x]);
+    __syncthreads();
   }
-  dot = wave_add(dot);
-  if (lane == 0) d_weights[task] = dot;
 }
 
 #define MB_ROUTE_REGISTER_V(T, NAME, V)                                            \
@@ -398,8 +468,10 @@ __global__ void __launch_bounds__(256)
   MB_ROUTE_REGISTER_V(T, NAME, 4);                              \
   MB_ROUTE_REGISTER_V(T, NAME, 8);                              \
   MB_ROUTE_REGISTER_V(T, NAME, 16);                             \
-  MB_REGISTER_KERNEL("combine_" NAME, combine_kernel<T>);       \
-  MB_REGISTER_KERNEL("combine_backward_" NAME, combine_backward_kernel<T>)
+  MB_REGISTER_KERNEL("combine_" NAME, (combine_kernel<T, false>));                            \
+  MB_REGISTER_KERNEL("combine_" NAME "_stream", (combine_kernel<T, true>));                   \
+  MB_REGISTER_KERNEL("combine_backward_" NAME, (combine_backward_kernel<T, false>));          \
+  MB_REGISTER_KERNEL("combine_backward_" NAME "_stream", (combine_backward_kernel<T, true>))
 MB_ROUTE_REGISTER(float, "f32");
 MB_ROUTE_REGISTER(_Float16, "f16");
 MB_ROUTE_REGISTER(__bf16, "bf16");
@@ -558,8 +630,8 @@ static int check_combine(const char* entry, int dtype, const void* y, uint64_t y
   if (tokens > (1u << 24) || y_rows > (1u << 24) || n > (1u << 20) || tokens * ((n + 511) / 512) > (1u << 25))
     return mb::fail(MB_ERR_UNSUPPORTED, "%s: %llu tokens of %llu columns exceed one launch", entry,
                     (unsigned long long)tokens, (unsigned long long)n);
-  if (tokens * n == 0) return MB_OK;
-  if (y_bytes < y_rows * n * item || (y == nullptr && y_rows))
+  if (tokens == 0) return MB_OK;
+  if (y_bytes < y_rows * n * item || (y == nullptr && y_rows * n))
     return mb::fail(MB_ERR_INVALID, "%s: y is NULL or too small for %llu x %llu", entry, (unsigned long long)y_rows,
                     (unsigned long long)n);
   if (!mb::aligned(y, item)) return mb::fail(MB_ERR_ALIGNMENT, "%s: y must lie on its elements' %u bytes", entry, item);
@@ -591,9 +663,18 @@ int mb_combine(int dtype, const void* y, uint64_t y_bytes, uint32_t y_rows, cons
   if (tokens == 0 || n == 0) return MB_OK;
   if (int rc = check_rows_out(entry, "out", out, out_bytes, tokens, n, mb::elem_bytes(dtype))) return rc;
   const uint64_t tasks = uint64_t{tokens} * ((n + 511) / 512);
-  MB_FOR_DTYPE(dtype, (mb::combine_kernel<T><<<dim3(static_cast<uint32_t>((tasks + 3) / 4)), dim3(256), 0,
-                                               static_cast<hipStream_t>(stream)>>>(
-                          static_cast<const T*>(y), y_rows, slots, weights, static_cast<T*>(out), tokens, top, n)));
+  auto launch = [&](auto kernel, auto t) {
+    using T = decltype(t);
+    kernel<<<dim3(static_cast<uint32_t>((tasks + 3) / 4)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const T*>(y), y_rows, slots, weights, static_cast<T*>(out), tokens, top, n);
+  };
+  const bool streamed = mb::streams(uint64_t{tokens} * n * mb::elem_bytes(dtype));
+  MB_FOR_DTYPE(dtype, {
+    if (streamed)
+      launch(mb::combine_kernel<T, true>, T());
+    else
+      launch(mb::combine_kernel<T, false>, T());
+  });
   return mb::launch_status("combine");
 }
 
@@ -606,16 +687,23 @@ int mb_combine_backward(int dtype, const void* d_out, uint64_t d_out_bytes, cons
                              n))
     return rc;
   const uint32_t item = mb::elem_bytes(dtype);
-  const uint64_t tasks = uint64_t{tokens} * top;
-  if (tasks > (1u << 24)) return mb::fail(MB_ERR_UNSUPPORTED, "%s: at most %u entries", entry, 1u << 24);
   if (tokens == 0) return MB_OK;
   if (int rc = check_rows_out(entry, "d_out", d_out, d_out_bytes, tokens, n, item)) return rc;
   if (int rc = check_rows_out(entry, "d_y", d_y, d_y_bytes, y_rows, n, item)) return rc;
   if (int rc = check_rows_out(entry, "d_weights", d_weights, d_weights_bytes, tokens, top, 4)) return rc;
-  MB_FOR_DTYPE(dtype, (mb::combine_backward_kernel<T><<<dim3(static_cast<uint32_t>((tasks + 3) / 4)), dim3(256), 0,
-                                                        static_cast<hipStream_t>(stream)>>>(
-                          static_cast<const T*>(d_out), static_cast<const T*>(y), y_rows, slots, weights,
-                          static_cast<T*>(d_y), d_weights, tokens, top, n)));
+  auto launch = [&](auto kernel, auto t) {
+    using T = decltype(t);
+    kernel<<<dim3(tokens), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+        static_cast<const T*>(d_out), static_cast<const T*>(y), y_rows, slots, weights, static_cast<T*>(d_y),
+        d_weights, top, n);
+  };
+  const bool streamed = mb::streams(uint64_t{y_rows} * n * item);
+  MB_FOR_DTYPE(dtype, {
+    if (streamed)
+      launch(mb::combine_backward_kernel<T, true>, T());
+    else
+      launch(mb::combine_backward_kernel<T, false>, T());
+  });
   return mb::launch_status("combine_backward");
 }
 
