@@ -7,17 +7,10 @@
 #include "mb_gemm_ring.h"
 #include "mb_mx.h"
 #include "mb_mx_device.h"
+#include "mb_mx_stream.h"
 
 namespace mb {
 namespace {
-
-// Rows first .. last - 1 of expert `e`; all of them without offsets. Clamped, so
-// that whatever `offsets` holds, no row outside 0 .. rows - 1 is touched.
-__device__ __forceinline__ void expert_rows(const int32_t* __restrict__ offsets, uint32_t e, int rows, int& first,
-                                            int& last) {
-  first = offsets ? max(0, min(offsets[e], rows)) : 0;
-  last = offsets ? max(first, min(offsets[e + 1], rows)) : rows;
-}
 
 // One wave computes 16 columns of 16 rows at a time with
 // v_mfma_scale_f32_16x16x128_f8f6f4: W's rows as the instruction's rows, X's as
@@ -374,6 +367,13 @@ void launch_ring(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const ui
       x, sx, w, sw, static_cast<T*>(y), rows, n, k, offsets, experts, band);
 }
 
+template <class T>
+void launch_stream(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const uint8_t* sw, void* y, int rows, int n,
+                   int k, const int32_t* offsets, int experts, uint32_t grid, int band, hipStream_t stream) {
+  mx_product_stream_kernel<T, 256, 128, 3><<<dim3(grid < 256 ? grid : 256), dim3(256), 0, stream>>>(
+      x, sx, w, sw, static_cast<T*>(y), rows, n, k, offsets, experts, band);
+}
+
 // A ring tile: BM features of BN rows.
 struct ProductKernel {
   int features, rows;
@@ -414,6 +414,8 @@ MB_FEW_REGISTER(__bf16, "bf16");
 MB_PRODUCT_REGISTER(float, "f32");
 MB_PRODUCT_REGISTER(_Float16, "f16");
 MB_PRODUCT_REGISTER(__bf16, "bf16");
+MB_REGISTER_KERNEL("mx_product_f16_256x128_stream", (mx_product_stream_kernel<_Float16, 256, 128, 3>));
+MB_REGISTER_KERNEL("mx_product_bf16_256x128_stream", (mx_product_stream_kernel<__bf16, 256, 128, 3>));
 
 constexpr uint32_t kMostExperts = 4096;
 
@@ -528,7 +530,11 @@ int launch_product(int dtype, const void* x_codes, const void* sx, const void* w
     }
     if (best) {
       const uint64_t grid = most_row_tiles(rows, experts, best->rows) * ((n + best->features - 1) / best->features);
-      best->launch[dtype](x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
+      ProductLauncher launch = best->launch[dtype];
+      if (best->features == 256 && dtype != MB_DTYPE_F32 && steps > 3 && experts <= kStreamExperts && n % 8 == 0 &&
+          aligned(y, 16))
+        launch = dtype == MB_DTYPE_F16 ? launch_stream<_Float16> : launch_stream<__bf16>;
+      launch(x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
                           offsets, static_cast<int>(experts), static_cast<uint32_t>((grid + 7) / 8 * 8), best->band,
                           stream);
       return launch_status("mx_product_ring");
