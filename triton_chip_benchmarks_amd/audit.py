@@ -40,7 +40,7 @@ _ELEMENT_TYPE = {"f": "f32", "DF16_": "f16", "DF16b": "bf16"}
 _ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)E")
 _LAYER_RE = re.compile(r"(mx_quantize|mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
                        r"_kernelI(f|DF16_|DF16b)(?:Lb([01])E)?E")
-_PRODUCT_RING_RE = re.compile(r"mx_product_(ring|stream)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi(\d+)EE")
+_PRODUCT_RING_RE = re.compile(r"mx_product_(ring|stream)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi\d+EE")
 _FEW_RE = re.compile(r"mx_few_kernelI(h|f|DF16_|DF16b)(S\d*_|T_|f|DF16_|DF16b)?Li(\d+)ELi(\d+)EE")
 _DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
 _VECTOR_RE = re.compile(r"vector_(\w+?)_kernelILi(\d+)E")
@@ -98,9 +98,8 @@ def registered_name(symbol: str) -> str | None:
         return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}{'_stream' if match.group(3) == '1' else ''}"
     match = _PRODUCT_RING_RE.search(symbol)
     if match:
-        kind, dtype, features, rows, stages = match.groups()
-        form = "_stream" if kind == "stream" else "_pair" if (features, stages) == ("128", "2") else ""
-        return f"mx_product_{_ELEMENT_TYPE[dtype]}_{features}x{rows}{form}"
+        kind, dtype, features, rows = match.groups()
+        return f"mx_product_{_ELEMENT_TYPE[dtype]}_{features}x{rows}{'_stream' if kind == 'stream' else ''}"
     match = _FEW_RE.search(symbol)
     if match:
         x, y, blocks, split = match.groups()

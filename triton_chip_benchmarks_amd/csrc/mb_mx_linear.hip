@@ -3,7 +3,6 @@
 #include <type_traits>
 
 #include "mb_elem.h"
-#include "mb_gemm_host.h"
 #include "mb_gemm_ring.h"
 #include "mb_mx.h"
 #include "mb_mx_device.h"
@@ -367,40 +366,60 @@ void launch_ring(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const ui
       x, sx, w, sw, static_cast<T*>(y), rows, n, k, offsets, experts, band);
 }
 
-template <class T>
+template <class T, int BM, int BN, int STAGES>
 void launch_stream(const uint8_t* x, const uint8_t* sx, const uint8_t* w, const uint8_t* sw, void* y, int rows, int n,
                    int k, const int32_t* offsets, int experts, uint32_t grid, int band, hipStream_t stream) {
-  mx_product_stream_kernel<T, 256, 128, 3><<<dim3(grid < 256 ? grid : 256), dim3(256), 0, stream>>>(
+  constexpr uint32_t kPlaces = 256 * RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT;
+  mx_product_stream_kernel<T, BM, BN, STAGES><<<dim3(grid < kPlaces ? grid : kPlaces), dim3(256), 0, stream>>>(
       x, sx, w, sw, static_cast<T*>(y), rows, n, k, offsets, experts, band);
 }
 
-// A ring tile: BM features of BN rows.
+// What a launch takes, in microseconds: `launch` once; for every round of its
+// workgroups `tile`, `ragged` more where the rows of Y are not on 16 bytes, and
+// for every 256 elements of K from `step_empty` to `step_full` with the filled
+// share of the round (the L2s and the power limit slow a step down as more CUs
+// run).
+struct ProductCost {
+  float launch, tile, ragged, step_empty, step_full;
+};
+
+// A kernel of BM features by BN rows a tile.
 struct ProductKernel {
   int features, rows;
+  int stages;    // of a persistent kernel, which K must exceed; 0 for the others
   int band;      // row tiles that share their weight's panels in an XCD's L2
   int resident;  // workgroups a CU holds
-  GemmCost cost;
+  ProductCost cost;
   ProductLauncher launch[3];  // by MB_DTYPE_*
 };
-#define MB_PRODUCT(BM, BN, STAGES, BAND, COST)                                                               \
-  ProductKernel {                                                                                            \
-    BM, BN, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, COST, {                                     \
-      launch_ring<float, BM, BN, STAGES>, launch_ring<_Float16, BM, BN, STAGES>, launch_ring<__bf16, BM, BN, STAGES> \
-    }                                                                                                        \
+#define MB_PRODUCT(KIND, BM, BN, STAGES, PERSISTENT, BAND, ...)                                  \
+  ProductKernel {                                                                                \
+    BM, BN, PERSISTENT, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, {__VA_ARGS__}, {    \
+      launch_##KIND<float, BM, BN, STAGES>, launch_##KIND<_Float16, BM, BN, STAGES>,             \
+          launch_##KIND<__bf16, BM, BN, STAGES>                                                  \
+    }                                                                                            \
   }
+// Fitted to 582 launches on an MI355X (17 to 32768 rows, n and K from 64 to 8192,
+// one weight or 8 to 256 experts of uneven popularity, half of the n odd): the
+// cheapest estimate costs 1.3% over the fastest of the five on average, over 10%
+// in one launch of 26, 27% at most. Twelve kernels were measured; these five's
+// best is 0.8% over the twelve's, the ring's 256x128, two 128x128 and 64x64 alone
+// 6%.
 const ProductKernel kProductKernels[] = {
-    MB_PRODUCT(256, 128, 3, 4, kCostMx256x128),
-    MB_PRODUCT(128, 128, 4, 6, kCostMx128),
-    MB_PRODUCT(128, 128, 2, 8, kCostMx128Pair),
-    MB_PRODUCT(64, 64, 3, 8, kCostMx64),
+    MB_PRODUCT(ring, 128, 128, 2, 0, 8, 1.62f, 3.71f, 0.40f, 0.349f, 1.485f),
+    MB_PRODUCT(ring, 64, 64, 3, 0, 8, 2.28f, 3.18f, 0.19f, 0.083f, 0.513f),
+    MB_PRODUCT(stream, 256, 128, 3, 3, 4, 4.70f, 2.38f, 1.47f, 0.510f, 1.380f),
+    MB_PRODUCT(stream, 128, 64, 3, 3, 8, 3.73f, 1.39f, 0.45f, 0.233f, 1.085f),
+    MB_PRODUCT(stream, 64, 64, 2, 2, 8, 3.36f, 1.74f, 0.34f, 0.172f, 1.678f),
 };
 
 #define MB_PRODUCT_REGISTER(T, NAME)                                                                        \
   MB_REGISTER_KERNEL("mx_product_" NAME, mx_product_kernel<T>);                                             \
-  MB_REGISTER_KERNEL("mx_product_" NAME "_256x128", (mx_product_ring_kernel<T, 256, 128, 3>));              \
-  MB_REGISTER_KERNEL("mx_product_" NAME "_128x128", (mx_product_ring_kernel<T, 128, 128, 4>));              \
-  MB_REGISTER_KERNEL("mx_product_" NAME "_128x128_pair", (mx_product_ring_kernel<T, 128, 128, 2>));         \
-  MB_REGISTER_KERNEL("mx_product_" NAME "_64x64", (mx_product_ring_kernel<T, 64, 64, 3>))
+  MB_REGISTER_KERNEL("mx_product_" NAME "_128x128", (mx_product_ring_kernel<T, 128, 128, 2>));              \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_64x64", (mx_product_ring_kernel<T, 64, 64, 3>));                  \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_256x128_stream", (mx_product_stream_kernel<T, 256, 128, 3>));     \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_128x64_stream", (mx_product_stream_kernel<T, 128, 64, 3>));       \
+  MB_REGISTER_KERNEL("mx_product_" NAME "_64x64_stream", (mx_product_stream_kernel<T, 64, 64, 2>))
 #define MB_FEW_REGISTER_SPLIT(T, NAME, FB, SPLIT, SIZE)                                             \
   MB_REGISTER_KERNEL("mx_linear_few_" NAME "_" SIZE, (mx_few_kernel<T, T, FB, SPLIT>));            \
   MB_REGISTER_KERNEL("mx_product_few_" NAME "_" SIZE, (mx_few_kernel<uint8_t, T, FB, SPLIT>))
@@ -414,8 +433,6 @@ MB_FEW_REGISTER(__bf16, "bf16");
 MB_PRODUCT_REGISTER(float, "f32");
 MB_PRODUCT_REGISTER(_Float16, "f16");
 MB_PRODUCT_REGISTER(__bf16, "bf16");
-MB_REGISTER_KERNEL("mx_product_f16_256x128_stream", (mx_product_stream_kernel<_Float16, 256, 128, 3>));
-MB_REGISTER_KERNEL("mx_product_bf16_256x128_stream", (mx_product_stream_kernel<__bf16, 256, 128, 3>));
 
 constexpr uint32_t kMostExperts = 4096;
 
@@ -460,15 +477,18 @@ double mean_row_tiles(uint32_t rows, uint32_t experts, int tile) {
   return experts * (each >= tile ? each / tile + 0.5 : each >= 1 ? 1.0 : each);
 }
 
-// Estimated microseconds of a launch (see GemmCost).
-double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint32_t steps, uint32_t experts) {
+// Estimated microseconds of a launch (see ProductCost).
+double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint32_t steps, uint32_t experts,
+                    bool ragged) {
   const double tiles = mean_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
   const double round = 256.0 * kernel.resident, whole = static_cast<double>(static_cast<uint64_t>(tiles / round));
   const double rest = tiles / round - whole;
+  const ProductCost& cost = kernel.cost;
   auto one = [&](double filled) {
-    return kernel.cost.tile + steps * (kernel.cost.step_empty + (kernel.cost.step_full - kernel.cost.step_empty) * filled);
+    return cost.tile + (ragged ? cost.ragged : 0.0f) +
+           steps * (cost.step_empty + (cost.step_full - cost.step_empty) * filled);
   };
-  return whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
+  return cost.launch + whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
 }
 
 // Whether mx_few_kernel takes a call: up to 16 rows of one weight, up to two an
@@ -522,22 +542,20 @@ int launch_product(int dtype, const void* x_codes, const void* sx, const void* w
   if (steps * scale_rows * 8 <= 0x7fffffffu) {
     const ProductKernel* best = nullptr;
     double best_cost = 0;
+    const bool ragged = uint64_t{n} * elem_bytes(dtype) % 16 != 0;
+    uint64_t best_grid = 0;
     for (const ProductKernel& kernel : kProductKernels) {
       const uint64_t grid = most_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
       if (grid > 0xffffff) continue;
-      const double cost = product_cost(kernel, rows, n, steps, experts);
-      if (best == nullptr || cost < best_cost) best = &kernel, best_cost = cost;
+      if (kernel.stages && (steps <= static_cast<uint32_t>(kernel.stages) || experts > kStreamExperts)) continue;
+      const double cost = product_cost(kernel, rows, n, steps, experts, ragged);
+      if (best == nullptr || cost < best_cost) best = &kernel, best_cost = cost, best_grid = grid;
     }
     if (best) {
-      const uint64_t grid = most_row_tiles(rows, experts, best->rows) * ((n + best->features - 1) / best->features);
-      ProductLauncher launch = best->launch[dtype];
-      if (best->features == 256 && dtype != MB_DTYPE_F32 && steps > 3 && experts <= kStreamExperts && n % 8 == 0 &&
-          aligned(y, 16))
-        launch = dtype == MB_DTYPE_F16 ? launch_stream<_Float16> : launch_stream<__bf16>;
-      launch(x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
-                          offsets, static_cast<int>(experts), static_cast<uint32_t>((grid + 7) / 8 * 8), best->band,
-                          stream);
-      return launch_status("mx_product_ring");
+      best->launch[dtype](x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
+                          offsets, static_cast<int>(experts), static_cast<uint32_t>((best_grid + 7) / 8 * 8),
+                          best->band, stream);
+      return launch_status(best->stages ? "mx_product_stream" : "mx_product_ring");
     }
   }
   const uint32_t tiles = (rows / experts + 15) / 16;

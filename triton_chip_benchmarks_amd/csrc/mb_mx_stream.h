@@ -72,8 +72,9 @@ struct RowTiles {
   }
 };
 
-// Y = X . W^T with 256 features of 128 rows a tile, as mx_product_ring_kernel,
-// one workgroup a CU for all of its tiles. That kernel's workgroup spends 5.9 us
+// Y = X . W^T with BM features of BN rows a tile, as mx_product_ring_kernel, a
+// workgroup for all the tiles of its place on a CU. That kernel's workgroup of
+// 256x128 spends 5.9 us
 // beside the 16 of a K of 4096: it waits for its first operands, and nothing else
 // runs on the CU while it stores. Here the DMAs run STAGES steps ahead of the
 // products over the ends of tiles, and a tile is stored from its registers, whose
@@ -84,8 +85,7 @@ struct RowTiles {
 // issued two steps before, after which one step's DMAs and, in the first two
 // steps of a tile, the stores of the tile before have been issued.
 //
-// n * sizeof(T) is a multiple of 16, y lies on 16 bytes, K has more than STAGES
-// steps, there are at most kStreamExperts experts.
+// K has more than STAGES steps, there are at most kStreamExperts experts.
 template <class T, int BM, int BN, int STAGES>
 __global__ void __launch_bounds__(256)
     mx_product_stream_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ sx,
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(256)
   using Tile = RingTile<Op, BM, BN, STAGES>;
   constexpr int ROWB = Tile::ROWB, FM = Tile::FM, FN = Tile::FN, CH = Tile::CHUNKS;
   constexpr int STORES = FM * FN * 16 * sizeof(T) / 16;  // of a lane and tile
-  static_assert(sizeof(T) == 2 && STAGES == 3 && (STAGES - 2) * Tile::DMAS + STORES < 64, "vmcnt counts DMAs and stores in flight");
+  static_assert((STAGES - 2) * Tile::DMAS + STORES < 64, "vmcnt counts DMAs and stores in flight");
   __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * Tile::STAGE];
   if (k < 0) lds[threadIdx.x] = 0;  // keeps DMA-written reads live; never executed
   const int lane = threadIdx.x & 63;
@@ -228,41 +228,73 @@ __global__ void __launch_bounds__(256)
       for (int j = 0; j < FN; ++j) acc[i][j] = typename Op::Acc{};
   };
 
-  // ---- the output tile: eight features, 16 bytes, a lane and store
+  // ---- the output tile: 16 bytes a lane and store, eight (fp32: four) features
+  constexpr int PIECE = 16 / sizeof(T);
   auto store = [&](const At& at) __attribute__((always_inline)) {
     constexpr int ES = sizeof(T);
     const int width = n - at.m0;  // features of the tile inside n, at least
     const __amdgpu_buffer_rsrc_t rc = __builtin_amdgcn_make_buffer_rsrc(
         y + static_cast<int64_t>(at.n0) * n + at.m0, (short)0, ((at.live - 1) * n + min(BM, width)) * ES, kBufferWord3);
+    // put(row of Y in elements, feature, its piece) for every piece of the lane.
+    auto pieces = [&](auto&& put) __attribute__((always_inline)) {
+      auto f = [&](int row, int feature, i32x4 value) __attribute__((always_inline)) {
+        asm volatile("" : "+v"(feature));  // one piece's masks at a time: all of them exceed the SGPRs
+        put(row, feature, value);
+      };
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int row = (wn * Tile::WN + j * 32 + (lane & 31)) * n;
+      for (int j = 0; j < FN; ++j) {
+        const int row = (wn * Tile::WN + j * 32 + (lane & 31)) * n;
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int column = wm * Tile::WM + i * 32;
-        auto put = [&](i32x4 value, int feature) __attribute__((always_inline)) {
-          __builtin_amdgcn_raw_buffer_store_b128(value, rc, feature < width ? (row + feature) * ES : kOutOfRange, 0, 0);
-        };
-        // Lanes 0-31 hold features 8q .. 8q + 3 of their row, lanes 32-63 the next four of the same rows.
+        for (int i = 0; i < FM; ++i) {
+          const int column = wm * Tile::WM + i * 32;
+          if constexpr (ES == 4) {
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          uint32_t word[2][2];
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const T pair[2] = {static_cast<T>(acc[i][j][4 * (q + p) + 2 * h]),
-                                 static_cast<T>(acc[i][j][4 * (q + p) + 2 * h + 1])};
-              __builtin_memcpy(&word[p][h], pair, 4);
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+              f(row, column + Op::out_row(lane, 4 * q), __builtin_bit_cast(i32x4, v));
             }
-          const auto low = __builtin_amdgcn_permlane32_swap(word[0][0], word[1][0], false, false);
-          const auto high = __builtin_amdgcn_permlane32_swap(word[0][1], word[1][1], false, false);
-          const i32x4 value = {static_cast<int>(low[0]), static_cast<int>(high[0]), static_cast<int>(low[1]),
-                               static_cast<int>(high[1])};
-          put(value, column + 8 * (q + (lane >> 5)));
+          } else {
+            // Lanes 0-31 hold features 8q .. 8q + 3 of their row, lanes 32-63 the next four of the same rows.
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+              uint32_t word[2][2];
+#pragma unroll
+              for (int p = 0; p < 2; ++p)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const T pair[2] = {static_cast<T>(acc[i][j][4 * (q + p) + 2 * h]),
+                                     static_cast<T>(acc[i][j][4 * (q + p) + 2 * h + 1])};
+                  __builtin_memcpy(&word[p][h], pair, 4);
+                }
+              const auto low = __builtin_amdgcn_permlane32_swap(word[0][0], word[1][0], false, false);
+              const auto high = __builtin_amdgcn_permlane32_swap(word[0][1], word[1][1], false, false);
+              f(row, column + 8 * (q + (lane >> 5)),
+                i32x4{static_cast<int>(low[0]), static_cast<int>(high[0]), static_cast<int>(low[1]),
+                      static_cast<int>(high[1])});
+            }
+          }
         }
       }
-    }
+    };
+    // Rows past `live` lie past the buffer. Every wave issues the same STORES,
+    // which vmcnt counts; those of an edge below only make it wait for more.
+    pieces([&](int row, int feature, i32x4 value) __attribute__((always_inline)) {
+      const int offset = feature + PIECE <= width ? (row + feature) * ES : kOutOfRange;
+      __builtin_amdgcn_raw_buffer_store_b128(value, rc, offset, 0, 0);
+    });
+    if (width < BM && n % PIECE)  // the pieces that n ends in
+      pieces([&](int row, int feature, i32x4 value) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < PIECE - 1; ++c) {
+          const bool inside = feature + PIECE > width && feature + c < width;
+          const int offset = inside ? (row + feature + c) * ES : kOutOfRange;
+          const int word = value[c * ES / 4];
+          if constexpr (ES == 4)
+            __builtin_amdgcn_raw_buffer_store_b32(word, rc, offset, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b16(static_cast<short>(c % 2 ? word >> 16 : word), rc, offset, 0, 0);
+        }
+      });
   };
 
   static_for<0, STAGES>([&](auto s_c) __attribute__((always_inline)) {
