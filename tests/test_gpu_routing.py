@@ -62,6 +62,55 @@ def test_route_and_gradient(gpu, tokens, experts, top, options):
     assert (np.abs(_host(d_logits) - exact) <= bound).all()
 
 
+@pytest.mark.parametrize("experts,top,groups,top_groups", [(8, 2, 1, 1), (60, 4, 4, 2), (64, 16, 16, 5), (128, 8, 1, 1),
+                                                           (232, 7, 1, 1), (256, 8, 8, 4), (256, 17, 1, 1),
+                                                           (300, 8, 1, 1)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_many_tokens(gpu, experts, top, groups, top_groups, scores):
+    """Enough tokens for every form of the kernels, logits of few values: of equal ones the lower index, whatever
+    lane holds it; the last tokens end inside a workgroup."""
+    import torch
+
+    from triton_chip_benchmarks_amd import routing
+
+    print(f"route many x {experts} top {top} of {groups}/{top_groups}", flush=True)
+    generator = torch.Generator(device="cuda").manual_seed(experts)
+    tokens = 4099
+    logits = (torch.randint(-40, 41, (tokens, experts), device="cuda", generator=generator) / 16.0).bfloat16()
+    logits[5::7] = -float("inf")
+    logits[:, 3] = -float("inf")
+    options = {"scores": scores, "groups": groups, "top_groups": top_groups, "scale": 2.0}
+    chosen, weights = routing.route(logits, top, **options)
+    sample = np.r_[0:40, tokens - 40:tokens]
+    expected, expected_weights = oracle.route(_host(logits)[sample], top, **_oracle_options(options))
+    if groups == 1:  # sums of two scores of few values may tie in 64 bits and not in 32
+        assert np.array_equal(chosen.cpu().numpy()[sample], expected)
+        assert np.allclose(_host(weights)[sample], expected_weights, rtol=SCORE_TOLERANCE, atol=0)
+    few = [routing.route(logits[i:i + 1000], top, **options) for i in range(0, tokens, 1000)]  # a wave a token
+    assert torch.equal(chosen, torch.cat([part[0] for part in few]))
+    assert torch.allclose(weights, torch.cat([part[1] for part in few]), rtol=SCORE_TOLERANCE, atol=0)
+    g = torch.randn(tokens, top, device="cuda", generator=generator)
+    d_logits = routing.route_backward(logits, chosen, g, scores=scores, scale=2.0)
+    exact = oracle.route_backward(_host(logits)[sample], chosen.cpu().numpy()[sample], _host(g)[sample], kind=scores,
+                                  scale=2.0)
+    bound = 8 * SCORE_TOLERANCE * np.abs(_host(g)[sample]).sum(axis=1, keepdims=True) + UNIT["bf16"] * np.abs(exact)
+    assert (np.abs(_host(d_logits)[sample] - exact) <= bound + 2.0**-25).all()
+
+
+def test_a_lone_choice_has_no_gradient(gpu):
+    """Renormalised, its weight is the scale whatever its logit."""
+    import torch
+
+    from triton_chip_benchmarks_amd import routing
+
+    for tokens in (33, 5000):
+        logits = torch.randn(tokens, 96, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+        for scores in ("softmax", "sigmoid"):
+            chosen, weights = routing.route(logits, 1, scores=scores, scale=1.5)
+            assert (weights == 1.5).all()
+            assert not routing.route_backward(logits, chosen, torch.ones_like(weights), scores=scores).any()
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16"])
 def test_route_takes_16_bit_logits_strided(gpu, dtype):
     import torch

@@ -37,8 +37,9 @@ _COPY_EDGES_RE = re.compile(r"copy_edges_kernelILi(\d+)ELi([012])E")
 _READ_RE = re.compile(r"read_sum_kernelI(f|DF16_|t)E")
 _READ_PACKED_RE = re.compile(r"read_sum_packed_kernelI(f|DF16_|t)Li(\d+)E")
 _ELEMENT_TYPE = {"f": "f32", "DF16_": "f16", "DF16b": "bf16"}
-_ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)E")
-_LAYER_RE = re.compile(r"(mx_quantize|mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
+_ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)E")
+_QUANTIZE_RE = re.compile(r"mx_quantize_kernelI(f|DF16_|DF16b)Li(\d+)ELb([01])E")
+_LAYER_RE = re.compile(r"(mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
                        r"_kernelI(f|DF16_|DF16b)(?:Lb([01])E)?E")
 _PRODUCT_RING_RE = re.compile(r"mx_product_(ring|stream)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi\d+EE")
 _FEW_RE = re.compile(r"mx_few_kernelI(h|f|DF16_|DF16b)(S\d*_|T_|f|DF16_|DF16b)?Li(\d+)ELi(\d+)EE")
@@ -92,7 +93,11 @@ def registered_name(symbol: str) -> str | None:
         return f"read_sum_{_READ_TYPE[match.group(1)]}_vec"
     match = _ROUTE_RE.search(symbol)
     if match:
-        return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}_v{match.group(3)}"
+        return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}_{match.group(4)}x{match.group(3)}"
+    match = _QUANTIZE_RE.search(symbol)
+    if match:
+        dtype, loads, stream = match.groups()
+        return f"mx_quantize_{_ELEMENT_TYPE[dtype]}_{512 * int(loads)}{'_stream' if stream == '1' else ''}"
     match = _LAYER_RE.search(symbol)
     if match:
         return f"{match.group(1)}_{_ELEMENT_TYPE[match.group(2)]}{'_stream' if match.group(3) == '1' else ''}"

@@ -119,6 +119,29 @@ __device__ __forceinline__ float wave_max(float v) {
   return wave_reduce(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
 }
 
+// f over the lane's team of TEAM lanes (a wave's 64, or its row of 16), the same
+// bits in every lane of the team: in a row, partners swap values (lanes 1 and 2
+// apart, then mirrored ones of 8 and of 16), so that both join the same two.
+template <int TEAM, class F>
+__device__ __forceinline__ float team_reduce(float v, float none, F&& f) {
+  static_assert(TEAM == 64 || TEAM == 16, "a wave or a row of it");
+  if constexpr (TEAM == 64) return wave_reduce(v, none, f);
+  v = f(v, dpp_lane<kQuadXor1, 0xf>(none, v));
+  v = f(v, dpp_lane<kQuadXor2, 0xf>(none, v));
+  v = f(v, dpp_lane<0x141, 0xf>(none, v));
+  return f(v, dpp_lane<0x140, 0xf>(none, v));
+}
+
+template <int TEAM>
+__device__ __forceinline__ float team_add(float v) {
+  return team_reduce<TEAM>(v, 0.0f, [](float a, float b) { return a + b; });
+}
+
+template <int TEAM>
+__device__ __forceinline__ float team_max(float v) {
+  return team_reduce<TEAM>(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
+}
+
 // Host: bytes of one element of MB_DTYPE_*, 0 for another code.
 inline uint32_t elem_bytes(int dtype) {
   return dtype == MB_DTYPE_F32 ? 4 : dtype == MB_DTYPE_F16 || dtype == MB_DTYPE_BF16 ? 2 : 0;

@@ -21,52 +21,59 @@ constexpr uint32_t kBlock = 256;  // elements along K whose 8 scales a row holds
 
 __device__ __forceinline__ float bits_float(uint32_t v) { return __builtin_bit_cast(float, v); }
 
-constexpr int kLaneRows = 2;                      // rows a lane loads at once
-constexpr int kRowsPerWorkgroup = 8 * kLaneRows;
-
 // Rows of x to codes and scales. A lane takes eight elements, four lanes a
-// group, half a wave one row's 256 elements, a workgroup 16 rows of them: bound by
-// HBM (8192x8192 bf16 30.1 us, 5.7 TB/s; with 32 rows 34.7, with 64 35.5). With
-// `slots` [rows][copies], row r goes to the operand's rows slots[r][0 .. copies),
-// those outside 0 .. out_rows - 1 left out; without, to row r.
-template <class T>
+// group, a wave U * 512 elements of one row, a workgroup four rows. With `slots`
+// [rows][copies], row r goes to the operand's rows slots[r][0 .. copies), those
+// outside 0 .. out_rows - 1 left out; without, to row r. STREAM as in store8.
+//
+// Bound by HBM: 8192x8192 bf16 29.0 us (5.9 TB/s; streamed 28.8), 8192x4096 to
+// four rows each 28.0 streamed (4.9 TB/s), not 30.7. Two loads a lane: with one
+// 30.8 and 29.0, with four 31.4 and 32.0; one where a row has no more (16384x512
+// 5.4 us, with two 6.2). Half a wave a row, whose operand rows are written in
+// pieces of 128 bytes, took 29.7 and 33.6.
+template <class T, int U, bool STREAM>
 __global__ void __launch_bounds__(256)
     mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t row_stride,
                        const int32_t* __restrict__ slots, uint32_t copies, uint32_t out_rows,
                        uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  constexpr int U = kLaneRows;
-  const uint32_t blocks = (k + kBlock - 1) / kBlock;
-  const uint32_t block = blockIdx.x % blocks;
-  const uint32_t row0 = blockIdx.x / blocks * kRowsPerWorkgroup + threadIdx.x / 32;
-  const uint32_t k0 = block * kBlock + threadIdx.x % 32 * 8;
-  const int count = static_cast<int>(k > k0 ? k - k0 : 0);
-  const uint32_t code_bytes = (k + kGroup - 1) / kGroup * 16;
+  const uint32_t lane = threadIdx.x & 63;
+  const uint32_t chunks = (k + U * 512 - 1) / (U * 512);
+  const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x / chunks * 4 + (threadIdx.x >> 6));
+  if (row >= rows) return;
+  const uint32_t start = blockIdx.x % chunks * (U * 512) + lane * 8;
+  const uint32_t code_bytes = (k + kGroup - 1) / kGroup * 16, blocks = (k + kBlock - 1) / kBlock;
   Raw8<T> raw[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t row = row0 + 8 * u;
-    if (row < rows)
-      raw[u].load(x + row * row_stride + k0, count);
-    else
-      raw[u].zero();
+    const uint32_t k0 = start + u * 512;
+    raw[u].load(x + row * row_stride + k0, static_cast<int>(k > k0 ? k - k0 : 0));
   }
+  uint32_t word[U], scale[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const uint32_t row = row0 + 8 * u;
     uint32_t largest = raw_magnitude(raw[u]);
     largest = join_magnitudes(T(), largest, quad_swap<kQuadXor1>(largest));
     largest = join_magnitudes(T(), largest, quad_swap<kQuadXor2>(largest));
-    const uint32_t scale = scale_byte(magnitude_bits<T>(largest));
-    const uint32_t word = encode8(raw[u], scale);
-    if (row >= rows) continue;
-    for (uint32_t c = 0; c < copies; ++c) {
-      const uint32_t out = slots ? static_cast<uint32_t>(slots[static_cast<uint64_t>(row) * copies + c]) : row;
-      if (out >= out_rows) continue;
-      if (k0 / 2 < code_bytes)
-        *reinterpret_cast<uint32_t*>(codes + static_cast<uint64_t>(out) * code_bytes + k0 / 2) = word;
-      if (threadIdx.x % 4 == 0)
-        scales[(static_cast<uint64_t>(block) * out_rows + out) * 8 + threadIdx.x % 32 / 4] =
-            static_cast<uint8_t>(k0 < k ? scale : 127);
+    scale[u] = scale_byte(magnitude_bits<T>(largest));
+    word[u] = encode8(raw[u], scale[u]);
+    if (start + u * 512 >= k) scale[u] = 127;  // groups past K
+  }
+  for (uint32_t c = 0; c < copies; ++c) {
+    const uint32_t out = slots ? static_cast<uint32_t>(slots[static_cast<uint64_t>(row) * copies + c]) : row;
+    if (out >= out_rows) continue;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t k0 = start + u * 512;
+      if (k0 / 2 < code_bytes) {
+        uint32_t* to = reinterpret_cast<uint32_t*>(codes + static_cast<uint64_t>(out) * code_bytes + k0 / 2);
+        if constexpr (STREAM)
+          __builtin_nontemporal_store(word[u], to);
+        else
+          *to = word[u];
+      }
+      if (lane % 4 == 0 && k0 / kBlock < blocks)
+        scales[(static_cast<uint64_t>(k0 / kBlock) * out_rows + out) * 8 + k0 % kBlock / kGroup] =
+            static_cast<uint8_t>(scale[u]);
     }
   }
 }
@@ -210,7 +217,9 @@ __global__ void __launch_bounds__(256)
 }
 
 #define MB_MX_REGISTER(T, NAME)                                      \
-  MB_REGISTER_KERNEL("mx_quantize_" NAME, mx_quantize_kernel<T>);    \
+  MB_REGISTER_KERNEL("mx_quantize_" NAME "_512", (mx_quantize_kernel<T, 1, false>));           \
+  MB_REGISTER_KERNEL("mx_quantize_" NAME "_1024", (mx_quantize_kernel<T, 2, false>));          \
+  MB_REGISTER_KERNEL("mx_quantize_" NAME "_1024_stream", (mx_quantize_kernel<T, 2, true>));    \
   MB_REGISTER_KERNEL("mx_quantize_columns_" NAME, mx_quantize_columns_kernel<T>); \
   MB_REGISTER_KERNEL("mx_dequantize_" NAME, (mx_dequantize_kernel<T, false>)); \
   MB_REGISTER_KERNEL("mx_dequantize_" NAME "_stream", (mx_dequantize_kernel<T, true>))
@@ -250,12 +259,23 @@ int check_rows(const char* entry, int dtype, const void* x, uint64_t x_bytes, ui
 
 int launch_quantize(int dtype, const void* x, uint32_t rows, uint32_t k, uint64_t row_stride, const int32_t* slots,
                     uint32_t copies, uint32_t out_rows, void* codes, void* scales, hipStream_t stream) {
-  const uint64_t grid = (rows + uint64_t{kRowsPerWorkgroup} - 1) / kRowsPerWorkgroup * ((k + kBlock - 1) / kBlock);
-  if (grid > 0xffffffu)
-    return fail(MB_ERR_UNSUPPORTED, "mx_quantize: %u x %u exceeds one launch", rows, k);
-  MB_FOR_DTYPE(dtype, (mx_quantize_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream>>>(
-                          static_cast<const T*>(x), rows, k, row_stride, slots, copies, out_rows,
-                          static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales))));
+  const uint32_t elements = k > 512 ? 1024 : 512;  // of a row and wave
+  const uint64_t grid = (rows + uint64_t{3}) / 4 * ((k + elements - 1) / elements);
+  if (grid > 0xffffffu) return fail(MB_ERR_UNSUPPORTED, "mx_quantize: %u x %u exceeds one launch", rows, k);
+  auto launch = [&](auto kernel, auto t) {
+    kernel<<<dim3(static_cast<uint32_t>(grid)), dim3(256), 0, stream>>>(
+        static_cast<const decltype(t)*>(x), rows, k, row_stride, slots, copies, out_rows,
+        static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales));
+  };
+  const bool streamed = streams(mx_code_bytes(uint64_t{rows} * copies, k));
+  MB_FOR_DTYPE(dtype, {
+    if (k <= 512)
+      launch(mx_quantize_kernel<T, 1, false>, T());
+    else if (streamed)
+      launch(mx_quantize_kernel<T, 2, true>, T());
+    else
+      launch(mx_quantize_kernel<T, 2, false>, T());
+  });
   return launch_status("mx_quantize");
 }
 

@@ -20,9 +20,10 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
-// Scores s of a token's logits, lane l holding experts l * V .. l * V + V - 1;
-// logits past the last expert and masked ones (-inf) are -inf and score 0.
-template <int V>
+// Scores s of a token's logits, lane l of its team holding experts l * V ..
+// l * V + V - 1; logits past the last expert and masked ones (-inf) are -inf and
+// score 0.
+template <int V, int TEAM>
 __device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax, float (&score)[V]) {
   if (!softmax) {
 #pragma unroll
@@ -32,7 +33,7 @@ __device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax,
   float top = kNegInf;
 #pragma unroll
   for (int i = 0; i < V; ++i) top = fmaxf(top, logit[i]);
-  top = wave_max(top);
+  top = team_max<TEAM>(top);
   if (top == kNegInf) top = 0.0f;  // nothing but masked experts
   float total = 0.0f;
 #pragma unroll
@@ -40,7 +41,7 @@ __device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax,
     score[i] = expf(logit[i] - top);
     total += score[i];
   }
-  total = wave_add(total);
+  total = team_add<TEAM>(total);
 #pragma unroll
   for (int i = 0; i < V; ++i) score[i] = total == 0.0f ? 0.0f : score[i] / total;
 }
@@ -64,22 +65,35 @@ __device__ __forceinline__ void load_logits(const T* __restrict__ row, uint32_t 
   }
 }
 
-// One wave a token. Selection values: score + bias; -inf where masked (a logit
-// of -inf) or outside the kept groups; a NaN counts as -1e38, below any score and
-// a finite sum with another, so that a token of NaNs still gets different
-// experts, with NaN weights.
-template <class T, int V>
+// A team of TEAM lanes a token: a wave, or, for many tokens, a quarter of one.
+// Selection values: score + bias; -inf where masked (a logit of -inf) or outside
+// the kept groups; a NaN counts as -1e38, below any score and a finite sum with
+// another, so that a token of NaNs still gets different experts, with NaN weights.
+//
+// Bound by the instructions of `top` rounds of a maximum over the team, which
+// cost the same for one token a wave as for four: 16384 tokens of 128 experts,
+// top 8, 15.6 us a wave each, 9.7 a quarter each. Few tokens are bound by the
+// latency of one: 16 of 256 experts 5.7 us a wave each, of which a launch is
+// about three.
+template <class T, int V, int TEAM>
 __global__ void __launch_bounds__(256)
     route_kernel(const T* __restrict__ logits, uint32_t tokens, uint32_t experts, uint64_t row_stride,
                  const float* __restrict__ bias, uint32_t top, bool softmax, uint32_t groups, uint32_t top_groups,
                  bool renormalize, float scale, int32_t* __restrict__ chosen, float* __restrict__ weights) {
-  __shared__ float lds[4][64 * V];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t token = blockIdx.x * 4 + wave;
+  constexpr int TOKENS = 256 / TEAM;
+  __shared__ float values_lds[TOKENS][TEAM * V];
+  __shared__ float groups_lds[TOKENS][TEAM];
+  struct Choice {
+    int32_t expert;
+    float score;
+  };
+  __shared__ Choice choices[TOKENS][TEAM];
+  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const uint32_t token = blockIdx.x * TOKENS + team;
   if (token >= tokens) return;
   float logit[V], score[V], value[V];
   load_logits(logits + token * row_stride, experts, lane, logit);
-  scores_of(logit, softmax, score);
+  scores_of<V, TEAM>(logit, softmax, score);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const uint32_t e = lane * V + i;
@@ -87,95 +101,90 @@ __global__ void __launch_bounds__(256)
     if (value[i] != value[i]) value[i] = -1e38f;
     if (logit[i] == kNegInf) value[i] = kNegInf;
   }
+  choices[team][lane] = Choice{-1, 0.0f};
   if (groups > 1) {
     const uint32_t size = experts / groups;
 #pragma unroll
-    for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = value[i];
+    for (int i = 0; i < V; ++i) values_lds[team][lane * V + i] = value[i];
     wave_lds_fence();
     float first = kNegInf, second = kNegInf;
     if (static_cast<uint32_t>(lane) < groups) {
 #pragma unroll 8
       for (uint32_t i = 0; i < size; ++i) {
-        const float v = lds[wave][lane * size + i];
+        const float v = values_lds[team][lane * size + i];
         second = fmaxf(second, fminf(first, v));
         first = fmaxf(first, v);
       }
     }
     const float mine = first + (second == kNegInf ? 0.0f : second);
+    groups_lds[team][lane] = mine;
+    wave_lds_fence();
     // A group is kept if fewer than top_groups come before it: larger ones, or
     // as large ones of a lower index.
     uint32_t before = 0;
+#pragma unroll 8
     for (uint32_t g = 0; g < groups; ++g) {
-      const float other = __builtin_bit_cast(
-          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), static_cast<int>(g)));
+      const float other = groups_lds[team][g];
       before += other > mine || (other == mine && g < static_cast<uint32_t>(lane));
     }
     const bool kept = static_cast<uint32_t>(lane) < groups && before < top_groups;
-    const uint64_t mask = __ballot(kept);
+    const uint64_t mask = __ballot(kept) >> (threadIdx.x % 64 - lane);
+    uint32_t group = lane * V / size, inside = lane * V % size;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const uint32_t e = lane * V + i;
-      if (e < experts && !(mask >> (e / size) & 1)) value[i] = kNegInf;
+      if (!(mask >> (group & 63) & 1)) value[i] = kNegInf;
+      if (++inside == size) inside = 0, ++group;
     }
   }
-  int mine = -1;
-  float mine_score = 0.0f;
   for (uint32_t j = 0; j < top; ++j) {
     float best = value[0];
-    int at = 0;
 #pragma unroll
-    for (int i = 1; i < V; ++i) {
-      if (value[i] > best) {
-        best = value[i];
-        at = i;
-      }
-    }
-    const float largest = wave_max(best);
-    if (largest == kNegInf) break;
-    const int winner = __builtin_ctzll(__ballot(best == largest));
-    float s = 0.0f;
+    for (int i = 1; i < V; ++i) best = fmaxf(best, value[i]);
+    const float largest = team_max<TEAM>(best);
+    // The first lane that has it, and there the first value.
+    const uint64_t winners = __ballot(best == largest) >> (threadIdx.x % 64 - lane);
+    const bool mine = __builtin_ctzll(winners | uint64_t{1} << 63) == lane && largest != kNegInf;
+    bool open = mine;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (i == at) {
-        s = score[i];
-        if (lane == winner) value[i] = kNegInf;
+      if (open && value[i] == largest) {
+        open = false;
+        value[i] = kNegInf;
+        choices[team][j] = Choice{static_cast<int32_t>(lane * V + i), score[i]};
       }
     }
-    const int expert = __builtin_amdgcn_readlane(lane * V + at, winner);
-    const int bits = __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), winner);
-    if (lane == static_cast<int>(j)) {
-      mine = expert;
-      mine_score = __builtin_bit_cast(float, bits);
-    }
   }
-  float weight = mine_score;
+  wave_lds_fence();
+  const Choice choice = choices[team][lane];
+  float weight = choice.score;
   if (renormalize) {
-    const float total = wave_add(mine_score);
+    const float total = team_add<TEAM>(choice.score);
     weight = total == 0.0f ? 0.0f : weight / total;
   }
   if (static_cast<uint32_t>(lane) < top) {
-    chosen[static_cast<uint64_t>(token) * top + lane] = mine;
+    chosen[static_cast<uint64_t>(token) * top + lane] = choice.expert;
     weights[static_cast<uint64_t>(token) * top + lane] = weight * scale;
   }
 }
 
-// Gradient of route's weights with respect to the logits, one wave a token.
-// With w_j = r s_j / Z over the chosen (Z = 1 unless renormalised) and g their
+// Gradient of route's weights with respect to the logits, a team a token. With
+// w_j = r s_j / Z over the chosen (Z = 1 unless renormalised) and g their
 // gradient, d s_j = r (g_j - sum_i g_i s_i / Z) / Z, then through the scores:
 // softmax d l = s (d s - sum d s s), sigmoid d l = d s s (1 - s). The choice
 // itself has no gradient.
-template <class T, int V>
+template <class T, int V, int TEAM>
 __global__ void __launch_bounds__(256)
     route_backward_kernel(const T* __restrict__ logits, uint32_t tokens, uint32_t experts, uint64_t row_stride,
                           const int32_t* __restrict__ chosen, const float* __restrict__ d_weights, uint32_t top,
                           bool softmax, bool renormalize, float scale, T* __restrict__ d_logits) {
-  __shared__ float lds[4][64 * V];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t token = blockIdx.x * 4 + wave;
+  constexpr int TOKENS = 256 / TEAM;
+  __shared__ float lds[TOKENS][TEAM * V];
+  const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+  const uint32_t token = blockIdx.x * TOKENS + team;
   if (token >= tokens) return;
   float logit[V], score[V];
   load_logits(logits + token * row_stride, experts, lane, logit);
-  scores_of(logit, softmax, score);
+  scores_of<V, TEAM>(logit, softmax, score);
   int expert = -1;
   float d = 0.0f;
   if (static_cast<uint32_t>(lane) < top) {
@@ -184,26 +193,27 @@ __global__ void __launch_bounds__(256)
     if (expert >= 0) d = d_weights[static_cast<uint64_t>(token) * top + lane] * scale;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = score[i];
+  for (int i = 0; i < V; ++i) lds[team][lane * V + i] = score[i];
   wave_lds_fence();
-  const float s = expert >= 0 ? lds[wave][expert] : 0.0f;
+  const float s = expert >= 0 ? lds[team][expert] : 0.0f;
   wave_lds_fence();
   if (renormalize) {
-    const float total = wave_add(s);
-    const float mean = total == 0.0f ? 0.0f : wave_add(d * s) / total;
+    const float total = team_add<TEAM>(s);
+    // By shares, so that a lone choice, whose weight is constant, has a gradient of exactly zero.
+    const float mean = team_add<TEAM>(total == 0.0f ? 0.0f : d * (s / total));
     d = expert < 0 || total == 0.0f ? 0.0f : (d - mean) / total;
   }
   // Renormalised softmax weights do not change with the unchosen logits.
-  const float common = softmax && !renormalize ? wave_add(d * s) : 0.0f;
+  const float common = softmax && !renormalize ? team_add<TEAM>(d * s) : 0.0f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) lds[wave][lane * V + i] = 0.0f;
+  for (int i = 0; i < V; ++i) lds[team][lane * V + i] = 0.0f;
   wave_lds_fence();
-  if (expert >= 0) lds[wave][expert] = d;
+  if (expert >= 0) lds[team][expert] = d;
   wave_lds_fence();
   LaneValues<T, V> out;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float ds = lds[wave][lane * V + i];
+    const float ds = lds[team][lane * V + i];
     out.at[i] = static_cast<T>(softmax ? score[i] * (ds - common) : ds * score[i] * (1.0f - score[i]));
   }
   T* to = d_logits + static_cast<uint64_t>(token) * experts + lane * V;
@@ -459,15 +469,18 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-#define MB_ROUTE_REGISTER_V(T, NAME, V)                                            \
-  MB_REGISTER_KERNEL("route_" NAME "_v" #V, (route_kernel<T, V>));                 \
-  MB_REGISTER_KERNEL("route_backward_" NAME "_v" #V, (route_backward_kernel<T, V>))
-#define MB_ROUTE_REGISTER(T, NAME)                              \
-  MB_ROUTE_REGISTER_V(T, NAME, 1);                              \
-  MB_ROUTE_REGISTER_V(T, NAME, 2);                              \
-  MB_ROUTE_REGISTER_V(T, NAME, 4);                              \
-  MB_ROUTE_REGISTER_V(T, NAME, 8);                              \
-  MB_ROUTE_REGISTER_V(T, NAME, 16);                             \
+#define MB_ROUTE_REGISTER_V(T, NAME, V, TEAM)                                               \
+  MB_REGISTER_KERNEL("route_" NAME "_" #TEAM "x" #V, (route_kernel<T, V, TEAM>));          \
+  MB_REGISTER_KERNEL("route_backward_" NAME "_" #TEAM "x" #V, (route_backward_kernel<T, V, TEAM>))
+#define MB_ROUTE_REGISTER(T, NAME)                                                            \
+  MB_ROUTE_REGISTER_V(T, NAME, 1, 64);                                                        \
+  MB_ROUTE_REGISTER_V(T, NAME, 2, 64);                                                        \
+  MB_ROUTE_REGISTER_V(T, NAME, 4, 64);                                                        \
+  MB_ROUTE_REGISTER_V(T, NAME, 8, 64);                                                        \
+  MB_ROUTE_REGISTER_V(T, NAME, 16, 64);                                                       \
+  MB_ROUTE_REGISTER_V(T, NAME, 4, 16);                                                        \
+  MB_ROUTE_REGISTER_V(T, NAME, 8, 16);                                                        \
+  MB_ROUTE_REGISTER_V(T, NAME, 16, 16);                                                       \
   MB_REGISTER_KERNEL("combine_" NAME, (combine_kernel<T, false>));                            \
   MB_REGISTER_KERNEL("combine_" NAME "_stream", (combine_kernel<T, true>));                   \
   MB_REGISTER_KERNEL("combine_backward_" NAME, (combine_backward_kernel<T, false>));          \
@@ -506,18 +519,31 @@ int check_chosen(const char* entry, const void* chosen, uint64_t chosen_bytes, c
   return MB_OK;
 }
 
+// f(values a lane, lanes a token): a quarter of a wave a token where there are
+// enough tokens to fill the chip's SIMDs so, and 16 lanes hold the experts, the
+// choices and the groups; else a wave.
 template <class F>
-void for_experts(uint32_t experts, F&& f) {
-  if (experts <= 64)
-    f(std::integral_constant<int, 1>{});
+void for_experts(uint32_t tokens, uint32_t experts, uint32_t top, uint32_t groups, F&& f) {
+  const bool quarter = tokens >= 4096 && experts <= 256 && top <= 16 && groups <= 16;
+  auto call = [&](auto v, auto team) { f(v, team); };
+  using Wave = std::integral_constant<int, 64>;
+  using Row = std::integral_constant<int, 16>;
+  if (quarter && experts <= 64)
+    call(std::integral_constant<int, 4>{}, Row{});
+  else if (quarter && experts <= 128)
+    call(std::integral_constant<int, 8>{}, Row{});
+  else if (quarter)
+    call(std::integral_constant<int, 16>{}, Row{});
+  else if (experts <= 64)
+    call(std::integral_constant<int, 1>{}, Wave{});
   else if (experts <= 128)
-    f(std::integral_constant<int, 2>{});
+    call(std::integral_constant<int, 2>{}, Wave{});
   else if (experts <= 256)
-    f(std::integral_constant<int, 4>{});
+    call(std::integral_constant<int, 4>{}, Wave{});
   else if (experts <= 512)
-    f(std::integral_constant<int, 8>{});
+    call(std::integral_constant<int, 8>{}, Wave{});
   else
-    f(std::integral_constant<int, 16>{});
+    call(std::integral_constant<int, 16>{}, Wave{});
 }
 
 uint64_t dispatch_blocks(uint64_t entries) { return (entries + kDispatchItems - 1) / kDispatchItems; }
@@ -545,9 +571,9 @@ int mb_route(int dtype, const void* logits, uint64_t logits_bytes, uint32_t toke
   if (tokens == 0) return MB_OK;
   if (int rc = mb::check_chosen(entry, chosen, chosen_bytes, weights, weights_bytes, uint64_t{tokens} * top))
     return rc;
-  const dim3 grid((tokens + 3) / 4);
-  MB_FOR_DTYPE(dtype, mb::for_experts(experts, [&](auto v) {
-    mb::route_kernel<T, decltype(v)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+  MB_FOR_DTYPE(dtype, mb::for_experts(tokens, experts, top, groups, [&](auto v, auto team) {
+    constexpr uint32_t kTokens = 256 / decltype(team)::value;
+    mb::route_kernel<T, decltype(v)::value, decltype(team)::value><<<(tokens + kTokens - 1) / kTokens, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
         static_cast<const T*>(logits), tokens, experts, row_stride, bias, top, scores == MB_SCORES_SOFTMAX,
         top_groups == groups ? 1 : groups, top_groups, renormalize != 0, scale, chosen, weights);
   }));
@@ -570,9 +596,9 @@ int mb_route_backward(int dtype, const void* logits, uint64_t logits_bytes, uint
                     experts);
   if (!mb::aligned(d_logits, item))
     return mb::fail(MB_ERR_ALIGNMENT, "%s: d_logits must lie on their elements' %u bytes", entry, item);
-  const dim3 grid((tokens + 3) / 4);
-  MB_FOR_DTYPE(dtype, mb::for_experts(experts, [&](auto v) {
-    mb::route_backward_kernel<T, decltype(v)::value><<<grid, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+  MB_FOR_DTYPE(dtype, mb::for_experts(tokens, experts, top, 1, [&](auto v, auto team) {
+    constexpr uint32_t kTokens = 256 / decltype(team)::value;
+    mb::route_backward_kernel<T, decltype(v)::value, decltype(team)::value><<<(tokens + kTokens - 1) / kTokens, dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
         static_cast<const T*>(logits), tokens, experts, row_stride, chosen, d_weights, top,
         scores == MB_SCORES_SOFTMAX, renormalize != 0, scale, static_cast<T*>(d_logits));
   }));
