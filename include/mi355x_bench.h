@@ -301,7 +301,8 @@ int mb_mx_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_
 /* Bytes of workspace (16-byte aligned) mb_mx_linear needs for `rows` rows of output. */
 uint64_t mb_mx_linear_workspace(uint32_t rows, uint32_t n, uint32_t k);
 
-/* Y = Q(X) . W^T: mb_mx_quantize of X, then mb_mx_product with the weight.
+/* Y = Q(X) . W^T: mb_mx_quantize of X, then mb_mx_product with the weight, in one
+ * launch for few rows and two for more.
  * offsets NULL: Y [tokens][n], one weight. With offsets and slots NULL: X's rows
  * are already in the order of the experts. With order and slots (mb_dispatch,
  * [tokens][copies]): X holds tokens, and Y [tokens*copies][n] their routed rows
@@ -312,6 +313,20 @@ int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, ui
                  uint32_t k, const int32_t* offsets, uint64_t offsets_bytes, const int32_t* order,
                  const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t experts, void* workspace,
                  uint64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace (16-byte aligned) of mb_mx_linear_backward. */
+uint64_t mb_mx_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k);
+
+/* Gradients of Y = Q(X) . Q(W)^T, straight through the quantisation, for d_out
+ * [rows][n]: d_x [rows][k] = Q(d_out) . Wc with the weight quantised by columns
+ * (mb_mx_quantize_columns of W: an operand of k rows and K = n), and d_w [n][k] =
+ * d_out^T . X, both quantised by columns, along the rows that the sum runs over.
+ * Five launches. */
+int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* x,
+                          uint64_t x_bytes, uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes,
+                          const void* scale_w, uint64_t scale_w_bytes, void* d_x, uint64_t d_x_bytes, void* d_w,
+                          uint64_t d_w_bytes, uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                          uint64_t workspace_bytes, void* stream);
 
 /* Scores of mb_route. */
 #define MB_SCORES_SOFTMAX 0u

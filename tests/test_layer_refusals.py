@@ -69,6 +69,22 @@ def test_product_and_linear():
     refused(INVALID, "mb_mx_linear", *linear(slots=P, offsets=P, order=P, copies=65), match="outside 1..64")
 
 
+def test_linear_backward():
+    call = lambda rows=8, d_out_bytes=8 * 64 * 2, x_bytes=8 * 96 * 2, d_x_bytes=8 * 96 * 2, d_w_bytes=64 * 96 * 2, workspace=P, workspace_bytes=BIG, w_bytes=BIG: (  # noqa: E731,E501
+        2, P, d_out_bytes, 64, P, x_bytes, 96, P, w_bytes, P, BIG, P, d_x_bytes, P, d_w_bytes, rows, 64, 96, workspace,
+        workspace_bytes, None)
+    refused(INVALID, "mb_mx_linear_backward", *call(rows=0), match="positive")
+    refused(INVALID, "mb_mx_linear_backward", *call(d_out_bytes=8 * 64 * 2 - 1), match="too small")
+    refused(INVALID, "mb_mx_linear_backward", *call(x_bytes=8 * 96 * 2 - 1), match="too small")
+    refused(INVALID, "mb_mx_linear_backward", *call(w_bytes=96 * 32 - 1), match="too small")
+    refused(INVALID, "mb_mx_linear_backward", *call(d_x_bytes=8 * 96 * 2 - 1), match="output")
+    refused(INVALID, "mb_mx_linear_backward", *call(d_w_bytes=64 * 96 * 2 - 1), match="output")
+    needed = _native.load().mb_mx_linear_backward_workspace(8, 64, 96)
+    refused(INVALID, "mb_mx_linear_backward", *call(workspace_bytes=needed - 1), match="workspace")
+    refused(UNSUPPORTED, "mb_mx_linear_backward", *call(rows=(1 << 20) + 1, d_out_bytes=BIG, x_bytes=BIG,
+                                                       d_x_bytes=BIG), match="at most")
+
+
 def test_route():
     call = lambda dtype=0, logits=P, logits_bytes=4 * 16 * 4, tokens=4, experts=16, stride=16, bias=None, bias_bytes=0, top=2, scores=0, groups=1, top_groups=1, chosen=P, chosen_bytes=32, weights_bytes=32: (  # noqa: E731,E501
         dtype, logits, logits_bytes, tokens, experts, stride, bias, bias_bytes, top, scores, groups, top_groups, 1, 1.0,

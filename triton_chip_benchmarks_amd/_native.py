@@ -119,6 +119,9 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mb_mx_linear_workspace": (_u64, [_u32, _u32, _u32]),
     "mb_mx_linear": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _ptr, _u64,
                             _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
+    "mb_mx_linear_backward_workspace": (_u64, [_u32, _u32, _u32]),
+    "mb_mx_linear_backward": (_i32, [_i32, _ptr, _u64, _u64, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr,
+                                     _u64, _u32, _u32, _u32, _ptr, _u64, _ptr]),
     "mb_route": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _u32, _u32, _u32, _u32, _u32, _f32, _ptr, _u64,
                         _ptr, _u64, _ptr]),
     "mb_route_backward": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _f32,

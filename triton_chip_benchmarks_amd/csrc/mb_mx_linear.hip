@@ -634,4 +634,58 @@ int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, ui
                             on);
 }
 
+// Operands of mb_mx_linear_backward in its workspace: Q(d_out) [rows][n], and the
+// columns of d_out [n][rows] and of x [k][rows].
+static uint64_t place_operand(uint64_t at, uint64_t rows, uint64_t k, uint64_t* codes, uint64_t* scales) {
+  *codes = at;
+  *scales = at + (mb::mx_code_bytes(rows, k) + 15) / 16 * 16;
+  return *scales + (mb::mx_scale_bytes(rows, k) + 15) / 16 * 16;
+}
+
+uint64_t mb_mx_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  uint64_t codes, scales, end = place_operand(0, rows, n, &codes, &scales);
+  end = place_operand(end, n, rows, &codes, &scales);
+  return place_operand(end, k, rows, &codes, &scales);
+}
+
+int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* x,
+                          uint64_t x_bytes, uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes,
+                          const void* scale_w, uint64_t scale_w_bytes, void* d_x, uint64_t d_x_bytes, void* d_w,
+                          uint64_t d_w_bytes, uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                          uint64_t workspace_bytes, void* stream) {
+  const char* entry = "mb_mx_linear_backward";
+  if (int rc = mb::check_shape(entry, dtype, rows, n, k, 1)) return rc;
+  if (rows == 0 || n == 0 || k == 0) return mb::fail(MB_ERR_INVALID, "%s: rows, n and K must be positive", entry);
+  if (rows > mb::kMxMostK)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: at most %u rows, which d_w sums over", entry, mb::kMxMostK);
+  if (int rc = mb::check_rows(entry, dtype, d_out, d_out_bytes, rows, n, d_out_stride)) return rc;
+  if (int rc = mb::check_rows(entry, dtype, x, x_bytes, rows, k, x_stride)) return rc;
+  if (int rc = mb::check_operand(entry, "the weight's columns", k, n, 1, w_columns, w_columns_bytes, scale_w,
+                                 scale_w_bytes))
+    return rc;
+  if (int rc = mb::check_output(entry, dtype, d_x, d_x_bytes, rows, k)) return rc;
+  if (int rc = mb::check_output(entry, dtype, d_w, d_w_bytes, n, k)) return rc;
+  uint64_t codes[3], scales[3], end = place_operand(0, rows, n, &codes[0], &scales[0]);
+  end = place_operand(end, n, rows, &codes[1], &scales[1]);
+  end = place_operand(end, k, rows, &codes[2], &scales[2]);
+  uint8_t* const space = static_cast<uint8_t*>(workspace);
+  if (space == nullptr || workspace_bytes < end)
+    return mb::fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
+                    (unsigned long long)end);
+  if (!mb::aligned(space, 16)) return mb::fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
+  const hipStream_t on = static_cast<hipStream_t>(stream);
+  if (int rc = mb::launch_quantize(dtype, d_out, rows, n, d_out_stride, nullptr, 1, rows, space + codes[0],
+                                   space + scales[0], on))
+    return rc;
+  if (int rc = mb::launch_quantize_columns(dtype, d_out, rows, n, d_out_stride, space + codes[1], space + scales[1], on))
+    return rc;
+  if (int rc = mb::launch_quantize_columns(dtype, x, rows, k, x_stride, space + codes[2], space + scales[2], on))
+    return rc;
+  if (int rc = mb::launch_product(dtype, space + codes[0], space + scales[0], w_columns, scale_w, d_x, rows, k, n,
+                                  nullptr, 1, on))
+    return rc;
+  return mb::launch_product(dtype, space + codes[1], space + scales[1], space + codes[2], space + scales[2], d_w, n, k,
+                            rows, nullptr, 1, on);
+}
+
 }  // extern "C"

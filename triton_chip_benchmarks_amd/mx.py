@@ -46,8 +46,9 @@ class Packed:
         self.experts = lead[0] if lead else None
 
 
-# The checks below run at every call, beside which a kernel takes a few microseconds: get_device and comparisons of
-# shapes cost tens of nanoseconds, tensor.device and torch.cuda.current_device several hundred.
+# The checks below run at every call, beside which a kernel takes a few microseconds. They read shapes, types and
+# device numbers, tens of nanoseconds each, and compare them; only a refusal builds anything (torch.device objects,
+# tuples of sizes and messages cost several hundred).
 
 
 def dtype_code(tensor, what: str) -> int:
@@ -57,41 +58,46 @@ def dtype_code(tensor, what: str) -> int:
     return code
 
 
-def check_device(*tensors) -> None:
+def launch_stream(stream, *tensors) -> int:
+    """The raw stream to launch on: `stream`, or the current one; every tensor must lie on the current device."""
     device = tensors[0].get_device()
-    if device != (torch._C._cuda_getDevice() if torch.cuda.is_initialized() else torch.cuda.current_device()):
-        raise ValueError(f"tensors must lie on the current HIP device (cuda:{torch.cuda.current_device()}), not "
-                         f"{tensors[0].device}")
     for tensor in tensors:
         if tensor.get_device() != device:
-            raise ValueError(f"tensors must lie on one device, cuda:{device}, not {tensor.device}")
+            raise ValueError(f"tensors must lie on one device, {tensors[0].device}, not {tensor.device}")
+    if device < 0 or device != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors must lie on the current HIP device, not {tensors[0].device}")
+    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
 
 
-def strided_rows(tensor, what: str) -> tuple[int, int]:
-    """(row stride, bytes spanned) of a 2-D tensor with contiguous rows."""
+def library():
+    return _native._library or _native.load()
+
+
+def strided_rows(tensor, what: str) -> tuple[int, int, int, int]:
+    """(rows, columns, row stride, elements spanned) of a 2-D tensor with contiguous rows."""
     if tensor.dim() != 2:
         raise ValueError(f"{what} must have two dimensions, not {tensor.dim()}")
     rows, columns = tensor.shape
     stride, step = tensor.stride()
     if columns > 1 and step != 1:
         raise ValueError(f"{what} must have contiguous rows (a stride of 1 along its last dimension)")
-    if not rows or not columns:
-        return columns, 0
-    return stride if rows > 1 else columns, ((rows - 1) * stride + columns) * tensor.element_size()
+    if rows > 1 and columns:
+        return rows, columns, stride, (rows - 1) * stride + columns
+    return rows, columns, columns, rows * columns
 
 
-def check_output(tensor, what: str, shape, dtype, device):
-    """`tensor`, checked, or a new one in its place."""
-    if tensor is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if tensor.shape != shape or tensor.dtype != dtype or not tensor.is_contiguous():
+def check_tensor(tensor, what: str, shape, dtype) -> None:
+    if tensor.shape != shape or tensor.dtype is not dtype or not tensor.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of {tuple(shape)}, not {tensor.dtype} of "
                          f"{tuple(tensor.shape)}")
+
+
+def check_output(tensor, what: str, shape, dtype, like):
+    """`tensor`, checked, or a new one on the device of `like` in its place."""
+    if tensor is None:
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    check_tensor(tensor, what, shape, dtype)
     return tensor
-
-
-def bytes_of(tensor) -> int:
-    return tensor.numel() * tensor.element_size()
 
 
 def empty(rows: int, k: int, device="cuda", experts: int | None = None) -> Packed:
@@ -110,33 +116,39 @@ def _check_experts(packed: Packed, what: str, experts: int | None) -> None:
 def quantize(x, packed: Packed | None = None, columns: bool = False, stream=None) -> Packed:
     """The MXFP4 operand of x's rows; with `columns`, of its columns (x transposed, groups along its rows)."""
     code = dtype_code(x, "x")
-    stride, span = strided_rows(x, "x")
-    rows, k = x.shape[::-1] if columns else x.shape
+    x_rows, x_columns, stride, span = strided_rows(x, "x")
+    rows, k = (x_columns, x_rows) if columns else (x_rows, x_columns)
     if packed is None:
         packed = empty(rows, k, x.device)
     _check_experts(packed, "packed", None)
-    if (packed.rows, packed.k) != (rows, k):
+    if packed.rows != rows or packed.k != k:
         raise ValueError(f"packed must be an operand of {rows} x {k}, not {packed.rows} x {packed.k}")
-    check_device(x, packed.codes, packed.scales)
-    out = (packed.codes.data_ptr(), packed.codes.numel(), packed.scales.data_ptr(), packed.scales.numel(),
-           _native.stream_handle(stream))
+    codes, scales = packed.codes, packed.scales
+    handle = launch_stream(stream, x, codes, scales)
+    span *= 2 if code else 4
     if columns:
-        _native.call("mb_mx_quantize_columns", code, x.data_ptr(), span, k, rows, stride, *out)
+        status = library().mb_mx_quantize_columns(code, x.data_ptr(), span, x_rows, x_columns, stride,
+                                                  codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
+                                                  handle)
     else:
-        _native.call("mb_mx_quantize", code, x.data_ptr(), span, rows, k, stride, None, 0, 1, rows, *out)
+        status = library().mb_mx_quantize(code, x.data_ptr(), span, rows, k, stride, None, 0, 1, rows,
+                                          codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(), handle)
+    if status:
+        _native.check(status)
     return packed
 
 
 def dequantize(packed: Packed, out=None, stream=None):
     """The values of an operand [rows][k]: bfloat16 (exact) unless `out` is of another type."""
     _check_experts(packed, "packed", None)
-    dtype = torch.bfloat16 if out is None else out.dtype
-    out = check_output(out, "out", (packed.rows, packed.k), dtype, packed.codes.device)
+    codes, scales, rows, k = packed.codes, packed.scales, packed.rows, packed.k
+    out = check_output(out, "out", (rows, k), torch.bfloat16 if out is None else out.dtype, codes)
     code = dtype_code(out, "out")
-    check_device(packed.codes, packed.scales, out)
-    _native.call("mb_mx_dequantize", code, packed.codes.data_ptr(), packed.codes.numel(), packed.scales.data_ptr(),
-                 packed.scales.numel(), out.data_ptr(), bytes_of(out), packed.rows, packed.k,
-                 _native.stream_handle(stream))
+    handle = launch_stream(stream, codes, scales, out)
+    status = library().mb_mx_dequantize(code, codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
+                                        out.data_ptr(), rows * k * (2 if code else 4), rows, k, handle)
+    if status:
+        _native.check(status)
     return out
 
 
@@ -153,36 +165,39 @@ def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=Non
         raise ValueError(f"a and b must have the same k, not {a.k} and {b.k}")
     if dtype is None:
         dtype = torch.bfloat16 if out is None else out.dtype
-    out = check_output(out, "out", (a.rows, b.rows), dtype, a.codes.device)
+    out = check_output(out, "out", (a.rows, b.rows), dtype, a.codes)
     code = dtype_code(out, "out")
     _check_indices(offsets, "offsets")
-    check_device(a.codes, a.scales, b.codes, b.scales, out, *(() if offsets is None else (offsets,)))
-    _native.call("mb_mx_product", code, a.codes.data_ptr(), a.codes.numel(), a.scales.data_ptr(), a.scales.numel(),
-                 b.codes.data_ptr(), b.codes.numel(), b.scales.data_ptr(), b.scales.numel(), out.data_ptr(),
-                 bytes_of(out), a.rows, b.rows, a.k, *_pointer(offsets), experts or 1, _native.stream_handle(stream))
+    handle = launch_stream(stream, a.codes, a.scales, b.codes, b.scales, out, *(() if offsets is None else (offsets,)))
+    status = library().mb_mx_product(
+        code, a.codes.data_ptr(), a.codes.numel(), a.scales.data_ptr(), a.scales.numel(), b.codes.data_ptr(),
+        b.codes.numel(), b.scales.data_ptr(), b.scales.numel(), out.data_ptr(), a.rows * b.rows * (2 if code else 4),
+        a.rows, b.rows, a.k, *_pointer(offsets), experts or 1, handle)
+    if status:
+        _native.check(status)
     return out
 
 
 def _check_indices(tensor, what: str) -> None:
-    if tensor is not None and (tensor.dtype != torch.int32 or not tensor.is_contiguous()):
+    if tensor is not None and (tensor.dtype is not torch.int32 or not tensor.is_contiguous()):
         raise ValueError(f"{what} must be a contiguous int32 tensor, not {tensor.dtype}")
 
 
 def _pointer(tensor) -> tuple[int | None, int]:
-    return (None, 0) if tensor is None else (tensor.data_ptr(), bytes_of(tensor))
+    return (None, 0) if tensor is None else (tensor.data_ptr(), 4 * tensor.numel())
 
 
-def _workspace(tensor, needed: int, device):
+def _workspace(tensor, needed: int, like):
     if tensor is None:
-        return torch.empty(needed, dtype=torch.uint8, device=device)
-    if tensor.dtype != torch.uint8 or not tensor.is_contiguous() or tensor.numel() < needed:
+        return torch.empty(needed, dtype=torch.uint8, device=like.device)
+    if tensor.dtype is not torch.uint8 or not tensor.is_contiguous() or tensor.numel() < needed:
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {needed} bytes")
     return tensor
 
 
 def linear_workspace(rows: int, n: int, k: int, dtype, experts: int = 1, device="cuda"):
     """A workspace for `linear` with `rows` output rows (routed ones, with a plan)."""
-    return torch.empty(_native.load().mb_mx_linear_workspace(rows, n, k), dtype=torch.uint8, device=device)
+    return torch.empty(library().mb_mx_linear_workspace(rows, n, k), dtype=torch.uint8, device=device)
 
 
 def linear(x, weight: Packed, out=None, plan=None, sorted_rows: bool = False, workspace=None, stream=None):
@@ -193,13 +208,12 @@ def linear(x, weight: Packed, out=None, plan=None, sorted_rows: bool = False, wo
     from plan.offsets[experts] on are not written.
     """
     code = dtype_code(x, "x")
-    stride, span = strided_rows(x, "x")
-    rows, k = x.shape
+    rows, k, stride, span = strided_rows(x, "x")
     offsets = order = slots = None
-    copies, experts = 1, None
+    copies, experts, indices = 1, None, ()
     if plan is not None:
         offsets = plan.offsets
-        experts = offsets.numel() - 1
+        experts, indices = offsets.numel() - 1, (offsets,)
         _check_indices(offsets, "plan.offsets")
         if not sorted_rows:
             order, slots = plan.order, plan.slots
@@ -207,47 +221,33 @@ def linear(x, weight: Packed, out=None, plan=None, sorted_rows: bool = False, wo
             _check_indices(slots, "plan.slots")
             if slots.dim() != 2 or slots.shape[0] != rows or order.numel() != slots.numel():
                 raise ValueError(f"the plan must route {rows} tokens, not slots of {tuple(slots.shape)}")
-            copies = slots.shape[1]
-        check_device(offsets, *(() if sorted_rows else (order, slots)))
+            copies, indices = slots.shape[1], (offsets, order, slots)
     elif sorted_rows:
         raise ValueError("sorted rows need the plan that they are sorted by")
     _check_experts(weight, "weight", experts)
     if weight.k != k:
         raise ValueError(f"the weight must have k = {k}, not {weight.k}")
-    n, routed = weight.rows, rows * copies
-    out = check_output(out, "out", (routed, n), x.dtype, x.device)
-    library = _native.load()
-    workspace = _workspace(workspace, library.mb_mx_linear_workspace(routed, n, k), x.device)
-    check_device(x, weight.codes, weight.scales, out, workspace)
-    _native.check(library.mb_mx_linear(
-        code, x.data_ptr(), span, rows, stride, weight.codes.data_ptr(), weight.codes.numel(),
-        weight.scales.data_ptr(), weight.scales.numel(), out.data_ptr(), bytes_of(out), n, k, *_pointer(offsets),
+    n, routed, codes, scales = weight.rows, rows * copies, weight.codes, weight.scales
+    out = check_output(out, "out", (routed, n), x.dtype, x)
+    native = library()
+    workspace = _workspace(workspace, native.mb_mx_linear_workspace(routed, n, k), x)
+    handle = launch_stream(stream, x, codes, scales, out, workspace, *indices)
+    item = 2 if code else 4
+    status = native.mb_mx_linear(
+        code, x.data_ptr(), span * item, rows, stride, codes.data_ptr(), codes.numel(), scales.data_ptr(),
+        scales.numel(), out.data_ptr(), routed * n * item, n, k, *_pointer(offsets),
         None if order is None else order.data_ptr(), *_pointer(slots), copies, experts or 1, workspace.data_ptr(),
-        workspace.numel(), _native.stream_handle(stream)))
+        workspace.numel(), handle)
+    if status:
+        _native.check(status)
     return out
-
-
-def _operand_bytes(rows: int, k: int) -> int:
-    """Bytes of an operand's codes and scales, each on 16 bytes."""
-    return -(-rows * (-(-k // GROUP) * 16) // 16) * 16 + -(-rows * (-(-k // STEP) * 8) // 16) * 16
-
-
-def _carve(workspace, at: int, rows: int, k: int) -> Packed:
-    codes = rows * (-(-k // GROUP) * 16)
-    start = at + -(-codes // 16) * 16
-    scales = rows * (-(-k // STEP) * 8)
-    return Packed(workspace[at:at + codes].view(rows, -(-k // GROUP) * 16),
-                  workspace[start:start + scales].view(-(-k // STEP), rows, 8), k)
 
 
 def linear_backward_workspace(rows: int, n: int, k: int, dtype, device="cuda"):
     """A workspace for `linear_backward`, and for `linear` of the same sizes."""
-    needed = max(_backward_bytes(rows, n, k), _native.load().mb_mx_linear_workspace(rows, n, k))
-    return torch.empty(needed, dtype=torch.uint8, device=device)
-
-
-def _backward_bytes(rows: int, n: int, k: int) -> int:
-    return _operand_bytes(rows, n) + _operand_bytes(n, rows) + _operand_bytes(k, rows)
+    native = library()
+    return torch.empty(max(native.mb_mx_linear_backward_workspace(rows, n, k),
+                           native.mb_mx_linear_workspace(rows, n, k)), dtype=torch.uint8, device=device)
 
 
 def linear_backward(d_out, x, weight_columns: Packed, d_x=None, d_weight=None, workspace=None, stream=None):
@@ -256,24 +256,29 @@ def linear_backward(d_out, x, weight_columns: Packed, d_x=None, d_weight=None, w
     d_x = Q(d_out) . W with `weight_columns` = quantize(w, columns=True); d_weight = d_out^T . x, both quantised
     along the rows that the sum runs over.
     """
-    rows, n = d_out.shape
-    k = x.shape[1] if x.dim() == 2 else -1
-    if d_out.dtype != x.dtype or x.dim() != 2 or x.shape[0] != rows:
+    code = dtype_code(x, "x")
+    rows, n, d_stride, d_span = strided_rows(d_out, "d_out")
+    x_rows, k, x_stride, x_span = strided_rows(x, "x")
+    if d_out.dtype is not x.dtype or x_rows != rows:
         raise ValueError(f"d_out and x must be of one type and number of rows, not {d_out.dtype} of "
                          f"{tuple(d_out.shape)} and {x.dtype} of {tuple(x.shape)}")
-    if (weight_columns.rows, weight_columns.k) != (k, n):
+    _check_experts(weight_columns, "weight_columns", None)
+    if weight_columns.rows != k or weight_columns.k != n:
         raise ValueError(f"weight_columns must be an operand of {k} x {n} (the weight quantised by columns), not "
                          f"{weight_columns.rows} x {weight_columns.k}")
-    workspace = _workspace(workspace, _backward_bytes(rows, n, k), x.device)
-    if not rows:
-        d_weight = check_output(d_weight, "d_weight", (n, k), x.dtype, x.device)
-        return check_output(d_x, "d_x", (rows, k), x.dtype, x.device), d_weight.zero_()
-    by_rows = _carve(workspace, 0, rows, n)
-    d_columns = _carve(workspace, _operand_bytes(rows, n), n, rows)
-    x_columns = _carve(workspace, _operand_bytes(rows, n) + _operand_bytes(n, rows), k, rows)
-    quantize(d_out, by_rows, stream=stream)
-    quantize(d_out, d_columns, columns=True, stream=stream)
-    quantize(x, x_columns, columns=True, stream=stream)
-    d_x = product(by_rows, weight_columns, d_x, dtype=x.dtype, stream=stream)
-    d_weight = product(d_columns, x_columns, d_weight, dtype=x.dtype, stream=stream)
+    d_x = check_output(d_x, "d_x", (rows, k), x.dtype, x)
+    d_weight = check_output(d_weight, "d_weight", (n, k), x.dtype, x)
+    if not rows or not n or not k:
+        return d_x.zero_(), d_weight.zero_()
+    native = library()
+    workspace = _workspace(workspace, native.mb_mx_linear_backward_workspace(rows, n, k), x)
+    codes, scales = weight_columns.codes, weight_columns.scales
+    handle = launch_stream(stream, d_out, x, codes, scales, d_x, d_weight, workspace)
+    item = 2 if code else 4
+    status = native.mb_mx_linear_backward(
+        code, d_out.data_ptr(), d_span * item, d_stride, x.data_ptr(), x_span * item, x_stride, codes.data_ptr(),
+        codes.numel(), scales.data_ptr(), scales.numel(), d_x.data_ptr(), rows * k * item, d_weight.data_ptr(),
+        n * k * item, rows, n, k, workspace.data_ptr(), workspace.numel(), handle)
+    if status:
+        _native.check(status)
     return d_x, d_weight

@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
-from .mx import bytes_of, check_device, check_output, dtype_code, strided_rows
+from .mx import check_output, check_tensor, dtype_code, launch_stream, library, strided_rows
 
 SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -47,18 +47,21 @@ def route(logits, top: int, bias=None, scores: str = "softmax", groups: int = 1,
     by their sum if `renormalize`, times `scale`.
     """
     code = dtype_code(logits, "logits")
-    stride, span = strided_rows(logits, "logits")
-    tokens, count = logits.shape
-    experts = check_output(experts, "experts", (tokens, top), torch.int32, logits.device)
-    weights = check_output(weights, "weights", (tokens, top), torch.float32, logits.device)
-    if bias is not None:
-        bias = check_output(bias, "bias", (count,), torch.float32, logits.device)
-        check_device(bias)
-    check_device(logits, experts, weights)
-    _native.call("mb_route", code, logits.data_ptr(), span, tokens, count, stride,
-                 None if bias is None else bias.data_ptr(), 0 if bias is None else bytes_of(bias), top,
-                 _score_code(scores), groups, top_groups, int(renormalize), scale, experts.data_ptr(),
-                 bytes_of(experts), weights.data_ptr(), bytes_of(weights), _native.stream_handle(stream))
+    tokens, count, stride, span = strided_rows(logits, "logits")
+    experts = check_output(experts, "experts", (tokens, top), torch.int32, logits)
+    weights = check_output(weights, "weights", (tokens, top), torch.float32, logits)
+    if bias is None:
+        handle = launch_stream(stream, logits, experts, weights)
+    else:
+        check_tensor(bias, "bias", (count,), torch.float32)
+        handle = launch_stream(stream, logits, experts, weights, bias)
+    entries = 4 * tokens * top
+    status = library().mb_route(code, logits.data_ptr(), span * (2 if code else 4), tokens, count, stride,
+                                None if bias is None else bias.data_ptr(), 4 * count, top, _score_code(scores), groups,
+                                top_groups, int(renormalize), scale, experts.data_ptr(), entries, weights.data_ptr(),
+                                entries, handle)
+    if status:
+        _native.check(status)
     return experts, weights
 
 
@@ -66,24 +69,27 @@ def route_backward(logits, experts, d_weights, scores: str = "softmax", renormal
                    d_logits=None, stream=None):
     """d_logits, in the logits' type, for the gradient d_weights of route's weights and the experts it chose."""
     code = dtype_code(logits, "logits")
-    stride, span = strided_rows(logits, "logits")
-    tokens, count = logits.shape
+    tokens, count, stride, span = strided_rows(logits, "logits")
     if experts.dim() != 2 or experts.shape[0] != tokens:
         raise ValueError(f"experts must be [{tokens}][top], not {tuple(experts.shape)}")
     top = experts.shape[1]
-    check_output(experts, "experts", (tokens, top), torch.int32, logits.device)
-    check_output(d_weights, "d_weights", (tokens, top), torch.float32, logits.device)
-    d_logits = check_output(d_logits, "d_logits", (tokens, count), logits.dtype, logits.device)
-    check_device(logits, experts, d_weights, d_logits)
-    _native.call("mb_route_backward", code, logits.data_ptr(), span, tokens, count, stride, experts.data_ptr(),
-                 bytes_of(experts), d_weights.data_ptr(), bytes_of(d_weights), top, _score_code(scores),
-                 int(renormalize), scale, d_logits.data_ptr(), bytes_of(d_logits), _native.stream_handle(stream))
+    check_tensor(experts, "experts", (tokens, top), torch.int32)
+    check_tensor(d_weights, "d_weights", (tokens, top), torch.float32)
+    d_logits = check_output(d_logits, "d_logits", (tokens, count), logits.dtype, logits)
+    handle = launch_stream(stream, logits, experts, d_weights, d_logits)
+    item, entries = 2 if code else 4, 4 * tokens * top
+    status = library().mb_route_backward(code, logits.data_ptr(), span * item, tokens, count, stride,
+                                         experts.data_ptr(), entries, d_weights.data_ptr(), entries, top,
+                                         _score_code(scores), int(renormalize), scale, d_logits.data_ptr(),
+                                         tokens * count * item, handle)
+    if status:
+        _native.check(status)
     return d_logits
 
 
 def empty_plan(tokens: int, top: int, experts: int, device="cuda") -> Plan:
     """A plan's buffers and workspace, for `dispatch` to fill."""
-    needed = _native.load().mb_dispatch_workspace(tokens * top, experts)
+    needed = library().mb_dispatch_workspace(tokens * top, experts)
     return Plan(torch.empty(experts + 1, dtype=torch.int32, device=device),
                 torch.empty(tokens * top, dtype=torch.int32, device=device),
                 torch.empty((tokens, top), dtype=torch.int32, device=device),
@@ -95,53 +101,64 @@ def dispatch(experts, count: int, plan: Plan | None = None, stream=None) -> Plan
     if experts.dim() != 2:
         raise ValueError(f"experts must be [tokens][top], not {tuple(experts.shape)}")
     tokens, top = experts.shape
-    check_output(experts, "experts", (tokens, top), torch.int32, experts.device)
+    entries = tokens * top
+    check_tensor(experts, "experts", (tokens, top), torch.int32)
     if plan is None:
         plan = empty_plan(tokens, top, count, experts.device)
-    check_output(plan.offsets, "plan.offsets", (count + 1,), torch.int32, experts.device)
-    check_output(plan.order, "plan.order", (tokens * top,), torch.int32, experts.device)
-    check_output(plan.slots, "plan.slots", (tokens, top), torch.int32, experts.device)
-    workspace = plan.workspace
-    check_device(experts, plan.offsets, plan.order, plan.slots, *(() if workspace is None else (workspace,)))
-    _native.call("mb_dispatch", experts.data_ptr(), bytes_of(experts), tokens * top, count, plan.offsets.data_ptr(),
-                 bytes_of(plan.offsets), plan.order.data_ptr(), bytes_of(plan.order), plan.slots.data_ptr(),
-                 bytes_of(plan.slots), None if workspace is None else workspace.data_ptr(),
-                 0 if workspace is None else bytes_of(workspace), _native.stream_handle(stream))
+    offsets, order, slots, workspace = plan
+    check_tensor(offsets, "plan.offsets", (count + 1,), torch.int32)
+    check_tensor(order, "plan.order", (entries,), torch.int32)
+    check_tensor(slots, "plan.slots", (tokens, top), torch.int32)
+    if workspace is None:
+        handle, space = launch_stream(stream, experts, offsets, order, slots), (None, 0)
+    else:
+        handle = launch_stream(stream, experts, offsets, order, slots, workspace)
+        space = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    status = library().mb_dispatch(experts.data_ptr(), 4 * entries, entries, count, offsets.data_ptr(), 4 * count + 4,
+                                   order.data_ptr(), 4 * entries, slots.data_ptr(), 4 * entries, *space, handle)
+    if status:
+        _native.check(status)
     return plan
 
 
 def _combine_sizes(y, slots, weights):
-    if y.dim() != 2 or slots.dim() != 2:
-        raise ValueError(f"y must be [rows][n] and slots [tokens][top], not {tuple(y.shape)} and {tuple(slots.shape)}")
-    check_output(y, "y", y.shape, y.dtype, y.device)
-    check_output(slots, "slots", slots.shape, torch.int32, y.device)
-    check_output(weights, "weights", slots.shape, torch.float32, y.device)
-    check_device(y, slots, weights)
-    return dtype_code(y, "y"), *y.shape, *slots.shape
+    if y.dim() != 2 or slots.dim() != 2 or not y.is_contiguous():
+        raise ValueError(f"y must be contiguous [rows][n] and slots [tokens][top], not {tuple(y.shape)} and "
+                         f"{tuple(slots.shape)}")
+    shape = slots.shape
+    check_tensor(slots, "slots", shape, torch.int32)
+    check_tensor(weights, "weights", shape, torch.float32)
+    return dtype_code(y, "y"), *y.shape, *shape
 
 
 def combine(y, slots, weights, out=None, stream=None):
     """out[t] = the sum over j of weights[t][j] * y[slots[t][j]], in y's type; slots of -1 are left out."""
     code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
-    out = check_output(out, "out", (tokens, n), y.dtype, y.device)
-    check_device(out)
-    _native.call("mb_combine", code, y.data_ptr(), bytes_of(y), rows, slots.data_ptr(), bytes_of(slots),
-                 weights.data_ptr(), bytes_of(weights), out.data_ptr(), bytes_of(out), tokens, top, n,
-                 _native.stream_handle(stream))
+    out = check_output(out, "out", (tokens, n), y.dtype, y)
+    handle = launch_stream(stream, y, slots, weights, out)
+    item, entries = 2 if code else 4, 4 * tokens * top
+    status = library().mb_combine(code, y.data_ptr(), rows * n * item, rows, slots.data_ptr(), entries,
+                                  weights.data_ptr(), entries, out.data_ptr(), tokens * n * item, tokens, top, n,
+                                  handle)
+    if status:
+        _native.check(status)
     return out
 
 
 def combine_backward(d_out, y, slots, weights, d_y=None, d_weights=None, stream=None):
     """(d_y, d_weights) of combine for the gradient d_out; rows of a given d_y that no slot names stay as they are."""
     code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
-    check_output(d_out, "d_out", (tokens, n), y.dtype, y.device)
+    check_tensor(d_out, "d_out", (tokens, n), y.dtype)
     if d_y is None:
         d_y = torch.zeros_like(y)
-    check_output(d_y, "d_y", (rows, n), y.dtype, y.device)
-    d_weights = check_output(d_weights, "d_weights", (tokens, top), torch.float32, y.device)
-    check_device(d_out, d_y, d_weights)
-    _native.call("mb_combine_backward", code, d_out.data_ptr(), bytes_of(d_out), y.data_ptr(), bytes_of(y), rows,
-                 slots.data_ptr(), bytes_of(slots), weights.data_ptr(), bytes_of(weights), d_y.data_ptr(),
-                 bytes_of(d_y), d_weights.data_ptr(), bytes_of(d_weights), tokens, top, n,
-                 _native.stream_handle(stream))
+    check_tensor(d_y, "d_y", (rows, n), y.dtype)
+    d_weights = check_output(d_weights, "d_weights", (tokens, top), torch.float32, y)
+    handle = launch_stream(stream, y, slots, weights, d_out, d_y, d_weights)
+    item, entries = 2 if code else 4, 4 * tokens * top
+    status = library().mb_combine_backward(code, d_out.data_ptr(), tokens * n * item, y.data_ptr(), rows * n * item,
+                                           rows, slots.data_ptr(), entries, weights.data_ptr(), entries,
+                                           d_y.data_ptr(), rows * n * item, d_weights.data_ptr(), entries, tokens, top,
+                                           n, handle)
+    if status:
+        _native.check(status)
     return d_y, d_weights
