@@ -81,8 +81,14 @@ __global__ void __launch_bounds__(256)
 // Columns of x to the rows of the transposed operand: groups of 32 run along
 // x's rows. A workgroup takes 256 rows of 128 columns, a wave a group of 32
 // rows, a lane two neighbouring columns, so that a group's largest magnitude
-// needs no other lane; the codes cross LDS, so that an operand row's 128 bytes
-// leave together.
+// needs no other lane and stays packed; the codes cross LDS, so that an operand
+// row's 128 bytes leave together.
+//
+// Bound by the memory's rate for 256 bytes a row: 8192x8192 bf16 36.9 us from HBM
+// (4.6 TB/s; with 512 bytes a row 37.5), 25.0 from the memory-side cache (6.8).
+// Rows off the lines lose if neighbouring strips run on different XCDs (8192x8190
+// 48.9 us, so 39.0). A column at a time and unpacked took 20 instructions an
+// element and 54 us from the cache.
 constexpr int kTileColumns = 128, kTilePitch = 128 + 16;  // LDS bytes of a column, a bank group apart
 
 // 32 rows of two columns, a pair a row as it is stored.
@@ -140,7 +146,7 @@ __device__ __forceinline__ void quantize_column(const ColumnPairs<T>& values, ui
   *scale_at = static_cast<uint8_t>(scale);
 }
 
-template <class T>
+template <class T, bool STREAM>
 __global__ void __launch_bounds__(512)
     mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -149,7 +155,10 @@ __global__ void __launch_bounds__(512)
   using Pair = typename ColumnPairs<T>::Pair;
   const uint32_t groups = (rows + kGroup - 1) / kGroup;
   const uint32_t strips = (columns + kTileColumns - 1) / kTileColumns;
-  const uint32_t strip = blockIdx.x % strips, block = blockIdx.x / strips;
+  // XCD c (workgroups c, c + 8, ..) takes neighbouring strips, whose pieces of a row share lines.
+  const uint32_t xcd = blockIdx.x % 8, count = gridDim.x;
+  const uint32_t pid = xcd * (count / 8) + min(xcd, count % 8) + blockIdx.x / 8;
+  const uint32_t strip = pid % strips, block = pid / strips;
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t local = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t group = block * 8 + local, column = lane * 2;
@@ -160,7 +169,10 @@ __global__ void __launch_bounds__(512)
     ColumnPairs<T> values;
     if (row0 + kGroup <= rows && live == kTileColumns) {
 #pragma unroll
-      for (int r = 0; r < 32; ++r, from += row_stride) values.at[r] = *reinterpret_cast<const Pair*>(from + column);
+      for (int r = 0; r < 32; ++r, from += row_stride) {
+        const Pair* pair = reinterpret_cast<const Pair*>(from + column);
+        values.at[r] = STREAM ? __builtin_nontemporal_load(pair) : *pair;
+      }
     } else {
 #pragma unroll
       for (int r = 0; r < 32; ++r, from += row_stride) {
@@ -184,9 +196,13 @@ __global__ void __launch_bounds__(512)
   const uint64_t first = strip * uint64_t{kTileColumns};
   for (uint32_t i = threadIdx.x; i < live * 8; i += 512) {
     const uint32_t c = i / 8, chunk = i % 8;
-    if (block * 8 + chunk < groups)
-      *reinterpret_cast<elem_u32x4*>(codes + ((first + c) * groups + block * 8 + chunk) * 16) =
-          *reinterpret_cast<const elem_u32x4*>(tile + c * kTilePitch + chunk * 16);
+    if (block * 8 + chunk >= groups) continue;
+    elem_u32x4* to = reinterpret_cast<elem_u32x4*>(codes + ((first + c) * groups + block * 8 + chunk) * 16);
+    const elem_u32x4 word = *reinterpret_cast<const elem_u32x4*>(tile + c * kTilePitch + chunk * 16);
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(word, to);
+    else
+      *to = word;
   }
   if (threadIdx.x < live)
     *reinterpret_cast<elem_u32x2*>(scales + (block * uint64_t{columns} + first + threadIdx.x) * 8) =
@@ -220,7 +236,8 @@ __global__ void __launch_bounds__(256)
   MB_REGISTER_KERNEL("mx_quantize_" NAME "_512", (mx_quantize_kernel<T, 1, false>));           \
   MB_REGISTER_KERNEL("mx_quantize_" NAME "_1024", (mx_quantize_kernel<T, 2, false>));          \
   MB_REGISTER_KERNEL("mx_quantize_" NAME "_1024_stream", (mx_quantize_kernel<T, 2, true>));    \
-  MB_REGISTER_KERNEL("mx_quantize_columns_" NAME, mx_quantize_columns_kernel<T>); \
+  MB_REGISTER_KERNEL("mx_quantize_columns_" NAME, (mx_quantize_columns_kernel<T, false>));     \
+  MB_REGISTER_KERNEL("mx_quantize_columns_" NAME "_stream", (mx_quantize_columns_kernel<T, true>)); \
   MB_REGISTER_KERNEL("mx_dequantize_" NAME, (mx_dequantize_kernel<T, false>)); \
   MB_REGISTER_KERNEL("mx_dequantize_" NAME "_stream", (mx_dequantize_kernel<T, true>))
 MB_MX_REGISTER(float, "f32");
@@ -284,9 +301,18 @@ int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint32_t co
   const uint64_t grid = (columns + uint64_t{kTileColumns} - 1) / kTileColumns * ((rows + uint64_t{kBlock} - 1) / kBlock);
   if (grid > 0x7fffffu)
     return fail(MB_ERR_UNSUPPORTED, "mx_quantize_columns: %u x %u exceeds one launch", rows, columns);
-  MB_FOR_DTYPE(dtype, (mx_quantize_columns_kernel<T><<<dim3(static_cast<uint32_t>(grid)), dim3(512), 0, stream>>>(
-                          static_cast<const T*>(x), rows, columns, row_stride, static_cast<uint8_t*>(codes),
-                          static_cast<uint8_t*>(scales))));
+  auto launch = [&](auto kernel, auto t) {
+    kernel<<<dim3(static_cast<uint32_t>(grid)), dim3(512), 0, stream>>>(
+        static_cast<const decltype(t)*>(x), rows, columns, row_stride, static_cast<uint8_t*>(codes),
+        static_cast<uint8_t*>(scales));
+  };
+  const bool streamed = streams(mx_code_bytes(columns, rows));
+  MB_FOR_DTYPE(dtype, {
+    if (streamed)
+      launch(mx_quantize_columns_kernel<T, true>, T());
+    else
+      launch(mx_quantize_columns_kernel<T, false>, T());
+  });
   return launch_status("mx_quantize_columns");
 }
 
