@@ -386,31 +386,31 @@ struct ProductCost {
 // A kernel of BM features by BN rows a tile.
 struct ProductKernel {
   int features, rows;
-  int stages;    // of a persistent kernel, which K must exceed; 0 for the others
+  bool persistent;
   int band;      // row tiles that share their weight's panels in an XCD's L2
   int resident;  // workgroups a CU holds
   ProductCost cost;
   ProductLauncher launch[3];  // by MB_DTYPE_*
 };
-#define MB_PRODUCT(KIND, BM, BN, STAGES, PERSISTENT, BAND, ...)                                  \
+constexpr bool kPersistent_ring = false, kPersistent_stream = true;
+#define MB_PRODUCT(KIND, BM, BN, STAGES, BAND, ...)                                              \
   ProductKernel {                                                                                \
-    BM, BN, PERSISTENT, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, {__VA_ARGS__}, {    \
+    BM, BN, kPersistent_##KIND, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, {__VA_ARGS__}, {    \
       launch_##KIND<float, BM, BN, STAGES>, launch_##KIND<_Float16, BM, BN, STAGES>,             \
           launch_##KIND<__bf16, BM, BN, STAGES>                                                  \
     }                                                                                            \
   }
-// Fitted to 582 launches on an MI355X (17 to 32768 rows, n and K from 64 to 8192,
+// Fitted to 414 launches on an MI355X (17 to 32768 rows, n and K from 64 to 8192,
 // one weight or 8 to 256 experts of uneven popularity, half of the n odd): the
-// cheapest estimate costs 1.3% over the fastest of the five on average, over 10%
-// in one launch of 26, 27% at most. Twelve kernels were measured; these five's
-// best is 0.8% over the twelve's, the ring's 256x128, two 128x128 and 64x64 alone
-// 6%.
+// cheapest estimate costs 2.1% over the fastest of the five on average, over 10%
+// in one launch of 17, at most 38% (2 us). Ten kernels were measured; these five's
+// best is 0.8% over the ten's, the two that are not persistent alone 12%.
 const ProductKernel kProductKernels[] = {
-    MB_PRODUCT(ring, 128, 128, 2, 0, 8, 1.62f, 3.71f, 0.40f, 0.349f, 1.485f),
-    MB_PRODUCT(ring, 64, 64, 3, 0, 8, 2.28f, 3.18f, 0.19f, 0.083f, 0.513f),
-    MB_PRODUCT(stream, 256, 128, 3, 3, 4, 4.70f, 2.38f, 1.47f, 0.510f, 1.380f),
-    MB_PRODUCT(stream, 128, 64, 3, 3, 8, 3.73f, 1.39f, 0.45f, 0.233f, 1.085f),
-    MB_PRODUCT(stream, 64, 64, 2, 2, 8, 3.36f, 1.74f, 0.34f, 0.172f, 1.678f),
+    MB_PRODUCT(ring, 128, 128, 2, 8, 2.10f, 3.59f, 0.25f, 0.303f, 1.426f),
+    MB_PRODUCT(ring, 64, 64, 3, 8, 2.90f, 2.86f, 0.12f, 0.056f, 0.495f),
+    MB_PRODUCT(stream, 256, 128, 3, 4, 5.45f, 2.34f, 1.66f, 0.510f, 1.204f),
+    MB_PRODUCT(stream, 128, 64, 3, 8, 5.31f, 0.90f, 0.48f, 0.179f, 0.918f),
+    MB_PRODUCT(stream, 64, 64, 3, 8, 4.84f, 0.83f, 0.28f, 0.102f, 0.768f),
 };
 
 #define MB_PRODUCT_REGISTER(T, NAME)                                                                        \
@@ -419,7 +419,7 @@ const ProductKernel kProductKernels[] = {
   MB_REGISTER_KERNEL("mx_product_" NAME "_64x64", (mx_product_ring_kernel<T, 64, 64, 3>));                  \
   MB_REGISTER_KERNEL("mx_product_" NAME "_256x128_stream", (mx_product_stream_kernel<T, 256, 128, 3>));     \
   MB_REGISTER_KERNEL("mx_product_" NAME "_128x64_stream", (mx_product_stream_kernel<T, 128, 64, 3>));       \
-  MB_REGISTER_KERNEL("mx_product_" NAME "_64x64_stream", (mx_product_stream_kernel<T, 64, 64, 2>))
+  MB_REGISTER_KERNEL("mx_product_" NAME "_64x64_stream", (mx_product_stream_kernel<T, 64, 64, 3>))
 #define MB_FEW_REGISTER_SPLIT(T, NAME, FB, SPLIT, SIZE)                                             \
   MB_REGISTER_KERNEL("mx_linear_few_" NAME "_" SIZE, (mx_few_kernel<T, T, FB, SPLIT>));            \
   MB_REGISTER_KERNEL("mx_product_few_" NAME "_" SIZE, (mx_few_kernel<uint8_t, T, FB, SPLIT>))
@@ -547,7 +547,7 @@ int launch_product(int dtype, const void* x_codes, const void* sx, const void* w
     for (const ProductKernel& kernel : kProductKernels) {
       const uint64_t grid = most_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
       if (grid > 0xffffff) continue;
-      if (kernel.stages && (steps <= static_cast<uint32_t>(kernel.stages) || experts > kStreamExperts)) continue;
+      if (kernel.persistent && experts > kStreamExperts) continue;
       const double cost = product_cost(kernel, rows, n, steps, experts, ragged);
       if (best == nullptr || cost < best_cost) best = &kernel, best_cost = cost, best_grid = grid;
     }
@@ -555,7 +555,7 @@ int launch_product(int dtype, const void* x_codes, const void* sx, const void* w
       best->launch[dtype](x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
                           offsets, static_cast<int>(experts), static_cast<uint32_t>((best_grid + 7) / 8 * 8),
                           best->band, stream);
-      return launch_status(best->stages ? "mx_product_stream" : "mx_product_ring");
+      return launch_status(best->persistent ? "mx_product_stream" : "mx_product_ring");
     }
   }
   const uint32_t tiles = (rows / experts + 15) / 16;

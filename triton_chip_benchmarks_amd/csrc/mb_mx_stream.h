@@ -85,7 +85,7 @@ struct RowTiles {
 // issued two steps before, after which one step's DMAs and, in the first two
 // steps of a tile, the stores of the tile before have been issued.
 //
-// K has more than STAGES steps, there are at most kStreamExperts experts.
+// There are at most kStreamExperts experts.
 template <class T, int BM, int BN, int STAGES>
 __global__ void __launch_bounds__(256)
     mx_product_stream_kernel(const uint8_t* __restrict__ x, const uint8_t* __restrict__ sx,
@@ -157,11 +157,11 @@ __global__ void __launch_bounds__(256)
   };
   int index = blockIdx.x / kXcds;
   if (index >= share) return;
-  // The DMAs reach at most the tile after the one multiplied, and enter it in one
-  // of that one's steps (k_steps > STAGES); past the last tile they load it once
-  // more.
-  At here = locate(index), next_at = locate(min(index + workers, share - 1));
+  // The DMAs run ahead of the products by STAGES steps, and tiles by as many as
+  // those make; past the last tile they load it once more.
+  At here = locate(index);
   Source from = source(here);
+  int dma_index = index;
   auto dma = [&](auto i_c, uint32_t stage) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
     const int kb = dma_step * ROWB;
@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(256)
   auto dma_advance = [&]() __attribute__((always_inline)) {
     if (++dma_step == k_steps) {
       dma_step = 0;
-      from = source(next_at);
+      dma_index += workers;
+      from = source(locate(min(dma_index, share - 1)));
     }
   };
 
@@ -297,11 +298,11 @@ __global__ void __launch_bounds__(256)
       });
   };
 
-  static_for<0, STAGES>([&](auto s_c) __attribute__((always_inline)) {
-    static_for<0, Tile::DMAS>(
-        [&](auto i_c) __attribute__((always_inline)) { dma(i_c, decltype(s_c)::value * Tile::STAGE); });
+#pragma unroll 1  // one copy of dma_advance
+  for (uint32_t at = 0; at < STAGES * Tile::STAGE; at += Tile::STAGE) {
+    static_for<0, Tile::DMAS>([&](auto i_c) __attribute__((always_inline)) { dma(i_c, at); });
     dma_advance();
-  });
+  }
   __builtin_amdgcn_s_waitcnt(vmcnt_only((STAGES - 1) * Tile::DMAS));
   lds_barrier();
   Set set0, set1;
@@ -355,8 +356,7 @@ __global__ void __launch_bounds__(256)
     with_stores = STAGES - 1;
     index += workers;
     if (index >= share) break;
-    here = next_at;
-    next_at = locate(min(index + workers, share - 1));
+    here = locate(index);
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_only(0));  // no DMA of a step past the last may land in a later workgroup's LDS
 #endif
