@@ -250,6 +250,99 @@ def test_experts(gpu, dtype, tokens, top, experts):
     assert torch.equal(again, out)
 
 
+# Sizes that run on every kernel of the products (256x128, 128x64 and 64x64 tiles, one or many a workgroup): K of one
+# step, of an odd number and with a last one in part, n off the pieces of 16 bytes, more tiles than places.
+TILED = [(4100, 4104, 1100), (2600, 3001, 300), (700, 2049, 255), (3000, 515, 5000), (130, 8190, 1056),
+         (20, 1000, 40), (90, 300, 7000), (9000, 131, 513)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,n,k", TILED)
+def test_products_of_many_tiles(gpu, dtype, rows, n, k):
+    """Against float64 on the device, from operands that the oracle's rules fix; twice, to the same bits."""
+    import torch
+
+    from triton_chip_benchmarks_amd import mx
+
+    print(f"product {dtype} {rows}x{n}x{k}", flush=True)
+    a, b = mx.quantize(_random(torch, dtype, rows, k, seed=1)), mx.quantize(_random(torch, dtype, n, k, seed=2))
+    va, vb = mx.dequantize(a).double(), mx.dequantize(b).double()
+    out = torch.full((rows, n), float("nan"), device="cuda", dtype=_dtype(torch, dtype))
+    mx.product(a, b, out)
+    expected, size = va @ vb.t().contiguous(), va.abs() @ vb.abs().t().contiguous()
+    bound = (k / 32 + 16) * 2.0**-23 * size
+    error = (out.double() - expected).abs()
+    assert bool((error <= bound + UNIT[dtype] * (expected.abs() + bound) + 2.0**-24).all()), error.max()
+    assert torch.equal(mx.product(a, b, dtype=out.dtype), out)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,experts,n,k", [(5000, 8, 1030, 600), (3000, 60, 264, 1025), (2000, 256, 136, 260),
+                                              (1500, 300, 72, 96), (4000, 4, 2056, 2300)])
+def test_products_of_many_experts(gpu, dtype, rows, experts, n, k):
+    """Uneven experts, some without a row; more of them than a wave's table holds; the rows behind stay."""
+    import torch
+
+    from triton_chip_benchmarks_amd import mx
+
+    print(f"product {dtype} {rows} of {experts} x {n}x{k}", flush=True)
+    generator = torch.Generator(device="cuda").manual_seed(experts)
+    share = torch.rand(experts, device="cuda", generator=generator) ** 4
+    share[1] = 0
+    counts = (share / share.sum() * (rows - 5)).long()
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+    offsets[1:] = counts.cumsum(0)
+    a = mx.quantize(_random(torch, dtype, rows, k, seed=1))
+    weights = [mx.quantize(_random(torch, dtype, n, k, seed=10 + e)) for e in range(experts)]
+    b = mx.Packed(torch.stack([w.codes for w in weights]), torch.stack([w.scales for w in weights]), k)
+    out = torch.full((rows, n), 7.0, device="cuda", dtype=_dtype(torch, dtype))
+    mx.product(a, b, out, offsets=offsets)
+    va, ends = mx.dequantize(a).double(), offsets.tolist()
+    for e in range(experts):
+        first, last = ends[e], ends[e + 1]
+        if last > first:
+            vb = mx.dequantize(weights[e]).double()
+            expected = va[first:last] @ vb.t().contiguous()
+            bound = (k / 32 + 16) * 2.0**-23 * (va[first:last].abs() @ vb.abs().t().contiguous())
+            error = (out[first:last].double() - expected).abs()
+            assert bool((error <= bound + UNIT[dtype] * (expected.abs() + bound) + 2.0**-24).all()), (e, error.max())
+    assert (out[ends[-1]:] == 7).all()
+
+
+def test_offsets_that_are_out_of_order_write_nothing_outside(gpu):
+    """Offsets past the rows, negative or falling are clamped: whatever lands in the output, nothing else is touched."""
+    import torch
+
+    from triton_chip_benchmarks_amd import mx
+
+    for rows in (8, 300):
+        guarded = torch.full((rows + 200, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+        a = mx.quantize(_random(torch, "bf16", rows, 96, seed=1))
+        b = mx.empty(64, 96, experts=4)
+        b.codes.zero_()
+        b.scales.fill_(127)
+        for offsets in ([0, -5, 10**6, 3, 2**31 - 1], [rows, 0, rows, 0, rows], [10**6] * 5):
+            mx.product(a, b, guarded[100:100 + rows], offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+            torch.cuda.synchronize()
+            assert (guarded[:100] == 7).all() and (guarded[100 + rows:] == 7).all()
+
+
+def test_a_weight_whose_scales_pass_32_bit_offsets(gpu):
+    """2^20 features of 257 K steps: 2.2 GB of scales, beyond the tiles' offsets."""
+    import torch
+
+    from triton_chip_benchmarks_amd import mx
+
+    n, k = 1 << 20, 257 * 256
+    b = mx.Packed(torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda"),
+                  torch.full((k // 256, n, 8), 127, dtype=torch.uint8, device="cuda"), k)
+    b.codes[n - 3] = 0x22  # ones
+    b.scales[256, n - 3] = 128  # twos in the last step
+    a = mx.quantize(torch.ones(17, k, device="cuda", dtype=torch.bfloat16))
+    out = mx.product(a, b, dtype=torch.float32)
+    assert (out[:, n - 3] == k + 256).all() and int(torch.count_nonzero(out)) == 17
+
+
 def test_empty_calls(gpu):
     import torch
 
