@@ -5,7 +5,9 @@ computations the reference suite uses to validate its kernels: the copy
 identity and read block sums (bench_bandwidth.py), the vector recurrences and
 their validators (bench_vector.py), the exact-lattice matrix references,
 tolerances and the OCP MX FP4 / FP8 formats (bench_tensor.py). Each function
-cites the reference file:line it follows.
+cites the reference file:line it follows. The operators of language models that
+the reference lacks (MXFP4 quantisation and linear layer, expert routing) are
+restated from their formulas, in float64.
 
 Only tests/, __graft_entry__.smoke() and bench.py's cpu_baseline leg may import
 it, and only as the checker or the timed CPU baseline. The product path
@@ -25,4 +27,8 @@ How each part is pinned (checks that a plausible mistake would fail):
              against torch.testing.assert_close and known answers a normwise
              rule would get wrong; the FP32/FP64 probe operands against the
              TF32/BF16/FP16/FP32 roundings they must expose.
+  mx       - the E2M1 table, nearest-even ties and saturation by known answers;
+             gradients against the formula written out and central differences.
+  routing  - known answers for ties, groups, masks and NaN; gradients against
+             central differences; a dispatch against its defining properties.
 """
