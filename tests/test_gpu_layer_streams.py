@@ -1,0 +1,72 @@
+"""Calls on a stream other than the current one: what they allocate is that stream's memory (the current stream's may
+still be in use, or be handed out again before the call's work is done), and the results are the same."""
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _calls(torch, mx, routing):
+    generator = torch.Generator(device="cuda").manual_seed(0)
+
+    def normal(*shape):
+        return torch.randn(shape, device="cuda", generator=generator).bfloat16()
+
+    def parts(operand):
+        return operand.codes, operand.scales
+
+    x, w, d_y, logits = normal(40, 96), normal(64, 96), normal(40, 64), normal(40, 8)
+    packed, columns = mx.quantize(w), mx.quantize(w, columns=True)
+    up = mx.empty(64, 96, experts=8)
+    for e in range(8):
+        mx.quantize(normal(64, 96), mx.Packed(up.codes[e], up.scales[e], 96))
+    chosen, weights = routing.route(logits, 2)
+    plan = routing.dispatch(chosen, 8)
+    y, d_out, d_weights = normal(80, 96), normal(40, 96), torch.rand(40, 2, device="cuda", generator=generator)
+    return {
+        "quantize": lambda stream: parts(mx.quantize(x, stream=stream)),
+        "quantize_columns": lambda stream: parts(mx.quantize(x, columns=True, stream=stream)),
+        "dequantize": lambda stream: (mx.dequantize(packed, stream=stream),),
+        "product": lambda stream: (mx.product(packed, packed, stream=stream),),
+        "linear": lambda stream: (mx.linear(x, packed, stream=stream),),
+        "routed": lambda stream: (mx.linear(x, up, plan=plan, stream=stream),),
+        "linear_backward": lambda stream: mx.linear_backward(d_y, x, columns, stream=stream),
+        "route": lambda stream: routing.route(logits, 2, stream=stream),
+        "route_backward": lambda stream: (routing.route_backward(logits, chosen, d_weights, stream=stream),),
+        "dispatch": lambda stream: routing.dispatch(chosen, 8, stream=stream)[:3],
+        "combine": lambda stream: (routing.combine(y, plan.slots, weights, stream=stream),),
+        "combine_backward": lambda stream: routing.combine_backward(d_out, y, plan.slots, weights, stream=stream),
+    }
+
+
+def test_outputs_and_workspaces_are_the_streams_memory(gpu, monkeypatch):
+    import torch
+
+    from triton_chip_benchmarks_amd import mx, routing
+
+    calls = _calls(torch, mx, routing)
+    side = torch.cuda.Stream()
+    made = []
+
+    def recorded(*arguments):
+        made.append(allocate(*arguments))
+        return made[-1]
+
+    allocate = mx.allocate
+    monkeypatch.setattr(mx, "allocate", recorded)
+    monkeypatch.setattr(routing, "allocate", recorded)
+    for name, call in calls.items():
+        print(f"streams {name}", flush=True)
+        here = [tensor.clone() for tensor in call(None)]
+        torch.cuda.synchronize()
+        del made[:]
+        there = call(side)
+        torch.cuda.synchronize()
+        segments = torch.cuda.memory_snapshot()
+        for tensor in (*made, *there):
+            if tensor.numel():
+                start = tensor.data_ptr()
+                owner = [s["stream"] for s in segments if s["address"] <= start < s["address"] + s["total_size"]]
+                assert owner == [side.cuda_stream], name
+        for mine, theirs in zip(here, there):
+            assert torch.equal(mine.view(torch.uint8), theirs.view(torch.uint8)), name

@@ -66,7 +66,20 @@ def launch_stream(stream, *tensors) -> int:
             raise ValueError(f"tensors must lie on one device, {tensors[0].device}, not {tensor.device}")
     if device < 0 or device != torch._C._cuda_getDevice():
         raise ValueError(f"tensors must lie on the current HIP device, not {tensors[0].device}")
-    return torch._C._cuda_getCurrentRawStream(device) if stream is None else stream.cuda_stream
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(device)
+    if stream.device_index != device:
+        raise ValueError(f"the stream must be of the tensors' device, {tensors[0].device}, not {stream.device}")
+    return stream.cuda_stream
+
+
+def allocate(shape, dtype, device, stream):
+    """A new tensor of the memory of the stream that the call runs on: the current stream's may be memory that it
+    still uses for earlier work, or hands out again before the call's work is done."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def library():
@@ -92,19 +105,19 @@ def check_tensor(tensor, what: str, shape, dtype) -> None:
                          f"{tuple(tensor.shape)}")
 
 
-def check_output(tensor, what: str, shape, dtype, like):
+def check_output(tensor, what: str, shape, dtype, like, stream):
     """`tensor`, checked, or a new one on the device of `like` in its place."""
     if tensor is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return allocate(shape, dtype, like.device, stream)
     check_tensor(tensor, what, shape, dtype)
     return tensor
 
 
-def empty(rows: int, k: int, device="cuda", experts: int | None = None) -> Packed:
+def empty(rows: int, k: int, device="cuda", experts: int | None = None, stream=None) -> Packed:
     """An operand's buffers, for `quantize` to fill."""
     lead = () if experts is None else (experts,)
-    return Packed(torch.empty((*lead, rows, -(-k // GROUP) * (GROUP // 2)), dtype=torch.uint8, device=device),
-                  torch.empty((*lead, -(-k // STEP), rows, STEP // GROUP), dtype=torch.uint8, device=device), k)
+    return Packed(allocate((*lead, rows, -(-k // GROUP) * (GROUP // 2)), torch.uint8, device, stream),
+                  allocate((*lead, -(-k // STEP), rows, STEP // GROUP), torch.uint8, device, stream), k)
 
 
 def _check_experts(packed: Packed, what: str, experts: int | None) -> None:
@@ -119,7 +132,7 @@ def quantize(x, packed: Packed | None = None, columns: bool = False, stream=None
     x_rows, x_columns, stride, span = strided_rows(x, "x")
     rows, k = (x_columns, x_rows) if columns else (x_rows, x_columns)
     if packed is None:
-        packed = empty(rows, k, x.device)
+        packed = empty(rows, k, x.device, stream=stream)
     _check_experts(packed, "packed", None)
     if packed.rows != rows or packed.k != k:
         raise ValueError(f"packed must be an operand of {rows} x {k}, not {packed.rows} x {packed.k}")
@@ -142,7 +155,7 @@ def dequantize(packed: Packed, out=None, stream=None):
     """The values of an operand [rows][k]: bfloat16 (exact) unless `out` is of another type."""
     _check_experts(packed, "packed", None)
     codes, scales, rows, k = packed.codes, packed.scales, packed.rows, packed.k
-    out = check_output(out, "out", (rows, k), torch.bfloat16 if out is None else out.dtype, codes)
+    out = check_output(out, "out", (rows, k), torch.bfloat16 if out is None else out.dtype, codes, stream)
     code = dtype_code(out, "out")
     handle = launch_stream(stream, codes, scales, out)
     status = library().mb_mx_dequantize(code, codes.data_ptr(), codes.numel(), scales.data_ptr(), scales.numel(),
@@ -165,7 +178,7 @@ def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=Non
         raise ValueError(f"a and b must have the same k, not {a.k} and {b.k}")
     if dtype is None:
         dtype = torch.bfloat16 if out is None else out.dtype
-    out = check_output(out, "out", (a.rows, b.rows), dtype, a.codes)
+    out = check_output(out, "out", (a.rows, b.rows), dtype, a.codes, stream)
     code = dtype_code(out, "out")
     _check_indices(offsets, "offsets")
     handle = launch_stream(stream, a.codes, a.scales, b.codes, b.scales, out, *(() if offsets is None else (offsets,)))
@@ -187,9 +200,9 @@ def _pointer(tensor) -> tuple[int | None, int]:
     return (None, 0) if tensor is None else (tensor.data_ptr(), 4 * tensor.numel())
 
 
-def _workspace(tensor, needed: int, like):
+def _workspace(tensor, needed: int, like, stream):
     if tensor is None:
-        return torch.empty(needed, dtype=torch.uint8, device=like.device)
+        return allocate(needed, torch.uint8, like.device, stream)
     if tensor.dtype is not torch.uint8 or not tensor.is_contiguous() or tensor.numel() < needed:
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {needed} bytes")
     return tensor
@@ -228,9 +241,9 @@ def linear(x, weight: Packed, out=None, plan=None, sorted_rows: bool = False, wo
     if weight.k != k:
         raise ValueError(f"the weight must have k = {k}, not {weight.k}")
     n, routed, codes, scales = weight.rows, rows * copies, weight.codes, weight.scales
-    out = check_output(out, "out", (routed, n), x.dtype, x)
+    out = check_output(out, "out", (routed, n), x.dtype, x, stream)
     native = library()
-    workspace = _workspace(workspace, native.mb_mx_linear_workspace(routed, n, k), x)
+    workspace = _workspace(workspace, native.mb_mx_linear_workspace(routed, n, k), x, stream)
     handle = launch_stream(stream, x, codes, scales, out, workspace, *indices)
     item = 2 if code else 4
     status = native.mb_mx_linear(
@@ -266,12 +279,12 @@ def linear_backward(d_out, x, weight_columns: Packed, d_x=None, d_weight=None, w
     if weight_columns.rows != k or weight_columns.k != n:
         raise ValueError(f"weight_columns must be an operand of {k} x {n} (the weight quantised by columns), not "
                          f"{weight_columns.rows} x {weight_columns.k}")
-    d_x = check_output(d_x, "d_x", (rows, k), x.dtype, x)
-    d_weight = check_output(d_weight, "d_weight", (n, k), x.dtype, x)
+    d_x = check_output(d_x, "d_x", (rows, k), x.dtype, x, stream)
+    d_weight = check_output(d_weight, "d_weight", (n, k), x.dtype, x, stream)
     if not rows or not n or not k:
         return d_x.zero_(), d_weight.zero_()
     native = library()
-    workspace = _workspace(workspace, native.mb_mx_linear_backward_workspace(rows, n, k), x)
+    workspace = _workspace(workspace, native.mb_mx_linear_backward_workspace(rows, n, k), x, stream)
     codes, scales = weight_columns.codes, weight_columns.scales
     handle = launch_stream(stream, d_out, x, codes, scales, d_x, d_weight, workspace)
     item = 2 if code else 4

@@ -15,7 +15,7 @@ from typing import NamedTuple
 import torch
 
 from . import _native
-from .mx import check_output, check_tensor, dtype_code, launch_stream, library, strided_rows
+from .mx import allocate, check_output, check_tensor, dtype_code, launch_stream, library, strided_rows
 
 SCORES = {"softmax": 0, "sigmoid": 1}
 
@@ -48,8 +48,8 @@ def route(logits, top: int, bias=None, scores: str = "softmax", groups: int = 1,
     """
     code = dtype_code(logits, "logits")
     tokens, count, stride, span = strided_rows(logits, "logits")
-    experts = check_output(experts, "experts", (tokens, top), torch.int32, logits)
-    weights = check_output(weights, "weights", (tokens, top), torch.float32, logits)
+    experts = check_output(experts, "experts", (tokens, top), torch.int32, logits, stream)
+    weights = check_output(weights, "weights", (tokens, top), torch.float32, logits, stream)
     if bias is None:
         handle = launch_stream(stream, logits, experts, weights)
     else:
@@ -75,7 +75,7 @@ def route_backward(logits, experts, d_weights, scores: str = "softmax", renormal
     top = experts.shape[1]
     check_tensor(experts, "experts", (tokens, top), torch.int32)
     check_tensor(d_weights, "d_weights", (tokens, top), torch.float32)
-    d_logits = check_output(d_logits, "d_logits", (tokens, count), logits.dtype, logits)
+    d_logits = check_output(d_logits, "d_logits", (tokens, count), logits.dtype, logits, stream)
     handle = launch_stream(stream, logits, experts, d_weights, d_logits)
     item, entries = 2 if code else 4, 4 * tokens * top
     status = library().mb_route_backward(code, logits.data_ptr(), span * item, tokens, count, stride,
@@ -87,13 +87,11 @@ def route_backward(logits, experts, d_weights, scores: str = "softmax", renormal
     return d_logits
 
 
-def empty_plan(tokens: int, top: int, experts: int, device="cuda") -> Plan:
+def empty_plan(tokens: int, top: int, experts: int, device="cuda", stream=None) -> Plan:
     """A plan's buffers and workspace, for `dispatch` to fill."""
     needed = library().mb_dispatch_workspace(tokens * top, experts)
-    return Plan(torch.empty(experts + 1, dtype=torch.int32, device=device),
-                torch.empty(tokens * top, dtype=torch.int32, device=device),
-                torch.empty((tokens, top), dtype=torch.int32, device=device),
-                torch.empty(needed, dtype=torch.uint8, device=device))
+    return Plan(allocate(experts + 1, torch.int32, device, stream), allocate(tokens * top, torch.int32, device, stream),
+                allocate((tokens, top), torch.int32, device, stream), allocate(needed, torch.uint8, device, stream))
 
 
 def dispatch(experts, count: int, plan: Plan | None = None, stream=None) -> Plan:
@@ -104,7 +102,7 @@ def dispatch(experts, count: int, plan: Plan | None = None, stream=None) -> Plan
     entries = tokens * top
     check_tensor(experts, "experts", (tokens, top), torch.int32)
     if plan is None:
-        plan = empty_plan(tokens, top, count, experts.device)
+        plan = empty_plan(tokens, top, count, experts.device, stream)
     offsets, order, slots, workspace = plan
     check_tensor(offsets, "plan.offsets", (count + 1,), torch.int32)
     check_tensor(order, "plan.order", (entries,), torch.int32)
@@ -134,7 +132,7 @@ def _combine_sizes(y, slots, weights):
 def combine(y, slots, weights, out=None, stream=None):
     """out[t] = the sum over j of weights[t][j] * y[slots[t][j]], in y's type; slots of -1 are left out."""
     code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
-    out = check_output(out, "out", (tokens, n), y.dtype, y)
+    out = check_output(out, "out", (tokens, n), y.dtype, y, stream)
     handle = launch_stream(stream, y, slots, weights, out)
     item, entries = 2 if code else 4, 4 * tokens * top
     status = library().mb_combine(code, y.data_ptr(), rows * n * item, rows, slots.data_ptr(), entries,
@@ -150,9 +148,10 @@ def combine_backward(d_out, y, slots, weights, d_y=None, d_weights=None, stream=
     code, rows, n, tokens, top = _combine_sizes(y, slots, weights)
     check_tensor(d_out, "d_out", (tokens, n), y.dtype)
     if d_y is None:
-        d_y = torch.zeros_like(y)
+        with torch.cuda.stream(stream):  # cleared in the order of the call's work
+            d_y = torch.zeros_like(y)
     check_tensor(d_y, "d_y", (rows, n), y.dtype)
-    d_weights = check_output(d_weights, "d_weights", (tokens, top), torch.float32, y)
+    d_weights = check_output(d_weights, "d_weights", (tokens, top), torch.float32, y, stream)
     handle = launch_stream(stream, y, slots, weights, d_out, d_y, d_weights)
     item, entries = 2 if code else 4, 4 * tokens * top
     status = library().mb_combine_backward(code, d_out.data_ptr(), tokens * n * item, y.data_ptr(), rows * n * item,
