@@ -39,7 +39,7 @@ _READ_PACKED_RE = re.compile(r"read_sum_packed_kernelI(f|DF16_|t)Li(\d+)E")
 _ELEMENT_TYPE = {"f": "f32", "DF16_": "f16", "DF16b": "bf16"}
 _ROUTE_RE = re.compile(r"(route(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)E")
 _QUANTIZE_RE = re.compile(r"mx_quantize_kernelI(f|DF16_|DF16b)Li(\d+)ELb([01])E")
-_LAYER_RE = re.compile(r"(mx_quantize_columns|mx_dequantize|mx_product|combine|combine_backward)"
+_LAYER_RE = re.compile(r"(mx_quantize_columns|mx_quantize_gradient|mx_dequantize|mx_product|combine|combine_backward)"
                        r"_kernelI(f|DF16_|DF16b)(?:Lb([01])E)?E")
 _PRODUCT_RING_RE = re.compile(r"mx_product_(ring|stream)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi\d+EE")
 _FEW_RE = re.compile(r"mx_few_kernelI(h|f|DF16_|DF16b)(S\d*_|T_|f|DF16_|DF16b)?Li(\d+)ELi(\d+)EE")

@@ -22,7 +22,7 @@ constexpr uint32_t kBlock = 256;  // elements along K whose 8 scales a row holds
 __device__ __forceinline__ float bits_float(uint32_t v) { return __builtin_bit_cast(float, v); }
 
 // Rows of x to codes and scales. A lane takes eight elements, four lanes a
-// group, a wave U * 512 elements of one row, a workgroup four rows. With `slots`
+// group, a wave U * 512 elements of one row, a workgroup WAVES rows. With `slots`
 // [rows][copies], row r goes to the operand's rows slots[r][0 .. copies), those
 // outside 0 .. out_rows - 1 left out; without, to row r. STREAM as in store8.
 //
@@ -31,16 +31,16 @@ __device__ __forceinline__ float bits_float(uint32_t v) { return __builtin_bit_c
 // 30.8 and 29.0, with four 31.4 and 32.0; one where a row has no more (16384x512
 // 5.4 us, with two 6.2). Half a wave a row, whose operand rows are written in
 // pieces of 128 bytes, took 29.7 and 33.6.
-template <class T, int U, bool STREAM>
-__global__ void __launch_bounds__(256)
-    mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t row_stride,
-                       const int32_t* __restrict__ slots, uint32_t copies, uint32_t out_rows,
-                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+template <class T, int U, bool STREAM, int WAVES>
+__device__ __forceinline__ void quantize_rows(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t row_stride,
+                                              const int32_t* __restrict__ slots, uint32_t copies, uint32_t out_rows,
+                                              uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                              uint32_t index) {
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t chunks = (k + U * 512 - 1) / (U * 512);
-  const uint32_t row = __builtin_amdgcn_readfirstlane(blockIdx.x / chunks * 4 + (threadIdx.x >> 6));
+  const uint32_t row = __builtin_amdgcn_readfirstlane(index / chunks * WAVES + (threadIdx.x >> 6));
   if (row >= rows) return;
-  const uint32_t start = blockIdx.x % chunks * (U * 512) + lane * 8;
+  const uint32_t start = index % chunks * (U * 512) + lane * 8;
   const uint32_t code_bytes = (k + kGroup - 1) / kGroup * 16, blocks = (k + kBlock - 1) / kBlock;
   Raw8<T> raw[U];
 #pragma unroll
@@ -76,6 +76,14 @@ __global__ void __launch_bounds__(256)
             static_cast<uint8_t>(scale[u]);
     }
   }
+}
+
+template <class T, int U, bool STREAM>
+__global__ void __launch_bounds__(256)
+    mx_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t row_stride,
+                       const int32_t* __restrict__ slots, uint32_t copies, uint32_t out_rows,
+                       uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  quantize_rows<T, U, STREAM, 4>(x, rows, k, row_stride, slots, copies, out_rows, codes, scales, blockIdx.x);
 }
 
 // Columns of x to the rows of the transposed operand: groups of 32 run along
@@ -147,17 +155,17 @@ __device__ __forceinline__ void quantize_column(const ColumnPairs<T>& values, ui
 }
 
 template <class T, bool STREAM>
-__global__ void __launch_bounds__(512)
-    mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
-                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+__device__ __forceinline__ void quantize_columns(const T* __restrict__ x, uint32_t rows, uint32_t columns,
+                                                 uint64_t row_stride, uint8_t* __restrict__ codes,
+                                                 uint8_t* __restrict__ scales, uint32_t index, uint32_t count) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[kTileColumns * kTilePitch];
   __shared__ __attribute__((aligned(8))) uint8_t tile_scales[kTileColumns * 8];
   using Pair = typename ColumnPairs<T>::Pair;
   const uint32_t groups = (rows + kGroup - 1) / kGroup;
   const uint32_t strips = (columns + kTileColumns - 1) / kTileColumns;
   // XCD c (workgroups c, c + 8, ..) takes neighbouring strips, whose pieces of a row share lines.
-  const uint32_t xcd = blockIdx.x % 8, count = gridDim.x;
-  const uint32_t pid = xcd * (count / 8) + min(xcd, count % 8) + blockIdx.x / 8;
+  const uint32_t xcd = index % 8;
+  const uint32_t pid = xcd * (count / 8) + min(xcd, count % 8) + index / 8;
   const uint32_t strip = pid % strips, block = pid / strips;
   const uint32_t lane = threadIdx.x & 63;
   const uint32_t local = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -209,6 +217,37 @@ __global__ void __launch_bounds__(512)
         *reinterpret_cast<const elem_u32x2*>(tile_scales + threadIdx.x * 8);
 }
 
+template <class T, bool STREAM>
+__global__ void __launch_bounds__(512)
+    mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                               uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  quantize_columns<T, STREAM>(x, rows, columns, row_stride, codes, scales, blockIdx.x, gridDim.x);
+}
+
+// The operands of a linear layer's gradient in one launch: the rows and the
+// columns of d [rows][n] and the columns of x [rows][k]. The tails of the three
+// run beside each other: 5000x3000 and 5000x4112 bf16 21.7 us, in three launches
+// 28.5; the gradient of a small layer (64x256x256), which the launches bound,
+// 14.2 for 19.6.
+template <class T, bool STREAM>
+__global__ void __launch_bounds__(512)
+    mx_quantize_gradient_kernel(const T* __restrict__ d, uint64_t d_stride, const T* __restrict__ x, uint64_t x_stride,
+                                uint32_t rows, uint32_t n, uint32_t k, uint8_t* __restrict__ d_codes,
+                                uint8_t* __restrict__ d_scales, uint8_t* __restrict__ d_columns,
+                                uint8_t* __restrict__ d_column_scales, uint8_t* __restrict__ x_columns,
+                                uint8_t* __restrict__ x_column_scales, uint32_t d_tiles, uint32_t x_tiles) {
+  const uint32_t index = blockIdx.x;
+  if (index < d_tiles + x_tiles) {
+    const bool first = index < d_tiles;
+    quantize_columns<T, STREAM>(first ? d : x, rows, first ? n : k, first ? d_stride : x_stride,
+                                first ? d_columns : x_columns, first ? d_column_scales : x_column_scales,
+                                first ? index : index - d_tiles, first ? d_tiles : x_tiles);
+  } else {
+    quantize_rows<T, 2, STREAM, 8>(d, rows, n, d_stride, nullptr, 1, rows, d_codes, d_scales,
+                                   index - d_tiles - x_tiles);
+  }
+}
+
 // Codes and scales to values, rounded once to T (exact in fp32 and bf16).
 template <class T, bool STREAM>
 __global__ void __launch_bounds__(256)
@@ -238,6 +277,8 @@ __global__ void __launch_bounds__(256)
   MB_REGISTER_KERNEL("mx_quantize_" NAME "_1024_stream", (mx_quantize_kernel<T, 2, true>));    \
   MB_REGISTER_KERNEL("mx_quantize_columns_" NAME, (mx_quantize_columns_kernel<T, false>));     \
   MB_REGISTER_KERNEL("mx_quantize_columns_" NAME "_stream", (mx_quantize_columns_kernel<T, true>)); \
+  MB_REGISTER_KERNEL("mx_quantize_gradient_" NAME, (mx_quantize_gradient_kernel<T, false>));   \
+  MB_REGISTER_KERNEL("mx_quantize_gradient_" NAME "_stream", (mx_quantize_gradient_kernel<T, true>)); \
   MB_REGISTER_KERNEL("mx_dequantize_" NAME, (mx_dequantize_kernel<T, false>)); \
   MB_REGISTER_KERNEL("mx_dequantize_" NAME "_stream", (mx_dequantize_kernel<T, true>))
 MB_MX_REGISTER(float, "f32");
@@ -296,9 +337,13 @@ int launch_quantize(int dtype, const void* x, uint32_t rows, uint32_t k, uint64_
   return launch_status("mx_quantize");
 }
 
-int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint32_t columns, uint64_t row_stride,
-                            void* codes, void* scales, hipStream_t stream) {
-  const uint64_t grid = (columns + uint64_t{kTileColumns} - 1) / kTileColumns * ((rows + uint64_t{kBlock} - 1) / kBlock);
+static uint64_t column_tiles(uint32_t rows, uint32_t columns) {
+  return (columns + uint64_t{kTileColumns} - 1) / kTileColumns * ((rows + uint64_t{kBlock} - 1) / kBlock);
+}
+
+static int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint32_t columns, uint64_t row_stride,
+                                   void* codes, void* scales, hipStream_t stream) {
+  const uint64_t grid = column_tiles(rows, columns);
   if (grid > 0x7fffffu)
     return fail(MB_ERR_UNSUPPORTED, "mx_quantize_columns: %u x %u exceeds one launch", rows, columns);
   auto launch = [&](auto kernel, auto t) {
@@ -314,6 +359,30 @@ int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint32_t co
       launch(mx_quantize_columns_kernel<T, false>, T());
   });
   return launch_status("mx_quantize_columns");
+}
+
+int launch_quantize_gradient(int dtype, const void* d, uint64_t d_stride, const void* x, uint64_t x_stride,
+                             uint32_t rows, uint32_t n, uint32_t k, void* d_codes, void* d_scales, void* d_columns,
+                             void* d_column_scales, void* x_columns, void* x_column_scales, hipStream_t stream) {
+  const uint64_t d_tiles = column_tiles(rows, n), x_tiles = column_tiles(rows, k);
+  const uint64_t grid = d_tiles + x_tiles + (rows + uint64_t{7}) / 8 * ((n + uint64_t{1023}) / 1024);
+  if (grid > 0x7fffffu)
+    return fail(MB_ERR_UNSUPPORTED, "mx_quantize_gradient: %u x %u x %u exceeds one launch", rows, n, k);
+  auto launch = [&](auto kernel, auto t) {
+    kernel<<<dim3(static_cast<uint32_t>(grid)), dim3(512), 0, stream>>>(
+        static_cast<const decltype(t)*>(d), d_stride, static_cast<const decltype(t)*>(x), x_stride, rows, n, k,
+        static_cast<uint8_t*>(d_codes), static_cast<uint8_t*>(d_scales), static_cast<uint8_t*>(d_columns),
+        static_cast<uint8_t*>(d_column_scales), static_cast<uint8_t*>(x_columns),
+        static_cast<uint8_t*>(x_column_scales), static_cast<uint32_t>(d_tiles), static_cast<uint32_t>(x_tiles));
+  };
+  const bool streamed = streams(mx_code_bytes(rows, n) + mx_code_bytes(n, rows) + mx_code_bytes(k, rows));
+  MB_FOR_DTYPE(dtype, {
+    if (streamed)
+      launch(mx_quantize_gradient_kernel<T, true>, T());
+    else
+      launch(mx_quantize_gradient_kernel<T, false>, T());
+  });
+  return launch_status("mx_quantize_gradient");
 }
 
 }  // namespace mb

@@ -674,12 +674,9 @@ int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, ui
                     (unsigned long long)end);
   if (!mb::aligned(space, 16)) return mb::fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (int rc = mb::launch_quantize(dtype, d_out, rows, n, d_out_stride, nullptr, 1, rows, space + codes[0],
-                                   space + scales[0], on))
-    return rc;
-  if (int rc = mb::launch_quantize_columns(dtype, d_out, rows, n, d_out_stride, space + codes[1], space + scales[1], on))
-    return rc;
-  if (int rc = mb::launch_quantize_columns(dtype, x, rows, k, x_stride, space + codes[2], space + scales[2], on))
+  if (int rc = mb::launch_quantize_gradient(dtype, d_out, d_out_stride, x, x_stride, rows, n, k, space + codes[0],
+                                            space + scales[0], space + codes[1], space + scales[1], space + codes[2],
+                                            space + scales[2], on))
     return rc;
   if (int rc = mb::launch_product(dtype, space + codes[0], space + scales[0], w_columns, scale_w, d_x, rows, k, n,
                                   nullptr, 1, on))
