@@ -27,9 +27,11 @@ int check_rows(const char* entry, int dtype, const void* x, uint64_t x_bytes, ui
 
 int launch_quantize(int dtype, const void* x, uint32_t rows, uint32_t k, uint64_t row_stride, const int32_t* slots,
                     uint32_t copies, uint32_t out_rows, void* codes, void* scales, hipStream_t stream);
-// The rows and the columns of d [rows][n] and the columns of x [rows][k].
+// The rows and the columns of d [rows][n] and the columns of x [rows][k]; the
+// columns with K = depth: rows, rounded up to 32 or to 256.
 int launch_quantize_gradient(int dtype, const void* d, uint64_t d_stride, const void* x, uint64_t x_stride,
-                             uint32_t rows, uint32_t n, uint32_t k, void* d_codes, void* d_scales, void* d_columns,
-                             void* d_column_scales, void* x_columns, void* x_column_scales, hipStream_t stream);
+                             uint32_t rows, uint32_t n, uint32_t k, uint32_t depth, void* d_codes, void* d_scales,
+                             void* d_columns, void* d_column_scales, void* x_columns, void* x_column_scales,
+                             hipStream_t stream);
 
 }  // namespace mb

@@ -90,7 +90,8 @@ __global__ void __launch_bounds__(256)
 // x's rows. A workgroup takes 256 rows of 128 columns, a wave a group of 32
 // rows, a lane two neighbouring columns, so that a group's largest magnitude
 // needs no other lane and stays packed; the codes cross LDS, so that an operand
-// row's 128 bytes leave together.
+// row's 128 bytes leave together. An operand row holds `groups` groups, as many as
+// the rows fill or, of zeros, up to the end of their block of 256.
 //
 // Bound by the memory's rate for 256 bytes a row: 8192x8192 bf16 36.9 us from HBM
 // (4.6 TB/s; with 512 bytes a row 37.5), 25.0 from the memory-side cache (6.8).
@@ -156,12 +157,11 @@ __device__ __forceinline__ void quantize_column(const ColumnPairs<T>& values, ui
 
 template <class T, bool STREAM>
 __device__ __forceinline__ void quantize_columns(const T* __restrict__ x, uint32_t rows, uint32_t columns,
-                                                 uint64_t row_stride, uint8_t* __restrict__ codes,
+                                                 uint64_t row_stride, uint32_t groups, uint8_t* __restrict__ codes,
                                                  uint8_t* __restrict__ scales, uint32_t index, uint32_t count) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[kTileColumns * kTilePitch];
   __shared__ __attribute__((aligned(8))) uint8_t tile_scales[kTileColumns * 8];
   using Pair = typename ColumnPairs<T>::Pair;
-  const uint32_t groups = (rows + kGroup - 1) / kGroup;
   const uint32_t strips = (columns + kTileColumns - 1) / kTileColumns;
   // XCD c (workgroups c, c + 8, ..) takes neighbouring strips, whose pieces of a row share lines.
   const uint32_t xcd = index % 8;
@@ -221,18 +221,20 @@ template <class T, bool STREAM>
 __global__ void __launch_bounds__(512)
     mx_quantize_columns_kernel(const T* __restrict__ x, uint32_t rows, uint32_t columns, uint64_t row_stride,
                                uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  quantize_columns<T, STREAM>(x, rows, columns, row_stride, codes, scales, blockIdx.x, gridDim.x);
+  quantize_columns<T, STREAM>(x, rows, columns, row_stride, (rows + kGroup - 1) / kGroup, codes, scales, blockIdx.x,
+                              gridDim.x);
 }
 
 // The operands of a linear layer's gradient in one launch: the rows and the
 // columns of d [rows][n] and the columns of x [rows][k]. The tails of the three
 // run beside each other: 5000x3000 and 5000x4112 bf16 21.7 us, in three launches
 // 28.5; the gradient of a small layer (64x256x256), which the launches bound,
-// 14.2 for 19.6.
+// 14.2 for 19.6. The columns' operands have `depth` >= rows elements of K, zeros
+// past the rows.
 template <class T, bool STREAM>
 __global__ void __launch_bounds__(512)
     mx_quantize_gradient_kernel(const T* __restrict__ d, uint64_t d_stride, const T* __restrict__ x, uint64_t x_stride,
-                                uint32_t rows, uint32_t n, uint32_t k, uint8_t* __restrict__ d_codes,
+                                uint32_t rows, uint32_t n, uint32_t k, uint32_t depth, uint8_t* __restrict__ d_codes,
                                 uint8_t* __restrict__ d_scales, uint8_t* __restrict__ d_columns,
                                 uint8_t* __restrict__ d_column_scales, uint8_t* __restrict__ x_columns,
                                 uint8_t* __restrict__ x_column_scales, uint32_t d_tiles, uint32_t x_tiles) {
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(512)
   if (index < d_tiles + x_tiles) {
     const bool first = index < d_tiles;
     quantize_columns<T, STREAM>(first ? d : x, rows, first ? n : k, first ? d_stride : x_stride,
-                                first ? d_columns : x_columns, first ? d_column_scales : x_column_scales,
+                                depth / kGroup, first ? d_columns : x_columns, first ? d_column_scales : x_column_scales,
                                 first ? index : index - d_tiles, first ? d_tiles : x_tiles);
   } else {
     quantize_rows<T, 2, STREAM, 8>(d, rows, n, d_stride, nullptr, 1, rows, d_codes, d_scales,
@@ -362,20 +364,21 @@ static int launch_quantize_columns(int dtype, const void* x, uint32_t rows, uint
 }
 
 int launch_quantize_gradient(int dtype, const void* d, uint64_t d_stride, const void* x, uint64_t x_stride,
-                             uint32_t rows, uint32_t n, uint32_t k, void* d_codes, void* d_scales, void* d_columns,
-                             void* d_column_scales, void* x_columns, void* x_column_scales, hipStream_t stream) {
+                             uint32_t rows, uint32_t n, uint32_t k, uint32_t depth, void* d_codes, void* d_scales,
+                             void* d_columns, void* d_column_scales, void* x_columns, void* x_column_scales,
+                             hipStream_t stream) {
   const uint64_t d_tiles = column_tiles(rows, n), x_tiles = column_tiles(rows, k);
   const uint64_t grid = d_tiles + x_tiles + (rows + uint64_t{7}) / 8 * ((n + uint64_t{1023}) / 1024);
   if (grid > 0x7fffffu)
     return fail(MB_ERR_UNSUPPORTED, "mx_quantize_gradient: %u x %u x %u exceeds one launch", rows, n, k);
   auto launch = [&](auto kernel, auto t) {
     kernel<<<dim3(static_cast<uint32_t>(grid)), dim3(512), 0, stream>>>(
-        static_cast<const decltype(t)*>(d), d_stride, static_cast<const decltype(t)*>(x), x_stride, rows, n, k,
+        static_cast<const decltype(t)*>(d), d_stride, static_cast<const decltype(t)*>(x), x_stride, rows, n, k, depth,
         static_cast<uint8_t*>(d_codes), static_cast<uint8_t*>(d_scales), static_cast<uint8_t*>(d_columns),
         static_cast<uint8_t*>(d_column_scales), static_cast<uint8_t*>(x_columns),
         static_cast<uint8_t*>(x_column_scales), static_cast<uint32_t>(d_tiles), static_cast<uint32_t>(x_tiles));
   };
-  const bool streamed = streams(mx_code_bytes(rows, n) + mx_code_bytes(n, rows) + mx_code_bytes(k, rows));
+  const bool streamed = streams(mx_code_bytes(rows, n) + mx_code_bytes(n, depth) + mx_code_bytes(k, depth));
   MB_FOR_DTYPE(dtype, {
     if (streamed)
       launch(mx_quantize_gradient_kernel<T, true>, T());

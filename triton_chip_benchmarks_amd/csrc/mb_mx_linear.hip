@@ -642,10 +642,16 @@ static uint64_t place_operand(uint64_t at, uint64_t rows, uint64_t k, uint64_t* 
   return *scales + (mb::mx_scale_bytes(rows, k) + 15) / 16 * 16;
 }
 
+// K of d_w's operands: whole blocks of 256 past the first, so that their rows'
+// 128-byte pieces lie on lines. 5000x3000 of K 4112 47.4 us, of 4352 (as many
+// steps) 44.3.
+static uint32_t gradient_depth(uint32_t rows) { return rows > 256 ? (rows + 255) / 256 * 256 : (rows + 31) / 32 * 32; }
+
 uint64_t mb_mx_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  const uint64_t depth = gradient_depth(rows < mb::kMxMostRows ? rows : mb::kMxMostRows);
   uint64_t codes, scales, end = place_operand(0, rows, n, &codes, &scales);
-  end = place_operand(end, n, rows, &codes, &scales);
-  return place_operand(end, k, rows, &codes, &scales);
+  end = place_operand(end, n, depth, &codes, &scales);
+  return place_operand(end, k, depth, &codes, &scales);
 }
 
 int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* x,
@@ -666,23 +672,24 @@ int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, ui
   if (int rc = mb::check_output(entry, dtype, d_x, d_x_bytes, rows, k)) return rc;
   if (int rc = mb::check_output(entry, dtype, d_w, d_w_bytes, n, k)) return rc;
   uint64_t codes[3], scales[3], end = place_operand(0, rows, n, &codes[0], &scales[0]);
-  end = place_operand(end, n, rows, &codes[1], &scales[1]);
-  end = place_operand(end, k, rows, &codes[2], &scales[2]);
+  const uint32_t depth = gradient_depth(rows);
+  end = place_operand(end, n, depth, &codes[1], &scales[1]);
+  end = place_operand(end, k, depth, &codes[2], &scales[2]);
   uint8_t* const space = static_cast<uint8_t*>(workspace);
   if (space == nullptr || workspace_bytes < end)
     return mb::fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
                     (unsigned long long)end);
   if (!mb::aligned(space, 16)) return mb::fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
   const hipStream_t on = static_cast<hipStream_t>(stream);
-  if (int rc = mb::launch_quantize_gradient(dtype, d_out, d_out_stride, x, x_stride, rows, n, k, space + codes[0],
-                                            space + scales[0], space + codes[1], space + scales[1], space + codes[2],
-                                            space + scales[2], on))
+  if (int rc = mb::launch_quantize_gradient(dtype, d_out, d_out_stride, x, x_stride, rows, n, k, depth,
+                                            space + codes[0], space + scales[0], space + codes[1], space + scales[1],
+                                            space + codes[2], space + scales[2], on))
     return rc;
   if (int rc = mb::launch_product(dtype, space + codes[0], space + scales[0], w_columns, scale_w, d_x, rows, k, n,
                                   nullptr, 1, on))
     return rc;
   return mb::launch_product(dtype, space + codes[1], space + scales[1], space + codes[2], space + scales[2], d_w, n, k,
-                            rows, nullptr, 1, on);
+                            depth, nullptr, 1, on);
 }
 
 }  // extern "C"
