@@ -70,3 +70,22 @@ def test_outputs_and_workspaces_are_the_streams_memory(gpu, monkeypatch):
                 assert owner == [side.cuda_stream], name
         for mine, theirs in zip(here, there):
             assert torch.equal(mine.view(torch.uint8), theirs.view(torch.uint8)), name
+
+
+def test_gradient_of_no_rows_is_cleared_in_the_streams_order(gpu):
+    """Work on the stream that is still to come when the call is made is ordered before its zeros."""
+    import torch
+
+    from triton_chip_benchmarks_amd import mx
+
+    side = torch.cuda.Stream()
+    columns = mx.quantize(torch.ones(64, 96, device="cuda", dtype=torch.bfloat16), columns=True)
+    d_weight = torch.zeros(64, 96, device="cuda", dtype=torch.bfloat16)
+    d_out, x = (torch.empty(0, width, device="cuda", dtype=torch.bfloat16) for width in (64, 96))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # about 10 ms
+        d_weight.fill_(1.0)
+    mx.linear_backward(d_out, x, columns, d_weight=d_weight, stream=side)
+    torch.cuda.synchronize()
+    assert not d_weight.any()

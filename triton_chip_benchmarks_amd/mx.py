@@ -282,7 +282,9 @@ def linear_backward(d_out, x, weight_columns: Packed, d_x=None, d_weight=None, w
     d_x = check_output(d_x, "d_x", (rows, k), x.dtype, x, stream)
     d_weight = check_output(d_weight, "d_weight", (n, k), x.dtype, x, stream)
     if not rows or not n or not k:
-        return d_x.zero_(), d_weight.zero_()
+        launch_stream(stream, d_out, x, weight_columns.codes, weight_columns.scales, d_x, d_weight)
+        with torch.cuda.stream(stream):  # cleared in the order of the call's work
+            return d_x.zero_(), d_weight.zero_()
     native = library()
     workspace = _workspace(workspace, native.mb_mx_linear_backward_workspace(rows, n, k), x, stream)
     codes, scales = weight_columns.codes, weight_columns.scales
