@@ -321,7 +321,7 @@ uint64_t mb_mx_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k);
  * [rows][n]: d_x [rows][k] = Q(d_out) . Wc with the weight quantised by columns
  * (mb_mx_quantize_columns of W: an operand of k rows and K = n), and d_w [n][k] =
  * d_out^T . X, both quantised by columns, along the rows that the sum runs over.
- * Five launches. */
+ * Three launches. */
 int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* x,
                           uint64_t x_bytes, uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes,
                           const void* scale_w, uint64_t scale_w_bytes, void* d_x, uint64_t d_x_bytes, void* d_w,
