@@ -59,3 +59,54 @@ def test_layer_agrees_with_the_oracle_and_with_its_graph(gpu, tokens, hidden, in
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(layer.out, eager)
+
+
+@pytest.mark.parametrize("tokens,n,k,count,top", [(3, 96, 40, 6, 2), (150, 72, 96, 4, 3)])
+def test_gradients_of_routed_rows_through_the_same_calls(gpu, tokens, n, k, count, top):
+    """The input's gradient is a routed product with the weights' columns and a sum over a token's choices; an
+    expert's weight gradient the linear layer's of its rows."""
+    import torch
+
+    from triton_chip_benchmarks_amd import mx, routing
+
+    print(f"routed gradients {tokens}x{n}x{k} experts={count} top={top}", flush=True)
+    generator = torch.Generator(device="cuda").manual_seed(tokens)
+
+    def normal(*shape):
+        return torch.randn(shape, device="cuda", generator=generator)
+
+    def host(tensor):
+        return tensor.double().cpu().numpy()
+
+    def close(got, expected, size, depth):
+        # fp32 sums as everywhere: a rounding for each of depth / 32 steps and 16 joins.
+        assert (np.abs(host(got) - expected) <= ((depth / 32 + 16) * 2.0**-23 + 2.0**-24) * size + 2.0**-149).all()
+
+    x, w, logits = normal(tokens, k), normal(count, n, k), normal(tokens, count)
+    logits[1] = float("-inf")  # a token without experts
+    chosen, _ = routing.route(logits, top)
+    plan = routing.dispatch(chosen, count)
+    offsets, order = plan.offsets.tolist(), plan.order.long()
+    d_y = normal(tokens * top, n)
+    columns = mx.empty(k, n, experts=count)
+    for e in range(count):
+        mx.quantize(w[e], mx.Packed(columns.codes[e], columns.scales[e], n), columns=True)
+    d_rows = mx.linear(d_y, columns, plan=plan, sorted_rows=True)
+    d_x = routing.combine(d_rows, plan.slots, torch.ones(tokens, top, device="cuda"))
+    expected, size = np.zeros((tokens, k)), np.zeros((tokens, k))
+    for e, (first, last) in enumerate(zip(offsets, offsets[1:])):
+        token = order[first:last] // top
+        part = mx.Packed(columns.codes[e], columns.scales[e], n)
+        _, d_w = mx.linear_backward(d_y[first:last], x[token], part)
+        assert d_w.shape == (n, k)
+        if first == last:
+            assert not d_w.any()
+            continue
+        (ex, sx), (ew, sw) = oracle_mx.linear_backward(host(d_y[first:last]), host(x[token]), host(w[e]))
+        close(d_w, ew, sw, last - first)
+        for t, row, rounding in zip(token.tolist(), ex, sx):
+            expected[t] += row
+            size[t] += rounding
+    # A token's `top` rows are rounded to fp32 and added.
+    close(d_x, expected, size, n + 32 * top)
+    assert not d_x[1].any()
