@@ -1,0 +1,70 @@
+"""Routing's gradients and weights where scores are far from 1: each value against its own size, not the row's.
+
+A score is one exponential, one addition and one division (together under 8 roundings of 2^-24, and one of 2^-150
+where it is below 2^-126), a sum of `top` scores adds log2(64) + top, and a renormalised gradient is a difference of
+values up to the sum of the magnitudes of `g`, times a share and a complement: 64 roundings of 2^-23 cover every chain.
+"""
+
+import numpy as np
+import pytest
+
+from oracle import routing as oracle
+
+pytestmark = pytest.mark.gpu
+
+ROUNDINGS = 64 * 2.0**-23
+
+
+def _host(tensor):
+    return tensor.double().cpu().numpy()
+
+
+def _gradient(logits, chosen, g, **options):
+    """(d_logits on the device, the float64 oracle's, and the size of the terms that each element is the sum of)."""
+    import torch
+
+    from triton_chip_benchmarks_amd import routing
+
+    on_device = [torch.tensor(part, device="cuda") for part in (logits, chosen, g)]
+    got = _host(routing.route_backward(*on_device, **options))
+    kind, scale = options.get("scores", "softmax"), options.get("scale", 1.0)
+    exact = oracle.route_backward(logits, chosen, g, kind=kind, renormalize=options.get("renormalize", True),
+                                  scale=scale)
+    return got, exact
+
+
+def _size(logits, chosen, g, scores, renormalize, scale):
+    """scale * share * complement * sum |g| of the chosen elements, 0 elsewhere."""
+    size = np.zeros(logits.shape)
+    for t in range(logits.shape[0]):
+        # In units of the row's largest exponential, so that float64 holds every share.
+        l = logits[t].astype(np.float64)
+        s = np.exp(l - l.max()) if scores == "softmax" else 1 / (1 + np.exp(-l))
+        s = s / s.sum() if scores == "softmax" else s
+        rest = 1.0 if scores == "softmax" else 1 / (1 + np.exp(l))
+        part = s / s[chosen[t]].sum() if renormalize else s
+        size[t, chosen[t]] = (scale * part * rest * np.abs(g[t]).sum())[chosen[t]]
+    return size
+
+
+@pytest.mark.parametrize("tokens", [3, 4100])
+@pytest.mark.parametrize("scores", ["sigmoid", "softmax"])
+def test_gradient_of_shares_of_scores_near_the_smallest(gpu, scores, tokens):
+    """Chosen scores of 1e-38: their shares, and the gradient, are of the size of any others'."""
+    print(f"gradient of small scores, {scores}, {tokens} tokens", flush=True)
+    row = np.array([-88.0, -88.2, -95.0, -95.5, -87.5, -90.0, -91.0, -96.0], dtype=np.float32)
+    logits = np.tile(row, (tokens, 1))
+    if scores == "softmax":
+        logits[:, 7] = 0.0  # takes the whole sum; not chosen
+    chosen = np.tile(np.array([0, 1], dtype=np.int32), (tokens, 1))
+    chosen[1] = 4, 0
+    g = np.tile(np.array([3.0, -3.0], dtype=np.float32), (tokens, 1))
+    got, exact = _gradient(logits, chosen, g, scores=scores, scale=2.5)
+    # The unchosen have no part in renormalised weights; the oracle's differences leave 2^-53 of the choices' there.
+    unchosen = np.ones(logits.shape, dtype=bool)
+    np.put_along_axis(unchosen, chosen, False, axis=1)
+    assert (got[unchosen] == 0).all()
+    # A score of e^-88.2 is 3.5e6 units of 2^-149: two more roundings of 2^-22.
+    bound = (ROUNDINGS + 2.0**-21) * _size(logits, chosen, g, scores, True, 2.5)
+    assert np.abs(exact).max() > 1
+    assert (np.abs(got - exact) <= bound)[~unchosen].all(), (got[:2], exact[:2])

@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(256)
 // Gradient of route's weights with respect to the logits, a team a token. With
 // w_j = r s_j / Z over the chosen (Z = 1 unless renormalised) and g their
 // gradient, d s_j = r (g_j - sum_i g_i s_i / Z) / Z, then through the scores:
-// softmax d l = s (d s - sum d s s), sigmoid d l = d s s (1 - s). The choice
+// softmax d l = s (d s - sum d s s), sigmoid d l = d s s (1 - s). Renormalised,
+// s d s is r (g_j - sum_i g_i p_i) p_j with the shares p = s / Z. The choice
 // itself has no gradient.
 template <class T, int V, int TEAM>
 __global__ void __launch_bounds__(256)
@@ -199,11 +200,12 @@ __global__ void __launch_bounds__(256)
   wave_lds_fence();
   if (renormalize) {
     const float total = team_add<TEAM>(s);
-    // By shares, so that a lone choice, whose weight is constant, has a gradient of exactly zero.
-    const float mean = team_add<TEAM>(total == 0.0f ? 0.0f : d * (s / total));
-    d = expert < 0 || total == 0.0f ? 0.0f : (d - mean) / total;
+    // By shares: a lone choice, whose weight is constant, has a gradient of exactly zero, and nothing
+    // overflows where the scores are small (1 / total is infinite for scores below 2^-128).
+    const float share = total == 0.0f ? 0.0f : s / total;
+    const float mean = team_add<TEAM>(d * share);
+    d = expert < 0 || total == 0.0f ? 0.0f : (d - mean) * share;
   }
-  // Renormalised softmax weights do not change with the unchosen logits.
   const float common = softmax && !renormalize ? team_add<TEAM>(d * s) : 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) lds[team][lane * V + i] = 0.0f;
@@ -213,8 +215,15 @@ __global__ void __launch_bounds__(256)
   LaneValues<T, V> out;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
+    // Renormalised: ds times the score. The softmax's weights do not change with the unchosen logits; a
+    // NaN score still gives NaN.
     const float ds = lds[team][lane * V + i];
-    out.at[i] = static_cast<T>(softmax ? score[i] * (ds - common) : ds * score[i] * (1.0f - score[i]));
+    float dl;
+    if (softmax)
+      dl = renormalize ? fmaf(score[i], 0.0f, ds) : score[i] * (ds - common);
+    else
+      dl = (renormalize ? fmaf(score[i], 0.0f, ds) : ds * score[i]) * (1.0f - score[i]);
+    out.at[i] = static_cast<T>(dl);
   }
   T* to = d_logits + static_cast<uint64_t>(token) * experts + lane * V;
   if (static_cast<uint32_t>(lane) * V + V <= experts) {
