@@ -68,3 +68,23 @@ def test_gradient_of_shares_of_scores_near_the_smallest(gpu, scores, tokens):
     bound = (ROUNDINGS + 2.0**-21) * _size(logits, chosen, g, scores, True, 2.5)
     assert np.abs(exact).max() > 1
     assert (np.abs(got - exact) <= bound)[~unchosen].all(), (got[:2], exact[:2])
+
+
+@pytest.mark.parametrize("tokens", [2, 4100])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_sigmoid_gradient_of_scores_near_one(gpu, renormalize, tokens):
+    """The gradient goes with 1 - s, which is far below a score's last bit from a logit of 17 on."""
+    print(f"gradient of scores near one, renormalize={renormalize}, {tokens} tokens", flush=True)
+    row = np.array([14.0, 16.0, 17.5, 20.0, 30.0, 86.0, -3.0, 0.5], dtype=np.float32)
+    logits = np.tile(row, (tokens, 1))
+    chosen = np.tile(np.array([5, 3, 0, 1, 2, 4, 6], dtype=np.int32), (tokens, 1))
+    g = np.tile(np.array([3.0, -3.0, 0.5, 1.0, -2.0, 1.5, 0.25], dtype=np.float32), (tokens, 1))
+    got, exact = _gradient(logits, chosen, g, scores="sigmoid", renormalize=renormalize, scale=2.5)
+    # The oracle's 1 - s is good to 2^-53; here the complement is the sigmoid of the logit's negative.
+    s = 1 / (1 + np.exp(-row.astype(np.float64)))
+    exact = exact * np.divide(1 / (1 + np.exp(row.astype(np.float64))), 1 - s, where=s < 1, out=np.ones(8))
+    part = s[chosen[0]] / s[chosen[0]].sum()
+    terms = 2.5 * ((g[0] - (g[0] * part).sum()) * part if renormalize else g[0] * s[chosen[0]])
+    exact[:, chosen[0]] = terms / (1 + np.exp(row[chosen[0]].astype(np.float64)))
+    bound = ROUNDINGS * _size(logits, chosen, g, "sigmoid", renormalize, 2.5) + 2.0**-149
+    assert (np.abs(got - exact) <= bound).all(), (got[0], exact[0])

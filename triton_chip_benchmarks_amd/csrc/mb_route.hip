@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256)
   if (token >= tokens) return;
   float logit[V], score[V];
   load_logits(logits + token * row_stride, experts, lane, logit);
-  scores_of<V, TEAM>(logit, softmax, score);
+  if (softmax) scores_of<V, TEAM>(logit, true, score);
   int expert = -1;
   float d = 0.0f;
   if (static_cast<uint32_t>(lane) < top) {
@@ -194,10 +194,11 @@ __global__ void __launch_bounds__(256)
     if (expert >= 0) d = d_weights[static_cast<uint64_t>(token) * top + lane] * scale;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) lds[team][lane * V + i] = score[i];
+  for (int i = 0; i < V; ++i) lds[team][lane * V + i] = softmax ? score[i] : logit[i];
   wave_lds_fence();
-  const float s = expert >= 0 ? lds[team][expert] : 0.0f;
+  const float held = expert >= 0 ? lds[team][expert] : kNegInf;
   wave_lds_fence();
+  const float s = softmax ? (expert >= 0 ? held : 0.0f) : sigmoid(held);
   if (renormalize) {
     const float total = team_add<TEAM>(s);
     // By shares: a lone choice, whose weight is constant, has a gradient of exactly zero, and nothing
@@ -207,6 +208,8 @@ __global__ void __launch_bounds__(256)
     d = expert < 0 || total == 0.0f ? 0.0f : (d - mean) * share;
   }
   const float common = softmax && !renormalize ? team_add<TEAM>(d * s) : 0.0f;
+  // 1 - s as the sigmoid of the negative logit: the difference is 6% off at a logit of 16 and 0 at 17.5.
+  if (!softmax && expert >= 0) d = (renormalize ? d : d * s) * sigmoid(-held);
 #pragma unroll
   for (int i = 0; i < V; ++i) lds[team][lane * V + i] = 0.0f;
   wave_lds_fence();
@@ -215,14 +218,14 @@ __global__ void __launch_bounds__(256)
   LaneValues<T, V> out;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    // Renormalised: ds times the score. The softmax's weights do not change with the unchosen logits; a
-    // NaN score still gives NaN.
+    // The gradient itself, but softmax scores that are not renormalised: there every logit has one, of the common
+    // sum. A NaN logit, or softmax score, still gives NaN.
     const float ds = lds[team][lane * V + i];
     float dl;
     if (softmax)
       dl = renormalize ? fmaf(score[i], 0.0f, ds) : score[i] * (ds - common);
     else
-      dl = (renormalize ? fmaf(score[i], 0.0f, ds) : ds * score[i]) * (1.0f - score[i]);
+      dl = logit[i] != logit[i] ? logit[i] : ds;
     out.at[i] = static_cast<T>(dl);
   }
   T* to = d_logits + static_cast<uint64_t>(token) * experts + lane * V;
