@@ -339,7 +339,10 @@ int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, ui
  * lower); among the rest the `top` largest c, in falling order, of equal ones the
  * lower index. chosen [tokens][top] is -1, with weight 0, where nothing is left;
  * weights are s, divided by their sum if renormalize, times scale. A NaN score
- * ranks below all others and gives a NaN weight.
+ * ranks below all others and gives a NaN weight. Scores are fp32 numbers: below
+ * 2^-126 (a sigmoid's logit of -87.3, a softmax's as far below the largest) they
+ * keep fewer bits, and below 2^-150 (-104) they are 0, as are the weights and
+ * gradients of a token that has chosen nothing else.
  * experts <= 1024, top <= 64, groups <= 64. */
 int mb_route(int dtype, const void* logits, uint64_t logits_bytes, uint32_t tokens, uint32_t experts,
              uint64_t row_stride, const float* bias, uint64_t bias_bytes, uint32_t top, uint32_t scores,

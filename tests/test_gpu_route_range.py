@@ -88,3 +88,23 @@ def test_sigmoid_gradient_of_scores_near_one(gpu, renormalize, tokens):
     exact[:, chosen[0]] = terms / (1 + np.exp(row[chosen[0]].astype(np.float64)))
     bound = ROUNDINGS * _size(logits, chosen, g, "sigmoid", renormalize, 2.5) + 2.0**-149
     assert (np.abs(got - exact) <= bound).all(), (got[0], exact[0])
+
+
+@pytest.mark.parametrize("tokens", [3, 4100])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_sigmoid_scores_down_to_the_smallest(gpu, renormalize, tokens):
+    """Logits whose scores fp32 still holds (from about -103 on) are told apart, and their shares are finite."""
+    import torch
+
+    from triton_chip_benchmarks_amd import routing
+
+    print(f"sigmoid scores near the smallest, renormalize={renormalize}, {tokens} tokens", flush=True)
+    row = np.array([-96.0, -89.5, -94.0, -88.9, -92.0, -90.5, -95.0, -200.0], dtype=np.float32)
+    logits = np.tile(row, (tokens, 1))
+    chosen, weights = routing.route(torch.tensor(logits, device="cuda"), 4, scores="sigmoid", renormalize=renormalize)
+    expected, exact = oracle.route(logits, 4, kind="sigmoid", renormalize=renormalize)
+    assert np.array_equal(chosen.cpu().numpy(), expected)
+    smallest = np.exp(row[expected[0]].astype(np.float64)).min()
+    bound = (ROUNDINGS + 2 * 2.0**-150 / smallest) * exact + (0 if renormalize else 2.0**-150)
+    assert (np.abs(_host(weights) - exact) <= bound).all(), (weights[0], exact[0])
+    assert (exact > 0).all()

@@ -11,7 +11,12 @@ namespace {
 constexpr uint32_t kMostExperts = 1024, kMostTop = 64;
 constexpr float kNegInf = -__builtin_inff();
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.0f / (1.0f + expf(-v)); }
+// 1 / (1 + e^-v); from -64 down e^v, which is the same in fp32 and does not pass through an infinite e^-v.
+__device__ __forceinline__ float sigmoid(float v) {
+  const bool far = v < -64.0f;
+  const float power = expf(far ? v : -v);
+  return far ? power : 1.0f / (1.0f + power);
+}
 
 // Orders a wave's LDS writes before its later LDS reads.
 __device__ __forceinline__ void wave_lds_fence() {
