@@ -108,3 +108,32 @@ def test_sigmoid_scores_down_to_the_smallest(gpu, renormalize, tokens):
     bound = (ROUNDINGS + 2 * 2.0**-150 / smallest) * exact + (0 if renormalize else 2.0**-150)
     assert (np.abs(_host(weights) - exact) <= bound).all(), (weights[0], exact[0])
     assert (exact > 0).all()
+
+
+@pytest.mark.parametrize("tokens", [5, 4100])
+def test_far_scores_of_a_token_leave_its_neighbours_alone(gpu, tokens):
+    """Tokens of far logits among ordinary and masked ones, in groups and with a bias: each as if it were alone."""
+    import torch
+
+    from triton_chip_benchmarks_amd import routing
+
+    print(f"far and near tokens, {tokens}", flush=True)
+    rng = np.random.default_rng(0)
+    logits = np.stack([rng.permutation(np.arange(32) / 8.0 - 2) for _ in range(tokens)]).astype(np.float32)
+    logits[1::3] -= 94.0
+    logits[1::3, 4:8] = -np.inf
+    logits[2::5] = -np.inf
+    logits[3::7, 16:] -= 300.0
+    options = {"scores": "sigmoid", "groups": 4, "top_groups": 2}
+    bias = np.zeros(32, dtype=np.float32)
+    bias[10:12] = 2.0  # chosen whatever they score
+    for offset in (None, bias):
+        on_device = None if offset is None else torch.tensor(offset, device="cuda")
+        chosen, weights = routing.route(torch.tensor(logits, device="cuda"), 5, on_device, **options)
+        kept = list(range(0, tokens, 1 if tokens < 100 else 89))
+        expected, exact = oracle.route(logits[kept], 5, offset, kind="sigmoid", groups=4, top_groups=2)
+        assert np.array_equal(chosen.cpu().numpy()[kept], expected)
+        # A score of e^-98 is 196 units of 2^-149.
+        assert (np.abs(_host(weights)[kept] - exact) <= (ROUNDINGS + 2.0**-6) * exact + 1e-30).all()
+        alone = [routing.route(torch.tensor(logits[t:t + 1], device="cuda"), 5, on_device, **options) for t in kept]
+        assert np.array_equal(chosen.cpu().numpy()[kept], np.concatenate([a[0].cpu().numpy() for a in alone]))

@@ -11,12 +11,6 @@ namespace {
 constexpr uint32_t kMostExperts = 1024, kMostTop = 64;
 constexpr float kNegInf = -__builtin_inff();
 
-// 1 / (1 + e^-v); from -64 down e^v, which is the same in fp32 and does not pass through an infinite e^-v.
-__device__ __forceinline__ float sigmoid(float v) {
-  const bool far = v < -64.0f;
-  const float power = expf(far ? v : -v);
-  return far ? power : 1.0f / (1.0f + power);
-}
 
 // Orders a wave's LDS writes before its later LDS reads.
 __device__ __forceinline__ void wave_lds_fence() {
@@ -27,12 +21,18 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 // Scores s of a token's logits, lane l of its team holding experts l * V ..
 // l * V + V - 1; logits past the last expert and masked ones (-inf) are -inf and
-// score 0.
+// score 0. So does a sigmoid's logit below -88.7, whose e^-l is infinite; `far`
+// takes e^l there, which fp32 still holds.
 template <int V, int TEAM>
-__device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax, float (&score)[V]) {
+__device__ __forceinline__ void scores_of(const float (&logit)[V], bool softmax, bool far, float (&score)[V]) {
   if (!softmax) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) score[i] = sigmoid(logit[i]);
+    for (int i = 0; i < V; ++i) score[i] = 1.0f / (1.0f + expf(-logit[i]));
+    if (far) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (score[i] == 0.0f) score[i] = expf(logit[i]);
+    }
     return;
   }
   float top = kNegInf;
@@ -98,69 +98,77 @@ __global__ void __launch_bounds__(256)
   if (token >= tokens) return;
   float logit[V], score[V], value[V];
   load_logits(logits + token * row_stride, experts, lane, logit);
-  scores_of<V, TEAM>(logit, softmax, score);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const uint32_t e = lane * V + i;
-    value[i] = score[i] + (bias && e < experts ? bias[e] : 0.0f);
-    if (value[i] != value[i]) value[i] = -1e38f;
-    if (logit[i] == kNegInf) value[i] = kNegInf;
-  }
-  choices[team][lane] = Choice{-1, 0.0f};
-  if (groups > 1) {
-    const uint32_t size = experts / groups;
-#pragma unroll
-    for (int i = 0; i < V; ++i) values_lds[team][lane * V + i] = value[i];
-    wave_lds_fence();
-    float first = kNegInf, second = kNegInf;
-    if (static_cast<uint32_t>(lane) < groups) {
-#pragma unroll 8
-      for (uint32_t i = 0; i < size; ++i) {
-        const float v = values_lds[team][lane * size + i];
-        second = fmaxf(second, fminf(first, v));
-        first = fmaxf(first, v);
-      }
-    }
-    const float mine = first + (second == kNegInf ? 0.0f : second);
-    groups_lds[team][lane] = mine;
-    wave_lds_fence();
-    // A group is kept if fewer than top_groups come before it: larger ones, or
-    // as large ones of a lower index.
-    uint32_t before = 0;
-#pragma unroll 8
-    for (uint32_t g = 0; g < groups; ++g) {
-      const float other = groups_lds[team][g];
-      before += other > mine || (other == mine && g < static_cast<uint32_t>(lane));
-    }
-    const bool kept = static_cast<uint32_t>(lane) < groups && before < top_groups;
-    const uint64_t mask = __ballot(kept) >> (threadIdx.x % 64 - lane);
-    uint32_t group = lane * V / size, inside = lane * V % size;
+  auto choose = [&](bool far) __attribute__((always_inline)) {
+    scores_of<V, TEAM>(logit, softmax, far, score);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      if (!(mask >> (group & 63) & 1)) value[i] = kNegInf;
-      if (++inside == size) inside = 0, ++group;
+      const uint32_t e = lane * V + i;
+      value[i] = score[i] + (bias && e < experts ? bias[e] : 0.0f);
+      if (value[i] != value[i]) value[i] = -1e38f;
+      if (logit[i] == kNegInf) value[i] = kNegInf;
     }
-  }
-  for (uint32_t j = 0; j < top; ++j) {
-    float best = value[0];
+    choices[team][lane] = Choice{-1, 0.0f};
+    if (groups > 1) {
+      const uint32_t size = experts / groups;
 #pragma unroll
-    for (int i = 1; i < V; ++i) best = fmaxf(best, value[i]);
-    const float largest = team_max<TEAM>(best);
-    // The first lane that has it, and there the first value.
-    const uint64_t winners = __ballot(best == largest) >> (threadIdx.x % 64 - lane);
-    const bool mine = __builtin_ctzll(winners | uint64_t{1} << 63) == lane && largest != kNegInf;
-    bool open = mine;
+      for (int i = 0; i < V; ++i) values_lds[team][lane * V + i] = value[i];
+      wave_lds_fence();
+      float first = kNegInf, second = kNegInf;
+      if (static_cast<uint32_t>(lane) < groups) {
+#pragma unroll 8
+        for (uint32_t i = 0; i < size; ++i) {
+          const float v = values_lds[team][lane * size + i];
+          second = fmaxf(second, fminf(first, v));
+          first = fmaxf(first, v);
+        }
+      }
+      const float mine = first + (second == kNegInf ? 0.0f : second);
+      groups_lds[team][lane] = mine;
+      wave_lds_fence();
+      // A group is kept if fewer than top_groups come before it: larger ones, or
+      // as large ones of a lower index.
+      uint32_t before = 0;
+#pragma unroll 8
+      for (uint32_t g = 0; g < groups; ++g) {
+        const float other = groups_lds[team][g];
+        before += other > mine || (other == mine && g < static_cast<uint32_t>(lane));
+      }
+      const bool kept = static_cast<uint32_t>(lane) < groups && before < top_groups;
+      const uint64_t mask = __ballot(kept) >> (threadIdx.x % 64 - lane);
+      uint32_t group = lane * V / size, inside = lane * V % size;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (open && value[i] == largest) {
-        open = false;
-        value[i] = kNegInf;
-        choices[team][j] = Choice{static_cast<int32_t>(lane * V + i), score[i]};
+      for (int i = 0; i < V; ++i) {
+        if (!(mask >> (group & 63) & 1)) value[i] = kNegInf;
+        if (++inside == size) inside = 0, ++group;
       }
     }
-  }
-  wave_lds_fence();
-  const Choice choice = choices[team][lane];
+    for (uint32_t j = 0; j < top; ++j) {
+      float best = value[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = fmaxf(best, value[i]);
+      const float largest = team_max<TEAM>(best);
+      // The first lane that has it, and there the first value.
+      const uint64_t winners = __ballot(best == largest) >> (threadIdx.x % 64 - lane);
+      const bool mine = __builtin_ctzll(winners | uint64_t{1} << 63) == lane && largest != kNegInf;
+      bool open = mine;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (open && value[i] == largest) {
+          open = false;
+          value[i] = kNegInf;
+          choices[team][j] = Choice{static_cast<int32_t>(lane * V + i), score[i]};
+        }
+      }
+    }
+    wave_lds_fence();
+    return choices[team][lane];
+  };
+  Choice choice = choose(false);
+  // Once more, with `far` scores, for a token with a choice that scored 0 (a comparison of every logit with -88
+  // would cost 16384 tokens of 256 experts 0.6 us of 14).
+  const uint64_t zeros = softmax ? 0 : __ballot(choice.expert >= 0 && choice.score == 0.0f);
+  if (__builtin_expect(zeros != 0, 0))
+    choice = choose((zeros >> (threadIdx.x % 64 - lane) & ~uint64_t{0} >> (64 - TEAM)) != 0);
   float weight = choice.score;
   if (renormalize) {
     const float total = team_add<TEAM>(choice.score);
@@ -188,22 +196,28 @@ __global__ void __launch_bounds__(256)
   const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
   const uint32_t token = blockIdx.x * TOKENS + team;
   if (token >= tokens) return;
-  float logit[V], score[V];
-  load_logits(logits + token * row_stride, experts, lane, logit);
-  if (softmax) scores_of<V, TEAM>(logit, true, score);
   int expert = -1;
   float d = 0.0f;
   if (static_cast<uint32_t>(lane) < top) {
     expert = chosen[static_cast<uint64_t>(token) * top + lane];
-    if (static_cast<uint32_t>(expert) >= experts) expert = -1;
-    if (expert >= 0) d = d_weights[static_cast<uint64_t>(token) * top + lane] * scale;
+    d = d_weights[static_cast<uint64_t>(token) * top + lane] * scale;
   }
+  float logit[V], score[V];
+  load_logits(logits + token * row_stride, experts, lane, logit);
+  if (softmax) scores_of<V, TEAM>(logit, true, false, score);
+  if (static_cast<uint32_t>(expert) >= experts) expert = -1, d = 0.0f;
 #pragma unroll
   for (int i = 0; i < V; ++i) lds[team][lane * V + i] = softmax ? score[i] : logit[i];
   wave_lds_fence();
   const float held = expert >= 0 ? lds[team][expert] : kNegInf;
   wave_lds_fence();
-  const float s = softmax ? (expert >= 0 ? held : 0.0f) : sigmoid(held);
+  float s = expert >= 0 ? held : 0.0f, rest = 1.0f;
+  if (!softmax) {
+    // s and 1 - s of a sigmoid, both from e^-|l|: the difference is 6% off at a logit of 16 and 0 at 17.5.
+    const float power = expf(-fabsf(held)), larger = 1.0f / (1.0f + power), smaller = power * larger;
+    s = held < 0.0f ? smaller : larger;
+    rest = held < 0.0f ? larger : smaller;
+  }
   if (renormalize) {
     const float total = team_add<TEAM>(s);
     // By shares: a lone choice, whose weight is constant, has a gradient of exactly zero, and nothing
@@ -213,8 +227,7 @@ __global__ void __launch_bounds__(256)
     d = expert < 0 || total == 0.0f ? 0.0f : (d - mean) * share;
   }
   const float common = softmax && !renormalize ? team_add<TEAM>(d * s) : 0.0f;
-  // 1 - s as the sigmoid of the negative logit: the difference is 6% off at a logit of 16 and 0 at 17.5.
-  if (!softmax && expert >= 0) d = (renormalize ? d : d * s) * sigmoid(-held);
+  if (!softmax) d = (renormalize ? d : d * s) * rest;
 #pragma unroll
   for (int i = 0; i < V; ++i) lds[team][lane * V + i] = 0.0f;
   wave_lds_fence();
