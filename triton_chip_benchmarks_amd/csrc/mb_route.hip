@@ -416,16 +416,16 @@ __global__ void __launch_bounds__(256)
   const uint32_t task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
   const uint32_t token = task / strips;
   if (token >= tokens) return;
-  const uint32_t column = task % strips * 512 + (threadIdx.x & 63) * 8;
-  // Lane j holds entry j: the loads of all slots and weights go out together.
-  const uint32_t lane = threadIdx.x & 63;
+  // Lane j holds entry j: the loads of all slots and weights go out together. Lanes past the row stay for their
+  // entries, on the row's last columns.
+  const uint32_t lane = threadIdx.x & 63, own = task % strips * 512 + lane * 8;
+  const uint32_t column = min(own, (n - 1) / 8 * 8);
   uint32_t my_slot = ~0u;
   float my_weight = 0.0f;
   if (lane < top) {
     my_slot = static_cast<uint32_t>(slots[uint64_t{token} * top + lane]);
     my_weight = weights[uint64_t{token} * top + lane];
   }
-  if (column >= n) return;
   const int count = static_cast<int>(min(8u, n - column));
   float sum[8] = {};
   for (uint32_t j0 = 0; j0 < top; j0 += kCombineRows) {
@@ -445,7 +445,7 @@ __global__ void __launch_bounds__(256)
       for (int i = 0; i < 8; ++i) sum[i] = fmaf(weight, raw[j][i], sum[i]);
     }
   }
-  store8<STREAM>(out + uint64_t{token} * n + column, sum, count);
+  if (column == own) store8<STREAM>(out + uint64_t{token} * n + column, sum, count);
 }
 
 constexpr int kGradientRows = 4;
