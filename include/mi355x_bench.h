@@ -298,6 +298,19 @@ int mb_mx_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_
                   uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets,
                   uint64_t offsets_bytes, uint32_t experts, void* stream);
 
+/* Registered name of the kernel that mb_mx_product launches for these sizes or,
+ * with `linear`, mb_mx_linear for `rows` rows of output (after quantising them,
+ * where the kernel takes operands); NULL, with the error set, for sizes that
+ * they refuse or that have no product. */
+const char* mb_mx_product_kernel(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts, uint32_t linear);
+
+/* mb_mx_product on the kernel of that name, for tests and measurements;
+ * MB_ERR_UNSUPPORTED if it does not take the type or these sizes. */
+int mb_mx_product_exact(const char* kernel, int dtype, const void* a, uint64_t a_bytes, const void* scale_a,
+                        uint64_t scale_a_bytes, const void* b, uint64_t b_bytes, const void* scale_b,
+                        uint64_t scale_b_bytes, void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                        const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream);
+
 /* Bytes of workspace (16-byte aligned) mb_mx_linear needs for `rows` rows of output. */
 uint64_t mb_mx_linear_workspace(uint32_t rows, uint32_t n, uint32_t k);
 

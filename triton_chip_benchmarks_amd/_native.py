@@ -116,6 +116,9 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mb_mx_dequantize": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _ptr]),
     "mb_mx_product": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _ptr,
                              _u64, _u32, _ptr]),
+    "mb_mx_product_kernel": (ctypes.c_char_p, [_i32, _u32, _u32, _u32, _u32, _u32]),
+    "mb_mx_product_exact": (_i32, [ctypes.c_char_p, _i32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64,
+                                   _u32, _u32, _u32, _ptr, _u64, _u32, _ptr]),
     "mb_mx_linear_workspace": (_u64, [_u32, _u32, _u32]),
     "mb_mx_linear": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _ptr, _u64,
                             _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),

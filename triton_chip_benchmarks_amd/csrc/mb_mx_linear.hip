@@ -1,5 +1,6 @@
 // Products of MXFP4 operands for linear layers: Y = X . W^T, each row of X with
 // the weight of its expert where there are several.
+#include <cstring>
 #include <type_traits>
 
 #include "mb_elem.h"
@@ -391,14 +392,19 @@ struct ProductKernel {
   int resident;  // workgroups a CU holds
   ProductCost cost;
   ProductLauncher launch[3];  // by MB_DTYPE_*
+  const char* name[3];
 };
 constexpr bool kPersistent_ring = false, kPersistent_stream = true;
-#define MB_PRODUCT(KIND, BM, BN, STAGES, BAND, ...)                                              \
-  ProductKernel {                                                                                \
-    BM, BN, kPersistent_##KIND, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, {__VA_ARGS__}, {    \
-      launch_##KIND<float, BM, BN, STAGES>, launch_##KIND<_Float16, BM, BN, STAGES>,             \
-          launch_##KIND<__bf16, BM, BN, STAGES>                                                  \
-    }                                                                                            \
+#define MB_SUFFIX_ring
+#define MB_SUFFIX_stream "_stream"
+#define MB_PRODUCT_NAME(T, KIND, BM, BN) "mx_product_" T "_" #BM "x" #BN MB_SUFFIX_##KIND
+#define MB_PRODUCT(KIND, BM, BN, STAGES, BAND, ...)                                                        \
+  ProductKernel {                                                                                          \
+    BM, BN, kPersistent_##KIND, BAND, RingTile<MfmaMxfp4, BM, BN, STAGES>::RESIDENT, {__VA_ARGS__},        \
+        {launch_##KIND<float, BM, BN, STAGES>, launch_##KIND<_Float16, BM, BN, STAGES>,                    \
+         launch_##KIND<__bf16, BM, BN, STAGES>},                                                           \
+        {MB_PRODUCT_NAME("f32", KIND, BM, BN), MB_PRODUCT_NAME("f16", KIND, BM, BN),                       \
+         MB_PRODUCT_NAME("bf16", KIND, BM, BN)}                                                            \
   }
 // Fitted to 414 launches on an MI355X (17 to 32768 rows, n and K from 64 to 8192,
 // one weight or 8 to 256 experts of uneven popularity, half of the n odd): the
@@ -491,6 +497,11 @@ double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint
   return cost.launch + whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
 }
 
+// Whether mx_few_kernel can: its rows' codes fit the LDS.
+bool few_fits(uint64_t rows, uint32_t k) {
+  return few_lds_bytes((k + 255) / 256, rows < kFewRows ? static_cast<uint32_t>(rows) : kFewRows) <= 128 * 1024;
+}
+
 // Whether mx_few_kernel takes a call: up to 16 rows of one weight, up to two an
 // expert on average (it reads a weight once for 16 rows, but its rows are
 // quantised, or copied, once a workgroup), whose codes fit the LDS. us, it and
@@ -498,16 +509,36 @@ double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint
 // 15.3; 128 experts of 2048x4096, two rows each 46 and 55, four 87 and 78.
 bool few_rows(uint64_t rows, uint32_t k, uint32_t experts) {
   const uint64_t most = experts > 1 ? 2 * uint64_t{experts} : kFewRows;
-  return rows <= most && few_lds_bytes((k + 255) / 256, rows < kFewRows ? rows : kFewRows) <= 128 * 1024;
+  return rows <= most && few_fits(rows, k);
+}
+
+// Forms of mx_few_kernel, by the number of features a workgroup takes: 32 where
+// that gives every CU a workgroup, else 16 (1x4096x14336 7.7 us, with 32 10.2);
+// with many workgroups, 64 and half the waves on each K (two rows of 128 experts
+// 46 us, with eight 58).
+enum FewForm { kFew16x8, kFew32x8, kFew32x4, kFewForms };
+constexpr uint32_t kFewColumns[kFewForms] = {16, 32, 64};
+#define MB_FEW_NAMES(KIND, SIZE) \
+  {"mx_" KIND "_few_f32_" SIZE, "mx_" KIND "_few_f16_" SIZE, "mx_" KIND "_few_bf16_" SIZE}
+// By form and MB_DTYPE_*: of rows quantised on the way, of operands.
+const char* const kLinearFewNames[kFewForms][3] = {MB_FEW_NAMES("linear", "16x8"), MB_FEW_NAMES("linear", "32x8"),
+                                                   MB_FEW_NAMES("linear", "32x4")};
+const char* const kProductFewNames[kFewForms][3] = {MB_FEW_NAMES("product", "16x8"), MB_FEW_NAMES("product", "32x8"),
+                                                    MB_FEW_NAMES("product", "32x4")};
+const char* const kPlainNames[3] = {"mx_product_f32", "mx_product_f16", "mx_product_bf16"};
+
+FewForm few_form(uint32_t rows, uint32_t n, uint32_t experts) {
+  const uint64_t wide = (n + uint64_t{31}) / 32 * (rows < experts ? rows : experts);
+  return wide < 256 ? kFew16x8 : wide < 2048 ? kFew32x8 : kFew32x4;
 }
 
 template <class X, class T>
-void launch_few(const void* x, uint64_t row_stride, const void* sx, const void* w, const void* sw, void* y,
-                uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, const int32_t* order, uint32_t copies,
-                uint32_t tokens, uint32_t experts, hipStream_t stream) {
+void launch_few(FewForm form, const void* x, uint64_t row_stride, const void* sx, const void* w, const void* sw,
+                void* y, uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, const int32_t* order,
+                uint32_t copies, uint32_t tokens, uint32_t experts, hipStream_t stream) {
   const uint32_t grid_rows = rows < experts ? rows : experts, lds_rows = rows < kFewRows ? rows : kFewRows;
-  const uint64_t wide = (n + uint64_t{31}) / 32 * grid_rows;
-  auto launch = [&](auto kernel, uint32_t columns) {
+  const uint32_t columns = kFewColumns[form];
+  auto launch = [&](auto kernel) {
     kernel<<<dim3((n + columns - 1) / columns, grid_rows), dim3(64 * kFewWaves),
              static_cast<uint32_t>(few_lds_bytes((k + 255) / 256, lds_rows)), stream>>>(
         static_cast<const X*>(x), row_stride, static_cast<const uint8_t*>(sx), static_cast<const uint8_t*>(w),
@@ -515,55 +546,99 @@ void launch_few(const void* x, uint64_t row_stride, const void* sx, const void* 
         static_cast<int>(k), offsets, order, static_cast<int>(copies), static_cast<int>(tokens),
         static_cast<int>(experts), static_cast<int>(lds_rows));
   };
-  // 32 features a workgroup where that gives every CU one, else 16 (1x4096x14336
-  // 7.7 us, with 32 10.2); with many workgroups, half the waves on each K (two
-  // rows of 128 experts 46 us, with eight 58).
-  if (wide < 256)
-    launch(mx_few_kernel<X, T, 1, 8>, 16);
-  else if (wide < 2048)
-    launch(mx_few_kernel<X, T, 2, 8>, 32);
+  if (form == kFew16x8)
+    launch(mx_few_kernel<X, T, 1, 8>);
+  else if (form == kFew32x8)
+    launch(mx_few_kernel<X, T, 2, 8>);
   else
-    launch(mx_few_kernel<X, T, 2, 4>, 64);
+    launch(mx_few_kernel<X, T, 2, 4>);
 }
 
-int launch_product(int dtype, const void* x_codes, const void* sx, const void* w_codes, const void* sw, void* y,
-                   uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, uint32_t experts,
-                   hipStream_t stream) {
-  const uint8_t *x = static_cast<const uint8_t*>(x_codes), *w = static_cast<const uint8_t*>(w_codes);
-  const uint8_t *sxb = static_cast<const uint8_t*>(sx), *swb = static_cast<const uint8_t*>(sw);
-  const uint32_t padded = (k + 31) / 32 * 32, steps = (k + 255) / 256;
-  if (few_rows(rows, k, experts)) {
-    MB_FOR_DTYPE(dtype, (launch_few<uint8_t, T>(x, 0, sx, w, sw, y, rows, n, k, offsets, nullptr, 1, rows, experts,
-                                                stream)));
-    return launch_status("mx_product_few");
+// The kernel that multiplies two operands: a form of mx_few_kernel, a kernel of
+// tiles, or, with neither, mx_product_kernel, which takes every size.
+struct ProductChoice {
+  int few = -1;
+  const ProductKernel* tiles = nullptr;
+  uint32_t grid = 0;  // of tiles
+  const char* name;
+};
+
+// By the rule for these sizes or, with `wanted`, the kernel of that name; false
+// if that one does not take them.
+bool choose_product(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts, const char* wanted,
+                    ProductChoice& out) {
+  auto is_wanted = [&](const char* name) { return wanted == nullptr || strcmp(wanted, name) == 0; };
+  if (wanted == nullptr ? few_rows(rows, k, experts) : few_fits(rows, k)) {
+    for (int form = 0; form < kFewForms; ++form) {
+      if (wanted == nullptr ? form != few_form(rows, n, experts) : !is_wanted(kProductFewNames[form][dtype])) continue;
+      out.few = form;
+      out.name = kProductFewNames[form][dtype];
+      return true;
+    }
   }
   // The ring addresses a matrix's scales, and a tile's rows, with 32-bit offsets.
   const uint64_t scale_rows = rows > n ? rows : n;
+  const uint32_t steps = (k + 255) / 256;
   if (steps * scale_rows * 8 <= 0x7fffffffu) {
-    const ProductKernel* best = nullptr;
     double best_cost = 0;
     const bool ragged = uint64_t{n} * elem_bytes(dtype) % 16 != 0;
-    uint64_t best_grid = 0;
     for (const ProductKernel& kernel : kProductKernels) {
       const uint64_t grid = most_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
       if (grid > 0xffffff) continue;
       if (kernel.persistent && experts > kStreamExperts) continue;
+      if (!is_wanted(kernel.name[dtype])) continue;
       const double cost = product_cost(kernel, rows, n, steps, experts, ragged);
-      if (best == nullptr || cost < best_cost) best = &kernel, best_cost = cost, best_grid = grid;
+      if (out.tiles && cost >= best_cost) continue;
+      best_cost = cost;
+      out.tiles = &kernel;
+      out.grid = static_cast<uint32_t>((grid + 7) / 8 * 8);
+      out.name = kernel.name[dtype];
     }
-    if (best) {
-      best->launch[dtype](x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), static_cast<int>(padded),
-                          offsets, static_cast<int>(experts), static_cast<uint32_t>((best_grid + 7) / 8 * 8),
-                          best->band, stream);
-      return launch_status(best->persistent ? "mx_product_stream" : "mx_product_ring");
-    }
+    if (out.tiles) return true;
   }
-  const uint32_t tiles = (rows / experts + 15) / 16;
-  const dim3 grid((n + 63) / 64, experts, tiles < 1 ? 1 : tiles < 256 ? tiles : 256);
-  MB_FOR_DTYPE(dtype, (mx_product_kernel<T><<<grid, dim3(256), 0, stream>>>(
-                          x, sxb, w, swb, static_cast<T*>(y), static_cast<int>(rows), static_cast<int>(n),
-                          static_cast<int>(k), offsets)));
-  return launch_status("mx_product");
+  out.name = kPlainNames[dtype];
+  return is_wanted(out.name);
+}
+
+int launch_product(int dtype, const void* x_codes, const void* sx, const void* w_codes, const void* sw, void* y,
+                   uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets, uint32_t experts,
+                   const char* wanted, hipStream_t stream) {
+  const uint8_t *x = static_cast<const uint8_t*>(x_codes), *w = static_cast<const uint8_t*>(w_codes);
+  const uint8_t *sxb = static_cast<const uint8_t*>(sx), *swb = static_cast<const uint8_t*>(sw);
+  ProductChoice choice;
+  if (!choose_product(dtype, rows, n, k, experts, wanted, choice))
+    return fail(MB_ERR_UNSUPPORTED, "mx_product: no kernel %s that takes %u x %u x %u and %u experts", wanted, rows, n,
+                k, experts);
+  if (choice.few >= 0) {
+    MB_FOR_DTYPE(dtype, (launch_few<uint8_t, T>(static_cast<FewForm>(choice.few), x, 0, sx, w, sw, y, rows, n, k,
+                                                offsets, nullptr, 1, rows, experts, stream)));
+  } else if (choice.tiles) {
+    const int padded = static_cast<int>((k + 31) / 32 * 32);
+    choice.tiles->launch[dtype](x, sxb, w, swb, y, static_cast<int>(rows), static_cast<int>(n), padded, offsets,
+                                static_cast<int>(experts), choice.grid, choice.tiles->band, stream);
+  } else {
+    const uint32_t tiles = (rows / experts + 15) / 16;
+    const dim3 grid((n + 63) / 64, experts, tiles < 1 ? 1 : tiles < 256 ? tiles : 256);
+    MB_FOR_DTYPE(dtype, (mx_product_kernel<T><<<grid, dim3(256), 0, stream>>>(
+                            x, sxb, w, swb, static_cast<T*>(y), static_cast<int>(rows), static_cast<int>(n),
+                            static_cast<int>(k), offsets)));
+  }
+  return launch_status(choice.name);
+}
+
+int run_product(const char* entry, const char* wanted, int dtype, const void* a, uint64_t a_bytes, const void* scale_a,
+                uint64_t scale_a_bytes, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
+                void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets,
+                uint64_t offsets_bytes, uint32_t experts, void* stream) {
+  if (int rc = check_shape(entry, dtype, rows, n, k, experts)) return rc;
+  if (int rc = check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
+  if (rows == 0 || n == 0) return MB_OK;
+  if (k == 0) return fail(MB_ERR_INVALID, "%s: K must be positive", entry);
+  if (int rc = check_operand(entry, "a", rows, k, 1, a, a_bytes, scale_a, scale_a_bytes)) return rc;
+  if (int rc = check_operand(entry, "b", n, k, experts, b, b_bytes, scale_b, scale_b_bytes)) return rc;
+  if (int rc = check_output(entry, dtype, c, c_bytes, rows, n)) return rc;
+  return launch_product(dtype, a, scale_a, b, scale_b, c, rows, n, k, offsets, experts, wanted,
+                        static_cast<hipStream_t>(stream));
 }
 
 }  // namespace
@@ -575,16 +650,29 @@ int mb_mx_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_
                   const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes, void* c,
                   uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k, const int32_t* offsets,
                   uint64_t offsets_bytes, uint32_t experts, void* stream) {
-  const char* entry = "mb_mx_product";
-  if (int rc = mb::check_shape(entry, dtype, rows, n, k, experts)) return rc;
-  if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
-  if (rows == 0 || n == 0) return MB_OK;
-  if (k == 0) return mb::fail(MB_ERR_INVALID, "%s: K must be positive", entry);
-  if (int rc = mb::check_operand(entry, "a", rows, k, 1, a, a_bytes, scale_a, scale_a_bytes)) return rc;
-  if (int rc = mb::check_operand(entry, "b", n, k, experts, b, b_bytes, scale_b, scale_b_bytes)) return rc;
-  if (int rc = mb::check_output(entry, dtype, c, c_bytes, rows, n)) return rc;
-  return mb::launch_product(dtype, a, scale_a, b, scale_b, c, rows, n, k, offsets, experts,
-                            static_cast<hipStream_t>(stream));
+  return mb::run_product("mb_mx_product", nullptr, dtype, a, a_bytes, scale_a, scale_a_bytes, b, b_bytes, scale_b,
+                         scale_b_bytes, c, c_bytes, rows, n, k, offsets, offsets_bytes, experts, stream);
+}
+
+int mb_mx_product_exact(const char* kernel, int dtype, const void* a, uint64_t a_bytes, const void* scale_a,
+                        uint64_t scale_a_bytes, const void* b, uint64_t b_bytes, const void* scale_b,
+                        uint64_t scale_b_bytes, void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                        const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream) {
+  if (kernel == nullptr) return mb::fail(MB_ERR_INVALID, "mb_mx_product_exact: the kernel's name is NULL");
+  return mb::run_product("mb_mx_product_exact", kernel, dtype, a, a_bytes, scale_a, scale_a_bytes, b, b_bytes, scale_b,
+                         scale_b_bytes, c, c_bytes, rows, n, k, offsets, offsets_bytes, experts, stream);
+}
+
+const char* mb_mx_product_kernel(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts, uint32_t linear) {
+  const char* entry = "mb_mx_product_kernel";
+  if (mb::check_shape(entry, dtype, rows, n, k, experts)) return nullptr;
+  if (rows == 0 || n == 0 || k == 0) {
+    mb::fail(MB_ERR_INVALID, "%s: empty product %u x %u x %u", entry, rows, n, k);
+    return nullptr;
+  }
+  mb::ProductChoice choice;
+  mb::choose_product(dtype, rows, n, k, experts, nullptr, choice);
+  return linear && choice.few >= 0 ? mb::kLinearFewNames[choice.few][dtype] : choice.name;
 }
 
 uint64_t mb_mx_linear_workspace(uint32_t rows, uint32_t n, uint32_t k) {
@@ -623,15 +711,16 @@ int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, ui
   uint8_t* scales = codes + codes_bytes;
   const hipStream_t on = static_cast<hipStream_t>(stream);
   if (mb::few_rows(rows, k, experts)) {
-    MB_FOR_DTYPE(dtype, (mb::launch_few<T, T>(x, row_stride, nullptr, w, scale_w, y, static_cast<uint32_t>(rows), n, k,
-                                              offsets, gathered ? order : nullptr, copies, tokens, experts, on)));
-    return mb::launch_status("mx_linear_few");
+    const mb::FewForm form = mb::few_form(static_cast<uint32_t>(rows), n, experts);
+    MB_FOR_DTYPE(dtype, (mb::launch_few<T, T>(form, x, row_stride, nullptr, w, scale_w, y, static_cast<uint32_t>(rows),
+                                              n, k, offsets, gathered ? order : nullptr, copies, tokens, experts, on)));
+    return mb::launch_status(mb::kLinearFewNames[form][dtype]);
   }
   if (int rc = mb::launch_quantize(dtype, x, tokens, k, row_stride, slots, gathered ? copies : 1,
                                    static_cast<uint32_t>(rows), codes, scales, on))
     return rc;
   return mb::launch_product(dtype, codes, scales, w, scale_w, y, static_cast<uint32_t>(rows), n, k, offsets, experts,
-                            on);
+                            nullptr, on);
 }
 
 // Operands of mb_mx_linear_backward in its workspace: Q(d_out) [rows][n], and the
@@ -686,10 +775,10 @@ int mb_mx_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, ui
                                             space + codes[2], space + scales[2], on))
     return rc;
   if (int rc = mb::launch_product(dtype, space + codes[0], space + scales[0], w_columns, scale_w, d_x, rows, k, n,
-                                  nullptr, 1, on))
+                                  nullptr, 1, nullptr, on))
     return rc;
   return mb::launch_product(dtype, space + codes[1], space + scales[1], space + codes[2], space + scales[2], d_w, n, k,
-                            depth, nullptr, 1, on);
+                            depth, nullptr, 1, nullptr, on);
 }
 
 }  // extern "C"

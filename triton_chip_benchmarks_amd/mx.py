@@ -165,11 +165,21 @@ def dequantize(packed: Packed, out=None, stream=None):
     return out
 
 
-def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=None):
+def product_kernel(rows: int, n: int, k: int, dtype=torch.bfloat16, experts: int = 1, linear: bool = False) -> str:
+    """Name of the kernel that `product` (with `linear`, `linear` for `rows` rows of output) launches."""
+    code = DTYPE_CODES.get(dtype, -1)
+    name = library().mb_mx_product_kernel(code, rows, n, k, experts, int(linear))
+    if name is None:
+        raise _native.NativeError(_native.MB_ERR_INVALID, _native.last_error())
+    return name.decode()
+
+
+def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=None, kernel: str | None = None):
     """A . B^T of two operands, in `dtype` (bfloat16 unless `out` or `dtype` says otherwise).
 
     With `offsets` ([experts + 1] int32, on the device) b holds a matrix for each expert, and a's rows offsets[e] ..
-    offsets[e + 1] - 1 meet matrix e; output rows from offsets[experts] on are not written.
+    offsets[e + 1] - 1 meet matrix e; output rows from offsets[experts] on are not written. `kernel` names the kernel
+    to run on, for tests and measurements.
     """
     experts = None if offsets is None else offsets.numel() - 1
     _check_experts(a, "a", None)
@@ -182,10 +192,13 @@ def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=Non
     code = dtype_code(out, "out")
     _check_indices(offsets, "offsets")
     handle = launch_stream(stream, a.codes, a.scales, b.codes, b.scales, out, *(() if offsets is None else (offsets,)))
-    status = library().mb_mx_product(
-        code, a.codes.data_ptr(), a.codes.numel(), a.scales.data_ptr(), a.scales.numel(), b.codes.data_ptr(),
-        b.codes.numel(), b.scales.data_ptr(), b.scales.numel(), out.data_ptr(), a.rows * b.rows * (2 if code else 4),
-        a.rows, b.rows, a.k, *_pointer(offsets), experts or 1, handle)
+    arguments = (code, a.codes.data_ptr(), a.codes.numel(), a.scales.data_ptr(), a.scales.numel(), b.codes.data_ptr(),
+                 b.codes.numel(), b.scales.data_ptr(), b.scales.numel(), out.data_ptr(),
+                 a.rows * b.rows * (2 if code else 4), a.rows, b.rows, a.k, *_pointer(offsets), experts or 1, handle)
+    if kernel is None:
+        status = library().mb_mx_product(*arguments)
+    else:
+        status = library().mb_mx_product_exact(kernel.encode(), *arguments)
     if status:
         _native.check(status)
     return out
