@@ -583,7 +583,8 @@ bool choose_product(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t e
     double best_cost = 0;
     const bool ragged = uint64_t{n} * elem_bytes(dtype) % 16 != 0;
     for (const ProductKernel& kernel : kProductKernels) {
-      const uint64_t grid = most_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
+      const uint64_t tiles = most_row_tiles(rows, experts, kernel.rows) * ((n + kernel.features - 1) / kernel.features);
+      const uint64_t grid = (tiles + kXcds - 1) / kXcds * kXcds;
       if (grid > 0xffffff) continue;
       if (kernel.persistent && experts > kStreamExperts) continue;
       if (!is_wanted(kernel.name[dtype])) continue;
@@ -591,7 +592,7 @@ bool choose_product(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t e
       if (out.tiles && cost >= best_cost) continue;
       best_cost = cost;
       out.tiles = &kernel;
-      out.grid = static_cast<uint32_t>((grid + 7) / 8 * 8);
+      out.grid = static_cast<uint32_t>(grid);
       out.name = kernel.name[dtype];
     }
     if (out.tiles) return true;
