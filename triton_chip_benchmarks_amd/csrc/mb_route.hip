@@ -747,6 +747,8 @@ int mb_combine_backward(int dtype, const void* d_out, uint64_t d_out_bytes, cons
   if (int rc = check_combine(entry, dtype, y, y_bytes, y_rows, slots, slots_bytes, weights, weights_bytes, tokens, top,
                              n))
     return rc;
+  // A workgroup of 256 a token, and a launch holds at most 2^32 - 1 work items.
+  if (tokens > 0xffffffu) return mb::fail(MB_ERR_UNSUPPORTED, "%s: at most %u tokens", entry, 0xffffffu);
   const uint32_t item = mb::elem_bytes(dtype);
   if (tokens == 0) return MB_OK;
   if (int rc = check_rows_out(entry, "d_out", d_out, d_out_bytes, tokens, n, item)) return rc;
