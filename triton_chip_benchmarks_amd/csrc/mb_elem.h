@@ -42,10 +42,6 @@ struct Raw8 {
     for (int i = 0; i < 8; ++i) v[i] = i < count ? p[i] : T(0);
     __builtin_memcpy(part, v, sizeof(part));
   }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) part[i] = elem_u32x4{0, 0, 0, 0};
-  }
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (sizeof(T) == 4) {
       const uint32_t word = part[i / 4][i % 4];  // __builtin_bit_cast of the element itself takes element 0
@@ -113,10 +109,6 @@ __device__ __forceinline__ float wave_reduce(float v, float none, F&& f) {
 
 __device__ __forceinline__ float wave_add(float v) {
   return wave_reduce(v, 0.0f, [](float a, float b) { return a + b; });
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-  return wave_reduce(v, -__builtin_inff(), [](float a, float b) { return fmaxf(a, b); });
 }
 
 // f over the lane's team of TEAM lanes (a wave's 64, or its row of 16), the same
