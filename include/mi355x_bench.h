@@ -261,7 +261,9 @@ const char* mb_gemm_exact_tile_kernel(int format, const mb_gemm_config* config, 
  *
  * Element types are MB_DTYPE_*. A tensor's rows are contiguous; inputs x and
  * logits take a row stride in elements (0 repeats a row) and lie at any
- * element's address. A size of zero is a call without work. */
+ * element's address. A size of zero is a call without work, except where an
+ * output would be a sum over nothing: a product, or a linear layer, refuses K = 0
+ * (with rows and n), and mb_mx_linear_backward any size of 0. */
 
 /* Rows of x [rows][k] to an MXFP4 operand: codes [out_rows][ceil(k/32)*16]
  * bytes (16-byte aligned; even k in the low nibble, zero past k) and scales
@@ -318,9 +320,9 @@ uint64_t mb_mx_linear_workspace(uint32_t rows, uint32_t n, uint32_t k);
  * launch for few rows and two for more.
  * offsets NULL: Y [tokens][n], one weight. With offsets and slots NULL: X's rows
  * are already in the order of the experts. With order and slots (mb_dispatch,
- * [tokens][copies]): X holds tokens, and Y [tokens*copies][n] their routed rows
- * in the order of the experts; Y's rows from offsets[experts] on are not
- * written. */
+ * [tokens][copies]; slots_bytes is what each of the two holds): X holds tokens,
+ * and Y [tokens*copies][n] their routed rows in the order of the experts; Y's
+ * rows from offsets[experts] on are not written. */
 int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,
                  uint64_t w_bytes, const void* scale_w, uint64_t scale_w_bytes, void* y, uint64_t y_bytes, uint32_t n,
                  uint32_t k, const int32_t* offsets, uint64_t offsets_bytes, const int32_t* order,

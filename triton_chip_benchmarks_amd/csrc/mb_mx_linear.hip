@@ -694,7 +694,7 @@ int mb_mx_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, ui
   if (int rc = mb::check_shape(entry, dtype, rows, n, k, experts)) return rc;
   if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
   if (gathered && (offsets == nullptr || order == nullptr || slots_bytes < rows * 4))
-    return mb::fail(MB_ERR_INVALID, "%s: slots need offsets, order and an entry for each of %llu rows", entry,
+    return mb::fail(MB_ERR_INVALID, "%s: slots need offsets, order and, in both, an entry for each of %llu rows", entry,
                     (unsigned long long)rows);
   if (!mb::aligned(slots, 4) || !mb::aligned(order, 4))
     return mb::fail(MB_ERR_ALIGNMENT, "%s: order and slots must lie on 4 bytes", entry);
