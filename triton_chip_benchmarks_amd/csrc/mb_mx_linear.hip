@@ -74,9 +74,12 @@ __global__ void __launch_bounds__(256)
 // launch and one pass over K. A wave keeps one turn's loads in flight (2.2 KiB of
 // 32 features): many waves cover the latency better than deep ones, whose
 // registers cost them (two turns deep 5 to 20% slower with many experts, four
-// 60%), and non-temporal loads lose 5 to 10%. Quantising in the kernel costs it
-// 0.4 us of 8.6 at 1x8192x8192, 4 of 42 for two rows of each of 128 experts of
-// 2048x4096, and spares a launch of 3.
+// 60%), and non-temporal loads lose 5 to 10%. With the weight from HBM (another
+// copy of it in each pass): 1x8192x8192 10.4 us (3.4 TB/s; the same weight again,
+// from the memory-side cache, 7.5), two rows for each of 128 experts of 2048x4096
+// 92 (6.2 TB/s). Quantising in the kernel spares a launch of 2.3 and costs 0.1 at
+// 1x8192x8192, nothing beside 128 experts and, since every workgroup does it for
+// every row, 2.9 of 16.0 at 16x8192x8192 and 5.2 of 18.5 at 16x4096x14336.
 constexpr int kFewWaves = 8, kFewRows = 16;
 
 // Expert and rows of a workgroup's blockIdx.y; false where it has none. With
@@ -504,18 +507,20 @@ bool few_fits(uint64_t rows, uint32_t k) {
 
 // Whether mx_few_kernel takes a call: up to 16 rows of one weight, up to two an
 // expert on average (it reads a weight once for 16 rows, but its rows are
-// quantised, or copied, once a workgroup), whose codes fit the LDS. us, it and
-// the ring with its quantisation: 1x8192x8192 9.0 and 15, 16x8192x8192 14.3 and
-// 15.3; 128 experts of 2048x4096, two rows each 46 and 55, four 87 and 78.
+// quantised, or copied, once a workgroup), whose codes fit the LDS. us, weights
+// from HBM, it and the tiles with their quantisation: 16x8192x8192 16.0 and 19.0,
+// 16x4096x14336 18.5 and 27.7; 128 experts of 2048x4096, two rows each 92 and 103
+// (128x64 tiles), four 107 on those, and 92 here for rows that are operands.
 bool few_rows(uint64_t rows, uint32_t k, uint32_t experts) {
   const uint64_t most = experts > 1 ? 2 * uint64_t{experts} : kFewRows;
   return rows <= most && few_fits(rows, k);
 }
 
 // Forms of mx_few_kernel, by the number of features a workgroup takes: 32 where
-// that gives every CU a workgroup, else 16 (1x4096x14336 7.7 us, with 32 10.2);
-// with many workgroups, 64 and half the waves on each K (two rows of 128 experts
-// 46 us, with eight 58).
+// that gives every CU a workgroup, else 16 (operands of 1x4096x14336 9.2 us, with
+// 32 11.2; at 8192x8192, with one workgroup of 32 a CU, 10.2 and with 16 9.6); with
+// many workgroups, 64 and half the waves on each K (two rows of 128 experts 92.7,
+// with all eight 95.1; four 92.2 and 98.9).
 enum FewForm { kFew16x8, kFew32x8, kFew32x4, kFewForms };
 constexpr uint32_t kFewColumns[kFewForms] = {16, 32, 64};
 #define MB_FEW_NAMES(KIND, SIZE) \
