@@ -398,6 +398,131 @@ int mb_combine_backward(int dtype, const void* d_out, uint64_t d_out_bytes, cons
                         uint64_t weights_bytes, void* d_y, uint64_t d_y_bytes, float* d_weights,
                         uint64_t d_weights_bytes, uint32_t tokens, uint32_t top, uint32_t n, void* stream);
 
+/* ---- layer operators: a feed-forward block in 8-bit floating point ---------
+ *
+ * FP8 operands with block scales, their products with a linear layer's gradients,
+ * the gated pair of projections and the root-mean-square norm. The reference has none
+ * of these. Conventions as for the MXFP4 operators above: element types MB_DTYPE_*,
+ * contiguous rows at a stride in elements, a size of zero is a call without work
+ * (K = 0 is refused, as are sizes of 0 of a backward call). */
+
+/* Rows of x [rows][k] to an FP8 operand with a scale for each 128 elements of a row:
+ * codes [out_rows][k rounded up to 16] E4M3 bytes (16-byte aligned; zero past k) and
+ * scales [ceil(k/512)][out_rows][4] (4-byte aligned; entry [b][r][g] is of elements
+ * 512b+128g .. +127, 127 for blocks past k). The scale byte of a block is e + 127, e
+ * the smallest integer with max|x| <= 448 * 2^e, at least -127, -127 for zeros; its
+ * elements are the E4M3 values nearest to x / 2^e, ties to the even code. A block that
+ * holds an infinity or NaN gets the byte 255 (NaN) and codes 0. slots, copies and
+ * out_rows as in mb_mx_quantize. */
+int mb_fp8_quantize(int dtype, const void* x, uint64_t x_bytes, uint32_t rows, uint32_t k, uint64_t row_stride,
+                    const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t out_rows, void* codes,
+                    uint64_t codes_bytes, void* scales, uint64_t scales_bytes, void* stream);
+
+/* The rows of x [rows][columns] to an operand of `rows` rows and K = columns, its
+ * columns to one of `columns` rows and K = rows (x transposed), or both in one pass; a
+ * NULL operand is left out. block = 1: scales as above. block = 128: one for 128 x 128
+ * elements, scales [ceil(K/512)][ceil(operand rows/128)][4], the same both ways, so
+ * that both operands hold the same values. */
+int mb_fp8_quantize_both(int dtype, const void* x, uint64_t x_bytes, uint32_t rows, uint32_t columns,
+                         uint64_t row_stride, uint32_t block, void* codes, uint64_t codes_bytes, void* scales,
+                         uint64_t scales_bytes, void* column_codes, uint64_t column_codes_bytes, void* column_scales,
+                         uint64_t column_scales_bytes, void* stream);
+
+/* An operand to the values it stands for, out [rows][k], rounded once to dtype. */
+int mb_fp8_dequantize(int dtype, const void* codes, uint64_t codes_bytes, const void* scales, uint64_t scales_bytes,
+                      uint32_t block, void* out, uint64_t out_bytes, uint32_t rows, uint32_t k, void* stream);
+
+/* C [rows][n] = A . B^T for operands A of `rows` rows and B of `experts` matrices of n
+ * rows (codes and scales one matrix after the other), a scale of A standing for
+ * a_block rows (1 or 128) and one of B for b_block. Sums in fp32, rounded once to
+ * dtype. offsets as in mb_mx_product; with them a_block is 1. */
+int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
+                   uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
+                   uint32_t b_block, void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                   const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream);
+
+/* Bytes of workspace (16-byte aligned) of mb_fp8_linear and mb_fp8_gated for `rows`
+ * rows of output. */
+uint64_t mb_fp8_linear_workspace(uint32_t rows, uint32_t n, uint32_t k);
+
+/* Y = Q(X) . W^T: mb_fp8_quantize of X, then mb_fp8_product with the weight. offsets,
+ * order, slots and copies as in mb_mx_linear. */
+int mb_fp8_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,
+                  uint64_t w_bytes, const void* scale_w, uint64_t scale_w_bytes, uint32_t w_block, void* y,
+                  uint64_t y_bytes, uint32_t n, uint32_t k, const int32_t* offsets, uint64_t offsets_bytes,
+                  const int32_t* order, const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t experts,
+                  void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace (16-byte aligned) of mb_fp8_linear_backward. */
+uint64_t mb_fp8_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k);
+
+/* Gradients of Y = Q(X) . Q(W)^T, straight through the quantisation, for d_out
+ * [rows][n]: d_x [rows][k] = Q(d_out) . Wc with the weight's columns (an operand of k
+ * rows and K = n, mb_fp8_quantize_both of W), and d_w [n][k] = d_out^T . X, both
+ * quantised by columns with block = 1. Three launches. */
+int mb_fp8_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* x,
+                           uint64_t x_bytes, uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes,
+                           const void* scale_w, uint64_t scale_w_bytes, uint32_t w_block, void* d_x,
+                           uint64_t d_x_bytes, void* d_w, uint64_t d_w_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                           void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Y [rows][n] = silu(G) * U with [G | U] = A . B^T, B's matrices of 2n rows: the n of
+ * the gate, then the n of the up projection. silu(g) = g / (1 + e^-g), in fp32.
+ * y_scales NULL: y in dtype, and, if gate_up is given, [G | U] as gate_up [rows][2n] in
+ * dtype. Else y is an FP8 operand's codes (K = n, a scale for each row's 128),
+ * quantised from the fp32 values, and gate_up must be NULL. Everything else as in
+ * mb_fp8_product. */
+int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
+                         uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
+                         uint32_t b_block, void* y, uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes,
+                         void* gate_up, uint64_t gate_up_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                         const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream);
+
+/* The same of Q(X), as mb_fp8_linear. */
+int mb_fp8_gated(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,
+                 uint64_t w_bytes, const void* scale_w, uint64_t scale_w_bytes, uint32_t w_block, void* y,
+                 uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes, void* gate_up, uint64_t gate_up_bytes,
+                 uint32_t n, uint32_t k, const int32_t* offsets, uint64_t offsets_bytes, const int32_t* order,
+                 const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t experts, void* workspace,
+                 uint64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace (16-byte aligned) of mb_fp8_gated_backward. */
+uint64_t mb_fp8_gated_backward_workspace(uint32_t rows, uint32_t n, uint32_t k);
+
+/* Gradients of mb_fp8_gated for d_out [rows][n], from the gate_up [rows][2n] that it
+ * kept: with s = 1 / (1 + e^-G), d_G = d_out U s (1 + G (1 - s)) and d_U = d_out G s
+ * are quantised from fp32, and go on as d_out [rows][2n] of mb_fp8_linear_backward,
+ * for the columns of W [2n][k]. Three launches. */
+int mb_fp8_gated_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride,
+                          const void* gate_up, uint64_t gate_up_bytes, const void* x, uint64_t x_bytes,
+                          uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes, const void* scale_w,
+                          uint64_t scale_w_bytes, uint32_t w_block, void* d_x, uint64_t d_x_bytes, void* d_w,
+                          uint64_t d_w_bytes, uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                          uint64_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm of rows: t = x + residual, rounded to dtype and written to
+ * total (both NULL: t = x), y = t * weight / sqrt(mean(t^2) + eps) in fp32, rounded
+ * once to out [rows][n] (dtype), to an FP8 operand (codes and scales, as
+ * mb_fp8_quantize of the fp32 values), or both; NULL ones are left out. weight [n] of
+ * dtype. total may be x or the residual itself. n <= 16384. */
+int mb_rms_norm(int dtype, const void* x, uint64_t x_bytes, uint64_t x_stride, const void* residual,
+                uint64_t residual_bytes, uint64_t residual_stride, const void* weight, uint64_t weight_bytes, float eps,
+                void* total, uint64_t total_bytes, void* out, uint64_t out_bytes, void* codes, uint64_t codes_bytes,
+                void* scales, uint64_t scales_bytes, uint32_t rows, uint32_t n, void* stream);
+
+/* Bytes of workspace (16-byte aligned) of mb_rms_norm_backward. */
+uint64_t mb_rms_norm_backward_workspace(uint32_t rows, uint32_t n);
+
+/* Gradients of mb_rms_norm for d_out [rows][n]: d_x [rows][n], of x and of the residual
+ * alike, with d_total (NULL: none), the gradient that t gets as an output, added; and
+ * d_weight [n], summed over the rows in a fixed order. d_x may be d_out or d_total
+ * itself. Two launches. */
+int mb_rms_norm_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* total,
+                         uint64_t total_bytes, uint64_t total_stride, const void* weight, uint64_t weight_bytes,
+                         float eps, const void* d_total, uint64_t d_total_bytes, uint64_t d_total_stride, void* d_x,
+                         uint64_t d_x_bytes, void* d_weight, uint64_t d_weight_bytes, uint32_t rows, uint32_t n,
+                         void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- vector: register-resident arithmetic chains ------------------------ */
 
 /* Vector chain kinds. Storage of input/output/coefficients per kind:

@@ -134,6 +134,31 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mb_combine": (_i32, [_i32, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _ptr]),
     "mb_combine_backward": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr, _u64,
                                    _u32, _u32, _u32, _ptr]),
+    "mb_fp8_quantize": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr, _u64,
+                               _ptr]),
+    "mb_fp8_quantize_both": (_i32, [_i32, _ptr, _u64, _u32, _u32, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr, _u64, _ptr,
+                                    _u64, _ptr]),
+    "mb_fp8_dequantize": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _u32, _u32, _ptr]),
+    "mb_fp8_product": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _u32, _u32,
+                              _u32, _ptr, _u64, _u32, _ptr]),
+    "mb_fp8_linear_workspace": (_u64, [_u32, _u32, _u32]),
+    "mb_fp8_linear": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _u32, _u32, _ptr,
+                             _u64, _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
+    "mb_fp8_linear_backward_workspace": (_u64, [_u32, _u32, _u32]),
+    "mb_fp8_linear_backward": (_i32, [_i32, _ptr, _u64, _u64, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _u32, _ptr,
+                                      _u64, _ptr, _u64, _u32, _u32, _u32, _ptr, _u64, _ptr]),
+    "mb_fp8_gated_product": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr,
+                                    _u64, _ptr, _u64, _u32, _u32, _u32, _ptr, _u64, _u32, _ptr]),
+    "mb_fp8_gated": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr,
+                            _u64, _u32, _u32, _ptr, _u64, _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
+    "mb_fp8_gated_backward_workspace": (_u64, [_u32, _u32, _u32]),
+    "mb_fp8_gated_backward": (_i32, [_i32, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _u32,
+                                     _ptr, _u64, _ptr, _u64, _u32, _u32, _u32, _ptr, _u64, _ptr]),
+    "mb_rms_norm": (_i32, [_i32, _ptr, _u64, _u64, _ptr, _u64, _u64, _ptr, _u64, _f32, _ptr, _u64, _ptr, _u64, _ptr,
+                           _u64, _ptr, _u64, _u32, _u32, _ptr]),
+    "mb_rms_norm_backward_workspace": (_u64, [_u32, _u32]),
+    "mb_rms_norm_backward": (_i32, [_i32, _ptr, _u64, _u64, _ptr, _u64, _u64, _ptr, _u64, _f32, _ptr, _u64, _u64, _ptr,
+                                    _u64, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
     "mb_vector_kernel_name": (ctypes.c_char_p, [_i32, _u32]),
     "mb_vector_chains": (_i32, [_i32, _ptr, _ptr, _ptr, _u64, _u32, _u32, _u32, _u64, _u64, _u64, _ptr]),
 }

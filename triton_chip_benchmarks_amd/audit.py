@@ -43,6 +43,14 @@ _LAYER_RE = re.compile(r"(mx_quantize_columns|mx_quantize_gradient|mx_dequantize
                        r"_kernelI(f|DF16_|DF16b)(?:Lb([01])E)?E")
 _PRODUCT_RING_RE = re.compile(r"mx_product_(ring|stream)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)ELi\d+EE")
 _FEW_RE = re.compile(r"mx_few_kernelI(h|f|DF16_|DF16b)(S\d*_|T_|f|DF16_|DF16b)?Li(\d+)ELi(\d+)EE")
+_FP8_TYPE = {**_ELEMENT_TYPE, "h": "e4m3"}
+_FP8_QUANTIZE_RE = re.compile(r"fp8_quantize_kernelI(f|DF16_|DF16b)Li(\d+)ELb([01])E")
+_FP8_TENSOR_RE = re.compile(r"(fp8_quantize_tiles|fp8_gradient|fp8_dequantize|rms_norm_weight)_kernelI(f|DF16_|DF16b)"
+                            r"(?:Lb([01])E)?E")
+_FP8_FLAG = {"fp8_quantize_tiles": "_square", "fp8_gradient": "_gated", "fp8_dequantize": "_stream"}
+_FP8_FEW_RE = re.compile(r"fp8_few_kernelI(h|f|DF16_|DF16b)(h|f|DF16_|DF16b)Li([012])ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)EE")
+_FP8_EPILOGUE = ("product", "gated", "gated_fp8")
+_NORM_RE = re.compile(r"(rms_norm(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)EE")
 _DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
 _VECTOR_RE = re.compile(r"vector_(\w+?)_kernelILi(\d+)E")
 _READ_TYPE = {"f": "f32", "DF16_": "f16", "t": "bf16"}
@@ -110,6 +118,22 @@ def registered_name(symbol: str) -> str | None:
         x, y, blocks, split = match.groups()
         family = "product" if x == "h" else "linear"
         return f"mx_{family}_few_{_ELEMENT_TYPE[y if x == 'h' else x]}_{16 * int(blocks)}x{split}"
+    match = _FP8_QUANTIZE_RE.search(symbol)
+    if match:
+        dtype, loads, stream = match.groups()
+        return f"fp8_quantize_{_ELEMENT_TYPE[dtype]}_{512 * int(loads)}{'_stream' if stream == '1' else ''}"
+    match = _FP8_TENSOR_RE.search(symbol)
+    if match:
+        family, dtype, flag = match.groups()
+        return f"{family}_{_ELEMENT_TYPE[dtype]}{_FP8_FLAG[family] if flag == '1' else ''}"
+    match = _FP8_FEW_RE.search(symbol)
+    if match:
+        x, y, epilogue, *sizes = match.groups()
+        return f"fp8_few_{_FP8_EPILOGUE[int(epilogue)]}_{_FP8_TYPE[x]}_{_FP8_TYPE[y]}_{'x'.join(sizes)}"
+    match = _NORM_RE.search(symbol)
+    if match:
+        family, dtype, waves, pieces = match.groups()
+        return f"{family}_{_ELEMENT_TYPE[dtype]}_{waves}x{pieces}"
     match = _DISPATCH_RE.search(symbol)
     if match:
         return match.group(1)

@@ -1,0 +1,412 @@
+// Products of FP8 operands with block scales: linear layers, their gradients and the
+// gated pair of projections, of one weight or one for each expert.
+#include "mb_fp8.h"
+#include "mb_fp8_few.h"
+
+namespace mb {
+namespace {
+
+// ---- few rows, and every size ---------------------------------------------------
+
+template <class X, class Y, int EPILOGUE, int FB, int RB, int WAVES, int SPLIT>
+void launch_few(const Fp8Product& p, hipStream_t stream) {
+  constexpr uint32_t kColumns = WAVES / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kRows = 16 * RB;
+  const uint32_t rows = static_cast<uint32_t>(p.rows), experts = static_cast<uint32_t>(p.experts);
+  const uint32_t lds_rows = rows < kRows ? rows : kRows;
+  const uint32_t chunks = (rows / (p.offsets ? experts : 1) + kRows - 1) / kRows;
+  const dim3 grid((static_cast<uint32_t>(p.n) + kColumns - 1) / kColumns,
+                  p.offsets ? (rows < experts ? rows : experts) : 1, chunks < 1 ? 1 : chunks < 256 ? chunks : 256);
+  const uint64_t lds = sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0;
+  fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>
+      <<<grid, dim3(64 * WAVES), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
+}
+
+template <class X, class Y>
+void launch_product_as(Fp8Epilogue epilogue, const Fp8Product& p, hipStream_t stream) {
+  if (epilogue == kFp8Plain)
+    launch_few<X, Y, kFp8Plain, 2, 1, 8, 8>(p, stream);
+  else if (epilogue == kFp8Gated)
+    launch_few<X, Y, kFp8Gated, 2, 1, 8, 8>(p, stream);
+  else
+    launch_few<X, uint8_t, kFp8GatedFp8, 2, 1, 8, 1>(p, stream);
+}
+
+#define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, RB, WAVES, SPLIT)                           \
+  MB_REGISTER_KERNEL("fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #RB "x" #WAVES "x" #SPLIT,       \
+                     (fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>))
+#define MB_FP8_REGISTER(T, NAME)                                              \
+  MB_FP8_FEW(uint8_t, "e4m3", T, NAME, kFp8Plain, "product", 2, 1, 8, 8);     \
+  MB_FP8_FEW(T, NAME, T, NAME, kFp8Plain, "product", 2, 1, 8, 8);             \
+  MB_FP8_FEW(uint8_t, "e4m3", T, NAME, kFp8Gated, "gated", 2, 1, 8, 8);       \
+  MB_FP8_FEW(T, NAME, T, NAME, kFp8Gated, "gated", 2, 1, 8, 8);               \
+  MB_FP8_FEW(T, NAME, uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)
+MB_FP8_REGISTER(float, "f32");
+MB_FP8_REGISTER(_Float16, "f16");
+MB_FP8_REGISTER(__bf16, "bf16");
+MB_FP8_FEW(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1);
+
+constexpr uint32_t kMostExperts = 4096;
+
+int check_shape(const char* entry, int dtype, uint64_t rows, uint64_t n, uint64_t k, uint32_t experts) {
+  if (!elem_bytes(dtype)) return fail(MB_ERR_INVALID, "%s: unknown element type %d", entry, dtype);
+  if (experts == 0 || experts > kMostExperts)
+    return fail(MB_ERR_INVALID, "%s: %u experts outside 1..%u", entry, experts, kMostExperts);
+  if (rows > kFp8MostRows || n > kFp8MostK || k > kFp8MostK)
+    return fail(MB_ERR_UNSUPPORTED, "%s: %llu x %llu x %llu: at most %u rows, %u columns and %u elements of K", entry,
+                (unsigned long long)rows, (unsigned long long)n, (unsigned long long)k, kFp8MostRows, kFp8MostK,
+                kFp8MostK);
+  return MB_OK;
+}
+
+int check_offsets(const char* entry, const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts) {
+  if (offsets == nullptr)
+    return experts == 1 ? MB_OK : fail(MB_ERR_INVALID, "%s: several experts need offsets", entry);
+  if (offsets_bytes < (uint64_t{experts} + 1) * 4)
+    return fail(MB_ERR_INVALID, "%s: offsets must hold %u entries", entry, experts + 1);
+  if (!aligned(offsets, 4)) return fail(MB_ERR_ALIGNMENT, "%s: offsets must lie on 4 bytes", entry);
+  return MB_OK;
+}
+
+// X's rows as a routed product gathers them.
+int check_routes(const char* entry, const int32_t* offsets, const int32_t* order, const int32_t* slots,
+                 uint64_t slots_bytes, uint64_t rows) {
+  if (slots && (offsets == nullptr || order == nullptr || slots_bytes < rows * 4))
+    return fail(MB_ERR_INVALID, "%s: slots need offsets, order and, in both, an entry for each of %llu rows", entry,
+                (unsigned long long)rows);
+  if (!aligned(slots, 4) || !aligned(order, 4))
+    return fail(MB_ERR_ALIGNMENT, "%s: order and slots must lie on 4 bytes", entry);
+  return MB_OK;
+}
+
+int shift_of(uint32_t block) { return block == 1 ? 0 : 7; }
+
+// X an operand: the product.
+int launch_operands(int dtype, Fp8Epilogue epilogue, const Fp8Product& p, hipStream_t stream) {
+  MB_FOR_DTYPE(dtype, (launch_product_as<uint8_t, T>(epilogue, p, stream)));
+  return launch_status("fp8_product");
+}
+
+// X of `dtype`, in one launch; its rows' codes fit the LDS.
+int launch_few_linear(int dtype, Fp8Epilogue epilogue, const Fp8Product& p, hipStream_t stream) {
+  MB_FOR_DTYPE(dtype, (launch_product_as<T, T>(epilogue, p, stream)));
+  return launch_status("fp8_linear");
+}
+
+bool few_fits(uint64_t rows, uint32_t k) {
+  return fp8_few_lds(k, rows < kFp8FewRows ? static_cast<uint32_t>(rows) : kFp8FewRows) <= 96 * 1024;
+}
+
+// Whether X is quantised in the product's launch.
+bool few_rows(uint64_t rows, uint32_t k, uint32_t experts) {
+  const uint64_t most = experts > 1 ? 2 * uint64_t{experts} : kFp8FewRows;
+  return rows <= most && few_fits(rows, k);
+}
+
+uint64_t workspace_codes(uint64_t rows, uint64_t k) { return (fp8_code_bytes(rows, k) + 15) / 16 * 16; }
+uint64_t workspace_bytes_of(uint64_t rows, uint64_t k) { return workspace_codes(rows, k) + fp8_scale_bytes(rows, k, 1); }
+
+// Quantises X (rows of tokens, to their slots, or rows in order) and multiplies. p holds
+// all but X's operand.
+int run_linear(const char* entry, int dtype, Fp8Epilogue epilogue, Fp8Product p, const int32_t* slots, void* workspace,
+               uint64_t workspace_bytes, hipStream_t stream) {
+  const uint32_t rows = static_cast<uint32_t>(p.rows), k = static_cast<uint32_t>(p.k);
+  const uint64_t needed = workspace_bytes_of(rows, k);
+  if (workspace == nullptr || workspace_bytes < needed)
+    return fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
+                (unsigned long long)needed);
+  if (!aligned(workspace, 16)) return fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
+  if (few_rows(rows, k, static_cast<uint32_t>(p.experts))) return launch_few_linear(dtype, epilogue, p, stream);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + workspace_codes(rows, k);
+  if (int rc = fp8_launch_quantize(dtype, p.x, static_cast<uint32_t>(p.tokens), k, p.row_stride, slots,
+                                   static_cast<uint32_t>(p.copies), rows, codes, scales, stream))
+    return rc;
+  p.x = codes;
+  p.sx = scales;
+  p.x_shift = 0;
+  return launch_operands(dtype, epilogue, p, stream);
+}
+
+// The outputs of a gated product.
+int check_gated_outputs(const char* entry, int dtype, void* y, uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes,
+                        void* gate_up, uint64_t gate_up_bytes, uint64_t rows, uint64_t n) {
+  if (y_scales) {
+    if (int rc = fp8_check_operand(entry, "the output", rows, n, 1, 1, y, y_bytes, y_scales, y_scales_bytes)) return rc;
+    if (gate_up)
+      return fail(MB_ERR_UNSUPPORTED, "%s: gate and up are kept beside an output of the tensors' type, not FP8", entry);
+    return MB_OK;
+  }
+  if (int rc = fp8_check_output(entry, "the output", dtype, y, y_bytes, rows, n)) return rc;
+  return gate_up ? fp8_check_output(entry, "gate_up", dtype, gate_up, gate_up_bytes, rows, 2 * n) : MB_OK;
+}
+
+// Operands of a product's gradients in its workspace: d's rows [rows][n], and the
+// columns of d [n][depth] and of x [k][depth].
+struct GradientSpace {
+  uint64_t codes[3], scales[3], end;
+};
+
+// K of d_w's operands: whole blocks past the first, so that their rows lie on lines.
+uint32_t gradient_depth(uint32_t rows) { return rows > 128 ? (rows + 127) / 128 * 128 : (rows + 15) / 16 * 16; }
+
+GradientSpace gradient_space(uint32_t rows, uint32_t n, uint32_t k) {
+  const uint32_t depth = gradient_depth(rows);
+  const uint64_t sizes[3][2] = {{rows, n}, {n, depth}, {k, depth}};
+  GradientSpace space{};
+  for (int i = 0; i < 3; ++i) {
+    space.codes[i] = space.end;
+    space.scales[i] = space.codes[i] + (fp8_code_bytes(sizes[i][0], sizes[i][1]) + 15) / 16 * 16;
+    space.end = space.scales[i] + (fp8_scale_bytes(sizes[i][0], sizes[i][1], 1) + 15) / 16 * 16;
+  }
+  return space;
+}
+
+// d_x [rows][k] and d_w [n][k] of a product of x [rows][k] with W [n][k] for the
+// gradient d [rows][n], or, with gate_up, d_out [rows][n / 2] of the gated product.
+int run_backward(const char* entry, int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_stride,
+                 const void* gate_up, uint64_t gate_up_bytes, bool gated, const void* x, uint64_t x_bytes,
+                 uint64_t x_stride, const void* w, uint64_t w_bytes, const void* sw, uint64_t sw_bytes,
+                 uint32_t w_block, void* d_x, uint64_t d_x_bytes, void* d_w, uint64_t d_w_bytes, uint32_t rows,
+                 uint32_t n, uint32_t k, void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
+  if (int rc = check_shape(entry, dtype, rows, n, k, 1)) return rc;
+  if (rows == 0 || n == 0 || k == 0) return fail(MB_ERR_INVALID, "%s: rows, n and K must be positive", entry);
+  if (rows > kFp8MostK)
+    return fail(MB_ERR_UNSUPPORTED, "%s: at most %u rows, which d_w sums over", entry, kFp8MostK);
+  if (int rc = fp8_check_rows(entry, "d_out", dtype, d_out, d_out_bytes, rows, gated ? n / 2 : n, d_stride)) return rc;
+  if (gated)
+    if (int rc = fp8_check_output(entry, "gate_up", dtype, gate_up, gate_up_bytes, rows, n)) return rc;
+  if (int rc = fp8_check_rows(entry, "x", dtype, x, x_bytes, rows, k, x_stride)) return rc;
+  if (int rc = fp8_check_operand(entry, "the weight's columns'", k, n, 1, w_block, w, w_bytes, sw, sw_bytes)) return rc;
+  if (int rc = fp8_check_output(entry, "d_x", dtype, d_x, d_x_bytes, rows, k)) return rc;
+  if (int rc = fp8_check_output(entry, "d_w", dtype, d_w, d_w_bytes, n, k)) return rc;
+  const GradientSpace at = gradient_space(rows, n, k);
+  uint8_t* const space = static_cast<uint8_t*>(workspace);
+  if (space == nullptr || workspace_bytes < at.end)
+    return fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
+                (unsigned long long)at.end);
+  if (!aligned(space, 16)) return fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
+  const uint32_t depth = gradient_depth(rows);
+  Fp8Out out[3];
+  for (int i = 0; i < 3; ++i) out[i] = Fp8Out{space + at.codes[i], space + at.scales[i]};
+  if (int rc = fp8_launch_gradient(dtype, d_out, d_stride, gated ? gate_up : nullptr, x, x_stride, rows, n, k, depth,
+                                   out[0], out[1], out[2], stream))
+    return rc;
+  Fp8Product p{};
+  p.copies = p.experts = 1;
+  p.x = out[0].codes;
+  p.sx = out[0].scales;
+  p.w = static_cast<const uint8_t*>(w);
+  p.sw = static_cast<const uint8_t*>(sw);
+  p.w_shift = shift_of(w_block);
+  p.y = d_x;
+  p.rows = p.tokens = static_cast<int>(rows);
+  p.n = static_cast<int>(k);
+  p.k = static_cast<int>(n);
+  if (int rc = launch_operands(dtype, kFp8Plain, p, stream)) return rc;
+  p.x = out[1].codes;
+  p.sx = out[1].scales;
+  p.w = out[2].codes;
+  p.sw = out[2].scales;
+  p.w_shift = 0;
+  p.y = d_w;
+  p.rows = p.tokens = static_cast<int>(n);
+  p.n = static_cast<int>(k);
+  p.k = static_cast<int>(depth);
+  return launch_operands(dtype, kFp8Plain, p, stream);
+}
+
+}  // namespace
+}  // namespace mb
+
+extern "C" {
+
+int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
+                   uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
+                   uint32_t b_block, void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                   const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream) {
+  const char* entry = "mb_fp8_product";
+  if (int rc = mb::check_shape(entry, dtype, rows, n, k, experts)) return rc;
+  if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
+  if (rows == 0 || n == 0) return MB_OK;
+  if (k == 0) return mb::fail(MB_ERR_INVALID, "%s: K must be positive", entry);
+  if (offsets && a_block != 1)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: rows of several experts have a scale each", entry);
+  if (int rc = mb::fp8_check_operand(entry, "a's", rows, k, 1, a_block, a, a_bytes, scale_a, scale_a_bytes)) return rc;
+  if (int rc = mb::fp8_check_operand(entry, "b's", n, k, experts, b_block, b, b_bytes, scale_b, scale_b_bytes))
+    return rc;
+  if (int rc = mb::fp8_check_output(entry, "the output", dtype, c, c_bytes, rows, n)) return rc;
+  mb::Fp8Product p{};
+  p.x = a;
+  p.sx = static_cast<const uint8_t*>(scale_a);
+  p.x_shift = mb::shift_of(a_block);
+  p.w = static_cast<const uint8_t*>(b);
+  p.sw = static_cast<const uint8_t*>(scale_b);
+  p.w_shift = mb::shift_of(b_block);
+  p.y = c;
+  p.rows = p.tokens = static_cast<int>(rows);
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.offsets = offsets;
+  p.copies = 1;
+  p.experts = static_cast<int>(experts);
+  return mb::launch_operands(dtype, mb::kFp8Plain, p, static_cast<hipStream_t>(stream));
+}
+
+uint64_t mb_fp8_linear_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  (void)n;
+  return mb::workspace_bytes_of(rows, k);
+}
+
+int mb_fp8_linear(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,
+                  uint64_t w_bytes, const void* scale_w, uint64_t scale_w_bytes, uint32_t w_block, void* y,
+                  uint64_t y_bytes, uint32_t n, uint32_t k, const int32_t* offsets, uint64_t offsets_bytes,
+                  const int32_t* order, const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t experts,
+                  void* workspace, uint64_t workspace_bytes, void* stream) {
+  const char* entry = "mb_fp8_linear";
+  if (slots && (copies == 0 || copies > 64))
+    return mb::fail(MB_ERR_INVALID, "%s: %u slots a token outside 1..64", entry, copies);
+  const uint64_t rows = uint64_t{tokens} * (slots ? copies : 1);
+  if (int rc = mb::check_shape(entry, dtype, rows, n, k, experts)) return rc;
+  if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
+  if (int rc = mb::check_routes(entry, offsets, order, slots, slots_bytes, rows)) return rc;
+  if (rows == 0 || n == 0) return MB_OK;
+  if (k == 0) return mb::fail(MB_ERR_INVALID, "%s: K must be positive", entry);
+  if (int rc = mb::fp8_check_rows(entry, "x", dtype, x, x_bytes, tokens, k, row_stride)) return rc;
+  if (int rc = mb::fp8_check_operand(entry, "the weight's", n, k, experts, w_block, w, w_bytes, scale_w, scale_w_bytes))
+    return rc;
+  if (int rc = mb::fp8_check_output(entry, "the output", dtype, y, y_bytes, rows, n)) return rc;
+  mb::Fp8Product p{};
+  p.x = x;
+  p.row_stride = row_stride;
+  p.w = static_cast<const uint8_t*>(w);
+  p.sw = static_cast<const uint8_t*>(scale_w);
+  p.w_shift = mb::shift_of(w_block);
+  p.y = y;
+  p.rows = static_cast<int>(rows);
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.offsets = offsets;
+  p.order = slots ? order : nullptr;
+  p.copies = slots ? static_cast<int>(copies) : 1;
+  p.tokens = static_cast<int>(tokens);
+  p.experts = static_cast<int>(experts);
+  return mb::run_linear(entry, dtype, mb::kFp8Plain, p, slots, workspace, workspace_bytes,
+                        static_cast<hipStream_t>(stream));
+}
+
+uint64_t mb_fp8_linear_backward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  return mb::gradient_space(rows < mb::kFp8MostRows ? rows : mb::kFp8MostRows, n, k).end;
+}
+
+int mb_fp8_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* x,
+                           uint64_t x_bytes, uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes,
+                           const void* scale_w, uint64_t scale_w_bytes, uint32_t w_block, void* d_x,
+                           uint64_t d_x_bytes, void* d_w, uint64_t d_w_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                           void* workspace, uint64_t workspace_bytes, void* stream) {
+  return mb::run_backward("mb_fp8_linear_backward", dtype, d_out, d_out_bytes, d_out_stride, nullptr, 0, false, x,
+                          x_bytes, x_stride, w_columns, w_columns_bytes, scale_w, scale_w_bytes, w_block, d_x,
+                          d_x_bytes, d_w, d_w_bytes, rows, n, k, workspace, workspace_bytes,
+                          static_cast<hipStream_t>(stream));
+}
+
+int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
+                         uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
+                         uint32_t b_block, void* y, uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes,
+                         void* gate_up, uint64_t gate_up_bytes, uint32_t rows, uint32_t n, uint32_t k,
+                         const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream) {
+  const char* entry = "mb_fp8_gated_product";
+  if (int rc = mb::check_shape(entry, dtype, rows, uint64_t{2} * n, k, experts)) return rc;
+  if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
+  if (rows == 0 || n == 0) return MB_OK;
+  if (k == 0) return mb::fail(MB_ERR_INVALID, "%s: K must be positive", entry);
+  if (offsets && a_block != 1)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: rows of several experts have a scale each", entry);
+  if (int rc = mb::fp8_check_operand(entry, "a's", rows, k, 1, a_block, a, a_bytes, scale_a, scale_a_bytes)) return rc;
+  if (int rc = mb::fp8_check_operand(entry, "b's", uint64_t{2} * n, k, experts, b_block, b, b_bytes, scale_b,
+                                     scale_b_bytes))
+    return rc;
+  if (int rc = mb::check_gated_outputs(entry, dtype, y, y_bytes, y_scales, y_scales_bytes, gate_up, gate_up_bytes, rows,
+                                       n))
+    return rc;
+  mb::Fp8Product p{};
+  p.x = a;
+  p.sx = static_cast<const uint8_t*>(scale_a);
+  p.x_shift = mb::shift_of(a_block);
+  p.w = static_cast<const uint8_t*>(b);
+  p.sw = static_cast<const uint8_t*>(scale_b);
+  p.w_shift = mb::shift_of(b_block);
+  p.y = y;
+  p.sy = static_cast<uint8_t*>(y_scales);
+  p.gate_up = gate_up;
+  p.rows = p.tokens = static_cast<int>(rows);
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.offsets = offsets;
+  p.copies = 1;
+  p.experts = static_cast<int>(experts);
+  return mb::launch_operands(dtype, y_scales ? mb::kFp8GatedFp8 : mb::kFp8Gated, p, static_cast<hipStream_t>(stream));
+}
+
+int mb_fp8_gated(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,
+                 uint64_t w_bytes, const void* scale_w, uint64_t scale_w_bytes, uint32_t w_block, void* y,
+                 uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes, void* gate_up, uint64_t gate_up_bytes,
+                 uint32_t n, uint32_t k, const int32_t* offsets, uint64_t offsets_bytes, const int32_t* order,
+                 const int32_t* slots, uint64_t slots_bytes, uint32_t copies, uint32_t experts, void* workspace,
+                 uint64_t workspace_bytes, void* stream) {
+  const char* entry = "mb_fp8_gated";
+  if (slots && (copies == 0 || copies > 64))
+    return mb::fail(MB_ERR_INVALID, "%s: %u slots a token outside 1..64", entry, copies);
+  const uint64_t rows = uint64_t{tokens} * (slots ? copies : 1);
+  if (int rc = mb::check_shape(entry, dtype, rows, uint64_t{2} * n, k, experts)) return rc;
+  if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
+  if (int rc = mb::check_routes(entry, offsets, order, slots, slots_bytes, rows)) return rc;
+  if (rows == 0 || n == 0) return MB_OK;
+  if (k == 0) return mb::fail(MB_ERR_INVALID, "%s: K must be positive", entry);
+  if (int rc = mb::fp8_check_rows(entry, "x", dtype, x, x_bytes, tokens, k, row_stride)) return rc;
+  if (int rc = mb::fp8_check_operand(entry, "the weight's", uint64_t{2} * n, k, experts, w_block, w, w_bytes, scale_w,
+                                     scale_w_bytes))
+    return rc;
+  if (int rc = mb::check_gated_outputs(entry, dtype, y, y_bytes, y_scales, y_scales_bytes, gate_up, gate_up_bytes, rows,
+                                       n))
+    return rc;
+  mb::Fp8Product p{};
+  p.x = x;
+  p.row_stride = row_stride;
+  p.w = static_cast<const uint8_t*>(w);
+  p.sw = static_cast<const uint8_t*>(scale_w);
+  p.w_shift = mb::shift_of(w_block);
+  p.y = y;
+  p.sy = static_cast<uint8_t*>(y_scales);
+  p.gate_up = gate_up;
+  p.rows = static_cast<int>(rows);
+  p.n = static_cast<int>(n);
+  p.k = static_cast<int>(k);
+  p.offsets = offsets;
+  p.order = slots ? order : nullptr;
+  p.copies = slots ? static_cast<int>(copies) : 1;
+  p.tokens = static_cast<int>(tokens);
+  p.experts = static_cast<int>(experts);
+  return mb::run_linear(entry, dtype, y_scales ? mb::kFp8GatedFp8 : mb::kFp8Gated, p, slots, workspace, workspace_bytes,
+                        static_cast<hipStream_t>(stream));
+}
+
+uint64_t mb_fp8_gated_backward_workspace(uint32_t rows, uint32_t n, uint32_t k) {
+  const uint64_t width = uint64_t{2} * n < mb::kFp8MostK ? uint64_t{2} * n : mb::kFp8MostK;
+  return mb::gradient_space(rows < mb::kFp8MostRows ? rows : mb::kFp8MostRows, static_cast<uint32_t>(width), k).end;
+}
+
+int mb_fp8_gated_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride,
+                          const void* gate_up, uint64_t gate_up_bytes, const void* x, uint64_t x_bytes,
+                          uint64_t x_stride, const void* w_columns, uint64_t w_columns_bytes, const void* scale_w,
+                          uint64_t scale_w_bytes, uint32_t w_block, void* d_x, uint64_t d_x_bytes, void* d_w,
+                          uint64_t d_w_bytes, uint32_t rows, uint32_t n, uint32_t k, void* workspace,
+                          uint64_t workspace_bytes, void* stream) {
+  const char* entry = "mb_fp8_gated_backward";
+  if (n > mb::kFp8MostK / 2)
+    return mb::fail(MB_ERR_UNSUPPORTED, "%s: n = %u: at most %u columns", entry, n, mb::kFp8MostK / 2);
+  return mb::run_backward(entry, dtype, d_out, d_out_bytes, d_out_stride, gate_up, gate_up_bytes, true, x, x_bytes,
+                          x_stride, w_columns, w_columns_bytes, scale_w, scale_w_bytes, w_block, d_x, d_x_bytes, d_w,
+                          d_w_bytes, rows, 2 * n, k, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"
