@@ -434,12 +434,30 @@ int mb_fp8_dequantize(int dtype, const void* codes, uint64_t codes_bytes, const 
 
 /* C [rows][n] = A . B^T for operands A of `rows` rows and B of `experts` matrices of n
  * rows (codes and scales one matrix after the other), a scale of A standing for
- * a_block rows (1 or 128) and one of B for b_block. Sums in fp32, rounded once to
- * dtype. offsets as in mb_mx_product; with them a_block is 1. */
+ * a_block rows (1 or 128) and one of B for b_block. Sums in fp32 (of a block's 128
+ * products, for fp16 and bf16 outputs, to about 2^-16 of the result, as the FP8 matrix
+ * instructions give it), rounded once to dtype. offsets as in mb_mx_product; with them
+ * a_block is 1. kernel: the name of the kernel to run on, for tests and measurements, or
+ * NULL. */
 int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
                    uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
                    uint32_t b_block, void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k,
-                   const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream);
+                   const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, const char* kernel, void* stream);
+
+/* What a product's sums become: themselves, silu(gate) * up, that with gate and up
+ * kept, or that as an FP8 operand. */
+#define MB_FP8_PLAIN 0u
+#define MB_FP8_GATED 1u
+#define MB_FP8_GATED_KEPT 2u
+#define MB_FP8_GATED_FP8 3u
+
+/* Registered name of the kernel that mb_fp8_product or, with `gated`,
+ * mb_fp8_gated_product launches for these sizes or, with `linear`, mb_fp8_linear or
+ * mb_fp8_gated for `rows` rows of output (after quantising them, where the kernel takes
+ * operands); NULL, with the error set, for sizes that they refuse or that have no
+ * product. */
+const char* mb_fp8_product_kernel(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts, uint32_t linear,
+                                  uint32_t gated);
 
 /* Bytes of workspace (16-byte aligned) of mb_fp8_linear and mb_fp8_gated for `rows`
  * rows of output. */
@@ -476,7 +494,8 @@ int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void*
                          uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
                          uint32_t b_block, void* y, uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes,
                          void* gate_up, uint64_t gate_up_bytes, uint32_t rows, uint32_t n, uint32_t k,
-                         const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream);
+                         const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, const char* kernel,
+                         void* stream);
 
 /* The same of Q(X), as mb_fp8_linear. */
 int mb_fp8_gated(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,

@@ -6,8 +6,8 @@ of the output's type:
   sums      16-bit outputs: the FP8 matrix instructions drop what lies some bits below a block's largest product, 2^-13
             of the sum of its 128 magnitudes where that was looked for; twice that. fp32 ones: products are exact, and a
             sum of K of them in any order is off by less than K 2^-24 of the magnitudes.
-Of a gated product g / (1 + e^-g) u the relative errors add up (d silu / d g is within 1.1), with eight roundings of 2^-24
-of the fp32 evaluation.
+Of a gated product g / (1 + e^-g) u the errors add up (d silu / d g is within 1.1), with eight roundings of 2^-24 of the
+fp32 evaluation.
 """
 
 import numpy as np
@@ -235,9 +235,9 @@ def test_linear_backward(gpu, dtype, rows, n, k):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,n,k", BACKWARD)
 def test_gated_backward(gpu, dtype, rows, n, k):
-    """The gradient of [gate | up] is evaluated in fp32 and rounded to codes: a value that fp32's error (under 16
-    roundings of 2^-24 of its terms) takes across a border is off by a step, 2^-3 of it, or, in a block whose largest lies
-    next to a border of the scale, by its smallest step. Where that happens is known from the exact values."""
+    """The gradient of [gate | up] is evaluated in fp32 and rounded to codes: a value that fp32's error (under 16 roundings
+    of 2^-24 of its terms) takes across a border is off by a step, 2^-3 of it, or, in a block whose largest lies next to a
+    border of the scale, by its smallest step. Where that happens is known from the exact values."""
     import torch
 
     from triton_chip_benchmarks_amd import fp8
@@ -298,7 +298,7 @@ def test_gated_gradient_against_differences(gpu):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_values_that_are_not_finite(gpu, dtype):
-    """A block with a NaN makes NaN of its row of the output alone, or, in a weight's block of 128 rows, of 128 columns."""
+    """A block with a NaN makes NaN of its row of the output alone, or, in a weight's block of 128 rows, of those columns."""
     import torch
 
     from triton_chip_benchmarks_amd import fp8

@@ -1,8 +1,8 @@
 """The root-mean-square norm with the residual's addition, and its gradients, against the float64 oracle.
 
-Tolerances: the sum of squares of n values in fp32, in any order, is off by less than n 2^-24 of itself, its root by half
-of that; six more roundings of 2^-24 make y, and one of half a step of the output's type (u). The gradient's terms are
-bounded the same way, by their magnitudes.
+Tolerances: the sum of squares of n values in fp32, in any order, is off by less than n 2^-24 of itself, its root by
+half of that; six more roundings of 2^-24 make y, and one of half a step of the output's type (u). The gradient's terms
+are bounded the same way, by their magnitudes.
 """
 
 import numpy as np

@@ -140,7 +140,8 @@ SIGNATURES: dict[str, tuple[object, list]] = {
                                     _u64, _ptr]),
     "mb_fp8_dequantize": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _u32, _u32, _ptr]),
     "mb_fp8_product": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _u32, _u32,
-                              _u32, _ptr, _u64, _u32, _ptr]),
+                              _u32, _ptr, _u64, _u32, ctypes.c_char_p, _ptr]),
+    "mb_fp8_product_kernel": (ctypes.c_char_p, [_i32, _u32, _u32, _u32, _u32, _u32, _u32]),
     "mb_fp8_linear_workspace": (_u64, [_u32, _u32, _u32]),
     "mb_fp8_linear": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _u32, _u32, _ptr,
                              _u64, _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
@@ -148,7 +149,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "mb_fp8_linear_backward": (_i32, [_i32, _ptr, _u64, _u64, _ptr, _u64, _u64, _ptr, _u64, _ptr, _u64, _u32, _ptr,
                                       _u64, _ptr, _u64, _u32, _u32, _u32, _ptr, _u64, _ptr]),
     "mb_fp8_gated_product": (_i32, [_i32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr,
-                                    _u64, _ptr, _u64, _u32, _u32, _u32, _ptr, _u64, _u32, _ptr]),
+                                    _u64, _ptr, _u64, _u32, _u32, _u32, _ptr, _u64, _u32, ctypes.c_char_p, _ptr]),
     "mb_fp8_gated": (_i32, [_i32, _ptr, _u64, _u32, _u64, _ptr, _u64, _ptr, _u64, _u32, _ptr, _u64, _ptr, _u64, _ptr,
                             _u64, _u32, _u32, _ptr, _u64, _ptr, _ptr, _u64, _u32, _u32, _ptr, _u64, _ptr]),
     "mb_fp8_gated_backward_workspace": (_u64, [_u32, _u32, _u32]),

@@ -49,7 +49,8 @@ _FP8_TENSOR_RE = re.compile(r"(fp8_quantize_tiles|fp8_gradient|fp8_dequantize|rm
                             r"(?:Lb([01])E)?E")
 _FP8_FLAG = {"fp8_quantize_tiles": "_square", "fp8_gradient": "_gated", "fp8_dequantize": "_stream"}
 _FP8_FEW_RE = re.compile(r"fp8_few_kernelI(h|f|DF16_|DF16b)(h|f|DF16_|DF16b)Li([012])ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)EE")
-_FP8_EPILOGUE = ("product", "gated", "gated_fp8")
+_FP8_TILES_RE = re.compile(r"fp8_tiles_kernelI(h|f|DF16_|DF16b)Li([0-3])ELi(\d+)ELi(\d+)ELi\d+EE")
+_FP8_EPILOGUE = ("product", "gated", "gated_fp8", "gated_kept")
 _NORM_RE = re.compile(r"(rms_norm(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)EE")
 _DISPATCH_RE = re.compile(r"(dispatch_(?:count|place))_kernelE")
 _VECTOR_RE = re.compile(r"vector_(\w+?)_kernelILi(\d+)E")
@@ -130,6 +131,10 @@ def registered_name(symbol: str) -> str | None:
     if match:
         x, y, epilogue, *sizes = match.groups()
         return f"fp8_few_{_FP8_EPILOGUE[int(epilogue)]}_{_FP8_TYPE[x]}_{_FP8_TYPE[y]}_{'x'.join(sizes)}"
+    match = _FP8_TILES_RE.search(symbol)
+    if match:
+        y, epilogue, features, rows = match.groups()
+        return f"fp8_tiles_{_FP8_EPILOGUE[int(epilogue)]}_{_FP8_TYPE[y]}_{features}x{rows}"
     match = _NORM_RE.search(symbol)
     if match:
         family, dtype, waves, pieces = match.groups()

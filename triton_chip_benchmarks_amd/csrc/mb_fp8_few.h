@@ -5,17 +5,9 @@
 #include <type_traits>
 
 #include "mb_fp8_device.h"
-#include "mb_mfma.h"
+#include "mb_mx_stream.h"
 
 namespace mb {
-
-// Rows first .. last - 1 of expert `e`; all of them without offsets. Clamped, so
-// that whatever `offsets` holds, no row outside 0 .. rows - 1 is touched.
-__device__ __forceinline__ void fp8_expert_rows(const int32_t* __restrict__ offsets, uint32_t e, int rows, int& first,
-                                                int& last) {
-  first = offsets ? max(0, min(offsets[e], rows)) : 0;
-  last = offsets ? max(first, min(offsets[e + 1], rows)) : rows;
-}
 
 // Expert and rows of a workgroup's blockIdx.y; false where it has none. With
 // fewer rows than experts there is one grid row a row of X, and the first row of
@@ -35,7 +27,7 @@ __device__ __forceinline__ bool fp8_few_expert(const int32_t* __restrict__ offse
       if (e >= experts || offsets[e] != static_cast<int>(blockIdx.y)) return false;
     }
   }
-  fp8_expert_rows(offsets, e, rows, first, last);
+  expert_rows(offsets, e, rows, first, last);
   return first < last;
 }
 

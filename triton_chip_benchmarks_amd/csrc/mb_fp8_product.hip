@@ -1,49 +1,131 @@
 // Products of FP8 operands with block scales: linear layers, their gradients and the
 // gated pair of projections, of one weight or one for each expert.
+#include <cstring>
+
 #include "mb_fp8.h"
-#include "mb_fp8_few.h"
+#include "mb_fp8_tiles.h"
 
 namespace mb {
 namespace {
 
-// ---- few rows, and every size ---------------------------------------------------
+// ---- the kernels of products -----------------------------------------------------
+
+constexpr int kE4m3 = 3;  // after MB_DTYPE_*: X an operand, or Y one
+
+template <class T>
+constexpr int type_code() {
+  return sizeof(T) == 1 ? kE4m3 : sizeof(T) == 4 ? MB_DTYPE_F32 : __is_same(T, __bf16) ? MB_DTYPE_BF16 : MB_DTYPE_F16;
+}
+
+// A kernel for X of `x` and Y of `y` by `epilogue` (Fp8TileEpilogue): of few rows, or of
+// tiles of `features` columns of W by `rows` rows.
+struct ProductKernel {
+  const char* name;
+  int x, y, epilogue;
+  bool tiles;
+  int features, rows;  // of a workgroup: columns of the output, rows
+  int resident;        // workgroups a CU holds
+  int band;            // row tiles that share their weight's panels in an XCD's L2
+  void (*launch)(const Fp8Product&, uint32_t grid, int band, hipStream_t);
+};
+
+// Workgroups of a kernel of few rows: columns, experts (rows, if there are fewer) and
+// chunks of an expert's rows.
+dim3 few_grid(uint32_t n, uint32_t columns, uint32_t rows, uint32_t chunk, uint32_t experts, bool routed) {
+  const uint32_t chunks = (rows / (routed ? experts : 1) + chunk - 1) / chunk;
+  return dim3((n + columns - 1) / columns, routed ? (rows < experts ? rows : experts) : 1,
+              chunks < 1 ? 1 : chunks < 256 ? chunks : 256);
+}
 
 template <class X, class Y, int EPILOGUE, int FB, int RB, int WAVES, int SPLIT>
-void launch_few(const Fp8Product& p, hipStream_t stream) {
+void launch_few(const Fp8Product& p, uint32_t, int, hipStream_t stream) {
   constexpr uint32_t kColumns = WAVES / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kRows = 16 * RB;
-  const uint32_t rows = static_cast<uint32_t>(p.rows), experts = static_cast<uint32_t>(p.experts);
-  const uint32_t lds_rows = rows < kRows ? rows : kRows;
-  const uint32_t chunks = (rows / (p.offsets ? experts : 1) + kRows - 1) / kRows;
-  const dim3 grid((static_cast<uint32_t>(p.n) + kColumns - 1) / kColumns,
-                  p.offsets ? (rows < experts ? rows : experts) : 1, chunks < 1 ? 1 : chunks < 256 ? chunks : 256);
+  const uint32_t rows = static_cast<uint32_t>(p.rows), lds_rows = rows < kRows ? rows : kRows;
   const uint64_t lds = sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0;
   fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>
-      <<<grid, dim3(64 * WAVES), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
+      <<<few_grid(static_cast<uint32_t>(p.n), kColumns, rows, kRows, static_cast<uint32_t>(p.experts), p.offsets),
+         dim3(64 * WAVES), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
 }
 
-template <class X, class Y>
-void launch_product_as(Fp8Epilogue epilogue, const Fp8Product& p, hipStream_t stream) {
-  if (epilogue == kFp8Plain)
-    launch_few<X, Y, kFp8Plain, 2, 1, 8, 8>(p, stream);
-  else if (epilogue == kFp8Gated)
-    launch_few<X, Y, kFp8Gated, 2, 1, 8, 8>(p, stream);
-  else
-    launch_few<X, uint8_t, kFp8GatedFp8, 2, 1, 8, 1>(p, stream);
+template <class Y, int EPILOGUE, int BM, int BN, int STAGES>
+void launch_tiles(const Fp8Product& p, uint32_t grid, int band, hipStream_t stream) {
+  constexpr uint32_t kPlaces = 256 * Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT;
+  fp8_tiles_kernel<Y, EPILOGUE, BM, BN, STAGES>
+      <<<dim3(grid < kPlaces ? grid : kPlaces), dim3(256), 0, stream>>>(p, band);
 }
 
-#define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, RB, WAVES, SPLIT)                           \
-  MB_REGISTER_KERNEL("fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #RB "x" #WAVES "x" #SPLIT,       \
-                     (fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>))
-#define MB_FP8_REGISTER(T, NAME)                                              \
-  MB_FP8_FEW(uint8_t, "e4m3", T, NAME, kFp8Plain, "product", 2, 1, 8, 8);     \
-  MB_FP8_FEW(T, NAME, T, NAME, kFp8Plain, "product", 2, 1, 8, 8);             \
-  MB_FP8_FEW(uint8_t, "e4m3", T, NAME, kFp8Gated, "gated", 2, 1, 8, 8);       \
-  MB_FP8_FEW(T, NAME, T, NAME, kFp8Gated, "gated", 2, 1, 8, 8);               \
-  MB_FP8_FEW(T, NAME, uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)
-MB_FP8_REGISTER(float, "f32");
-MB_FP8_REGISTER(_Float16, "f16");
-MB_FP8_REGISTER(__bf16, "bf16");
-MB_FP8_FEW(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1);
+#define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, RB, WAVES, SPLIT)                                 \
+  ProductKernel {                                                                                              \
+    "fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #RB "x" #WAVES "x" #SPLIT, type_code<X>(),               \
+        type_code<Y>(), EPILOGUE, false, WAVES / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), 16 * RB, 0, \
+        0, launch_few<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>                                                    \
+  }
+#define MB_FP8_TILES(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND)                                          \
+  ProductKernel {                                                                                              \
+    "fp8_tiles_" NAME "_" Y_NAME "_" #BM "x" #BN, kE4m3, type_code<Y>(), EPILOGUE, true,                       \
+        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, BAND,           \
+        launch_tiles<Y, EPILOGUE, BM, BN, STAGES>                                                              \
+  }
+// The forms, for a list M(arguments) of kernels and for their registration alike.
+#define MB_FP8_FEW_OF(M, X, X_NAME, Y, Y_NAME)                 \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 1, 8, 8)    \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 1, 8, 4)    \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 1, 8, 8)    \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 1, 8, 8)      \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 1, 8, 4)
+#define MB_FP8_FEW_MORE(M, X, X_NAME, Y, Y_NAME)               \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 2, 8, 4)    \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 8, 4)    \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 2, 8, 4)      \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 8, 4)
+#define MB_FP8_FEW_ALL(M)                                                              \
+  MB_FP8_FEW_OF(M, uint8_t, "e4m3", float, "f32")                                      \
+  MB_FP8_FEW_OF(M, uint8_t, "e4m3", _Float16, "f16")                                   \
+  MB_FP8_FEW_OF(M, uint8_t, "e4m3", __bf16, "bf16")                                    \
+  MB_FP8_FEW_MORE(M, uint8_t, "e4m3", float, "f32")                                    \
+  MB_FP8_FEW_MORE(M, uint8_t, "e4m3", _Float16, "f16")                                 \
+  MB_FP8_FEW_MORE(M, uint8_t, "e4m3", __bf16, "bf16")                                  \
+  MB_FP8_FEW_OF(M, float, "f32", float, "f32")                                         \
+  MB_FP8_FEW_OF(M, _Float16, "f16", _Float16, "f16")                                   \
+  MB_FP8_FEW_OF(M, __bf16, "bf16", __bf16, "bf16")                                     \
+  M(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)           \
+  M(float, "f32", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)              \
+  M(_Float16, "f16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)           \
+  M(__bf16, "bf16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)
+#define MB_FP8_TILES_PLAIN(M, Y, Y_NAME)                          \
+  M(Y, Y_NAME, kTilePlain, "product", 256, 128, 3, 4)             \
+  M(Y, Y_NAME, kTilePlain, "product", 128, 128, 4, 6)             \
+  M(Y, Y_NAME, kTilePlain, "product", 128, 64, 3, 8)              \
+  M(Y, Y_NAME, kTilePlain, "product", 64, 64, 3, 8)               \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 64, 3, 8)                \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 64, 3, 8)
+#define MB_FP8_TILES_GATED(M, Y, Y_NAME)                          \
+  M(Y, Y_NAME, kTilePlain, "product", 256, 256, 2, 4)             \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 256, 2, 4)               \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 256, 2, 4)      \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 128, 3, 4)               \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 128, 3, 4)
+#define MB_FP8_TILES_ALL(M)                                       \
+  MB_FP8_TILES_PLAIN(M, float, "f32")                             \
+  MB_FP8_TILES_PLAIN(M, _Float16, "f16")                          \
+  MB_FP8_TILES_PLAIN(M, __bf16, "bf16")                           \
+  MB_FP8_TILES_GATED(M, _Float16, "f16")                          \
+  MB_FP8_TILES_GATED(M, __bf16, "bf16")                           \
+  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 256, 2, 4)  \
+  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 128, 3, 4)  \
+  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 64, 3, 8)
+
+#define MB_FP8_FEW_ENTRY(...) MB_FP8_FEW(__VA_ARGS__),
+#define MB_FP8_TILES_ENTRY(...) MB_FP8_TILES(__VA_ARGS__),
+const ProductKernel kKernels[] = {MB_FP8_FEW_ALL(MB_FP8_FEW_ENTRY) MB_FP8_TILES_ALL(MB_FP8_TILES_ENTRY)};
+
+#define MB_FP8_FEW_REGISTER(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, RB, WAVES, SPLIT)              \
+  MB_REGISTER_KERNEL("fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #RB "x" #WAVES "x" #SPLIT,    \
+                     (fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>));
+#define MB_FP8_TILES_REGISTER(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND)                       \
+  MB_REGISTER_KERNEL("fp8_tiles_" NAME "_" Y_NAME "_" #BM "x" #BN, (fp8_tiles_kernel<Y, EPILOGUE, BM, BN, STAGES>));
+MB_FP8_FEW_ALL(MB_FP8_FEW_REGISTER)
+MB_FP8_TILES_ALL(MB_FP8_TILES_REGISTER)
 
 constexpr uint32_t kMostExperts = 4096;
 
@@ -80,16 +162,9 @@ int check_routes(const char* entry, const int32_t* offsets, const int32_t* order
 
 int shift_of(uint32_t block) { return block == 1 ? 0 : 7; }
 
-// X an operand: the product.
-int launch_operands(int dtype, Fp8Epilogue epilogue, const Fp8Product& p, hipStream_t stream) {
-  MB_FOR_DTYPE(dtype, (launch_product_as<uint8_t, T>(epilogue, p, stream)));
-  return launch_status("fp8_product");
-}
-
-// X of `dtype`, in one launch; its rows' codes fit the LDS.
-int launch_few_linear(int dtype, Fp8Epilogue epilogue, const Fp8Product& p, hipStream_t stream) {
-  MB_FOR_DTYPE(dtype, (launch_product_as<T, T>(epilogue, p, stream)));
-  return launch_status("fp8_linear");
+// Row tiles of `tile` rows, at most: an expert's rows start one of their own.
+uint64_t most_row_tiles(uint32_t rows, uint32_t experts, int tile) {
+  return experts > 1 ? rows / tile + (rows < experts ? rows : experts) : (rows + uint64_t{1} * tile - 1) / tile;
 }
 
 bool few_fits(uint64_t rows, uint32_t k) {
@@ -100,6 +175,62 @@ bool few_fits(uint64_t rows, uint32_t k) {
 bool few_rows(uint64_t rows, uint32_t k, uint32_t experts) {
   const uint64_t most = experts > 1 ? 2 * uint64_t{experts} : kFp8FewRows;
   return rows <= most && few_fits(rows, k);
+}
+
+struct ProductChoice {
+  const ProductKernel* kernel = nullptr;
+  uint32_t grid = 0;  // of tiles
+};
+
+// The kernel for X of type `x` by the rule or, with `wanted`, the one of that name; none
+// if it does not take the sizes.
+ProductChoice choose_product(int x, int y, int epilogue, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts,
+                             const char* wanted) {
+  ProductChoice best;
+  const uint64_t width = epilogue == kTilePlain ? n : uint64_t{2} * n, steps = (k + uint64_t{511}) / 512;
+  double best_cost = 0;
+  for (const ProductKernel& kernel : kKernels) {
+    // A kernel of few rows keeps the gate and up, if it is given where to.
+    const int asked = epilogue == kTileGatedKept && !kernel.tiles ? static_cast<int>(kTileGated) : epilogue;
+    if (kernel.x != x || kernel.y != y || kernel.epilogue != asked) continue;
+    if (wanted && strcmp(wanted, kernel.name) != 0) continue;
+    double cost;
+    uint64_t grid = 0;
+    if (kernel.tiles) {
+      if (experts > kStreamExperts) continue;
+      // The tiles address a matrix's scales, and a tile's rows, with 32-bit offsets.
+      if (steps * (rows > width ? rows : width) * 4 > 0x7fffffffu) continue;
+      if (fp8_pitch(k) * 256 > 0x7fffffffu || uint64_t{1} * kernel.rows * width * 4 > 0x7fffffffu) continue;
+      const uint64_t tiles =
+          most_row_tiles(rows, experts, kernel.rows) * ((n + uint64_t{1} * kernel.features - 1) / kernel.features);
+      grid = (tiles + kXcds - 1) / kXcds * kXcds;
+      if (grid > 0xffffff) continue;
+      cost = 5.0 + static_cast<double>((tiles + 255) / 256) * (k + 127) / 128 * kernel.features * kernel.rows / 32768;
+    } else {
+      const dim3 few = few_grid(n, static_cast<uint32_t>(kernel.features), rows, static_cast<uint32_t>(kernel.rows),
+                                experts, experts > 1);
+      if (uint64_t{few.x} * few.y * few.z > 0x3fffff) continue;  // of 1024 threads at most: 2^32 - 1 a launch
+      cost = static_cast<double>(rows) / experts * n * k * 1e-9;
+    }
+    if (best.kernel && cost >= best_cost) continue;
+    best_cost = cost;
+    best.kernel = &kernel;
+    best.grid = static_cast<uint32_t>(grid);
+  }
+  return best;
+}
+
+int launch_product(const char* entry, const char* wanted, int x, int dtype, Fp8Epilogue epilogue, const Fp8Product& p,
+                   hipStream_t stream) {
+  const int asked = epilogue == kFp8Gated && p.gate_up ? static_cast<int>(kTileGatedKept) : static_cast<int>(epilogue);
+  const ProductChoice choice =
+      choose_product(x, epilogue == kFp8GatedFp8 ? kE4m3 : dtype, asked, static_cast<uint32_t>(p.rows),
+                     static_cast<uint32_t>(p.n), static_cast<uint32_t>(p.k), static_cast<uint32_t>(p.experts), wanted);
+  if (choice.kernel == nullptr)
+    return fail(MB_ERR_UNSUPPORTED, "%s: no kernel %s that takes %d x %d x %d and %d experts", entry,
+                wanted ? wanted : "", p.rows, p.n, p.k, p.experts);
+  choice.kernel->launch(p, choice.grid, choice.kernel->band, stream);
+  return launch_status(choice.kernel->name);
 }
 
 uint64_t workspace_codes(uint64_t rows, uint64_t k) { return (fp8_code_bytes(rows, k) + 15) / 16 * 16; }
@@ -115,7 +246,8 @@ int run_linear(const char* entry, int dtype, Fp8Epilogue epilogue, Fp8Product p,
     return fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
                 (unsigned long long)needed);
   if (!aligned(workspace, 16)) return fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
-  if (few_rows(rows, k, static_cast<uint32_t>(p.experts))) return launch_few_linear(dtype, epilogue, p, stream);
+  if (few_rows(rows, k, static_cast<uint32_t>(p.experts)))
+    return launch_product(entry, nullptr, dtype, dtype, epilogue, p, stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + workspace_codes(rows, k);
   if (int rc = fp8_launch_quantize(dtype, p.x, static_cast<uint32_t>(p.tokens), k, p.row_stride, slots,
@@ -124,7 +256,7 @@ int run_linear(const char* entry, int dtype, Fp8Epilogue epilogue, Fp8Product p,
   p.x = codes;
   p.sx = scales;
   p.x_shift = 0;
-  return launch_operands(dtype, epilogue, p, stream);
+  return launch_product(entry, nullptr, kE4m3, dtype, epilogue, p, stream);
 }
 
 // The outputs of a gated product.
@@ -202,7 +334,7 @@ int run_backward(const char* entry, int dtype, const void* d_out, uint64_t d_out
   p.rows = p.tokens = static_cast<int>(rows);
   p.n = static_cast<int>(k);
   p.k = static_cast<int>(n);
-  if (int rc = launch_operands(dtype, kFp8Plain, p, stream)) return rc;
+  if (int rc = launch_product(entry, nullptr, kE4m3, dtype, kFp8Plain, p, stream)) return rc;
   p.x = out[1].codes;
   p.sx = out[1].scales;
   p.w = out[2].codes;
@@ -212,7 +344,7 @@ int run_backward(const char* entry, int dtype, const void* d_out, uint64_t d_out
   p.rows = p.tokens = static_cast<int>(n);
   p.n = static_cast<int>(k);
   p.k = static_cast<int>(depth);
-  return launch_operands(dtype, kFp8Plain, p, stream);
+  return launch_product(entry, nullptr, kE4m3, dtype, kFp8Plain, p, stream);
 }
 
 }  // namespace
@@ -223,7 +355,8 @@ extern "C" {
 int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
                    uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
                    uint32_t b_block, void* c, uint64_t c_bytes, uint32_t rows, uint32_t n, uint32_t k,
-                   const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream) {
+                   const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, const char* kernel,
+                   void* stream) {
   const char* entry = "mb_fp8_product";
   if (int rc = mb::check_shape(entry, dtype, rows, n, k, experts)) return rc;
   if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
@@ -249,7 +382,21 @@ int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale
   p.offsets = offsets;
   p.copies = 1;
   p.experts = static_cast<int>(experts);
-  return mb::launch_operands(dtype, mb::kFp8Plain, p, static_cast<hipStream_t>(stream));
+  return mb::launch_product(entry, kernel, mb::kE4m3, dtype, mb::kFp8Plain, p, static_cast<hipStream_t>(stream));
+}
+
+const char* mb_fp8_product_kernel(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts, uint32_t linear,
+                                  uint32_t gated) {
+  const char* entry = "mb_fp8_product_kernel";
+  const bool fp8 = gated == MB_FP8_GATED_FP8;
+  if (mb::check_shape(entry, dtype, rows, gated ? uint64_t{2} * n : n, k, experts)) return nullptr;
+  if (rows == 0 || n == 0 || k == 0 || gated > MB_FP8_GATED_FP8) {
+    mb::fail(MB_ERR_INVALID, "%s: no product of %u x %u x %u and kind %u", entry, rows, n, k, gated);
+    return nullptr;
+  }
+  const int kinds[] = {mb::kTilePlain, mb::kTileGated, mb::kTileGatedKept, mb::kTileGatedFp8};
+  const int x = linear && mb::few_rows(rows, k, experts) ? dtype : mb::kE4m3;
+  return mb::choose_product(x, fp8 ? mb::kE4m3 : dtype, kinds[gated], rows, n, k, experts, nullptr).kernel->name;
 }
 
 uint64_t mb_fp8_linear_workspace(uint32_t rows, uint32_t n, uint32_t k) {
@@ -313,7 +460,8 @@ int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void*
                          uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
                          uint32_t b_block, void* y, uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes,
                          void* gate_up, uint64_t gate_up_bytes, uint32_t rows, uint32_t n, uint32_t k,
-                         const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, void* stream) {
+                         const int32_t* offsets, uint64_t offsets_bytes, uint32_t experts, const char* kernel,
+                         void* stream) {
   const char* entry = "mb_fp8_gated_product";
   if (int rc = mb::check_shape(entry, dtype, rows, uint64_t{2} * n, k, experts)) return rc;
   if (int rc = mb::check_offsets(entry, offsets, offsets_bytes, experts)) return rc;
@@ -344,7 +492,8 @@ int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void*
   p.offsets = offsets;
   p.copies = 1;
   p.experts = static_cast<int>(experts);
-  return mb::launch_operands(dtype, y_scales ? mb::kFp8GatedFp8 : mb::kFp8Gated, p, static_cast<hipStream_t>(stream));
+  return mb::launch_product(entry, kernel, mb::kE4m3, dtype, y_scales ? mb::kFp8GatedFp8 : mb::kFp8Gated, p,
+                            static_cast<hipStream_t>(stream));
 }
 
 int mb_fp8_gated(int dtype, const void* x, uint64_t x_bytes, uint32_t tokens, uint64_t row_stride, const void* w,

@@ -134,11 +134,25 @@ def dequantize(packed: Packed, out=None, stream=None):
     return out
 
 
-def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=None):
+KINDS = {"product": 0, "gated": 1, "gated_kept": 2, "gated_fp8": 3}
+
+
+def product_kernel(rows: int, n: int, k: int, dtype=torch.bfloat16, experts: int = 1, linear: bool = False,
+                   kind: str = "product") -> str:
+    """Name of the kernel that `product` or, by `kind`, `gated` (with gate_up, or to an operand) of an operand launches;
+    with `linear`, `linear` or `gated` of a tensor for `rows` rows of output."""
+    name = library().mb_fp8_product_kernel(DTYPE_CODES.get(dtype, -1), rows, n, k, experts, int(linear), KINDS[kind])
+    if name is None:
+        raise _native.NativeError(_native.MB_ERR_INVALID, _native.last_error())
+    return name.decode()
+
+
+def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=None, kernel: str | None = None):
     """A . B^T of two operands, in `dtype` (bfloat16 unless `out` or `dtype` says otherwise).
 
     With `offsets` ([experts + 1] int32, on the device) b holds a matrix for each expert, and a's rows offsets[e] ..
-    offsets[e + 1] - 1 meet matrix e; output rows from offsets[experts] on are not written.
+    offsets[e + 1] - 1 meet matrix e; output rows from offsets[experts] on are not written. `kernel` names the kernel
+    to run on, for tests and measurements.
     """
     experts = None if offsets is None else offsets.numel() - 1
     _check_product(a, b, experts)
@@ -150,7 +164,7 @@ def product(a: Packed, b: Packed, out=None, dtype=None, offsets=None, stream=Non
     handle = launch_stream(stream, a.codes, a.scales, b.codes, b.scales, out, *(() if offsets is None else (offsets,)))
     status = library().mb_fp8_product(code, *_parts(a), a.block, *_parts(b), b.block, out.data_ptr(),
                                       a.rows * b.rows * (2 if code else 4), a.rows, b.rows, a.k, *_pointer(offsets),
-                                      experts or 1, handle)
+                                      experts or 1, None if kernel is None else kernel.encode(), handle)
     if status:
         _native.check(status)
     return out
@@ -283,13 +297,14 @@ def gated_workspace(rows: int, n: int, k: int, dtype, experts: int = 1, device="
 
 
 def gated(x, weight: Packed, out=None, packed: Packed | None = None, gate_up=None, plan=None,
-          sorted_rows: bool = False, dtype=None, workspace=None, stream=None):
+          sorted_rows: bool = False, dtype=None, workspace=None, stream=None, kernel: str | None = None):
     """silu(x . G^T) * (x . U^T): x [rows][k], a tensor, quantised on the way, or an operand; weight an operand of 2n
     rows, G's and then U's (with a `plan`, a matrix for each expert, as for `linear`; an operand's rows are sorted).
 
     The result, rounded once from fp32, is `out` [rows][n] of x's type (of an operand: of `dtype`, bfloat16 unless
     given) or, if `packed` is given, that operand, with a scale for each row's 128. `gate_up` [rows][2n], if given, gets
-    [x . G^T | x . U^T], which `gated_backward` takes.
+    [x . G^T | x . U^T], which `gated_backward` takes. `kernel` names the kernel to run an operand on, for tests and
+    measurements.
     """
     operand = isinstance(x, Packed)
     if operand:
@@ -309,6 +324,8 @@ def gated(x, weight: Packed, out=None, packed: Packed | None = None, gate_up=Non
     _check_experts(weight, "weight", routes.experts)
     if operand:
         _check_product(x, weight, routes.experts)
+    if kernel is not None and not operand:
+        raise ValueError("a kernel is named for an operand, not for a tensor")
     if weight.k != k or weight.rows % 2:
         raise ValueError(f"the weight must have k = {k} and an even number of rows, not {weight.k} and {weight.rows}")
     n, routed, item = weight.rows // 2, rows * routes.copies, 2 if code else 4
@@ -329,7 +346,8 @@ def gated(x, weight: Packed, out=None, packed: Packed | None = None, gate_up=Non
         handle = launch_stream(stream, like, x.scales, weight.codes, weight.scales, *tensors, *routes.tensors)
         offsets, size = routes.arguments[:2]
         status = native.mb_fp8_gated_product(code, *_parts(x), x.block, *_parts(weight), weight.block, *output, *saved,
-                                             rows, n, k, offsets, size, routes.experts or 1, handle)
+                                             rows, n, k, offsets, size, routes.experts or 1,
+                                             None if kernel is None else kernel.encode(), handle)
     else:
         workspace = _workspace(workspace, native.mb_fp8_linear_workspace(routed, n, k), x, stream)
         handle = launch_stream(stream, x, weight.codes, weight.scales, workspace, *tensors, *routes.tensors)
