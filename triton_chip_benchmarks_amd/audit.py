@@ -48,7 +48,7 @@ _FP8_QUANTIZE_RE = re.compile(r"fp8_quantize_kernelI(f|DF16_|DF16b)Li(\d+)ELb([0
 _FP8_TENSOR_RE = re.compile(r"(fp8_quantize_tiles|fp8_gradient|fp8_dequantize|rms_norm_weight)_kernelI(f|DF16_|DF16b)"
                             r"(?:Lb([01])E)?E")
 _FP8_FLAG = {"fp8_quantize_tiles": "_square", "fp8_gradient": "_gated", "fp8_dequantize": "_stream"}
-_FP8_FEW_RE = re.compile(r"fp8_few_kernelI(h|f|DF16_|DF16b)(h|f|DF16_|DF16b)Li([012])ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)EE")
+_FP8_FEW_RE = re.compile(r"fp8_few_kernelI(h|f|DF16_|DF16b)(h|f|DF16_|DF16b)Li([012])ELi(\d+)ELi(\d+)EE")
 _FP8_TILES_RE = re.compile(r"fp8_tiles_kernelI(h|f|DF16_|DF16b)Li([0-3])ELi(\d+)ELi(\d+)ELi\d+EE")
 _FP8_EPILOGUE = ("product", "gated", "gated_fp8", "gated_kept")
 _NORM_RE = re.compile(r"(rms_norm(?:_backward)?)_kernelI(f|DF16_|DF16b)Li(\d+)ELi(\d+)EE")

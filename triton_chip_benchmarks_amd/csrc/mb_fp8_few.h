@@ -53,7 +53,7 @@ struct Fp8Product {
   int copies, tokens, experts;
 };
 
-constexpr int kFp8FewRows = 16;
+constexpr int kFp8FewWaves = 8, kFp8FewRows = 16;
 
 // LDS of the quantised rows: a row's codes, then a row's scales, each row a bank
 // group past the one before. Pairs of blocks: a turn of the kernel takes two.
@@ -126,21 +126,20 @@ __device__ __forceinline__ f32x4 fp8_mma16(const Fp8Fragment<true, SEL>& a, cons
   return c;
 }
 
-// A workgroup takes up to 16 * RB rows at a time (of one expert) and TILES tiles of
+// A workgroup takes up to 16 rows at a time (of one expert) and TILES tiles of
 // FB * 16 rows of W (gated: 16 of the gates' and the same 16 of the ups' each two),
 // SPLIT waves sharing a tile's K in turns of 256 elements; they add their parts in LDS
 // in a fixed order. X is of fp32, fp16 or bf16, quantised into LDS on the way, or
 // (uint8_t) an operand, read where it is. W's rows are the instruction's rows, X's its
 // columns: a lane holds 32 bytes of K of a row of each, and four neighbouring features
 // of one row of the output.
-template <class X, class Y, int EPILOGUE, int FB, int RB, int WAVES, int SPLIT>
-__global__ void __launch_bounds__(64 * WAVES) fp8_few_kernel(Fp8Product p, int lds_rows) {
+template <class X, class Y, int EPILOGUE, int FB, int SPLIT>
+__global__ void __launch_bounds__(64 * kFp8FewWaves) fp8_few_kernel(Fp8Product p, int lds_rows) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool GATED = EPILOGUE != kFp8Plain, STAGED = sizeof(X) > 1, WIDE = sizeof(Y) == 4;
-  constexpr int TILES = WAVES / SPLIT, WIDTH = FB * 16, COLUMNS = GATED ? WIDTH / 2 : WIDTH, ROWS = 16 * RB;
+  constexpr int WAVES = kFp8FewWaves, TILES = WAVES / SPLIT, WIDTH = FB * 16, COLUMNS = GATED ? WIDTH / 2 : WIDTH, ROWS = kFp8FewRows;
   static_assert(!GATED || FB % 2 == 0, "pairs");
   static_assert(EPILOGUE != kFp8GatedFp8 || TILES * COLUMNS == 128, "a workgroup holds whole blocks of the output");
-  static_assert(!STAGED || RB == 1, "16 rows are staged");
   __shared__ float parts[WAVES][ROWS][WIDTH + 1];
   extern __shared__ __attribute__((aligned(16))) uint8_t staged[];
   const int lane = threadIdx.x & 63, part = lane >> 4, l16 = lane & 15;
@@ -198,59 +197,52 @@ __global__ void __launch_bounds__(64 * WAVES) fp8_few_kernel(Fp8Product p, int l
       }
       __syncthreads();
     }
-    const uint8_t* xc[RB];
-    const uint8_t* xs[RB];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      const int mine = min(16 * r + l16, live - 1);
-      if constexpr (STAGED) {
-        xc[r] = staged + mine * code_stride + part * 32;
-        xs[r] = staged_scales + mine * scale_stride;
-      } else {
-        xc[r] = static_cast<const uint8_t*>(p.x) + static_cast<int64_t>(m0 + mine) * pitch + part * 32;
-        xs[r] = p.sx + static_cast<int64_t>((m0 + mine) >> p.x_shift) * 4;
-      }
+    const int mine = min(l16, live - 1);
+    const uint8_t *xc, *xs;
+    if constexpr (STAGED) {
+      xc = staged + mine * code_stride + part * 32;
+      xs = staged_scales + mine * scale_stride;
+    } else {
+      xc = static_cast<const uint8_t*>(p.x) + static_cast<int64_t>(m0 + mine) * pitch + part * 32;
+      xs = p.sx + static_cast<int64_t>((m0 + mine) >> p.x_shift) * 4;
     }
-    f32x4 acc[RB][FB] = {};
+    f32x4 acc[FB] = {};
     auto multiply = [&](const Unit& unit, int turn) __attribute__((always_inline)) {
       const int b = (turn0 + turn * SPLIT) * 2;
       const bool tail = !STAGED && (b + 2) * 128 > pitch;
       const bool past = b + 1 >= blocks;  // of the turn's second block: nothing of it counts, its scales neither
+      Fp8Codes codes[2];
+      uint32_t scales;
+      if constexpr (STAGED) {
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        Fp8Codes codes[2];
-        uint32_t scales;
-        if constexpr (STAGED) {
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            codes[h].at[q] = *reinterpret_cast<const i32x4*>(xc + (b + h) * 128 + q * 16);
+        scales = *reinterpret_cast<const uint16_t*>(xs + b);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            codes[h].at[q] =
+                *reinterpret_cast<const i32x4*>(xc + min((b + h) * 128 + q * 16, pitch - 16 - part * 32));
+        scales = *reinterpret_cast<const uint16_t*>(xs + (int64_t{b >> 2} * x_scales * 4 + (b & 3)));
+        if (tail) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int q = 0; q < 2; ++q)
-              codes[h].at[q] = *reinterpret_cast<const i32x4*>(xc[r] + (b + h) * 128 + q * 16);
-          scales = *reinterpret_cast<const uint16_t*>(xs[r] + b);
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-              codes[h].at[q] = *reinterpret_cast<const i32x4*>(
-                  xc[r] + min((b + h) * 128 + q * 16, pitch - 16 - part * 32));
-          scales = *reinterpret_cast<const uint16_t*>(xs[r] + (int64_t{b >> 2} * x_scales * 4 + (b & 3)));
-          if (tail) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int q = 0; q < 2; ++q)
-                if ((b + h) * 128 + part * 32 + q * 16 >= pitch) codes[h].at[q] = i32x4{0, 0, 0, 0};
-          }
+              if ((b + h) * 128 + part * 32 + q * 16 >= pitch) codes[h].at[q] = i32x4{0, 0, 0, 0};
         }
-        if (past) scales &= 0xff;
-        const Fp8Fragment<WIDE, 0> x0(codes[0], scales);
-        const Fp8Fragment<WIDE, 1> x1(codes[1], scales);
+      }
+      if (past) scales &= 0xff;
+      const Fp8Fragment<WIDE, 0> x0(codes[0], scales);
+      const Fp8Fragment<WIDE, 1> x1(codes[1], scales);
 #pragma unroll
-        for (int f = 0; f < FB; ++f) {
-          acc[r][f] = fp8_mma16(Fp8Fragment<WIDE, 0>(unit.w[f][0], unit.s[f]), x0, acc[r][f]);
-          acc[r][f] = fp8_mma16(Fp8Fragment<WIDE, 1>(unit.w[f][1], past ? unit.s[f] & 0xff : unit.s[f]), x1, acc[r][f]);
-        }
+      for (int f = 0; f < FB; ++f) {
+        acc[f] = fp8_mma16(Fp8Fragment<WIDE, 0>(unit.w[f][0], unit.s[f]), x0, acc[f]);
+        acc[f] = fp8_mma16(Fp8Fragment<WIDE, 1>(unit.w[f][1], past ? unit.s[f] & 0xff : unit.s[f]), x1, acc[f]);
       }
     };
     for (int turn = 0; turn < turns; ++turn) {
@@ -258,11 +250,9 @@ __global__ void __launch_bounds__(64 * WAVES) fp8_few_kernel(Fp8Product p, int l
       if (turn + 1 < turns) load(unit, turn + 1);
     }
 #pragma unroll
-    for (int r = 0; r < RB; ++r)
+    for (int f = 0; f < FB; ++f)
 #pragma unroll
-      for (int f = 0; f < FB; ++f)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) parts[wave][16 * r + l16][f * 16 + 4 * part + i] = acc[r][f][i];
+      for (int i = 0; i < 4; ++i) parts[wave][l16][f * 16 + 4 * part + i] = acc[f][i];
     __syncthreads();
     // Column `column` of the workgroup's and row r, of W's rows of parity `odd`.
     auto sum = [&](int r, int column, int odd) __attribute__((always_inline)) {

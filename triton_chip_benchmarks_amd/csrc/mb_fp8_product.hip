@@ -1,5 +1,7 @@
 // Products of FP8 operands with block scales: linear layers, their gradients and the
 // gated pair of projections, of one weight or one for each expert.
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "mb_fp8.h"
@@ -10,12 +12,25 @@ namespace {
 
 // ---- the kernels of products -----------------------------------------------------
 
+// Microseconds of a quantisation's launch, and of 4096 elements quantised in a product's.
+constexpr double kQuantizeLaunch = 2.8, kStaging = 0.25;
+
 constexpr int kE4m3 = 3;  // after MB_DTYPE_*: X an operand, or Y one
 
 template <class T>
 constexpr int type_code() {
   return sizeof(T) == 1 ? kE4m3 : sizeof(T) == 4 ? MB_DTYPE_F32 : __is_same(T, __bf16) ? MB_DTYPE_BF16 : MB_DTYPE_F16;
 }
+
+// What a launch takes, in microseconds. Of tiles: `launch` once; for every round of the
+// chip's workgroups `tile`, `ragged` more where the rows of Y are not on 16 bytes, and for
+// every 128 elements of K from `step_empty` to `step` with the filled share of the round
+// (the L2s and the power limit slow a step down as more CUs run). Of few rows: `launch`;
+// for every round `tile` and, for every 256 elements of K that a wave takes, `step`; and
+// `megabyte` for every 10^6 bytes of weights.
+struct ProductCost {
+  float launch, tile, ragged, step_empty, step, megabyte;
+};
 
 // A kernel for X of `x` and Y of `y` by `epilogue` (Fp8TileEpilogue): of few rows, or of
 // tiles of `features` columns of W by `rows` rows.
@@ -26,6 +41,8 @@ struct ProductKernel {
   int features, rows;  // of a workgroup: columns of the output, rows
   int resident;        // workgroups a CU holds
   int band;            // row tiles that share their weight's panels in an XCD's L2
+  int split;           // waves that share a tile's K
+  ProductCost cost;
   void (*launch)(const Fp8Product&, uint32_t grid, int band, hipStream_t);
 };
 
@@ -37,14 +54,15 @@ dim3 few_grid(uint32_t n, uint32_t columns, uint32_t rows, uint32_t chunk, uint3
               chunks < 1 ? 1 : chunks < 256 ? chunks : 256);
 }
 
-template <class X, class Y, int EPILOGUE, int FB, int RB, int WAVES, int SPLIT>
+template <class X, class Y, int EPILOGUE, int FB, int SPLIT>
 void launch_few(const Fp8Product& p, uint32_t, int, hipStream_t stream) {
-  constexpr uint32_t kColumns = WAVES / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kRows = 16 * RB;
+  constexpr uint32_t kColumns = kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2);
+  constexpr uint32_t kRows = kFp8FewRows;
   const uint32_t rows = static_cast<uint32_t>(p.rows), lds_rows = rows < kRows ? rows : kRows;
   const uint64_t lds = sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0;
-  fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>
+  fp8_few_kernel<X, Y, EPILOGUE, FB, SPLIT>
       <<<few_grid(static_cast<uint32_t>(p.n), kColumns, rows, kRows, static_cast<uint32_t>(p.experts), p.offsets),
-         dim3(64 * WAVES), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
+         dim3(64 * kFp8FewWaves), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
 }
 
 template <class Y, int EPILOGUE, int BM, int BN, int STAGES>
@@ -54,75 +72,82 @@ void launch_tiles(const Fp8Product& p, uint32_t grid, int band, hipStream_t stre
       <<<dim3(grid < kPlaces ? grid : kPlaces), dim3(256), 0, stream>>>(p, band);
 }
 
-#define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, RB, WAVES, SPLIT)                                 \
+#define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, SPLIT, ...)                                       \
   ProductKernel {                                                                                              \
-    "fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #RB "x" #WAVES "x" #SPLIT, type_code<X>(),               \
-        type_code<Y>(), EPILOGUE, false, WAVES / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), 16 * RB, 0, \
-        0, launch_few<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>                                                    \
+    "fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #SPLIT, type_code<X>(), type_code<Y>(), EPILOGUE, false, \
+        kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kFp8FewRows, 2, 0, SPLIT,            \
+        {__VA_ARGS__}, launch_few<X, Y, EPILOGUE, FB, SPLIT>                                                   \
   }
-#define MB_FP8_TILES(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND)                                          \
+#define MB_FP8_TILES(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND, ...)                                     \
   ProductKernel {                                                                                              \
     "fp8_tiles_" NAME "_" Y_NAME "_" #BM "x" #BN, kE4m3, type_code<Y>(), EPILOGUE, true,                       \
-        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, BAND,           \
-        launch_tiles<Y, EPILOGUE, BM, BN, STAGES>                                                              \
+        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, BAND, 1,        \
+        {__VA_ARGS__}, launch_tiles<Y, EPILOGUE, BM, BN, STAGES>                                               \
   }
-// The forms, for a list M(arguments) of kernels and for their registration alike.
-#define MB_FP8_FEW_OF(M, X, X_NAME, Y, Y_NAME)                 \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 1, 8, 8)    \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 1, 8, 4)    \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 1, 8, 8)    \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 1, 8, 8)      \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 1, 8, 4)
-#define MB_FP8_FEW_MORE(M, X, X_NAME, Y, Y_NAME)               \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 2, 8, 4)    \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 8, 4)    \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 2, 8, 4)      \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 8, 4)
-#define MB_FP8_FEW_ALL(M)                                                              \
-  MB_FP8_FEW_OF(M, uint8_t, "e4m3", float, "f32")                                      \
-  MB_FP8_FEW_OF(M, uint8_t, "e4m3", _Float16, "f16")                                   \
-  MB_FP8_FEW_OF(M, uint8_t, "e4m3", __bf16, "bf16")                                    \
-  MB_FP8_FEW_MORE(M, uint8_t, "e4m3", float, "f32")                                    \
-  MB_FP8_FEW_MORE(M, uint8_t, "e4m3", _Float16, "f16")                                 \
-  MB_FP8_FEW_MORE(M, uint8_t, "e4m3", __bf16, "bf16")                                  \
-  MB_FP8_FEW_OF(M, float, "f32", float, "f32")                                         \
-  MB_FP8_FEW_OF(M, _Float16, "f16", _Float16, "f16")                                   \
-  MB_FP8_FEW_OF(M, __bf16, "bf16", __bf16, "bf16")                                     \
-  M(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)           \
-  M(float, "f32", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)              \
-  M(_Float16, "f16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)           \
-  M(__bf16, "bf16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 8, 1)
-#define MB_FP8_TILES_PLAIN(M, Y, Y_NAME)                          \
-  M(Y, Y_NAME, kTilePlain, "product", 256, 128, 3, 4)             \
-  M(Y, Y_NAME, kTilePlain, "product", 128, 128, 4, 6)             \
-  M(Y, Y_NAME, kTilePlain, "product", 128, 64, 3, 8)              \
-  M(Y, Y_NAME, kTilePlain, "product", 64, 64, 3, 8)               \
-  M(Y, Y_NAME, kTileGated, "gated", 256, 64, 3, 8)                \
-  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 64, 3, 8)
-#define MB_FP8_TILES_GATED(M, Y, Y_NAME)                          \
-  M(Y, Y_NAME, kTilePlain, "product", 256, 256, 2, 4)             \
-  M(Y, Y_NAME, kTileGated, "gated", 256, 256, 2, 4)               \
-  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 256, 2, 4)      \
-  M(Y, Y_NAME, kTileGated, "gated", 256, 128, 3, 4)               \
-  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 128, 3, 4)
-#define MB_FP8_TILES_ALL(M)                                       \
-  MB_FP8_TILES_PLAIN(M, float, "f32")                             \
-  MB_FP8_TILES_PLAIN(M, _Float16, "f16")                          \
-  MB_FP8_TILES_PLAIN(M, __bf16, "bf16")                           \
-  MB_FP8_TILES_GATED(M, _Float16, "f16")                          \
-  MB_FP8_TILES_GATED(M, __bf16, "bf16")                           \
-  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 256, 2, 4)  \
-  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 128, 3, 4)  \
-  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 64, 3, 8)
+// The forms, for a list M(arguments) of kernels and for their registration alike. Costs
+// are fitted to 8700 sizes on an MI355X (1 to 16384 rows, n and K from 64 to 8192, one
+// weight or 8 to 128 experts of uneven popularity, two of five off the tiles): the
+// cheapest estimate costs 1.3% over the fastest of the tiles on average for products and
+// 0.3% for gated ones, and 1.8% over the fastest of all where there are few rows; the
+// worst are 6 to 27 us of launches of 7 to 60 in which a few experts had all the rows.
+#define MB_FP8_FEW_16(M, X, X_NAME, Y, Y_NAME)                                           \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 8, 5.68f, 1.01f, 0, 0, 0, 0.071f)     \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 8, 4.15f, 2.46f, 0, 0, 0.18f, 0.078f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 3.52f, 2.43f, 0, 0, 0.78f, 0.082f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 8, 4.87f, 2.39f, 0, 0, 0.03f, 0.089f)   \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 4.26f, 2.36f, 0, 0, 0.72f, 0.072f)
+#define MB_FP8_TILES_16(M, Y, Y_NAME)                                                                 \
+  M(Y, Y_NAME, kTilePlain, "product", 256, 256, 2, 4, 4.56f, 3.81f, 4.15f, 0.958f, 1.700f, 0)         \
+  M(Y, Y_NAME, kTilePlain, "product", 256, 128, 3, 4, 3.83f, 2.87f, 2.05f, 0.620f, 1.095f, 0)         \
+  M(Y, Y_NAME, kTilePlain, "product", 128, 128, 4, 6, 4.51f, 1.71f, 0.69f, 0.391f, 0.594f, 0)         \
+  M(Y, Y_NAME, kTilePlain, "product", 128, 64, 3, 8, 4.48f, 1.72f, 0.10f, 0.214f, 0.740f, 0)          \
+  M(Y, Y_NAME, kTilePlain, "product", 64, 64, 3, 8, 5.16f, 1.14f, 0.05f, 0.134f, 0.417f, 0)           \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 256, 2, 4, 4.90f, 6.88f, 1.70f, 1.005f, 1.755f, 0)           \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 128, 3, 4, 4.55f, 3.70f, 0.77f, 0.613f, 1.043f, 0)           \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 64, 3, 8, 4.50f, 2.24f, 0.27f, 0.427f, 0.746f, 0)            \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 256, 2, 4, 3.99f, 10.97f, 5.85f, 0.989f, 1.719f, 0) \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 128, 3, 4, 3.75f, 6.17f, 2.81f, 0.614f, 1.010f, 0)  \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 64, 3, 8, 3.70f, 3.74f, 1.41f, 0.429f, 0.712f, 0)
+#define MB_FP8_FEW_32(M, X, X_NAME, Y, Y_NAME)                                           \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 8, 5.72f, 1.00f, 0, 0, 0, 0.085f)     \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 8, 4.07f, 2.48f, 0, 0, 0.29f, 0.094f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 3.34f, 2.44f, 0, 0, 0.99f, 0.093f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 8, 5.08f, 1.91f, 0, 0, 0.23f, 0.111f)   \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 4.30f, 1.96f, 0, 0, 1.02f, 0.094f)
+#define MB_FP8_TILES_32(M, Y, Y_NAME)                                                         \
+  M(Y, Y_NAME, kTilePlain, "product", 256, 128, 3, 4, 1.98f, 5.02f, 0.85f, 1.290f, 1.771f, 0) \
+  M(Y, Y_NAME, kTilePlain, "product", 128, 128, 4, 6, 3.53f, 2.70f, 0.06f, 0.720f, 0.946f, 0) \
+  M(Y, Y_NAME, kTilePlain, "product", 128, 64, 3, 8, 3.25f, 2.81f, 0, 0.423f, 1.040f, 0)      \
+  M(Y, Y_NAME, kTilePlain, "product", 64, 64, 3, 8, 4.76f, 1.41f, 0, 0.256f, 0.622f, 0)       \
+  M(Y, Y_NAME, kTileGated, "gated", 256, 64, 3, 8, 3.98f, 2.87f, 0.04f, 0.820f, 1.108f, 0)    \
+  M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 64, 3, 8, 2.83f, 4.91f, 0.71f, 0.825f, 1.105f, 0)
+#define MB_FP8_FEW_ALL(M)                                                                                 \
+  MB_FP8_FEW_32(M, uint8_t, "e4m3", float, "f32")                                                         \
+  MB_FP8_FEW_16(M, uint8_t, "e4m3", _Float16, "f16")                                                      \
+  MB_FP8_FEW_16(M, uint8_t, "e4m3", __bf16, "bf16")                                                       \
+  MB_FP8_FEW_32(M, float, "f32", float, "f32")                                                            \
+  MB_FP8_FEW_16(M, _Float16, "f16", _Float16, "f16")                                                      \
+  MB_FP8_FEW_16(M, __bf16, "bf16", __bf16, "bf16")                                                        \
+  M(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f) \
+  M(float, "f32", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f)    \
+  M(_Float16, "f16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f) \
+  M(__bf16, "bf16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f)
+#define MB_FP8_TILES_ALL(M)                                                                          \
+  MB_FP8_TILES_32(M, float, "f32")                                                                   \
+  MB_FP8_TILES_16(M, _Float16, "f16")                                                                \
+  MB_FP8_TILES_16(M, __bf16, "bf16")                                                                 \
+  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 256, 2, 4, 4.51f, 7.60f, 0, 1.018f, 1.830f, 0) \
+  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 128, 3, 4, 4.38f, 4.14f, 0, 0.631f, 1.061f, 0) \
+  M(uint8_t, "e4m3", kTileGatedFp8, "gated_fp8", 256, 64, 3, 8, 4.20f, 2.60f, 0, 0.452f, 0.729f, 0)
 
 #define MB_FP8_FEW_ENTRY(...) MB_FP8_FEW(__VA_ARGS__),
 #define MB_FP8_TILES_ENTRY(...) MB_FP8_TILES(__VA_ARGS__),
 const ProductKernel kKernels[] = {MB_FP8_FEW_ALL(MB_FP8_FEW_ENTRY) MB_FP8_TILES_ALL(MB_FP8_TILES_ENTRY)};
 
-#define MB_FP8_FEW_REGISTER(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, RB, WAVES, SPLIT)              \
-  MB_REGISTER_KERNEL("fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #RB "x" #WAVES "x" #SPLIT,    \
-                     (fp8_few_kernel<X, Y, EPILOGUE, FB, RB, WAVES, SPLIT>));
-#define MB_FP8_TILES_REGISTER(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND)                       \
+#define MB_FP8_FEW_REGISTER(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, SPLIT, ...)          \
+  MB_REGISTER_KERNEL("fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #SPLIT,             \
+                     (fp8_few_kernel<X, Y, EPILOGUE, FB, SPLIT>));
+#define MB_FP8_TILES_REGISTER(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND, ...)        \
   MB_REGISTER_KERNEL("fp8_tiles_" NAME "_" Y_NAME "_" #BM "x" #BN, (fp8_tiles_kernel<Y, EPILOGUE, BM, BN, STAGES>));
 MB_FP8_FEW_ALL(MB_FP8_FEW_REGISTER)
 MB_FP8_TILES_ALL(MB_FP8_TILES_REGISTER)
@@ -167,19 +192,47 @@ uint64_t most_row_tiles(uint32_t rows, uint32_t experts, int tile) {
   return experts > 1 ? rows / tile + (rows < experts ? rows : experts) : (rows + uint64_t{1} * tile - 1) / tile;
 }
 
-bool few_fits(uint64_t rows, uint32_t k) {
-  return fp8_few_lds(k, rows < kFp8FewRows ? static_cast<uint32_t>(rows) : kFp8FewRows) <= 96 * 1024;
+// Experts with rows, if all were as popular.
+double used_experts(uint32_t rows, uint32_t experts) {
+  return experts == 1 ? 1.0 : experts * (1.0 - std::exp(-static_cast<double>(rows) / experts));
 }
 
-// Whether X is quantised in the product's launch.
-bool few_rows(uint64_t rows, uint32_t k, uint32_t experts) {
-  const uint64_t most = experts > 1 ? 2 * uint64_t{experts} : kFp8FewRows;
-  return rows <= most && few_fits(rows, k);
+double mean_row_tiles(uint32_t rows, uint32_t experts, int tile) {
+  if (experts == 1) return static_cast<double>(most_row_tiles(rows, 1, tile));
+  const double each = static_cast<double>(rows) / experts;
+  return experts * (each >= tile ? each / tile + 0.5 : each >= 1 ? 1.0 : each);
+}
+
+// Estimated microseconds of a launch (see ProductCost).
+double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts) {
+  const ProductCost& cost = kernel.cost;
+  const double across = (n + uint64_t{1} * kernel.features - 1) / kernel.features;
+  if (!kernel.tiles) {
+    const double used = used_experts(rows, experts), each = rows / used;
+    const double chunks = experts == 1 ? (rows + kFp8FewRows - 1) / kFp8FewRows : std::max(1.0, each / kFp8FewRows);
+    const double rounds = std::max(1.0, across * used * chunks / (256.0 * kernel.resident));
+    const double turns = ((k + 255) / 256 + kernel.split - 1) / kernel.split;
+    const double width = kernel.epilogue == kFp8Plain ? n : 2.0 * n;
+    // A workgroup quantises its rows, 4096 elements at a time.
+    const double staging = kernel.x == kE4m3 ? 0 : rounds * std::min(each, 1.0 * kFp8FewRows) * k / 4096 * kStaging;
+    return cost.launch + rounds * (cost.tile + turns * cost.step) + used * width * k * 1e-6 * chunks * cost.megabyte +
+           staging;
+  }
+  const double tiles = mean_row_tiles(rows, experts, kernel.rows) * across;
+  const double round = 256.0 * kernel.resident, whole = static_cast<double>(static_cast<uint64_t>(tiles / round));
+  const double rest = tiles / round - whole, steps = (k + 127) / 128;
+  const bool ragged = kernel.y != kE4m3 && uint64_t{n} * elem_bytes(kernel.y) % 16 != 0;
+  auto one = [&](double filled) {
+    return cost.tile + (ragged ? cost.ragged : 0.0f) +
+           steps * (cost.step_empty + (cost.step - cost.step_empty) * filled);
+  };
+  return cost.launch + whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
 }
 
 struct ProductChoice {
   const ProductKernel* kernel = nullptr;
   uint32_t grid = 0;  // of tiles
+  double cost = 0;
 };
 
 // The kernel for X of type `x` by the rule or, with `wanted`, the one of that name; none
@@ -188,13 +241,11 @@ ProductChoice choose_product(int x, int y, int epilogue, uint32_t rows, uint32_t
                              const char* wanted) {
   ProductChoice best;
   const uint64_t width = epilogue == kTilePlain ? n : uint64_t{2} * n, steps = (k + uint64_t{511}) / 512;
-  double best_cost = 0;
   for (const ProductKernel& kernel : kKernels) {
     // A kernel of few rows keeps the gate and up, if it is given where to.
     const int asked = epilogue == kTileGatedKept && !kernel.tiles ? static_cast<int>(kTileGated) : epilogue;
     if (kernel.x != x || kernel.y != y || kernel.epilogue != asked) continue;
     if (wanted && strcmp(wanted, kernel.name) != 0) continue;
-    double cost;
     uint64_t grid = 0;
     if (kernel.tiles) {
       if (experts > kStreamExperts) continue;
@@ -205,32 +256,49 @@ ProductChoice choose_product(int x, int y, int epilogue, uint32_t rows, uint32_t
           most_row_tiles(rows, experts, kernel.rows) * ((n + uint64_t{1} * kernel.features - 1) / kernel.features);
       grid = (tiles + kXcds - 1) / kXcds * kXcds;
       if (grid > 0xffffff) continue;
-      cost = 5.0 + static_cast<double>((tiles + 255) / 256) * (k + 127) / 128 * kernel.features * kernel.rows / 32768;
     } else {
-      const dim3 few = few_grid(n, static_cast<uint32_t>(kernel.features), rows, static_cast<uint32_t>(kernel.rows),
-                                experts, experts > 1);
-      if (uint64_t{few.x} * few.y * few.z > 0x3fffff) continue;  // of 1024 threads at most: 2^32 - 1 a launch
-      cost = static_cast<double>(rows) / experts * n * k * 1e-9;
+      // A row's codes fit the LDS, and the workgroups of 512 a launch's 2^32 - 1.
+      if (x != kE4m3 && fp8_few_lds(k, rows < kFp8FewRows ? rows : kFp8FewRows) > 96 * 1024) continue;
+      const dim3 few = few_grid(n, static_cast<uint32_t>(kernel.features), rows, kFp8FewRows, experts, experts > 1);
+      if (uint64_t{few.x} * few.y * few.z > 0x7fffff) continue;
     }
-    if (best.kernel && cost >= best_cost) continue;
-    best_cost = cost;
-    best.kernel = &kernel;
-    best.grid = static_cast<uint32_t>(grid);
+    const double cost = product_cost(kernel, rows, n, k, experts);
+    if (best.kernel && cost >= best.cost) continue;
+    best = ProductChoice{&kernel, static_cast<uint32_t>(grid), cost};
   }
   return best;
 }
 
-int launch_product(const char* entry, const char* wanted, int x, int dtype, Fp8Epilogue epilogue, const Fp8Product& p,
-                   hipStream_t stream) {
-  const int asked = epilogue == kFp8Gated && p.gate_up ? static_cast<int>(kTileGatedKept) : static_cast<int>(epilogue);
-  const ProductChoice choice =
-      choose_product(x, epilogue == kFp8GatedFp8 ? kE4m3 : dtype, asked, static_cast<uint32_t>(p.rows),
-                     static_cast<uint32_t>(p.n), static_cast<uint32_t>(p.k), static_cast<uint32_t>(p.experts), wanted);
+// Whether X, of `dtype`, is quantised in the product's launch, and the choice for either.
+bool choose_linear(int dtype, int y, int epilogue, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts,
+                   ProductChoice& choice) {
+  const ProductChoice inside = choose_product(dtype, y, epilogue, rows, n, k, experts, nullptr);
+  choice = choose_product(kE4m3, y, epilogue, rows, n, k, experts, nullptr);
+  if (inside.kernel == nullptr || (choice.kernel && inside.cost > choice.cost + kQuantizeLaunch)) return false;
+  choice = inside;
+  return true;
+}
+
+int kind_of(Fp8Epilogue epilogue, const Fp8Product& p) {
+  return epilogue == kFp8Gated && p.gate_up ? static_cast<int>(kTileGatedKept) : static_cast<int>(epilogue);
+}
+
+int launch_choice(const char* entry, const ProductChoice& choice, const char* wanted, const Fp8Product& p,
+                  hipStream_t stream) {
   if (choice.kernel == nullptr)
     return fail(MB_ERR_UNSUPPORTED, "%s: no kernel %s that takes %d x %d x %d and %d experts", entry,
                 wanted ? wanted : "", p.rows, p.n, p.k, p.experts);
   choice.kernel->launch(p, choice.grid, choice.kernel->band, stream);
   return launch_status(choice.kernel->name);
+}
+
+// X an operand.
+int launch_product(const char* entry, const char* wanted, int dtype, Fp8Epilogue epilogue, const Fp8Product& p,
+                   hipStream_t stream) {
+  const ProductChoice choice = choose_product(
+      kE4m3, epilogue == kFp8GatedFp8 ? kE4m3 : dtype, kind_of(epilogue, p), static_cast<uint32_t>(p.rows),
+      static_cast<uint32_t>(p.n), static_cast<uint32_t>(p.k), static_cast<uint32_t>(p.experts), wanted);
+  return launch_choice(entry, choice, wanted, p, stream);
 }
 
 uint64_t workspace_codes(uint64_t rows, uint64_t k) { return (fp8_code_bytes(rows, k) + 15) / 16 * 16; }
@@ -246,8 +314,10 @@ int run_linear(const char* entry, int dtype, Fp8Epilogue epilogue, Fp8Product p,
     return fail(MB_ERR_INVALID, "%s: the workspace is NULL or too small: %llu bytes needed", entry,
                 (unsigned long long)needed);
   if (!aligned(workspace, 16)) return fail(MB_ERR_ALIGNMENT, "%s: the workspace must lie on 16 bytes", entry);
-  if (few_rows(rows, k, static_cast<uint32_t>(p.experts)))
-    return launch_product(entry, nullptr, dtype, dtype, epilogue, p, stream);
+  ProductChoice choice;
+  if (choose_linear(dtype, epilogue == kFp8GatedFp8 ? kE4m3 : dtype, kind_of(epilogue, p), rows,
+                    static_cast<uint32_t>(p.n), k, static_cast<uint32_t>(p.experts), choice))
+    return launch_choice(entry, choice, nullptr, p, stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + workspace_codes(rows, k);
   if (int rc = fp8_launch_quantize(dtype, p.x, static_cast<uint32_t>(p.tokens), k, p.row_stride, slots,
@@ -256,7 +326,7 @@ int run_linear(const char* entry, int dtype, Fp8Epilogue epilogue, Fp8Product p,
   p.x = codes;
   p.sx = scales;
   p.x_shift = 0;
-  return launch_product(entry, nullptr, kE4m3, dtype, epilogue, p, stream);
+  return launch_choice(entry, choice, nullptr, p, stream);
 }
 
 // The outputs of a gated product.
@@ -334,7 +404,7 @@ int run_backward(const char* entry, int dtype, const void* d_out, uint64_t d_out
   p.rows = p.tokens = static_cast<int>(rows);
   p.n = static_cast<int>(k);
   p.k = static_cast<int>(n);
-  if (int rc = launch_product(entry, nullptr, kE4m3, dtype, kFp8Plain, p, stream)) return rc;
+  if (int rc = launch_product(entry, nullptr, dtype, kFp8Plain, p, stream)) return rc;
   p.x = out[1].codes;
   p.sx = out[1].scales;
   p.w = out[2].codes;
@@ -344,7 +414,7 @@ int run_backward(const char* entry, int dtype, const void* d_out, uint64_t d_out
   p.rows = p.tokens = static_cast<int>(n);
   p.n = static_cast<int>(k);
   p.k = static_cast<int>(depth);
-  return launch_product(entry, nullptr, kE4m3, dtype, kFp8Plain, p, stream);
+  return launch_product(entry, nullptr, dtype, kFp8Plain, p, stream);
 }
 
 }  // namespace
@@ -382,7 +452,7 @@ int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale
   p.offsets = offsets;
   p.copies = 1;
   p.experts = static_cast<int>(experts);
-  return mb::launch_product(entry, kernel, mb::kE4m3, dtype, mb::kFp8Plain, p, static_cast<hipStream_t>(stream));
+  return mb::launch_product(entry, kernel, dtype, mb::kFp8Plain, p, static_cast<hipStream_t>(stream));
 }
 
 const char* mb_fp8_product_kernel(int dtype, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts, uint32_t linear,
@@ -395,8 +465,15 @@ const char* mb_fp8_product_kernel(int dtype, uint32_t rows, uint32_t n, uint32_t
     return nullptr;
   }
   const int kinds[] = {mb::kTilePlain, mb::kTileGated, mb::kTileGatedKept, mb::kTileGatedFp8};
-  const int x = linear && mb::few_rows(rows, k, experts) ? dtype : mb::kE4m3;
-  return mb::choose_product(x, fp8 ? mb::kE4m3 : dtype, kinds[gated], rows, n, k, experts, nullptr).kernel->name;
+  const int y = fp8 ? mb::kE4m3 : dtype;
+  mb::ProductChoice choice;
+  if (linear)
+    mb::choose_linear(dtype, y, kinds[gated], rows, n, k, experts, choice);
+  else
+    choice = mb::choose_product(mb::kE4m3, y, kinds[gated], rows, n, k, experts, nullptr);
+  if (choice.kernel) return choice.kernel->name;
+  mb::fail(MB_ERR_UNSUPPORTED, "%s: no kernel that takes %u x %u x %u and %u experts", entry, rows, n, k, experts);
+  return nullptr;
 }
 
 uint64_t mb_fp8_linear_workspace(uint32_t rows, uint32_t n, uint32_t k) {
@@ -492,7 +569,7 @@ int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void*
   p.offsets = offsets;
   p.copies = 1;
   p.experts = static_cast<int>(experts);
-  return mb::launch_product(entry, kernel, mb::kE4m3, dtype, y_scales ? mb::kFp8GatedFp8 : mb::kFp8Gated, p,
+  return mb::launch_product(entry, kernel, dtype, y_scales ? mb::kFp8GatedFp8 : mb::kFp8Gated, p,
                             static_cast<hipStream_t>(stream));
 }
 
