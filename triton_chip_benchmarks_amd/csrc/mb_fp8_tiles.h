@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(256, (Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESID
     dma_advance();
   };
   [[maybe_unused]] auto rolled = [&](int kt, Set& set) __attribute__((always_inline)) {
-    constexpr int NQ = Tile::MFMAS, BARRIER = 4, SPREAD = 20;
+    constexpr int NQ = Tile::MFMAS, BARRIER = 2, SPREAD = 22;
     const uint32_t next_stage = stage == 0 ? Tile::STAGE : 0;
     const int next = kt + 1 == k_steps ? 0 : kt + 1;
     static_for<0, NQ>([&](auto q_c) __attribute__((always_inline)) {

@@ -179,31 +179,24 @@ def _check_product(a: Packed, b: Packed, experts: int | None) -> None:
         raise ValueError("rows of several experts have a scale each")
 
 
-class _Routes:
-    """What a call takes from a plan: its experts, copies of a row, and the C arguments."""
-
-    __slots__ = ("experts", "copies", "tensors", "arguments")
-
-    def __init__(self, plan, rows: int, sorted_rows: bool):
-        self.experts, self.copies, self.tensors = None, 1, ()
-        self.arguments = (None, 0, None, None, 0, 1, 1)
-        if plan is None:
-            if sorted_rows:
-                raise ValueError("sorted rows need the plan that they are sorted by")
-            return
-        offsets, order, slots = plan.offsets, plan.order, plan.slots
-        _check_indices(offsets, "plan.offsets")
-        self.experts = offsets.numel() - 1
-        self.tensors = (offsets,)
+def _routes(plan, rows: int, sorted_rows: bool):
+    """What a call takes from a plan: (experts, copies of a row, tensors, the C arguments)."""
+    if plan is None:
         if sorted_rows:
-            self.arguments = (*_pointer(offsets), None, None, 0, 1, self.experts)
-            return
-        _check_indices(order, "plan.order")
-        _check_indices(slots, "plan.slots")
-        if slots.dim() != 2 or slots.shape[0] != rows or order.numel() != slots.numel():
-            raise ValueError(f"the plan must route {rows} tokens, not slots of {tuple(slots.shape)}")
-        self.copies, self.tensors = slots.shape[1], (offsets, order, slots)
-        self.arguments = (*_pointer(offsets), order.data_ptr(), *_pointer(slots), self.copies, self.experts)
+            raise ValueError("sorted rows need the plan that they are sorted by")
+        return None, 1, (), (None, 0, None, None, 0, 1, 1)
+    offsets, order, slots = plan.offsets, plan.order, plan.slots
+    _check_indices(offsets, "plan.offsets")
+    experts = offsets.numel() - 1
+    if sorted_rows:
+        return experts, 1, (offsets,), (*_pointer(offsets), None, None, 0, 1, experts)
+    _check_indices(order, "plan.order")
+    _check_indices(slots, "plan.slots")
+    if slots.dim() != 2 or slots.shape[0] != rows or order.numel() != slots.numel():
+        raise ValueError(f"the plan must route {rows} tokens, not slots of {tuple(slots.shape)}")
+    copies = slots.shape[1]
+    return (experts, copies, (offsets, order, slots),
+            (*_pointer(offsets), order.data_ptr(), *_pointer(slots), copies, experts))
 
 
 def linear_workspace(rows: int, n: int, k: int, dtype, experts: int = 1, device="cuda"):
@@ -220,18 +213,18 @@ def linear(x, weight: Packed, out=None, plan=None, sorted_rows: bool = False, wo
     """
     code = dtype_code(x, "x")
     rows, k, stride, span = strided_rows(x, "x")
-    routes = _Routes(plan, rows, sorted_rows)
-    _check_experts(weight, "weight", routes.experts)
+    experts, copies, indices, routes = _routes(plan, rows, sorted_rows)
+    _check_experts(weight, "weight", experts)
     if weight.k != k:
         raise ValueError(f"the weight must have k = {k}, not {weight.k}")
-    n, routed = weight.rows, rows * routes.copies
+    n, routed = weight.rows, rows * copies
     out = check_output(out, "out", (routed, n), x.dtype, x, stream)
     native = library()
     workspace = _workspace(workspace, native.mb_fp8_linear_workspace(routed, n, k), x, stream)
-    handle = launch_stream(stream, x, weight.codes, weight.scales, out, workspace, *routes.tensors)
+    handle = launch_stream(stream, x, weight.codes, weight.scales, out, workspace, *indices)
     item = 2 if code else 4
     status = native.mb_fp8_linear(code, x.data_ptr(), span * item, rows, stride, *_parts(weight), weight.block,
-                                  out.data_ptr(), routed * n * item, n, k, *routes.arguments, workspace.data_ptr(),
+                                  out.data_ptr(), routed * n * item, n, k, *routes, workspace.data_ptr(),
                                   workspace.numel(), handle)
     if status:
         _native.check(status)
@@ -320,15 +313,15 @@ def gated(x, weight: Packed, out=None, packed: Packed | None = None, gate_up=Non
             raise ValueError(f"the output of a tensor of {x.dtype} is of its type, not {dtype}")
         rows, k, stride, span = strided_rows(x, "x")
         like, dtype = x, x.dtype
-    routes = _Routes(plan, rows, sorted_rows)
-    _check_experts(weight, "weight", routes.experts)
+    experts, copies, indices, routes = _routes(plan, rows, sorted_rows)
+    _check_experts(weight, "weight", experts)
     if operand:
-        _check_product(x, weight, routes.experts)
+        _check_product(x, weight, experts)
     if kernel is not None and not operand:
         raise ValueError("a kernel is named for an operand, not for a tensor")
     if weight.k != k or weight.rows % 2:
         raise ValueError(f"the weight must have k = {k} and an even number of rows, not {weight.k} and {weight.rows}")
-    n, routed, item = weight.rows // 2, rows * routes.copies, 2 if code else 4
+    n, routed, item = weight.rows // 2, rows * copies, 2 if code else 4
     if packed is None:
         result = out = check_output(out, "out", (routed, n), dtype, like, stream)
         output, tensors = (out.data_ptr(), routed * n * item, None, 0), (out,)
@@ -343,16 +336,16 @@ def gated(x, weight: Packed, out=None, packed: Packed | None = None, gate_up=Non
         saved, tensors = (gate_up.data_ptr(), routed * 2 * n * item), (*tensors, gate_up)
     native = library()
     if operand:
-        handle = launch_stream(stream, like, x.scales, weight.codes, weight.scales, *tensors, *routes.tensors)
-        offsets, size = routes.arguments[:2]
+        handle = launch_stream(stream, like, x.scales, weight.codes, weight.scales, *tensors, *indices)
+        offsets, size = routes[:2]
         status = native.mb_fp8_gated_product(code, *_parts(x), x.block, *_parts(weight), weight.block, *output, *saved,
-                                             rows, n, k, offsets, size, routes.experts or 1,
+                                             rows, n, k, offsets, size, experts or 1,
                                              None if kernel is None else kernel.encode(), handle)
     else:
         workspace = _workspace(workspace, native.mb_fp8_linear_workspace(routed, n, k), x, stream)
-        handle = launch_stream(stream, x, weight.codes, weight.scales, workspace, *tensors, *routes.tensors)
+        handle = launch_stream(stream, x, weight.codes, weight.scales, workspace, *tensors, *indices)
         status = native.mb_fp8_gated(code, x.data_ptr(), span * item, rows, stride, *_parts(weight), weight.block,
-                                     *output, *saved, n, k, *routes.arguments, workspace.data_ptr(), workspace.numel(),
+                                     *output, *saved, n, k, *routes, workspace.data_ptr(), workspace.numel(),
                                      handle)
     if status:
         _native.check(status)

@@ -28,11 +28,6 @@ class Normed(NamedTuple):
     total: object
 
 
-def _weight(weight, n: int, dtype) -> tuple[int, int]:
-    check_tensor(weight, "weight", (n,), dtype)
-    return weight.data_ptr(), n * weight.element_size()
-
-
 def rms_norm(x, weight, eps: float = 1e-6, residual=None, out=None, packed=None, total=None, stream=None) -> Normed:
     """y = t * weight / sqrt(mean(t^2) + eps) of rows t = x [rows][n], or x + residual rounded to x's type (`total`, which
     may be x or the residual itself).
@@ -41,35 +36,37 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None, out=None, packed=None,
     """
     code = dtype_code(x, "x")
     rows, n, stride, span = strided_rows(x, "x")
-    item = 2 if code else 4
-    weight_arguments = _weight(weight, n, x.dtype)
-    tensors = [x, weight]
-    added, sums = (None, 0, 0), (None, 0)
-    if residual is not None:
-        if residual.dtype is not x.dtype or residual.shape != x.shape:
-            raise ValueError(f"the residual must be a {x.dtype} tensor of {tuple(x.shape)}, not {residual.dtype} of "
+    item, dtype, shape = 2 if code else 4, x.dtype, x.shape
+    size = rows * n * item
+    check_tensor(weight, "weight", (n,), dtype)
+    added, sums, outputs, operand = (None, 0, 0), (None, 0), (None, 0), (None, 0, None, 0)
+    tensors = (x, weight)
+    if residual is None:
+        if total is not None:
+            raise ValueError("without a residual the total is x itself")
+        total = x
+    else:
+        if residual.dtype is not dtype or residual.shape != shape:
+            raise ValueError(f"the residual must be a {dtype} tensor of {tuple(shape)}, not {residual.dtype} of "
                              f"{tuple(residual.shape)}")
         _, _, residual_stride, residual_span = strided_rows(residual, "residual")
-        total = check_output(total, "total", (rows, n), x.dtype, x, stream)
-        added, sums = (residual.data_ptr(), residual_span * item, residual_stride), (total.data_ptr(), rows * n * item)
-        tensors += [residual, total]
-    elif total is not None:
-        raise ValueError("without a residual the total is x itself")
-    outputs, operand = (None, 0), (None, 0, None, 0)
+        total = check_output(total, "total", shape, dtype, x, stream)
+        added, sums = (residual.data_ptr(), residual_span * item, residual_stride), (total.data_ptr(), size)
+        tensors = (x, weight, residual, total)
     if packed is not None:
         packed = fp8._operand(packed, "packed", rows, n, 1, x, stream)
         operand = fp8._parts(packed)
-        tensors += [packed.codes, packed.scales]
+        tensors += (packed.codes, packed.scales)
     if out is not None or packed is None:
-        out = check_output(out, "out", (rows, n), x.dtype, x, stream)
-        outputs = (out.data_ptr(), rows * n * item)
-        tensors.append(out)
+        out = check_output(out, "out", shape, dtype, x, stream)
+        outputs = (out.data_ptr(), size)
+        tensors += (out,)
     handle = launch_stream(stream, *tensors)
-    status = library().mb_rms_norm(code, x.data_ptr(), span * item, stride, *added, *weight_arguments, eps, *sums,
-                                   *outputs, *operand, rows, n, handle)
+    status = library().mb_rms_norm(code, x.data_ptr(), span * item, stride, *added, weight.data_ptr(), n * item, eps,
+                                   *sums, *outputs, *operand, rows, n, handle)
     if status:
         _native.check(status)
-    return Normed(out, packed, x if residual is None else total)
+    return Normed(out, packed, total)
 
 
 def rms_norm_backward_workspace(rows: int, n: int, device="cuda"):
@@ -87,7 +84,7 @@ def rms_norm_backward(d_out, total, weight, eps: float = 1e-6, d_total=None, d_x
     code = dtype_code(total, "total")
     rows, n, stride, span = strided_rows(total, "total")
     item = 2 if code else 4
-    weight_arguments = _weight(weight, n, total.dtype)
+    check_tensor(weight, "weight", (n,), total.dtype)
     tensors, strides = [d_out, total, weight], []
     for name, tensor in (("d_out", d_out), ("d_total", d_total)):
         if tensor is None:
@@ -109,8 +106,8 @@ def rms_norm_backward(d_out, total, weight, eps: float = 1e-6, d_total=None, d_x
     native = library()
     workspace = _workspace(workspace, native.mb_rms_norm_backward_workspace(rows, n), total, stream)
     handle = launch_stream(stream, *tensors, d_x, d_weight, workspace)
-    status = native.mb_rms_norm_backward(code, *strides[0], total.data_ptr(), span * item, stride, *weight_arguments,
-                                         eps, *strides[1], d_x.data_ptr(), rows * n * item, d_weight.data_ptr(),
+    status = native.mb_rms_norm_backward(code, *strides[0], total.data_ptr(), span * item, stride,
+                                         weight.data_ptr(), n * item, eps, *strides[1], d_x.data_ptr(), rows * n * item, d_weight.data_ptr(),
                                          n * item, rows, n, workspace.data_ptr(), workspace.numel(), handle)
     if status:
         _native.check(status)
