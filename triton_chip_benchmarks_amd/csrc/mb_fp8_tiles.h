@@ -63,6 +63,12 @@ struct Kept {
 // fragments of this step have arrived, so that its stage may be loaded again, and the
 // next step's loads, issued behind the last barrier, have had a step's time to land.
 //
+// The matrix cores bound it, and the clock that the power limit leaves them: 8192^3 from
+// operands in the caches takes 388 us (2.83 PFLOP/s; this library's FP8 product without
+// scales 376 to 404), with cold ones 424 to 450. With the barrier after the fourth
+// product instead of the second 433 cold, with two barriers a step, each for half of the
+// operands, 464. By 256x128 the same product takes 474: its loads are half as many again.
+//
 // There are at most kStreamExperts experts.
 template <class Y, int EPILOGUE, int BM, int BN, int STAGES>
 __global__ void __launch_bounds__(256, (Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT))
@@ -524,15 +530,15 @@ __global__ void __launch_bounds__(256, (Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESID
 #pragma unroll 1
       for (int kt = 0; kt < k_steps; ++kt) rolled(kt, set0);
     } else {
-    int kt = 0;
-    do {
-      step(kt, set0, set1);
-      if (kt + 1 < k_steps)
-        step(kt + 1, set1, set0);
-      else
-        set0 = set1;  // the next tile's first fragments
-      kt += 2;
-    } while (kt < k_steps);
+      int kt = 0;
+      do {
+        step(kt, set0, set1);
+        if (kt + 1 < k_steps)
+          step(kt + 1, set1, set0);
+        else
+          set0 = set1;  // the next tile's first fragments
+        kt += 2;
+      } while (kt < k_steps);
     }
     store(At{0, here_m0, here_n0, here_live});
     with_stores = STAGES - 1;

@@ -285,12 +285,20 @@ void for_width(uint32_t n, bool spread, F&& call) {
 }
 
 template <class T>
-void launch_norm(const NormArguments& a, hipStream_t stream) {
+int launch_norm(const char* entry, const NormArguments& a, hipStream_t stream) {
+  int status = MB_OK;
   for_width(a.n, a.rows <= 512, [&](auto waves, auto pieces) {
     constexpr int W = decltype(waves)::value, P = decltype(pieces)::value;
-    rms_norm_kernel<T, W, P>
-        <<<dim3(W == 1 ? (a.rows + 3) / 4 : a.rows), dim3(W > 4 ? 64 * W : 256), 0, stream>>>(a);
+    constexpr uint32_t kThreads = W > 4 ? 64 * W : 256;
+    const uint32_t grid = W == 1 ? (a.rows + 3) / 4 : a.rows;
+    if (uint64_t{grid} * kThreads > 0xffffffffu) {
+      status = fail(MB_ERR_UNSUPPORTED, "%s: %u rows of %u exceed one launch", entry, a.rows, a.n);
+      return;
+    }
+    rms_norm_kernel<T, W, P><<<dim3(grid), dim3(kThreads), 0, stream>>>(a);
+    status = launch_status("rms_norm");
   });
+  return status;
 }
 
 template <class T>
@@ -370,8 +378,9 @@ int mb_rms_norm(int dtype, const void* x, uint64_t x_bytes, uint64_t x_stride, c
       return rc;
   const mb::NormArguments a{x,     x_stride, residual, residual_stride, weight, eps, total, out,
                             static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, n};
-  MB_FOR_DTYPE(dtype, mb::launch_norm<T>(a, static_cast<hipStream_t>(stream)));
-  return mb::launch_status("rms_norm");
+  int status = MB_OK;
+  MB_FOR_DTYPE(dtype, status = mb::launch_norm<T>(entry, a, static_cast<hipStream_t>(stream)));
+  return status;
 }
 
 uint64_t mb_rms_norm_backward_workspace(uint32_t rows, uint32_t n) {
