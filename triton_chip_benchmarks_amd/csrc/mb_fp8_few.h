@@ -63,6 +63,7 @@ constexpr uint32_t fp8_scale_stride(uint32_t k) { return fp8_staged_blocks(k) + 
 constexpr uint64_t fp8_few_lds(uint32_t k, uint32_t rows) {
   return uint64_t{rows} * (fp8_code_stride(k) + fp8_scale_stride(k));
 }
+constexpr uint64_t fp8_few_parts(int width) { return uint64_t{kFp8FewWaves} * kFp8FewRows * (width + 1) * 4; }
 
 // A lane's 32 codes of a block of K and the dword with its scale.
 //
@@ -133,15 +134,26 @@ __device__ __forceinline__ f32x4 fp8_mma16(const Fp8Fragment<true, SEL>& a, cons
 // (uint8_t) an operand, read where it is. W's rows are the instruction's rows, X's its
 // columns: a lane holds 32 bytes of K of a row of each, and four neighbouring features
 // of one row of the output.
+//
+// Reading the weights bounds it, so the next turn's are in flight while one's are
+// multiplied, and nothing else waits for them: one row by 8192 x 8192 takes 14.4 us
+// (4.7 TB/s, two of them the launch), 16 by the gated pair of 14336 x 4096 25.7 (4.6),
+// 256 by those of 110 experts of 1024 x 4096 138 (6.7). SPLIT 8 is for the fewest
+// columns, and FB 2 for as many as leave a wave more to do: 4096 x 4096 5.7 us by 1x8;
+// 14336 x 1024 4.7 by 2x4. With X's codes or a third turn in flight as well, a wave's
+// registers leave a CU half the waves, at 1.1 to 1.3 times the time.
 template <class X, class Y, int EPILOGUE, int FB, int SPLIT>
 __global__ void __launch_bounds__(64 * kFp8FewWaves) fp8_few_kernel(Fp8Product p, int lds_rows) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool GATED = EPILOGUE != kFp8Plain, STAGED = sizeof(X) > 1, WIDE = sizeof(Y) == 4;
-  constexpr int WAVES = kFp8FewWaves, TILES = WAVES / SPLIT, WIDTH = FB * 16, COLUMNS = GATED ? WIDTH / 2 : WIDTH, ROWS = kFp8FewRows;
+  constexpr int WAVES = kFp8FewWaves, ROWS = kFp8FewRows, TILES = WAVES / SPLIT, WIDTH = FB * 16;
+  constexpr int COLUMNS = GATED ? WIDTH / 2 : WIDTH;
   static_assert(!GATED || FB % 2 == 0, "pairs");
   static_assert(EPILOGUE != kFp8GatedFp8 || TILES * COLUMNS == 128, "a workgroup holds whole blocks of the output");
-  __shared__ float parts[WAVES][ROWS][WIDTH + 1];
+  // The staged rows, and then, in their place, the waves' sums: two workgroups of 16
+  // rows of K = 4096 fit a CU.
   extern __shared__ __attribute__((aligned(16))) uint8_t staged[];
+  float(*const parts)[ROWS][WIDTH + 1] = reinterpret_cast<float(*)[ROWS][WIDTH + 1]>(staged);
   const int lane = threadIdx.x & 63, part = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int e, first, last;
@@ -184,16 +196,49 @@ __global__ void __launch_bounds__(64 * kFp8FewWaves) fp8_few_kernel(Fp8Product p
     if (turns > 0) load(unit, 0);  // in flight while the rows are quantised
     const int live = min(ROWS, last - m0);
     if constexpr (STAGED) {
-      const int piece = threadIdx.x % 16, all = fp8_staged_blocks(k);
-      for (int task = threadIdx.x / 16; task < live * all; task += 4 * WAVES) {
-        const int row = task / all, block = task % all, k0 = block * 128 + piece * 8;
-        int token = m0 + row;
-        if (p.order) token = max(0, min(p.order[token] / p.copies, p.tokens - 1));
-        Raw8<X> raw;
-        raw.load(static_cast<const X*>(p.x) + static_cast<uint64_t>(token) * p.row_stride + k0, k - k0);
-        const uint32_t scale = fp8_scale_byte(magnitude_bits<X>(row16_magnitude<X>(raw_magnitude(raw))));
-        *reinterpret_cast<elem_u32x2*>(staged + row * code_stride + k0) = fp8_encode8(raw, scale);
-        if (piece == 0) staged_scales[row * scale_stride + block] = static_cast<uint8_t>(scale);
+      // A wave takes 512 elements of a row at a time, BATCH of them in flight, so that
+      // rows and places are the wave's and cost its lanes nothing: quantisation is bound
+      // by instructions here, since every workgroup of the launch does it anew.
+      constexpr int BATCH = 2;
+      const int chunks = (k + 511) / 512, all = fp8_staged_blocks(k);
+      int row = 0, chunk = wave;
+      auto settle = [&]() __attribute__((always_inline)) {
+        while (chunk >= chunks) {
+          chunk -= chunks;
+          ++row;
+        }
+      };
+      settle();
+      while (row < live) {
+        Raw8<X> raw[BATCH];
+        int rows_at[BATCH], chunk_at[BATCH];
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          rows_at[u] = row;
+          chunk_at[u] = chunk;
+          if (row < live) {
+            int token = m0 + row;
+            if (p.order) token = max(0, min(p.order[token] / p.copies, p.tokens - 1));
+            const X* from = static_cast<const X*>(p.x) + static_cast<uint64_t>(token) * p.row_stride + chunk * 512;
+            if ((chunk + 1) * 512 <= k)
+              raw[u].load(from + lane * 8);
+            else
+              raw[u].load(from + lane * 8, k - chunk * 512 - lane * 8);
+          }
+          chunk += WAVES;
+          settle();
+        }
+#pragma unroll
+        for (int u = 0; u < BATCH; ++u) {
+          if (rows_at[u] >= live) break;
+          const uint32_t scale = fp8_scale_byte(magnitude_bits<X>(row16_magnitude<X>(raw_magnitude(raw[u]))));
+          const int block = chunk_at[u] * 4 + lane / 16;
+          if (block < all) {
+            *reinterpret_cast<elem_u32x2*>(staged + rows_at[u] * code_stride + chunk_at[u] * 512 + lane * 8) =
+                fp8_encode8(raw[u], scale);
+            if (lane % 16 == 0) staged_scales[rows_at[u] * scale_stride + block] = static_cast<uint8_t>(scale);
+          }
+        }
       }
       __syncthreads();
     }
@@ -249,6 +294,7 @@ __global__ void __launch_bounds__(64 * kFp8FewWaves) fp8_few_kernel(Fp8Product p
       multiply(unit, turn);
       if (turn + 1 < turns) load(unit, turn + 1);
     }
+    if constexpr (STAGED) __syncthreads();  // every wave has read the rows
 #pragma unroll
     for (int f = 0; f < FB; ++f)
 #pragma unroll

@@ -12,8 +12,11 @@ namespace {
 
 // ---- the kernels of products -----------------------------------------------------
 
-// Microseconds of a quantisation's launch, and of 4096 elements quantised in a product's.
-constexpr double kQuantizeLaunch = 2.8, kStaging = 0.25;
+// Microseconds of a quantisation's launch before a product's, and of 4096 elements that a
+// workgroup quantises in the product's own. Inside and before, in graphs: 4096 x 4096, 1,
+// 8 and 16 rows 5.7 and 7.4, 7.9 and 8.3, 10.6 and 9.0; the gated pair of 14336 x 4096,
+// 1, 4, 8 and 16 rows 24.3 and 25.9, 25.4 and 26.9, 28.0 and 27.7, 33.8 and 30.0.
+constexpr double kQuantizeLaunch = 2.0, kStaging = 0.22;
 
 constexpr int kE4m3 = 3;  // after MB_DTYPE_*: X an operand, or Y one
 
@@ -39,7 +42,8 @@ struct ProductKernel {
   int x, y, epilogue;
   bool tiles;
   int features, rows;  // of a workgroup: columns of the output, rows
-  int resident;        // workgroups a CU holds
+  int resident;        // workgroups a CU holds; of few rows, those of a round of the costs
+  int staged;          // of few rows, those that a CU's registers hold at once
   int band;            // row tiles that share their weight's panels in an XCD's L2
   int split;           // waves that share a tile's K
   ProductCost cost;
@@ -59,7 +63,8 @@ void launch_few(const Fp8Product& p, uint32_t, int, hipStream_t stream) {
   constexpr uint32_t kColumns = kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2);
   constexpr uint32_t kRows = kFp8FewRows;
   const uint32_t rows = static_cast<uint32_t>(p.rows), lds_rows = rows < kRows ? rows : kRows;
-  const uint64_t lds = sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0;
+  const uint64_t lds =
+      std::max(sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0, fp8_few_parts(FB * 16));
   fp8_few_kernel<X, Y, EPILOGUE, FB, SPLIT>
       <<<few_grid(static_cast<uint32_t>(p.n), kColumns, rows, kRows, static_cast<uint32_t>(p.experts), p.offsets),
          dim3(64 * kFp8FewWaves), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
@@ -75,13 +80,13 @@ void launch_tiles(const Fp8Product& p, uint32_t grid, int band, hipStream_t stre
 #define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, SPLIT, ...)                                       \
   ProductKernel {                                                                                              \
     "fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #SPLIT, type_code<X>(), type_code<Y>(), EPILOGUE, false, \
-        kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kFp8FewRows, 2, 0, SPLIT,            \
+        kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kFp8FewRows, 2, FB == 1 ? 2 : 1, 0, SPLIT, \
         {__VA_ARGS__}, launch_few<X, Y, EPILOGUE, FB, SPLIT>                                                   \
   }
 #define MB_FP8_TILES(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND, ...)                                     \
   ProductKernel {                                                                                              \
     "fp8_tiles_" NAME "_" Y_NAME "_" #BM "x" #BN, kE4m3, type_code<Y>(), EPILOGUE, true,                       \
-        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, BAND, 1,        \
+        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, 1, BAND, 1,     \
         {__VA_ARGS__}, launch_tiles<Y, EPILOGUE, BM, BN, STAGES>                                               \
   }
 // The forms, for a list M(arguments) of kernels and for their registration alike. Costs
@@ -213,8 +218,9 @@ double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint
     const double rounds = std::max(1.0, across * used * chunks / (256.0 * kernel.resident));
     const double turns = ((k + 255) / 256 + kernel.split - 1) / kernel.split;
     const double width = kernel.epilogue == kFp8Plain ? n : 2.0 * n;
-    // A workgroup quantises its rows, 4096 elements at a time.
-    const double staging = kernel.x == kE4m3 ? 0 : rounds * std::min(each, 1.0 * kFp8FewRows) * k / 4096 * kStaging;
+    const double turns_staged = std::max(1.0, across * used * chunks / (256.0 * kernel.staged));
+    const double staging =
+        kernel.x == kE4m3 ? 0 : turns_staged * std::min(each, 1.0 * kFp8FewRows) * k / 4096 * kStaging;
     return cost.launch + rounds * (cost.tile + turns * cost.step) + used * width * k * 1e-6 * chunks * cost.megabyte +
            staging;
   }
