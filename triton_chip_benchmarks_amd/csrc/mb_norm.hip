@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_backwar
   __shared__ float parts[2][2][WAVES];  // sums of even and odd rows in turn
   // Where a lane's registers hold no more (16 waves have 128 each), d_total is read when
   // it is added, and the parts of d_w lie in LDS, each lane's its own.
-  constexpr bool LATE = WAVES == 16 && sizeof(T) == 4;
+  constexpr bool LATE = WAVES * P == 32 && sizeof(T) == 4;
   __shared__ float kept[LATE ? P * 8 * WAVES * 64 : 1];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t worker = blockIdx.x * PER_GROUP + (WAVES == 1 ? wave : 0);
@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// call(integral_constant<WAVES>, integral_constant<P>) for a row of n elements: one
-// wave up to 1024, four up to 8192, else 16; with `spread`, as many as fill.
+// call(integral_constant<WAVES>, integral_constant<P>) for a row of n elements: one wave
+// up to 1024, four up to 8192, else 16; with `spread`, as many as have a piece each.
 template <class F>
 void for_width(uint32_t n, bool spread, F&& call) {
   auto with = [&](auto waves, auto pieces) { call(waves, pieces); };
@@ -287,6 +287,7 @@ void for_width(uint32_t n, bool spread, F&& call) {
 template <class T>
 int launch_norm(const char* entry, const NormArguments& a, hipStream_t stream) {
   int status = MB_OK;
+  // Few rows are spread: one of 8192 takes 2.8 us by 16 waves.
   for_width(a.n, a.rows <= 512, [&](auto waves, auto pieces) {
     constexpr int W = decltype(waves)::value, P = decltype(pieces)::value;
     constexpr uint32_t kThreads = W > 4 ? 64 * W : 256;
@@ -303,9 +304,12 @@ int launch_norm(const char* entry, const NormArguments& a, hipStream_t stream) {
 
 template <class T>
 void launch_norm_backward(const NormGradient& a, T* d_weight, hipStream_t stream) {
-  for_width(a.n, false, [&](auto waves, auto pieces) {
+  // Past 4096 columns 16 waves a row, half as many workers for the same waves: 4096 rows
+  // of 8192 in fp32 100 to 103 us, by four waves 108; 1000 of 5003 20 to 23 and 24; 8192
+  // of 8192 in bf16 108 to 112 by both.
+  for_width(a.n, a.n > 4096, [&](auto waves, auto pieces) {
     constexpr int W = decltype(waves)::value, P = decltype(pieces)::value;
-    if constexpr (W != 16 || P != 1)  // that form is of rows that are spread
+    if constexpr (W != 4 || P != 4)
       rms_norm_backward_kernel<T, W, P>
           <<<dim3(W == 1 ? (a.workers + 3) / 4 : a.workers), dim3(W > 4 ? 64 * W : 256), 0, stream>>>(a);
   });
@@ -314,10 +318,10 @@ void launch_norm_backward(const NormGradient& a, T* d_weight, hipStream_t stream
 
 // Workers of the gradient: as many waves as hide the memory's latency, and no more, for
 // each worker's part of d_w is written and read again. Microseconds with 256, 512, 1024
-// and 2048 of them: 512 columns of bf16 by one wave 419, 222, 124, 85 (100000 rows);
-// 8192 by four 117, 108, 114, 129 (8192 rows); 16384 by 16: 109, 115, 127, 155 (4096).
+// and 2048 of them: 512 columns of bf16 by one wave 419, 222, 124, 85 (100000 rows); 4096
+// by four 128, 105, 111, 118 (16384 rows); 16384 by 16: 109, 115, 127, 155 (4096).
 uint32_t norm_workers(uint32_t rows, uint32_t n) {
-  const uint32_t most = n <= 1024 ? 2048 : n <= 8192 ? 512 : 256;
+  const uint32_t most = n <= 1024 ? 2048 : n <= 4096 ? 512 : 256;
   return rows < most ? rows : most;
 }
 
@@ -331,8 +335,8 @@ uint32_t norm_workers(uint32_t rows, uint32_t n) {
   MB_NORM_REGISTER_BACKWARD(T, NAME, 1, 2);      \
   MB_NORM_REGISTER_BACKWARD(T, NAME, 4, 1);      \
   MB_NORM_REGISTER_BACKWARD(T, NAME, 4, 2);      \
-  MB_NORM_REGISTER_BACKWARD(T, NAME, 4, 4);      \
-  MB_NORM_REGISTER_FORM(T, NAME, 16, 1);         \
+  MB_NORM_REGISTER_FORM(T, NAME, 4, 4);          \
+  MB_NORM_REGISTER_BACKWARD(T, NAME, 16, 1);     \
   MB_NORM_REGISTER_BACKWARD(T, NAME, 16, 2);     \
   MB_REGISTER_KERNEL("rms_norm_weight_" NAME, rms_norm_weight_kernel<T>)
 MB_NORM_REGISTER(float, "f32");
