@@ -65,20 +65,25 @@ def test_layer_agrees_with_the_oracle_and_with_its_graph(gpu, tokens, hidden, in
     for _ in range(3):
         for tensor in (layer.out, layer.normed, layer.total, layer.y):
             tensor.fill_(float("nan"))
-        layer.inner.codes.view(torch.uint8).fill_(0x7f)
+        if layer.few:
+            layer.inner.fill_(float("nan"))
+        else:
+            layer.inner.codes.view(torch.uint8).fill_(0x7f)
         layer.experts.fill_(-1)
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(layer.out, eager)
 
 
+@pytest.mark.parametrize("tokens", [5, 40])
 @pytest.mark.parametrize("which", ["up_weight", "down_weight"])
-def test_another_experts_weight_does_not_pass_the_check(gpu, monkeypatch, which):
+def test_another_experts_weight_does_not_pass_the_check(gpu, monkeypatch, which, tokens):
     import torch
 
     from triton_chip_benchmarks_amd import experts
 
-    layer = experts.Fp8Layer(5, 256, 96, 8, 2, torch.bfloat16)
+    layer = experts.Fp8Layer(tokens, 256, 96, 8, 2, torch.bfloat16)
+    assert layer.few == (tokens == 5)
     right = experts._values
     monkeypatch.setattr(experts, "_values", lambda packed, e: right(packed, (e + 1) % 8) if packed is getattr(layer, which)
                         else right(packed, e))

@@ -24,6 +24,9 @@ constexpr uint32_t kBlock = kFp8Block;
 // elements, 16 lanes a block, a wave U * 512 elements of one row: whole dwords of
 // scales. With `slots` [rows][copies], row r goes to the operand's rows slots[r][0 ..
 // copies), those outside 0 .. out_rows - 1 left out; without, to row r.
+//
+// Bound by memory: 8192 x 8192 of bf16 take 45 us cold (4.5 TB/s), 5000 x 4112 14.5,
+// where a launch's start and end are a fifth; 4096 rows of 4096 to eight places each 34.
 template <class T, int U, bool STREAM>
 __global__ void __launch_bounds__(256)
     fp8_quantize_kernel(const T* __restrict__ x, uint32_t rows, uint32_t k, uint64_t row_stride,
@@ -103,7 +106,8 @@ __device__ __forceinline__ void put_scale(const TileOut& out, uint32_t scale_row
 // group, so that neither side meets its banks), and leave a column's 128 bytes
 // together. SQUARE: one scale for the whole tile, the same both ways.
 //
-// Bound by memory: the tile is read once for both.
+// Bound by memory, the tile read once for both: a weight of 6000 x 4112 in bf16 both ways
+// takes 25 us (3.9 TB/s).
 template <class T, bool SQUARE>
 __device__ __forceinline__ void quantize_tile(const Raw8<T> (&at)[8], uint32_t row_tile, uint32_t column_tile,
                                               const TileOut& by_rows, const TileOut& by_columns, TileShared& shared) {
@@ -285,6 +289,11 @@ struct GatePiece {
 // The operands of a product's gradients in one launch: d's rows and columns, tile by
 // tile, and x's columns. With gate_up, d is computed on the way: a tile of d_up follows
 // the tile of d_gate that reads the same, which it then finds in the XCD's L2.
+//
+// d 5000 x 3000 and x 5000 x 4112 in bf16 take 26 us, by memory (4.7 TB/s). With gate_up
+// 67, for 42 of memory at that rate, by instructions: about 30 us of sigmoids and scales
+// do not lie under the loads. Tiles of one side that leave out the other's half of the
+// gradient, and four rows' loads in flight at a time, changed nothing (66 to 76).
 template <class T, bool GATED>
 __global__ void __launch_bounds__(kTileThreads)
     fp8_gradient_kernel(const T* __restrict__ d, uint64_t d_stride, const T* __restrict__ gate_up,
@@ -332,7 +341,7 @@ __global__ void __launch_bounds__(kTileThreads)
 }
 
 // Codes and scales to values, rounded once to T (exact in fp32, and in bf16 from 2^-133
-// to its largest). A lane takes eight.
+// to its largest). A lane takes eight. 16384 x 8192 to bf16 take 74 us (5.4 TB/s).
 template <class T, bool STREAM>
 __global__ void __launch_bounds__(256)
     fp8_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,

@@ -114,6 +114,12 @@ class Layer:
         return self.out
 
 
+# Up to so many rows the gated pair goes to 16 bits, and the projection behind it quantises: a workgroup of the pair that
+# writes an operand has whole blocks of it, 128 columns, and so few of those leave most CUs without one. One token of the
+# command's layer takes 40 us so and 49 with an operand between, eight tokens 153 and 143.
+FEW_ROWS = 16
+
+
 class Fp8Layer(Layer):
     """A layer on FP8 operands, from the residual stream on. Normed rows are quantised as they are gathered, so that a
     token's row is read once for each of its experts and its operand is never read twice."""
@@ -133,17 +139,24 @@ class Fp8Layer(Layer):
         self.before = normal(tokens, hidden).to(dtype)
         self.norm_weight = (1 + 0.1 * normal(hidden)).to(dtype)
         self.total, self.normed = buffer(tokens, hidden), buffer(tokens, hidden)
-        self.inner = fp8.empty(rows, inner, device=device)
-        self.space = fp8.gated_workspace(rows, inner, hidden, dtype, experts, device)
+        self.few = rows <= FEW_ROWS
+        self.inner = buffer(rows, inner) if self.few else fp8.empty(rows, inner, device=device)
+        self.up_space = fp8.gated_workspace(rows, inner, hidden, dtype, experts, device)
+        self.down_space = fp8.linear_workspace(rows, hidden, inner, dtype, experts, device)
 
     def norm(self):
         norm.rms_norm(self.before, self.norm_weight, residual=self.x, out=self.normed, total=self.total)
 
     def gated(self):
-        fp8.gated(self.normed, self.up_weight, packed=self.inner, plan=self.plan, workspace=self.space)
+        to = {"out" if self.few else "packed": self.inner}
+        fp8.gated(self.normed, self.up_weight, **to, plan=self.plan, workspace=self.up_space)
 
     def down(self):
-        fp8.product(self.inner, self.down_weight, self.y, offsets=self.plan.offsets)
+        if self.few:
+            fp8.linear(self.inner, self.down_weight, self.y, plan=self.plan, sorted_rows=True,
+                       workspace=self.down_space)
+        else:
+            fp8.product(self.inner, self.down_weight, self.y, offsets=self.plan.offsets)
 
     STEPS = ("norm", "route", "dispatch", "gated", "down", "combine")
 
@@ -162,11 +175,11 @@ def work(layer: Layer, step: str) -> dict:
         def packed(n, k, block=fp8.BLOCK):
             return n * k + -(-n // block) * -(-k // fp8.BLOCK)
 
+        between = rows * inner * item if rows <= FEW_ROWS else packed(rows, inner, 1)
         products = {"norm": {"bytes": (4 * tokens + 1) * hidden * item, "flops": 5 * tokens * hidden},
-                    "gated": {"bytes": tokens * hidden * item + used * packed(2 * inner, hidden)
-                                       + packed(rows, inner, 1),
+                    "gated": {"bytes": tokens * hidden * item + used * packed(2 * inner, hidden) + between,
                               "flops": 4 * rows * inner * hidden},
-                    "down": {"bytes": packed(rows, inner, 1) + used * packed(hidden, inner) + rows * hidden * item,
+                    "down": {"bytes": between + used * packed(hidden, inner) + rows * hidden * item,
                              "flops": 2 * rows * inner * hidden}}
     else:
         def packed(n, k):
@@ -210,7 +223,7 @@ def check(layer: Layer, tokens: int = 32) -> float:
         compare("norm", layer.normed[:tokens],
                 total * (total.square().mean(1, keepdim=True) + 1e-6).rsqrt() * layer.norm_weight.double())
         x = fp8.dequantize(fp8.quantize(layer.normed[:tokens])).double()
-        held = fp8.dequantize(layer.inner).double()
+        held = fp8.dequantize(fp8.quantize(layer.inner) if layer.few else layer.inner).double()
     else:
         x = mx.dequantize(mx.quantize(layer.x[:tokens])).double()
     for t, (shares, chosen, slots) in enumerate(zip(layer.weights[:tokens].tolist(), layer.experts[:tokens].tolist(),
@@ -222,7 +235,7 @@ def check(layer: Layer, tokens: int = 32) -> float:
             if on_fp8:
                 gate, up = (x[t:t + 1] @ _values(layer.up_weight, e).t().contiguous()).chunk(2, 1)
                 inner = held[slot:slot + 1]
-                compare("gated", inner, torch.nn.functional.silu(gate) * up)
+                compare("gated", layer.inner[slot:slot + 1] if layer.few else inner, torch.nn.functional.silu(gate) * up)
             else:
                 gate_up, inner = (part[slot:slot + 1] for part in (layer.gate_up, layer.gate))
                 compare("up", gate_up, x[t:t + 1] @ _values(layer.up_weight, e).t().contiguous())
@@ -232,7 +245,7 @@ def check(layer: Layer, tokens: int = 32) -> float:
             compare("down", y, inner @ _values(layer.down_weight, e).t().contiguous())
             expected[t] += share * y[0].double()
     compare("combine", layer.out[:tokens], expected)
-    if on_fp8:  # its operand's codes are rounded to 2^-4, four times the tolerance: counted as a quarter
+    if on_fp8 and not layer.few:  # its codes are rounded to 2^-4, four times the tolerance: counted as a quarter
         squares["gated"][0] /= 16
     distances = [(error / size)**0.5 if size else float(error != 0) for error, size in squares.values()]
     return max(distances) if all(distance == distance for distance in distances) else float("nan")
