@@ -7,22 +7,23 @@ from triton_chip_benchmarks_amd import _native, fp8
 
 DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 
-# (rows, n, k, experts, of a tensor) of each kernel of an output type, by the kind of product.
+# (rows, n, k, experts) of each kernel of an output type, by the kind of product; of few rows, X a tensor or an operand.
 FEW = {
-    "product": {"1x8": (1, 16, 16, 8, True), "2x4": (64, 1408, 2048, 64, True), "2x8": (12000, 22, 20, 400, True)},
-    "gated": {"2x4": (444, 17, 16, 400, True), "2x8": (1, 16, 16, 8, True)},
+    "product": {"1x4": (1, 4096, 1024, 1), "1x8": (1, 4096, 4096, 1), "2x4": (1, 14336, 1024, 1)},
+    "gated": {"2x4": (1, 4096, 1024, 1), "2x8": (1, 1024, 4096, 1)},
+    "gated_fp8": {"2x1": (1, 16, 16, 8)},
 }
 TILES = {
-    "product": {"64x64": (1, 17, 18, 1), "128x64": (27, 1248, 16, 128), "128x128": (22859, 96, 18, 1),
+    "product": {"64x64": (21391, 34, 20, 8), "128x64": (36, 3541, 19, 128), "128x128": (22859, 96, 18, 1),
                 "256x128": (2545, 1704, 16, 8), "256x256": (2850, 3080, 16, 8)},
-    "gated": {"256x64": (5, 4222, 18, 32), "256x128": (15640, 16, 16, 32), "256x256": (12177, 412, 17, 8)},
-    "gated_kept": {"256x64": (7, 4166, 17, 128), "256x128": (16462, 34, 16, 8), "256x256": (2545, 1704, 16, 8)},
-    "gated_fp8": {"256x64": (3, 4655, 126, 128), "256x128": (15640, 16, 16, 32), "256x256": (16399, 134, 19, 32)},
+    "gated": {"256x64": (6, 10559, 18, 128), "256x128": (18037, 36, 18, 1), "256x256": (12177, 412, 17, 8)},
+    "gated_kept": {"256x64": (688, 1000, 17, 32), "256x128": (15907, 72, 18, 32), "256x256": (2545, 1704, 16, 8)},
+    "gated_fp8": {"256x64": (1, 19, 524, 1), "256x128": (15640, 16, 16, 32), "256x256": (16399, 134, 19, 32)},
 }
 TILES_32 = {
-    "product": {"64x64": (1, 16, 16, 8), "128x64": (27, 1248, 16, 128), "128x128": (4028, 862, 16, 32),
+    "product": {"64x64": (18037, 36, 18, 1), "128x64": (31, 7921, 24, 128), "128x128": (4028, 862, 16, 32),
                 "256x128": (9225, 335, 18, 128)},
-    "gated": {"256x64": (5, 4222, 18, 32)}, "gated_kept": {"256x64": (11, 2676, 16, 32)},
+    "gated": {"256x64": (24, 11380, 20, 128)}, "gated_kept": {"256x64": (5609, 120, 18, 1)},
 }
 
 
@@ -34,15 +35,13 @@ def _choices(name):
         for tile, (rows, n, k, experts) in sizes.items():
             yield f"fp8_tiles_{kind}_{form}_{tile}", fp8.product_kernel(rows, n, k, dtype, experts, False, kind)
     for kind, sizes in FEW.items():
-        for shape, (rows, n, k, experts, _) in sizes.items():
-            yield (f"fp8_few_{kind}_{name}_{name}_{shape}",
-                   fp8.product_kernel(rows, n, k, dtype, experts, True, kind))
-    yield f"fp8_few_gated_fp8_{name}_e4m3_2x1", fp8.product_kernel(1, 16, 16, dtype, 8, True, "gated_fp8")
-    yield "fp8_few_gated_fp8_e4m3_e4m3_2x1", fp8.product_kernel(1, 16, 16, dtype, 8, False, "gated_fp8")
-    for shape, size in (("1x8", (1, 19, 16, 400)), ("2x4", (77, 124, 16, 400)), ("2x8", (12592, 22, 21, 400))):
-        yield f"fp8_few_product_e4m3_{name}_{shape}", fp8.product_kernel(*size[:3], dtype, size[3])
-    for shape, kind, size in (("2x4", "gated", (444, 17, 16, 400)), ("2x8", "gated_kept", (1, 16, 16, 8))):
-        yield f"fp8_few_gated_e4m3_{name}_{shape}", fp8.product_kernel(*size[:3], dtype, size[3], False, kind)
+        form = "e4m3" if kind == "gated_fp8" else name
+        for shape, (rows, n, k, experts) in sizes.items():
+            yield f"fp8_few_{kind}_{name}_{form}_{shape}", fp8.product_kernel(rows, n, k, dtype, experts, True, kind)
+            yield f"fp8_few_{kind}_e4m3_{form}_{shape}", fp8.product_kernel(rows, n, k, dtype, experts, False, kind)
+            if kind == "gated":  # of few rows the same kernels keep the gate and up
+                yield (f"fp8_few_{kind}_e4m3_{form}_{shape}",
+                       fp8.product_kernel(rows, n, k, dtype, experts, False, "gated_kept"))
 
 
 @pytest.mark.parametrize("name", sorted(DTYPES))

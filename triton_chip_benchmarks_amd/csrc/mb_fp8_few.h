@@ -53,7 +53,10 @@ struct Fp8Product {
   int copies, tokens, experts;
 };
 
-constexpr int kFp8FewWaves = 8, kFp8FewRows = 16;
+constexpr int kFp8FewRows = 16;
+// Waves of a workgroup, and the workgroups of which a CU's registers hold the waves.
+constexpr int fp8_few_waves(int split) { return split == 4 ? 4 : 8; }
+constexpr int fp8_few_resident(int fb, int split) { return (fb == 1 ? 16 : 12) / fp8_few_waves(split); }
 
 // LDS of the quantised rows: a row's codes, then a row's scales, each row a bank
 // group past the one before. Pairs of blocks: a turn of the kernel takes two.
@@ -63,7 +66,7 @@ constexpr uint32_t fp8_scale_stride(uint32_t k) { return fp8_staged_blocks(k) + 
 constexpr uint64_t fp8_few_lds(uint32_t k, uint32_t rows) {
   return uint64_t{rows} * (fp8_code_stride(k) + fp8_scale_stride(k));
 }
-constexpr uint64_t fp8_few_parts(int width) { return uint64_t{kFp8FewWaves} * kFp8FewRows * (width + 1) * 4; }
+constexpr uint64_t fp8_few_parts(int waves, int width) { return uint64_t{1} * waves * kFp8FewRows * (width + 1) * 4; }
 
 // A lane's 32 codes of a block of K and the dword with its scale.
 //
@@ -136,17 +139,18 @@ __device__ __forceinline__ f32x4 fp8_mma16(const Fp8Fragment<true, SEL>& a, cons
 // of one row of the output.
 //
 // Reading the weights bounds it, so the next turn's are in flight while one's are
-// multiplied, and nothing else waits for them: one row by 8192 x 8192 takes 14.4 us
-// (4.7 TB/s, two of them the launch), 16 by the gated pair of 14336 x 4096 25.7 (4.6),
-// 256 by those of 110 experts of 1024 x 4096 138 (6.7). SPLIT 8 is for the fewest
-// columns, and FB 2 for as many as leave a wave more to do: 4096 x 4096 5.7 us by 1x8;
-// 14336 x 1024 4.7 by 2x4. With X's codes or a third turn in flight as well, a wave's
-// registers leave a CU half the waves, at 1.1 to 1.3 times the time.
+// multiplied (131 to 160 registers with two fragments of W, 12 waves a CU). Workgroups of
+// four waves fill those where one of eight leaves four out: the gated pair of 14336 x 4096
+// takes 16 rows in 27.5 us and not 31, 64 tokens of eight of 128 experts of 2048 x 2048
+// 170 and not 194 (6.3 TB/s). A SPLIT of eight is for as few columns as leave CUs without
+// a workgroup, where a wave's turns one after the other are the time: one row of 8192 by
+// 2048 columns takes 7.7 us, by four 10.4. With X's codes or a third turn in flight as
+// well, a CU holds half the waves, at 1.1 to 1.3 times the time.
 template <class X, class Y, int EPILOGUE, int FB, int SPLIT>
-__global__ void __launch_bounds__(64 * kFp8FewWaves) fp8_few_kernel(Fp8Product p, int lds_rows) {
+__global__ void __launch_bounds__(64 * fp8_few_waves(SPLIT)) fp8_few_kernel(Fp8Product p, int lds_rows) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr bool GATED = EPILOGUE != kFp8Plain, STAGED = sizeof(X) > 1, WIDE = sizeof(Y) == 4;
-  constexpr int WAVES = kFp8FewWaves, ROWS = kFp8FewRows, TILES = WAVES / SPLIT, WIDTH = FB * 16;
+  constexpr int WAVES = fp8_few_waves(SPLIT), ROWS = kFp8FewRows, TILES = WAVES / SPLIT, WIDTH = FB * 16;
   constexpr int COLUMNS = GATED ? WIDTH / 2 : WIDTH;
   static_assert(!GATED || FB % 2 == 0, "pairs");
   static_assert(EPILOGUE != kFp8GatedFp8 || TILES * COLUMNS == 128, "a workgroup holds whole blocks of the output");

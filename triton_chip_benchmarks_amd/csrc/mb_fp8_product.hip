@@ -12,11 +12,13 @@ namespace {
 
 // ---- the kernels of products -----------------------------------------------------
 
-// Microseconds of a quantisation's launch before a product's, and of 4096 elements that a
-// workgroup quantises in the product's own. Inside and before, in graphs: 4096 x 4096, 1,
-// 8 and 16 rows 5.7 and 7.4, 7.9 and 8.3, 10.6 and 9.0; the gated pair of 14336 x 4096,
-// 1, 4, 8 and 16 rows 24.3 and 25.9, 25.4 and 26.9, 28.0 and 27.7, 33.8 and 30.0.
-constexpr double kQuantizeLaunch = 2.0, kStaging = 0.22;
+// Microseconds of a quantisation's launch before a product's (with what an operand in
+// memory costs the product over one in LDS), and of 4096 elements that a workgroup of
+// eight waves quantises in the product's own, alone on a CU or for every workgroup that
+// the CU has. Inside and before, in graphs: 14336 x 4096, 1, 4 and 8 rows 13.8 and 16.9,
+// 16.4 and 18.4, 20.5 and 18.7; the gated pair of it 26.1 and 27.0, 27.4 and 27.5, 33.4
+// and 27.8; 1024 x 4096, 1, 4 and 8 rows 5.4 and 6.7, 7.2 and 7.2, 9.5 and 7.5.
+constexpr double kQuantizeLaunch = 2.5, kStagingAlone = 0.22, kStaging = 0.3;
 
 constexpr int kE4m3 = 3;  // after MB_DTYPE_*: X an operand, or Y one
 
@@ -28,9 +30,11 @@ constexpr int type_code() {
 // What a launch takes, in microseconds. Of tiles: `launch` once; for every round of the
 // chip's workgroups `tile`, `ragged` more where the rows of Y are not on 16 bytes, and for
 // every 128 elements of K from `step_empty` to `step` with the filled share of the round
-// (the L2s and the power limit slow a step down as more CUs run). Of few rows: `launch`;
-// for every round `tile` and, for every 256 elements of K that a wave takes, `step`; and
-// `megabyte` for every 10^6 bytes of weights.
+// (the L2s and the power limit slow a step down as more CUs run), and kMegabyte for every
+// 10^6 bytes of weights at least. Of few rows: `launch`, and the root of the squares of
+// `tile` and, for every 256 elements of K that a wave takes, `step` a round, and of
+// `megabyte` for every 10^6 bytes of weights (either alone where the other is small).
+constexpr double kMegabyte = 0.25;
 struct ProductCost {
   float launch, tile, ragged, step_empty, step, megabyte;
 };
@@ -42,8 +46,7 @@ struct ProductKernel {
   int x, y, epilogue;
   bool tiles;
   int features, rows;  // of a workgroup: columns of the output, rows
-  int resident;        // workgroups a CU holds; of few rows, those of a round of the costs
-  int staged;          // of few rows, those that a CU's registers hold at once
+  int resident;        // workgroups a CU holds
   int band;            // row tiles that share their weight's panels in an XCD's L2
   int split;           // waves that share a tile's K
   ProductCost cost;
@@ -60,14 +63,14 @@ dim3 few_grid(uint32_t n, uint32_t columns, uint32_t rows, uint32_t chunk, uint3
 
 template <class X, class Y, int EPILOGUE, int FB, int SPLIT>
 void launch_few(const Fp8Product& p, uint32_t, int, hipStream_t stream) {
-  constexpr uint32_t kColumns = kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2);
+  constexpr uint32_t kColumns = fp8_few_waves(SPLIT) / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2);
   constexpr uint32_t kRows = kFp8FewRows;
   const uint32_t rows = static_cast<uint32_t>(p.rows), lds_rows = rows < kRows ? rows : kRows;
   const uint64_t lds =
-      std::max(sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0, fp8_few_parts(FB * 16));
+      std::max(sizeof(X) > 1 ? fp8_few_lds(static_cast<uint32_t>(p.k), lds_rows) : 0, fp8_few_parts(fp8_few_waves(SPLIT), FB * 16));
   fp8_few_kernel<X, Y, EPILOGUE, FB, SPLIT>
       <<<few_grid(static_cast<uint32_t>(p.n), kColumns, rows, kRows, static_cast<uint32_t>(p.experts), p.offsets),
-         dim3(64 * kFp8FewWaves), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
+         dim3(64 * fp8_few_waves(SPLIT)), static_cast<uint32_t>(lds), stream>>>(p, static_cast<int>(lds_rows));
 }
 
 template <class Y, int EPILOGUE, int BM, int BN, int STAGES>
@@ -80,27 +83,28 @@ void launch_tiles(const Fp8Product& p, uint32_t grid, int band, hipStream_t stre
 #define MB_FP8_FEW(X, X_NAME, Y, Y_NAME, EPILOGUE, NAME, FB, SPLIT, ...)                                       \
   ProductKernel {                                                                                              \
     "fp8_few_" NAME "_" X_NAME "_" Y_NAME "_" #FB "x" #SPLIT, type_code<X>(), type_code<Y>(), EPILOGUE, false, \
-        kFp8FewWaves / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kFp8FewRows, 2, FB == 1 ? 2 : 1, 0, SPLIT, \
+        fp8_few_waves(SPLIT) / SPLIT * FB * 16 / (EPILOGUE == kFp8Plain ? 1 : 2), kFp8FewRows, fp8_few_resident(FB, SPLIT), 0, SPLIT, \
         {__VA_ARGS__}, launch_few<X, Y, EPILOGUE, FB, SPLIT>                                                   \
   }
 #define MB_FP8_TILES(Y, Y_NAME, EPILOGUE, NAME, BM, BN, STAGES, BAND, ...)                                     \
   ProductKernel {                                                                                              \
     "fp8_tiles_" NAME "_" Y_NAME "_" #BM "x" #BN, kE4m3, type_code<Y>(), EPILOGUE, true,                       \
-        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, 1, BAND, 1,     \
+        EPILOGUE == kTilePlain ? BM : BM / 2, BN, Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESIDENT, BAND, 1,        \
         {__VA_ARGS__}, launch_tiles<Y, EPILOGUE, BM, BN, STAGES>                                               \
   }
 // The forms, for a list M(arguments) of kernels and for their registration alike. Costs
-// are fitted to 8700 sizes on an MI355X (1 to 16384 rows, n and K from 64 to 8192, one
-// weight or 8 to 128 experts of uneven popularity, two of five off the tiles): the
-// cheapest estimate costs 1.3% over the fastest of the tiles on average for products and
-// 0.3% for gated ones, and 1.8% over the fastest of all where there are few rows; the
-// worst are 6 to 27 us of launches of 7 to 60 in which a few experts had all the rows.
+// are fitted to sizes timed on an MI355X, two of five off the tiles: of tiles to 8700 (1
+// to 16384 rows, n and K from 64 to 8192, one weight or 8 to 128 experts of uneven
+// popularity), where the cheapest estimate costs 1.3% over the fastest on average for
+// products and 0.3% for gated ones; of few rows to 17800 in graphs (up to 40 rows of one
+// weight and six an expert), where it costs 1.4% over the fastest of all and 4% at the
+// ninth decile; the worst are up to twice the time, 30 us, where K is 128 or 256.
 #define MB_FP8_FEW_16(M, X, X_NAME, Y, Y_NAME)                                           \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 8, 5.68f, 1.01f, 0, 0, 0, 0.071f)     \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 8, 4.15f, 2.46f, 0, 0, 0.18f, 0.078f) \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 3.52f, 2.43f, 0, 0, 0.78f, 0.082f) \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 8, 4.87f, 2.39f, 0, 0, 0.03f, 0.089f)   \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 4.26f, 2.36f, 0, 0, 0.72f, 0.072f)
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 8, 1.89f, 0.33f, 0, 0, 1.18f, 0.243f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 4, 2.04f, 0.61f, 0, 0, 0.64f, 0.220f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 1.80f, 0.69f, 0, 0, 1.07f, 0.211f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 8, 2.13f, 0, 0, 0, 1.60f, 0.230f)       \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 1.82f, 0.81f, 0, 0, 1.04f, 0.207f)
 #define MB_FP8_TILES_16(M, Y, Y_NAME)                                                                 \
   M(Y, Y_NAME, kTilePlain, "product", 256, 256, 2, 4, 4.56f, 3.81f, 4.15f, 0.958f, 1.700f, 0)         \
   M(Y, Y_NAME, kTilePlain, "product", 256, 128, 3, 4, 3.83f, 2.87f, 2.05f, 0.620f, 1.095f, 0)         \
@@ -114,11 +118,11 @@ void launch_tiles(const Fp8Product& p, uint32_t grid, int band, hipStream_t stre
   M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 128, 3, 4, 3.75f, 6.17f, 2.81f, 0.614f, 1.010f, 0)  \
   M(Y, Y_NAME, kTileGatedKept, "gated_kept", 256, 64, 3, 8, 3.70f, 3.74f, 1.41f, 0.429f, 0.712f, 0)
 #define MB_FP8_FEW_32(M, X, X_NAME, Y, Y_NAME)                                           \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 8, 5.72f, 1.00f, 0, 0, 0, 0.085f)     \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 8, 4.07f, 2.48f, 0, 0, 0.29f, 0.094f) \
-  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 3.34f, 2.44f, 0, 0, 0.99f, 0.093f) \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 8, 5.08f, 1.91f, 0, 0, 0.23f, 0.111f)   \
-  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 4.30f, 1.96f, 0, 0, 1.02f, 0.094f)
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 8, 1.91f, 0.41f, 0, 0, 1.21f, 0.243f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 1, 4, 2.01f, 0.48f, 0, 0, 0.94f, 0.223f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Plain, "product", 2, 4, 1.80f, 0.47f, 0, 0, 1.46f, 0.220f) \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 8, 2.22f, 0, 0, 0, 1.73f, 0.239f)       \
+  M(X, X_NAME, Y, Y_NAME, kFp8Gated, "gated", 2, 4, 1.94f, 0.45f, 0, 0, 1.46f, 0.209f)
 #define MB_FP8_TILES_32(M, Y, Y_NAME)                                                         \
   M(Y, Y_NAME, kTilePlain, "product", 256, 128, 3, 4, 1.98f, 5.02f, 0.85f, 1.290f, 1.771f, 0) \
   M(Y, Y_NAME, kTilePlain, "product", 128, 128, 4, 6, 3.53f, 2.70f, 0.06f, 0.720f, 0.946f, 0) \
@@ -133,10 +137,10 @@ void launch_tiles(const Fp8Product& p, uint32_t grid, int band, hipStream_t stre
   MB_FP8_FEW_32(M, float, "f32", float, "f32")                                                            \
   MB_FP8_FEW_16(M, _Float16, "f16", _Float16, "f16")                                                      \
   MB_FP8_FEW_16(M, __bf16, "bf16", __bf16, "bf16")                                                        \
-  M(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f) \
-  M(float, "f32", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f)    \
-  M(_Float16, "f16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f) \
-  M(__bf16, "bf16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 2.58f, 3.06f, 0, 0, 1.36f, 0.113f)
+  M(uint8_t, "e4m3", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 0.74f, 3.04f, 0, 0, 1.99f, 0.217f) \
+  M(float, "f32", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 0.74f, 3.04f, 0, 0, 1.99f, 0.217f)    \
+  M(_Float16, "f16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 0.74f, 3.04f, 0, 0, 1.99f, 0.217f) \
+  M(__bf16, "bf16", uint8_t, "e4m3", kFp8GatedFp8, "gated_fp8", 2, 1, 0.74f, 3.04f, 0, 0, 1.99f, 0.217f)
 #define MB_FP8_TILES_ALL(M)                                                                          \
   MB_FP8_TILES_32(M, float, "f32")                                                                   \
   MB_FP8_TILES_16(M, _Float16, "f16")                                                                \
@@ -212,17 +216,20 @@ double mean_row_tiles(uint32_t rows, uint32_t experts, int tile) {
 double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint32_t k, uint32_t experts) {
   const ProductCost& cost = kernel.cost;
   const double across = (n + uint64_t{1} * kernel.features - 1) / kernel.features;
+  const double used = used_experts(rows, experts);
+  const double megabytes = used * (kernel.epilogue == kTilePlain ? 1 : 2) * n * k * 1e-6;  // of weights
   if (!kernel.tiles) {
-    const double used = used_experts(rows, experts), each = rows / used;
+    const double each = rows / used;
     const double chunks = experts == 1 ? (rows + kFp8FewRows - 1) / kFp8FewRows : std::max(1.0, each / kFp8FewRows);
     const double rounds = std::max(1.0, across * used * chunks / (256.0 * kernel.resident));
     const double turns = ((k + 255) / 256 + kernel.split - 1) / kernel.split;
-    const double width = kernel.epilogue == kFp8Plain ? n : 2.0 * n;
-    const double turns_staged = std::max(1.0, across * used * chunks / (256.0 * kernel.staged));
-    const double staging =
-        kernel.x == kE4m3 ? 0 : turns_staged * std::min(each, 1.0 * kFp8FewRows) * k / 4096 * kStaging;
-    return cost.launch + rounds * (cost.tile + turns * cost.step) + used * width * k * 1e-6 * chunks * cost.megabyte +
-           staging;
+    // Every workgroup quantises its rows.
+    const double each_cu = across * used * chunks / 256.0, waves = fp8_few_waves(kernel.split);
+    const double staging = kernel.x == kE4m3 ? 0
+                                             : std::min(each, 1.0 * kFp8FewRows) * k / 4096 *
+                                                   std::max(kStagingAlone * 8 / waves, kStaging * each_cu);
+    return cost.launch + staging +
+           std::hypot(rounds * (cost.tile + turns * cost.step), megabytes * chunks * cost.megabyte);
   }
   const double tiles = mean_row_tiles(rows, experts, kernel.rows) * across;
   const double round = 256.0 * kernel.resident, whole = static_cast<double>(static_cast<uint64_t>(tiles / round));
@@ -232,7 +239,8 @@ double product_cost(const ProductKernel& kernel, uint32_t rows, uint32_t n, uint
     return cost.tile + (ragged ? cost.ragged : 0.0f) +
            steps * (cost.step_empty + (cost.step - cost.step_empty) * filled);
   };
-  return cost.launch + whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
+  const double all = cost.launch + whole * one(1.0) + (rest > 0 ? one(rest) : 0.0);
+  return std::max(all, 1.0 + megabytes * kMegabyte) + 0.01 * all;  // of two that memory bounds the quicker
 }
 
 struct ProductChoice {
