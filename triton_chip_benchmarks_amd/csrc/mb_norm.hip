@@ -6,7 +6,9 @@
 //   d_t = r (w dy - t r^2 mean(w dy t)) + d_total,  d_w = sum over rows of dy t r
 //
 // The norm is taken of t as it is rounded, so that the gradient, which reads the stream
-// again, differentiates what was computed. Sums are of fp32.
+// again, differentiates what was computed. The norm's sum, root and products are of 64
+// bits, at the rate of fp32's and under the loads: an FP8 code beside a border is then the
+// exact value's, but for fp32's rounding. The gradients' sums are of fp32.
 #include <type_traits>
 
 #include "mb_fp8.h"
@@ -21,12 +23,13 @@ constexpr uint32_t kMostColumns = 16384;  // of a row, which a workgroup holds i
 
 // Sum over a row's WAVES waves, the same in every lane; `parts` has a place for each.
 template <int WAVES>
-__device__ __forceinline__ float row_sum(float v, float* parts, uint32_t wave) {
-  v = wave_add(v);
+__device__ __forceinline__ double row_sum(double v, double* parts, uint32_t wave) {
+#pragma unroll
+  for (int offset = 32; offset > 0; offset >>= 1) v += __shfl_xor(v, offset, 64);
   if constexpr (WAVES > 1) {
     if ((threadIdx.x & 63) == 0) parts[wave] = v;
     __syncthreads();
-    v = 0.0f;
+    v = 0.0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) v += parts[w];
   }
@@ -43,16 +46,17 @@ struct NormArguments {
   void *total, *out;
   uint8_t *codes, *scales;
   uint32_t rows, n;
+  double per_column;  // 1 / n
 };
 
 // A row by WAVES waves, each lane P pieces of eight neighbouring elements: the row is
 // read once and stays in registers. 16 lanes hold a block of the FP8 output, a wave a
 // dword of its scales. Memory bounds it: 16384 rows of 8192 in bf16 with the residual,
-// its sum and the FP8 output take 159 us, 5.9 TB/s.
+// its sum and the FP8 output take 160 to 164 us, 5.8 TB/s.
 template <class T, int WAVES, int P>
 __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_kernel(NormArguments a) {
   constexpr uint32_t PER_GROUP = WAVES == 1 ? 4 : 1;  // rows of a workgroup
-  __shared__ float parts[WAVES];
+  __shared__ double parts[WAVES];
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t row = blockIdx.x * PER_GROUP + (WAVES == 1 ? wave : 0);
   if (row >= a.rows) return;
@@ -72,14 +76,15 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_kernel(
     const uint32_t c = (p * WAVES * 64 + thread) * 8;
     weight[p].load(static_cast<const T*>(a.weight) + c, static_cast<int>(n > c ? n - c : 0));
   }
-  float t[P][8], sum = 0.0f;
+  float t[P][8];
+  double sum = 0.0;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       t[p][i] = raw[p][i];
       if (a.residual) t[p][i] = widen(static_cast<T>(t[p][i] + added[p][i]));
-      sum = fmaf(t[p][i], t[p][i], sum);
+      sum = fma(static_cast<double>(t[p][i]), static_cast<double>(t[p][i]), sum);
     }
   }
   if (a.total) {
@@ -90,14 +95,22 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_kernel(
     }
   }
   sum = row_sum<WAVES>(sum, parts, wave);
-  const float inverse = 1.0f / sqrtf(sum / static_cast<float>(n) + a.eps);
+  const double mean = sum * a.per_column + a.eps;
+  double inverse;
+  if (mean > 1e-30 && mean < 1e30) {  // a step of Newton from fp32's: within 2^-45 of it
+    inverse = __builtin_amdgcn_rsqf(static_cast<float>(mean));
+    inverse *= 1.5 - 0.5 * mean * inverse * inverse;
+  } else {
+    inverse = 1.0 / sqrt(mean);
+  }
   const uint32_t pitch = (n + 15) / 16 * 16;
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const uint32_t c = (p * WAVES * 64 + thread) * 8;
     float y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = t[p][i] * inverse * weight[p][i];
+    for (int i = 0; i < 8; ++i)
+      y[i] = static_cast<float>(t[p][i] * inverse * static_cast<double>(weight[p][i]));
     if (a.out && c < n)
       store8<false>(static_cast<T*>(a.out) + static_cast<uint64_t>(row) * n + c, y, static_cast<int>(n - c));
     if (a.codes) {
@@ -287,7 +300,8 @@ void for_width(uint32_t n, bool spread, F&& call) {
 template <class T>
 int launch_norm(const char* entry, const NormArguments& a, hipStream_t stream) {
   int status = MB_OK;
-  // Few rows are spread: one of 8192 takes 2.8 us by 16 waves.
+  // Few rows are spread: one of 8192 takes 3.6 us by 16 waves, 0.8 of them for the sums
+  // of 64 bits.
   for_width(a.n, a.rows <= 512, [&](auto waves, auto pieces) {
     constexpr int W = decltype(waves)::value, P = decltype(pieces)::value;
     constexpr uint32_t kThreads = W > 4 ? 64 * W : 256;
@@ -381,7 +395,7 @@ int mb_rms_norm(int dtype, const void* x, uint64_t x_bytes, uint64_t x_stride, c
     if (int rc = mb::fp8_check_operand(entry, "the output's", rows, n, 1, 1, codes, codes_bytes, scales, scales_bytes))
       return rc;
   const mb::NormArguments a{x,     x_stride, residual, residual_stride, weight, eps, total, out,
-                            static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, n};
+                            static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), rows, n, 1.0 / n};
   int status = MB_OK;
   MB_FOR_DTYPE(dtype, status = mb::launch_norm<T>(entry, a, static_cast<hipStream_t>(stream)));
   return status;

@@ -116,7 +116,7 @@ class Layer:
 
 # Up to so many rows the gated pair goes to 16 bits, and the projection behind it quantises: a workgroup of the pair that
 # writes an operand has whole blocks of it, 128 columns, and so few of those leave most CUs without one. One token of the
-# command's layer takes 40 us so and 49 with an operand between, eight tokens 153 and 143.
+# command's layer takes 37 us so and 49 with an operand between, eight tokens 153 and 143.
 FEW_ROWS = 16
 
 
