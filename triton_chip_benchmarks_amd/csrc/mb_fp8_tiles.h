@@ -19,7 +19,7 @@ struct Fp8Tile {
   static constexpr bool GATED = EPILOGUE != kTilePlain;
   static constexpr int ROWB = 128, WM = BM / 2, WN = BN / 2, FM = WM / 32, FN = WN / 32, CHUNKS = 4;
   static constexpr int DMA_A = BM / 32, DMA_B = BN / 32, DMAS = DMA_A + DMA_B + 1;  // per wave and step
-  static constexpr int OPERANDS = (BM + BN) * ROWB, STAGE = OPERANDS + (GATED ? 3072 : 2048);
+  static constexpr int OPERANDS = (BM + BN) * ROWB, STAGE = OPERANDS + (GATED ? 3 : 2) * 1024;
   static constexpr int MFMAS = FM * FN * 2, READS = (FM + FN) * CHUNKS;
   static constexpr int SHARED = STAGES * STAGE + (EPILOGUE == kTileGatedFp8 ? 2 * BN * 4 : 0);
   static constexpr int RESIDENT = 160 * 1024 / SHARED;  // workgroups a CU's LDS holds

@@ -64,8 +64,8 @@ def empty(rows: int, k: int, block: int = 1, device="cuda", experts: int | None 
 
 def _check_experts(packed: Packed, what: str, experts: int | None) -> None:
     if packed.experts != experts:
-        raise ValueError(f"{what} must hold {'one matrix' if experts is None else f'a matrix for each of {experts} experts'},"
-                         f" not codes of {tuple(packed.codes.shape)}")
+        wanted = "one matrix" if experts is None else f"a matrix for each of {experts} experts"
+        raise ValueError(f"{what} must hold {wanted}, not codes of {tuple(packed.codes.shape)}")
 
 
 def _operand(packed: Packed | None, what: str, rows: int, k: int, block: int, like, stream) -> Packed:
@@ -84,8 +84,8 @@ def _parts(packed: Packed) -> tuple[int, int, int, int]:
 
 
 def quantize(x, packed: Packed | None = None, columns: bool = False, block: int = 1, stream=None) -> Packed:
-    """The operand of x's rows; with `columns`, of its columns (x transposed, blocks along its rows). `block` rows of the
-    operand, 1 or 128, share a scale."""
+    """The operand of x's rows; with `columns`, of its columns (x transposed, blocks along its rows). `block` rows of
+    the operand, 1 or 128, share a scale."""
     code = dtype_code(x, "x")
     x_rows, x_columns, stride, span = strided_rows(x, "x")
     rows, k = (x_columns, x_rows) if columns else (x_rows, x_columns)

@@ -29,8 +29,8 @@ class Normed(NamedTuple):
 
 
 def rms_norm(x, weight, eps: float = 1e-6, residual=None, out=None, packed=None, total=None, stream=None) -> Normed:
-    """y = t * weight / sqrt(mean(t^2) + eps) of rows t = x [rows][n], or x + residual rounded to x's type (`total`, which
-    may be x or the residual itself).
+    """y = t * weight / sqrt(mean(t^2) + eps) of rows t = x [rows][n], or x + residual rounded to x's type (`total`,
+    which may be x or the residual itself).
 
     y goes to `packed` (fp8.Packed of rows x n), if given, and to `out`, if given or if packed is not.
     """
@@ -107,8 +107,9 @@ def rms_norm_backward(d_out, total, weight, eps: float = 1e-6, d_total=None, d_x
     workspace = _workspace(workspace, native.mb_rms_norm_backward_workspace(rows, n), total, stream)
     handle = launch_stream(stream, *tensors, d_x, d_weight, workspace)
     status = native.mb_rms_norm_backward(code, *strides[0], total.data_ptr(), span * item, stride,
-                                         weight.data_ptr(), n * item, eps, *strides[1], d_x.data_ptr(), rows * n * item, d_weight.data_ptr(),
-                                         n * item, rows, n, workspace.data_ptr(), workspace.numel(), handle)
+                                         weight.data_ptr(), n * item, eps, *strides[1], d_x.data_ptr(),
+                                         rows * n * item, d_weight.data_ptr(), n * item, rows, n,
+                                         workspace.data_ptr(), workspace.numel(), handle)
     if status:
         _native.check(status)
     return d_x, d_weight
