@@ -7,6 +7,7 @@ can never silently measure something other than the hand-written kernels.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from pathlib import Path
 import threading
@@ -179,6 +180,10 @@ def load(path: Path | None = None) -> ctypes.CDLL:
             raise NativeLibraryMissing(
                 f"{target} is missing; build it with `python -m triton_chip_benchmarks_amd.build` "
                 "(or __graft_entry__.build()) before running a benchmark")
+        # torch brings a HIP runtime of its own, which the library takes if it is there already. Loaded the other way
+        # round there are two, and the library's finds no device beside torch's.
+        with contextlib.suppress(ImportError):
+            import torch  # noqa: F401
         try:
             library = ctypes.CDLL(str(target))
         except OSError as exc:
