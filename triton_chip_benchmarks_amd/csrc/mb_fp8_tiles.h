@@ -385,6 +385,23 @@ __global__ void __launch_bounds__(256, (Fp8Tile<EPILOGUE, BM, BN, STAGES>::RESID
         int here_lane = lane;
         asm volatile("" : "+v"(here_lane));
         const int lrow = here_lane % 32, lgroup = here_lane / 32;
+        // Columns past n have codes of zero, but scales of other rows or steps: a NaN among those is not the block's.
+        if (limit < COLUMNS) {
+#pragma unroll
+          for (int i = 0; i < FM / 2; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+              int left = limit - (wm * (FM / 2) + i) * 32;
+              pin(acc[2 * i][j]);
+              asm volatile("" : "+v"(left));
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                if (out_row_32(here_lane, r) >= left) acc[2 * i][j][r] = 0.0f;
+                __builtin_amdgcn_sched_barrier(0);
+              }
+              pin(acc[2 * i][j]);
+            }
+        }
         uint32_t largest[FN];
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
