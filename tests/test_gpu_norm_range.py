@@ -1,0 +1,55 @@
+"""The norm's gradients of rows whose squares pass fp32's range, either way: those of what the forward pass computed.
+
+Tolerances: a row's sums of n terms in fp32, in any order, are off by less than n 2^-24 of their magnitudes, the root by
+half of that, and a dozen roundings of 2^-24 make d_x of them, and one of half a step (u) its type. A term of d_weight has
+the root's error and a few roundings; a sum over the rows is off by less than rows 2^-24 of their magnitudes. Rows are
+scaled by powers of two, which is exact but for values that end below 2^-126.
+"""
+
+import numpy as np
+import pytest
+
+from oracle import norm as oracle
+
+pytestmark = pytest.mark.gpu
+
+
+def host(tensor):
+    return tensor.double().cpu().numpy()
+
+
+@pytest.mark.parametrize("size,eps", [(1e20, 1e-6), (3e37, 1e-6), (1e-25, 0.0), (1e-36, 0.0), (1.0, 1e-6)])
+@pytest.mark.parametrize("also", [False, True])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows,n", [(1, 100), (9, 700), (3, 2048), (520, 4000), (4, 8192), (300, 8200), (5, 16384)])
+def test_gradients_of_large_and_small_rows(gpu, rows, n, dtype, also, size, eps):
+    import torch
+
+    from triton_chip_benchmarks_amd import norm
+
+    of = getattr(torch, dtype)
+    generator = torch.Generator(device="cuda").manual_seed(rows + n)
+
+    def normal(*shape, scale=1.0):
+        return (scale * torch.randn(shape, device="cuda", generator=generator)).to(of)
+
+    total, weight, d_out = normal(rows, n, scale=size), normal(n), normal(rows, n)
+    d_total = normal(rows, n, scale=1 / size) if also else None  # as large as the norm's own part
+    assert torch.isfinite(norm.rms_norm(total, weight, eps).out).all()
+    d_x, d_weight = norm.rms_norm_backward(d_out, total, weight, eps, d_total=d_total)
+    t, w, d = host(total), host(weight), host(d_out)
+    eps = float(np.float32(eps))
+    exact_x, exact_w = oracle.rms_norm_backward(d, t, w, eps, None if d_total is None else host(d_total))
+    inverse = 1 / np.sqrt((t * t).mean(axis=1, keepdims=True) + eps)
+    dw, normed = np.abs(d * w), np.abs(t) * inverse
+    terms_x = inverse * (dw + normed * (dw * normed).mean(axis=1, keepdims=True))
+    terms_w = (np.abs(d) * normed).sum(axis=0)
+    info = torch.finfo(of)
+    u = info.eps / 2 * (1 + 2.0**-7)
+    floor = info.smallest_normal * info.eps + 2.0**-148  # half a step each of the norm's part and of its sum with d_total
+    off = (2 * n + 12) * 2.0**-24 * terms_x + 2.0**-24 * np.abs(exact_x)
+    assert np.isfinite(host(d_x)).all()
+    assert (np.abs(host(d_x) - exact_x) <= off + u * (np.abs(exact_x) + off) + floor).all()
+    off = (rows + n / 2 + 8) * 2.0**-24 * terms_w
+    assert (np.abs(host(d_weight) - exact_w) <= off + u * (np.abs(exact_w) + off) + floor).all()
+    assert np.abs(host(d_x)).max() > 0 and np.abs(host(d_weight)).max() > 0
