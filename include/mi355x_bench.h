@@ -520,9 +520,9 @@ int mb_fp8_gated_backward(int dtype, const void* d_out, uint64_t d_out_bytes, ui
                           uint64_t workspace_bytes, void* stream);
 
 /* Root-mean-square norm of rows: t = x + residual, rounded to dtype and written to
- * total (both NULL: t = x), y = t * weight / sqrt(mean(t^2) + eps) in fp32, rounded
- * once to out [rows][n] (dtype), to an FP8 operand (codes and scales, as
- * mb_fp8_quantize of the fp32 values), or both; NULL ones are left out. weight [n] of
+ * total (both NULL: t = x), y = t * weight / sqrt(mean(t^2) + eps) in 64 bits, rounded
+ * to fp32 and from there to out [rows][n] (dtype), to an FP8 operand (codes and scales,
+ * as mb_fp8_quantize of the fp32 values), or both; NULL ones are left out. weight [n] of
  * dtype. total may be x or the residual itself. n <= 16384. */
 int mb_rms_norm(int dtype, const void* x, uint64_t x_bytes, uint64_t x_stride, const void* residual,
                 uint64_t residual_bytes, uint64_t residual_stride, const void* weight, uint64_t weight_bytes, float eps,
@@ -534,8 +534,9 @@ uint64_t mb_rms_norm_backward_workspace(uint32_t rows, uint32_t n);
 
 /* Gradients of mb_rms_norm for d_out [rows][n]: d_x [rows][n], of x and of the residual
  * alike, with d_total (NULL: none), the gradient that t gets as an output, added; and
- * d_weight [n], summed over the rows in a fixed order. d_x may be d_out or d_total
- * itself. Two launches. */
+ * d_weight [n], summed over the rows in a fixed order. Sums in fp32, of rows scaled by a
+ * power of two where their squares pass its range. d_x may be d_out or d_total itself.
+ * Two launches. */
 int mb_rms_norm_backward(int dtype, const void* d_out, uint64_t d_out_bytes, uint64_t d_out_stride, const void* total,
                          uint64_t total_bytes, uint64_t total_stride, const void* weight, uint64_t weight_bytes,
                          float eps, const void* d_total, uint64_t d_total_bytes, uint64_t d_total_stride, void* d_x,

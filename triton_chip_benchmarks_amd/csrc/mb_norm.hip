@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_kernel(
   sum = row_sum<WAVES>(sum, parts, wave);
   const double mean = sum * a.per_column + a.eps;
   double inverse;
-  if (mean > 1e-30 && mean < 1e30) {  // a step of Newton from fp32's: within 2^-45 of it
+  if (mean > 1e-30 && mean < 1e30) {  // a step of Newton from fp32's: within 2^-44 of it
     inverse = __builtin_amdgcn_rsqf(static_cast<float>(mean));
     inverse *= 1.5 - 0.5 * mean * inverse * inverse;
   } else {
