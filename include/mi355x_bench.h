@@ -434,9 +434,10 @@ int mb_fp8_dequantize(int dtype, const void* codes, uint64_t codes_bytes, const 
 
 /* C [rows][n] = A . B^T for operands A of `rows` rows and B of `experts` matrices of n
  * rows (codes and scales one matrix after the other), a scale of A standing for
- * a_block rows (1 or 128) and one of B for b_block. Sums in fp32 (of a block's 128
- * products, for fp16 and bf16 outputs, to about 2^-16 of the result, as the FP8 matrix
- * instructions give it), rounded once to dtype. offsets as in mb_mx_product; with them
+ * a_block rows (1 or 128) and one of B for b_block. Sums in fp32, rounded once to
+ * dtype; for fp16 and bf16 outputs a block's 128 products are summed as the FP8 matrix
+ * instructions do, to 2^-12 of their magnitudes at worst (2^-16 to 2^-14 of the result
+ * by its 2-norm). offsets as in mb_mx_product; with them
  * a_block is 1. kernel: the name of the kernel to run on, for tests and measurements, or
  * NULL. */
 int mb_fp8_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
@@ -488,8 +489,9 @@ int mb_fp8_linear_backward(int dtype, const void* d_out, uint64_t d_out_bytes, u
  * the gate, then the n of the up projection. silu(g) = g / (1 + e^-g), in fp32.
  * y_scales NULL: y in dtype, and, if gate_up is given, [G | U] as gate_up [rows][2n] in
  * dtype. Else y is an FP8 operand's codes (K = n, a scale for each row's 128),
- * quantised from the fp32 values, and gate_up must be NULL. Everything else as in
- * mb_fp8_product. */
+ * quantised from the fp32 values, and gate_up must be NULL; its sums are then those of
+ * 16-bit outputs, whatever dtype (for sums in fp32, y in fp32 and mb_fp8_quantize of
+ * it). Everything else as in mb_fp8_product. */
 int mb_fp8_gated_product(int dtype, const void* a, uint64_t a_bytes, const void* scale_a, uint64_t scale_a_bytes,
                          uint32_t a_block, const void* b, uint64_t b_bytes, const void* scale_b, uint64_t scale_b_bytes,
                          uint32_t b_block, void* y, uint64_t y_bytes, void* y_scales, uint64_t y_scales_bytes,

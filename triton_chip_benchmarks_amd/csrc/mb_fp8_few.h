@@ -139,7 +139,7 @@ __device__ __forceinline__ f32x4 fp8_mma16(const Fp8Fragment<true, SEL>& a, cons
 // of one row of the output.
 //
 // Reading the weights bounds it, so the next turn's are in flight while one's are
-// multiplied (131 to 160 registers with two fragments of W, 12 waves a CU). Workgroups of
+// multiplied (132 to 152 registers with two fragments of W, 12 waves a CU). Workgroups of
 // four waves fill those where one of eight leaves four out: the gated pair of 14336 x 4096
 // takes 16 rows in 27.5 us and not 31, 64 tokens of eight of 128 experts of 2048 x 2048
 // 170 and not 194 (6.3 TB/s). A SPLIT of eight is for as few columns as leave CUs without

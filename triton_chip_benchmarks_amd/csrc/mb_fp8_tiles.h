@@ -65,7 +65,7 @@ struct Kept {
 //
 // The matrix cores bound it, and the clock that the power limit leaves them: 8192^3 from
 // operands in the caches takes 388 us (2.83 PFLOP/s; this library's FP8 product without
-// scales 376 to 404), with cold ones 424 to 450. With the barrier after the fourth
+// scales 376 to 404), with cold ones 418 to 450. With the barrier after the fourth
 // product instead of the second 433 cold, with two barriers a step, each for half of the
 // operands, 464. By 256x128 the same product takes 474: its loads are half as many again.
 //

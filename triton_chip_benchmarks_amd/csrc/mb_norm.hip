@@ -53,7 +53,7 @@ struct NormArguments {
 // A row by WAVES waves, each lane P pieces of eight neighbouring elements: the row is
 // read once and stays in registers. 16 lanes hold a block of the FP8 output, a wave a
 // dword of its scales. Memory bounds it: 16384 rows of 8192 in bf16 with the residual,
-// its sum and the FP8 output take 160 to 164 us, 5.8 TB/s.
+// its sum and the FP8 output take 156 to 164 us, 5.8 to 6.0 TB/s.
 template <class T, int WAVES, int P>
 __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_kernel(NormArguments a) {
   constexpr uint32_t PER_GROUP = WAVES == 1 ? 4 : 1;  // rows of a workgroup
@@ -154,8 +154,8 @@ constexpr float kMeanMost = 0x1p110f, kMeanLeast = 0x1p-40f;
 
 // Rows worker, worker + workers, .. of the gradient, by WAVES waves as above: both sums
 // of a row in one pass over it, and the worker's part of d_w in registers. Memory bounds
-// it: 8192 rows of 8192 in bf16, three read and one written, take 108 us with the sum
-// below, 5.0 TB/s.
+// it: 8192 rows of 8192 in bf16, three read and one written, take 104 to 112 us, 4.8 to 5.2
+// TB/s, and the sum below 4.6.
 template <class T, int WAVES, int P>
 __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_backward_kernel(NormGradient a) {
   constexpr uint32_t PER_GROUP = WAVES == 1 ? 4 : 1;

@@ -200,7 +200,8 @@ def _routes(plan, rows: int, sorted_rows: bool):
 
 
 def linear_workspace(rows: int, n: int, k: int, dtype, experts: int = 1, device="cuda"):
-    """A workspace for `linear` with `rows` output rows (routed ones, with a plan)."""
+    """A workspace for `linear` with `rows` output rows (routed ones, with a plan); for every n, type and number of experts
+    the same."""
     return torch.empty(library().mb_fp8_linear_workspace(rows, n, k), dtype=torch.uint8, device=device)
 
 
@@ -295,7 +296,8 @@ def gated(x, weight: Packed, out=None, packed: Packed | None = None, gate_up=Non
     rows, G's and then U's (with a `plan`, a matrix for each expert, as for `linear`; an operand's rows are sorted).
 
     The result, rounded once from fp32, is `out` [rows][n] of x's type (of an operand: of `dtype`, bfloat16 unless
-    given) or, if `packed` is given, that operand, with a scale for each row's 128. `gate_up` [rows][2n], if given, gets
+    given) or, if `packed` is given, that operand, with a scale for each row's 128, its sums those of 16-bit outputs
+    whatever x's type (`quantize` of an fp32 `out` has fp32's). `gate_up` [rows][2n], if given, gets
     [x . G^T | x . U^T], which `gated_backward` takes. `kernel` names the kernel to run an operand on, for tests and
     measurements.
     """
