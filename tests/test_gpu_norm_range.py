@@ -53,3 +53,39 @@ def test_gradients_of_large_and_small_rows(gpu, rows, n, dtype, also, size, eps)
     off = (rows + n / 2 + 8) * 2.0**-24 * terms_w
     assert (np.abs(host(d_weight) - exact_w) <= off + u * (np.abs(exact_w) + off) + floor).all()
     assert np.abs(host(d_x)).max() > 0 and np.abs(host(d_weight)).max() > 0
+
+
+@pytest.mark.parametrize("n", [300, 1800, 4000, 9000, 16384])
+def test_rows_of_every_kind_stand_by_themselves(gpu, n):
+    """Rows that are summed once and rows that are summed again, with zeros, infinities and NaN among them, give each what it
+    gives alone; those that are finite what the formula says, with an eps of any size."""
+    import torch
+
+    from triton_chip_benchmarks_amd import norm
+
+    generator = torch.Generator(device="cuda").manual_seed(n)
+    total = torch.randn(700, n, device="cuda", generator=generator)
+    size = torch.tensor([1.0, 1e25, 0.0, 1e-30, 3e37, 1.0, 1e-44], device="cuda").repeat(100)[:, None]
+    total *= size
+    total[5::7, 3], total[12::14, 3] = float("nan"), float("inf")
+    weight, d_out = (torch.randn(shape, device="cuda", generator=generator) for shape in ((n,), (700, n)))
+    finite = torch.isfinite(total).all(dim=1).cpu().numpy()
+    assert finite.sum() == 600
+    for eps in (0.0, 1e-6, 1e-20, 1e35):
+        d_x, _ = norm.rms_norm_backward(d_out, total, weight, eps)
+        for row in (0, 1, 2, 3, 4, 5, 6, 12, 699):
+            alone, _ = norm.rms_norm_backward(d_out[row:row + 1], total[row:row + 1], weight, eps)
+            assert torch.equal(alone.nan_to_num(7.0), d_x[row:row + 1].nan_to_num(7.0)), (eps, row)
+        assert torch.isnan(d_x[5::7, 3]).all()
+        t, w, d = host(total)[finite], host(weight), host(d_out)[finite]
+        kept = np.abs(t).max(axis=1) > (0 if eps else 1e-40)  # 0 / 0, and roots past fp32, are not numbers
+        if eps:
+            kept[:] = True
+        t, d = t[kept], d[kept]
+        wide = float(np.float32(eps))
+        exact, _ = oracle.rms_norm_backward(d, t, w, wide)
+        inverse = 1 / np.sqrt((t * t).mean(axis=1, keepdims=True) + wide)
+        dw, normed = np.abs(d * w), np.abs(t) * inverse
+        terms = inverse * (dw + normed * (dw * normed).mean(axis=1, keepdims=True))
+        off = (2 * n + 12) * 2.0**-24 * terms + 2.0**-23 * np.abs(exact) + 2.0**-148
+        assert (np.abs(host(d_x)[finite][kept] - exact) <= off).all(), eps
