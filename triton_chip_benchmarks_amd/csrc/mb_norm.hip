@@ -248,8 +248,9 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_backwar
       sums(scale, scaled_parts, squares, along);
       mean = squares / static_cast<float>(n) + a.eps * scale * scale;
     }
-    const float inverse = 1.0f / sqrtf(mean);
+    float inverse = 1.0f / sqrtf(mean);
     const float share = along / static_cast<float>(n) * inverse;
+    inverse *= scale;  // of t itself: past fp32 only where all of a row lies below 2^-126, and eps with it
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const uint32_t c = (p * WAVES * 64 + thread) * 8;
@@ -258,9 +259,9 @@ __global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) rms_norm_backwar
       float d_x[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float normed = t[p][i] * scale * inverse;
+        const float normed = t[p][i] * inverse;
         sum_at(p, i) = fmaf(d[p][i], normed, sum_at(p, i));
-        d_x[i] = inverse * (d[p][i] * weight[p][i] - normed * share) * scale;
+        d_x[i] = inverse * (d[p][i] * weight[p][i] - normed * share);
         if (a.d_total) d_x[i] += d_total[LATE ? 0 : p][i];
       }
       if (live > 0) store8<false>(static_cast<T*>(a.d_x) + static_cast<uint64_t>(row) * n + c, d_x, live);
