@@ -24,8 +24,8 @@ def host(tensor):
     return tensor.double().cpu().numpy()
 
 
-@pytest.mark.parametrize("size,eps", SIZES)
-@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("dtype,size,eps", [(dtype, *size) for dtype in ("float32", "float16", "bfloat16")
+                                            for size in SIZES[:1 if dtype == "float16" else 3]])  # (fp16 holds no others)
 @pytest.mark.parametrize("rows,n", [(3, 1), (40, 130), (514, 512), (5, 1024), (514, 1025), (7, 4096), (514, 4104),
                                     (6, 8192), (514, 8192), (3, 16384), (514, 16384)])
 def test_outputs_and_codes_are_the_exact_values(gpu, rows, n, dtype, size, eps):
@@ -33,8 +33,6 @@ def test_outputs_and_codes_are_the_exact_values(gpu, rows, n, dtype, size, eps):
 
     from triton_chip_benchmarks_amd import fp8, norm
 
-    if dtype == "float16" and size != 1.0:
-        pytest.skip("fp16 holds no such rows")
     of = getattr(torch, dtype)
     generator = torch.Generator(device="cuda").manual_seed(rows + n)
     x = (size * torch.randn(rows, n, device="cuda", generator=generator)).to(of)
